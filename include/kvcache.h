@@ -516,6 +516,61 @@ int kvc_rotary_plan_resolve_slots(kvc_rotary_plan* plan, int64_t* slots, void* s
 /* As kvc_write_plan_set_slots. */
 int kvc_rotary_plan_set_slots(kvc_rotary_plan* plan, const int64_t* slots);
 
+/* ---------------------------------------------------------------------------
+ * Causal attention over the paged cache, for the queries of a step.
+ * Stands where the reference calls BatchPrefillWithPagedKVCacheWrapper.run /
+ * BatchDecodeWithPagedKVCacheWrapper.run behind the write
+ *   (runtime/worker/llm_worker/models/layers/attention.py:87-99), with the index
+ * tensors of the write and qo_indptr (the reference's cu_seqlens_q,
+ * runtime/worker/llm_worker/model_worker.py:362-365).
+ * Request b has the query rows [qo_indptr[b], qo_indptr[b+1]) and the keys
+ *   len_b = max(pages_b - 1, 0) * page_size + kv_last_page_len[b],
+ * pages_b = kv_indptr[b+1] - kv_indptr[b] (no pages: no keys). Its j-th token stands at position len_b - n_b + j
+ * and attends to the keys up to its own position; query head x reads key head
+ * x / (num_heads / num_kv_heads):
+ *   out = softmax(sm_scale * q.k) v,  lse = log(sum exp(sm_scale * q.k)).
+ * A row without keys (also: one whose every score is -inf) is zero, its lse
+ * -inf. A page outside [0, num_pages) has no keys. What lies behind a request's
+ * last key, or is masked, does not reach the result, infinities and NaN included.
+ * Rows behind qo_indptr[batch_size] are left as they were. Sums and softmax
+ * statistics are fp32, the weights are rounded to the storage type for the
+ * matrix instruction, the output once.
+ *
+ * shared_pages: the leading pages that the requests of the batch share (a
+ * common prompt). They are read once for the rows of all requests whose block
+ * table begins with the same pages as that of the first request with tokens and
+ * so many pages; a request that begins with others is computed by itself. The number
+ * changes how the work is cut, not what is computed.
+ *
+ * A plan is made once per step and holds the ARGUMENTS, not the arrays; sizes
+ * are capacities (num_tokens: rows of query and out), so a recorded
+ * kvc_attention_plan_build and _run serve every later step written into the
+ * same index buffers. _build lays the step's work out in `buffer`
+ * (kvc_attention_plan_bytes, device memory, aligned to 256, kept by the caller while the plan
+ * is used); _run must be ordered after it. _run works in `workspace`
+ * (kvc_attention_workspace_bytes, aligned to 256): runs that may overlap need a workspace each.
+ * query [num_tokens, num_heads*head_dim] with a token stride in elements,
+ * rows and pages aligned to 16 bytes; out [num_tokens, num_heads*head_dim]
+ * contiguous; lse fp32 [num_tokens, num_heads] or NULL. dtype bf16 or f16;
+ * head_dim a multiple of 8 up to 256. */
+typedef struct kvc_attention_plan kvc_attention_plan;
+
+int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indices,
+                              const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                              int64_t batch_size, int64_t num_tokens, int64_t num_kv_indices,
+                              int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                              int64_t page_size, int64_t shared_pages, float sm_scale, int dtype,
+                              kvc_attention_plan** out);
+int64_t kvc_attention_plan_bytes(const kvc_attention_plan* plan);
+int64_t kvc_attention_workspace_bytes(const kvc_attention_plan* plan);
+int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buffer_bytes,
+                             void* stream);
+int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query,
+                           int64_t q_token_stride, const void* paged_kv_cache,
+                           int64_t page_stride, int64_t num_pages, void* out, float* lse,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+int kvc_attention_plan_destroy(kvc_attention_plan* plan);
+
 /* The on-device half of a swap on its own: gather scattered pool blocks into a
  * dense device buffer laid out like the host pool, [n, layer_end-layer_begin,
  * block_bytes], or scatter such a buffer back:

@@ -5,6 +5,7 @@
     paged       append_paged_kv_cache(_layers), get_seq_lens, get_batch_indices_positions
     kv_worker   KVWorker (GPU <-> pinned host swap), Device, BlockMapping
     index_prep  host-side block-table / slot-mapping construction
+    attention   causal attention over the paged cache, a shared prefix read once for the batch
     rotary      rotary position embedding, alone or fused with the K/V write
     disk_tier   DiskTier (host <-> block file, native positional I/O)
     kv_pool     pool sizing, layer-sync handle and model-side hooks, hand-over to a second process
@@ -18,6 +19,7 @@ C ABI of include/kvcache.h; the disk tier is host-side file I/O in the same
 library. Nothing here has a CPU fallback.
 """
 from . import _lib
+from .attention import PagedAttentionPlan, paged_attention
 from .cache_ops import (check_block_maps, copy_blocks, fill_key_cache, flatten_block_maps,
                         gather_blocks, reshape_and_cache, reshape_and_cache_layers, scatter_blocks,
                         swap_in, swap_out)
@@ -52,4 +54,5 @@ __all__ = [
     "InferInput", "KVIndexInputs", "make_kv_index_inputs", "to_device", "to_device_one_launch",
     "build_write_index", "BlockRuns", "max_block_runs", "slot_block_runs", "write_block_runs_layers",
     "KVWriteStep",
+    "PagedAttentionPlan", "paged_attention",
 ]

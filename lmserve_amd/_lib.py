@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 from typing import Optional
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -136,6 +136,13 @@ SIGNATURES = {
                                                     _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64,
                                                     _P, _P, _P, _I64, _I64, _I64, _I64, _I64, c_int,
                                                     _P]),
+    "kvc_attention_plan_create": (c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, c_float,
+                                          c_int, ctypes.POINTER(_P)]),
+    "kvc_attention_plan_bytes": (_I64, [_P]),
+    "kvc_attention_workspace_bytes": (_I64, [_P]),
+    "kvc_attention_plan_build": (c_int, [_P, _P, _I64, _P]),
+    "kvc_attention_plan_run": (c_int, [_P, _P, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P]),
+    "kvc_attention_plan_destroy": (c_int, [_P]),
     "kvc_copy_blocks": (c_int, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P]),
     "kvc_gather_blocks": (c_int, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
     "kvc_scatter_blocks": (c_int, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P]),

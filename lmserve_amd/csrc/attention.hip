@@ -1,0 +1,758 @@
+// Causal attention of a step's queries over the paged K/V cache (gfx950).
+//
+// Row r of a request is (token, query head): with G = query heads per key head, the G heads of a token that share a key
+// head are G rows of one matrix, so grouped heads read a key once. For a row with limit `lim` (its position + 1):
+//   s_k = scale q.k,  m = max s,  l = sum_k exp(s_k - m),  o = sum_k exp(s_k - m) v_k / l     over k < lim,
+// in one pass over the keys: where the running maximum grows, what was summed is scaled by exp(m_old - m_new).
+// Ranges of keys that different workgroups took are joined by their lse = m + log l: o = sum_c exp(lse_c - lse) o_c.
+// Exponentials are taken to base 2, with scale * log2(e) in the exponent's multiply-add.
+//
+// A step's work is laid out on the device, from the index tensors (two small launches, once per step): items of
+// (row tile, key range) of about equal length, as many as fill the card, however the lengths are spread. The leading
+// pages that the requests of a batch share are items of their own, whose rows are those of ALL these requests.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <new>
+
+#include "common.h"
+#include "device.h"
+#include "kvcache.h"
+
+namespace {
+
+using kvc::fail;
+using kvc::log2_exact;
+using kvc::u32x4;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kTile = 16;          // rows of an item
+constexpr int kBlock = 32;         // keys that a wavefront takes at once
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// ---- the step's layout ---------------------------------------------------------------------------------------------
+struct Request {  // 16 bytes
+  int32_t q_begin, n, len, table;  // first token, tokens, keys, first entry of its block table
+};
+struct Item {  // 32 bytes
+  int32_t q_begin;  // first token of the request; -1: the rows of all sharing requests, through shared_tokens
+  int32_t row0, rows, table, key_begin, key_end;
+  int32_t slot;     // where its partial goes; -1: the only item of its rows
+  int32_t pad;
+};
+struct Entry {  // 32 bytes: a row tile that is joined from partials (or has no keys at all)
+  int32_t q_begin, row0, rows, slot, chunks;
+  int32_t shared_row0;  // the tile's first row among those of the sharing requests, or -1
+  int32_t pad[2];
+};
+struct Header {
+  int32_t items, entries, shared_chunks, shared_tokens;
+};
+
+struct Layout {  // the plan's device buffer
+  Header* header;
+  Request* requests;
+  int32_t* shares;         // [B] 1: its leading pages are the shared ones
+  int32_t* offsets;        // [B][4] first item, slot, entry, shared token
+  int32_t* limits;         // [T] keys that a token sees
+  int32_t* shared_tokens;  // [T]
+  Item* items;
+  Entry* entries;
+};
+
+struct PlanArgs {
+  const int32_t *qo_indptr, *kv_indices, *kv_indptr, *kv_last_page_len;
+  int32_t batch_size, num_tokens, num_kv_indices, page_size, shared_pages, group;
+  int32_t target;      // items that a step is cut into, about
+  int32_t min_chunk;   // keys
+  int32_t max_items, max_entries;
+  Layout l;
+};
+
+__device__ __forceinline__ int32_t clamp(int32_t x, int32_t lo, int32_t hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+struct Table {
+  int32_t begin, pages;
+};
+__device__ __forceinline__ Table table_of(const PlanArgs& a, int32_t b) {
+  const int32_t begin = clamp(a.kv_indptr[b], 0, a.num_kv_indices);
+  return {begin, clamp(a.kv_indptr[b + 1], begin, a.num_kv_indices) - begin};
+}
+__device__ __forceinline__ Table tokens_of(const PlanArgs& a, int32_t b) {
+  const int32_t begin = clamp(a.qo_indptr[b], 0, a.num_tokens);
+  return {begin, clamp(a.qo_indptr[b + 1], begin, a.num_tokens) - begin};
+}
+
+// A workgroup per request: its lengths, its tokens' limits, and whether it begins with the shared pages. Which pages these
+// are is what the first request with tokens and that many pages holds; a request that holds others is a request by itself,
+// so that the number of shared pages changes how the work is cut and never the result.
+__global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
+  __shared__ int32_t first, differ;
+  const int32_t b = blockIdx.x, tid = threadIdx.x;
+  const Table q = tokens_of(a, b), t = table_of(a, b);
+  const int64_t room = (int64_t)t.pages * a.page_size;
+  const int64_t want = t.pages ? room - a.page_size + clamp(a.kv_last_page_len[b], 0, a.page_size) : 0;
+  const int32_t len = (int32_t)(want < INT32_MAX - 64 ? want : INT32_MAX - 64);
+  for (int32_t j = tid; j < q.pages; j += 256) {
+    const int32_t lim = len - q.pages + j + 1;
+    a.l.limits[q.begin + j] = lim > 0 ? lim : 0;
+  }
+  bool shares = a.shared_pages > 0 && q.pages > 0 && t.pages >= a.shared_pages;
+  if (shares) {
+    if (tid == 0) {
+      first = b;
+      differ = 0;
+    }
+    __syncthreads();
+    for (int32_t c0 = 0; c0 < b; c0 += 256) {
+      const int32_t c = c0 + tid;
+      if (c < b && tokens_of(a, c).pages > 0 && table_of(a, c).pages >= a.shared_pages) atomicMin(&first, c);
+      __syncthreads();
+      const bool found = first < b;
+      __syncthreads();  // everyone has looked before someone lowers it further
+      if (found) break;
+    }
+    const int32_t* mine = a.kv_indices + t.begin;
+    const int32_t* theirs = a.kv_indices + table_of(a, first).begin;
+    bool other = false;
+    for (int32_t i = tid; i < a.shared_pages; i += 256) other = other || mine[i] != theirs[i];
+    if (other) differ = 1;
+    __syncthreads();
+    shares = !differ;
+  }
+  if (tid == 0) {
+    a.l.requests[b] = {q.begin, q.pages, len, t.begin};
+    a.l.shares[b] = shares;
+  }
+}
+
+struct Counts {
+  int32_t v[4];  // items, slots, entries, shared tokens
+};
+__device__ __forceinline__ int32_t ceil_div(int32_t x, int32_t y) { return (x + y - 1) / y; }
+
+struct Cut {
+  int32_t tiles, chunks, begin;  // row tiles, key ranges of each, first key of its own
+};
+__device__ __forceinline__ Cut cut_of(const PlanArgs& a, const Request& r, bool shares, int32_t chunk) {
+  Cut c;
+  c.begin = shares ? min(a.shared_pages * a.page_size, r.len) : 0;
+  c.tiles = ceil_div(r.n * a.group, kTile);
+  c.chunks = ceil_div(r.len - c.begin, chunk);
+  return c;
+}
+
+// One workgroup: the keys of an item, from all the work there is; how many items, slots and entries come before each
+// request's, by a scan; the lists. A request of few tokens is one tile and takes a few lines of its own, so a wavefront
+// does a request.
+__global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
+  __shared__ int64_t total_work, total_shared;
+  __shared__ int32_t wave_sums[16][4], carry[4], some_request;
+  const int32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) {
+    total_work = total_shared = 0;
+    some_request = INT32_MAX;
+  }
+  __syncthreads();
+  int64_t work = 0, shared = 0;
+  for (int32_t b = tid; b < a.batch_size; b += 1024) {
+    const Request r = a.l.requests[b];
+    const bool sh = a.l.shares[b];
+    const Cut c = cut_of(a, r, sh, 1 << 30);
+    work += (int64_t)c.tiles * (r.len - c.begin);
+    if (sh) {
+      shared += r.n;
+      atomicMin(&some_request, b);
+    }
+  }
+  atomicAdd((unsigned long long*)&total_work, (unsigned long long)work);
+  atomicAdd((unsigned long long*)&total_shared, (unsigned long long)shared);
+  __syncthreads();
+  const int32_t shared_tokens = (int32_t)total_shared;
+  const int32_t shared_len = a.shared_pages * a.page_size;
+  const int32_t shared_tiles = ceil_div(shared_tokens * a.group, kTile);
+  const int64_t all = total_work + (int64_t)shared_tiles * shared_len;
+  int64_t per = (all + a.target - 1) / a.target;
+  per = (per + kBlock - 1) / kBlock * kBlock;
+  const int32_t chunk = (int32_t)(per < a.min_chunk ? a.min_chunk : per < (1 << 30) ? per : 1 << 30);
+  const int32_t shared_chunks = shared_tokens ? ceil_div(shared_len, chunk) : 0;
+  const int32_t shared_items = shared_tiles * shared_chunks;
+  if (tid < 4) carry[tid] = tid < 2 ? shared_items : 0;
+  __syncthreads();
+  for (int32_t b0 = 0; b0 < a.batch_size; b0 += 1024) {
+    const int32_t b = b0 + tid;
+    Counts n = {};
+    if (b < a.batch_size) {
+      const Request r = a.l.requests[b];
+      const bool sh = a.l.shares[b];
+      const Cut c = cut_of(a, r, sh, chunk);
+      n.v[0] = c.tiles * c.chunks;
+      n.v[1] = sh || c.chunks > 1 ? n.v[0] : 0;
+      n.v[2] = sh || c.chunks != 1 ? c.tiles : 0;
+      n.v[3] = sh ? r.n : 0;
+    }
+    Counts before = n;  // inclusive, then exclusive
+    for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int32_t x = __shfl_up(before.v[i], d);
+        if (lane >= d) before.v[i] += x;
+      }
+    if (lane == 63)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wave_sums[wave][i] = before.v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int32_t base = carry[i];
+      for (int w = 0; w < wave; ++w) base += wave_sums[w][i];
+      before.v[i] += base - n.v[i];
+    }
+    if (b < a.batch_size) *reinterpret_cast<int4*>(a.l.offsets + 4 * b) = *reinterpret_cast<const int4*>(before.v);
+    __syncthreads();
+    if (tid == 1023)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) carry[i] = before.v[i] + n.v[i];
+    __syncthreads();
+  }
+  if (tid == 0) *a.l.header = {min(carry[0], a.max_items), min(carry[2], a.max_entries), shared_chunks, shared_tokens};
+
+  for (int32_t b = wave; b < a.batch_size; b += 16) {
+    const Request r = a.l.requests[b];
+    const bool sh = a.l.shares[b];
+    const Cut c = cut_of(a, r, sh, chunk);
+    const int4 first = *reinterpret_cast<const int4*>(a.l.offsets + 4 * b);
+    const int32_t rows = r.n * a.group;
+    const bool partial = sh || c.chunks > 1;
+    for (int32_t i = lane; i < c.tiles * c.chunks; i += 64) {
+      const int32_t tile = i / c.chunks, part = i - tile * c.chunks;
+      const int32_t row0 = tile * kTile, last_row = min(row0 + kTile, rows) - 1;
+      const int32_t end = clamp(r.len - r.n + last_row / a.group + 1, c.begin, r.len);  // keys that the tile's last token sees
+      const int32_t each = (ceil_div(end - c.begin, c.chunks) + kBlock - 1) / kBlock * kBlock;
+      const int32_t from = min(c.begin + part * each, end), to = min(from + each, end);
+      if (first.x + i < a.max_items)
+        a.l.items[first.x + i] = {r.q_begin, row0, last_row + 1 - row0, r.table, from, to, partial ? first.y + i : -1, 0};
+    }
+    if (sh || c.chunks != 1)
+      for (int32_t i = lane; i < c.tiles; i += 64) {
+        const int32_t row0 = i * kTile;
+        if (first.z + i < a.max_entries)
+          a.l.entries[first.z + i] = {r.q_begin, row0, min(kTile, rows - row0), first.y + i * c.chunks, c.chunks,
+                                      sh ? first.w * a.group + row0 : -1, {}};
+      }
+    if (sh)
+      for (int32_t i = lane; i < r.n; i += 64) a.l.shared_tokens[first.w + i] = r.q_begin + i;
+  }
+  if (shared_items) {
+    const int32_t table = a.l.requests[some_request].table;
+    const int32_t each = (ceil_div(shared_len, shared_chunks) + kBlock - 1) / kBlock * kBlock;
+    for (int32_t i = tid; i < shared_items && i < a.max_items; i += 1024) {
+      const int32_t tile = i / shared_chunks, part = i - tile * shared_chunks, row0 = tile * kTile;
+      const int32_t from = min(part * each, shared_len);
+      a.l.items[i] = {-1, row0, min(kTile, shared_tokens * a.group - row0), table, from, min(from + each, shared_len), i, 0};
+    }
+  }
+}
+
+// ---- storage types -------------------------------------------------------------------------------------------------
+struct BF16 {
+  typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2));
+  }
+  static __device__ __forceinline__ float wide(uint32_t half) { return __uint_as_float(half << 16); }
+  static constexpr uint32_t kExponent = 0x7f80u;
+};
+struct F16 {
+  typedef _Float16 V8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 v = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  static __device__ __forceinline__ float wide(uint32_t half) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)half);
+  }
+  static constexpr uint32_t kExponent = 0x7c00u;
+};
+// Two 16-bit values side by side: is one infinite or not a number?
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t two) {
+  return (two & T::kExponent) == T::kExponent || (two >> 16 & T::kExponent) == T::kExponent;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t finite_part(uint32_t two) {
+  return ((two & T::kExponent) == T::kExponent ? 0 : two & 0xffffu) |
+         ((two >> 16 & T::kExponent) == T::kExponent ? 0 : two & 0xffff0000u);
+}
+
+struct AttendArgs {
+  const char* query;
+  const char* cache;
+  const int32_t* kv_indices;
+  char* out;
+  float* lse;              // may be null
+  float* partial;          // [slots][kv heads][kTile][head_dim]
+  float* partial_lse;      // [slots][kv heads][kTile], to base 2
+  int64_t q_stride;        // bytes
+  uint32_t page_stride, row_stride, plane;  // bytes: page to page, key to key in a page, K to V
+  int32_t num_pages, page_size, page_shift;
+  int32_t kv_heads, group, head_dim;
+  float scale;             // times log2(e)
+  Layout l;
+};
+
+// Byte offset of a key's row, or -1 where there is none to read: beyond `end`, or on a page that the cache does not have
+__device__ __forceinline__ int64_t key_offset(const AttendArgs& a, int32_t table, int32_t key, int32_t end) {
+  if (key >= end) return -1;
+  const int32_t p = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+  const int32_t page = a.kv_indices[table + p];
+  if (page < 0 || page >= a.num_pages) return -1;
+  return (int64_t)page * a.page_stride + (int64_t)(key - p * a.page_size) * a.row_stride;
+}
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A workgroup per (item, key head); its wavefronts take blocks of 32 keys in turn, each with a maximum and a sum of its
+// own, joined at the end through LDS.
+//   S^T = K Q^T: the keys' rows are the matrix instruction's A operand as they lie in memory, 16 bytes a lane.
+//   O^T = V^T P^T: a lane's 8 probabilities, of keys 4q..4q+3 and 16+4q..16+4q+3 (q = lane / 16), are the B operand as S^T
+//   left them; the A operand wants the same keys of one column of V, which the transposing LDS read gives.
+// P is rounded to the storage type for the matrix instruction, each weight by at most half a step of itself, as the inputs
+// were; the sum l is of the weights before that, since lse is an output in 32 bits.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void attend_rows_kernel(AttendArgs a) {
+  constexpr int KSTEPS = DP / 32, DTILES = DP / 16;
+  constexpr int LPR = DP <= 32 ? 4 : DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // lanes to a row of V
+  constexpr int RPI = 64 / LPR, VLOADS = kBlock / RPI;
+  constexpr int VSTRIDE = DP * 2 + 32;           // rows 32 bytes apart in the banks: a transposing read takes 4 of them
+  constexpr int OSTRIDE = DP + 4;
+  static_assert(kTile * OSTRIDE * 4 <= kBlock * VSTRIDE, "a wavefront's O takes the place of its V");
+  __shared__ __attribute__((aligned(16))) char v_lds[kWaves][kBlock * VSTRIDE];
+  __shared__ float stats[kWaves][2][kTile];
+  const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t n = lane & 15, quad = lane >> 4;
+  const int32_t num_items = a.l.header->items;
+  for (int32_t at = blockIdx.x; at < num_items * a.kv_heads; at += gridDim.x) {
+    const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
+    const Item item = a.l.items[it];
+    const int32_t D = a.head_dim;
+
+    u32x4 q[KSTEPS] = {};
+    int32_t limit = 0;
+    if (n < item.rows) {
+      const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
+      const int32_t token = item.q_begin >= 0 ? item.q_begin + i : a.l.shared_tokens[i];
+      limit = a.l.limits[token];
+      const char* p = a.query + (int64_t)token * a.q_stride + ((int64_t)(h * a.group + g) * D + quad * 8) * 2;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k)
+        if (k * 32 + quad * 8 < D) q[k] = *reinterpret_cast<const u32x4*>(p + k * 64);
+    }
+    limit = min(limit, item.key_end);
+    float m = -INFINITY, l = 0;
+    f32x4 o[DTILES] = {};
+    const char* k_base = a.cache + (int64_t)h * D * 2;
+    char* my_v = v_lds[wave];
+    for (int32_t k0 = item.key_begin + wave * kBlock; k0 < item.key_end; k0 += kWaves * kBlock) {
+      u32x4 kr[2][KSTEPS] = {}, vr[VLOADS] = {};
+      bool have[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t off = key_offset(a, item.table, k0 + i * 16 + n, item.key_end);
+        have[i] = off >= 0;
+        if (have[i])
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k)
+            if (k * 32 + quad * 8 < D) kr[i][k] = *reinterpret_cast<const u32x4*>(k_base + off + k * 64 + quad * 16);
+      }
+      const int32_t vrow = lane / LPR, vcol = lane % LPR;
+#pragma unroll
+      for (int i = 0; i < VLOADS; ++i) {
+        const int64_t off = key_offset(a, item.table, k0 + i * RPI + vrow, item.key_end);
+        if (off >= 0 && vcol * 8 < D) vr[i] = *reinterpret_cast<const u32x4*>(k_base + a.plane + off + vcol * 16);
+      }
+      // which of the block's keys are there: bit n of half i
+      const uint32_t present = ((uint32_t)__ballot(have[0]) & 0xffffu) | (uint32_t)__ballot(have[1]) << 16;
+
+      f32x4 s[2] = {};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k) s[i] = T::mfma(kr[i][k], q[k], s[i]);
+      // does a row stop inside the block, and is there a value in it that 0 does not cancel?
+      bool odd_v = false;
+#pragma unroll
+      for (int i = 0; i < VLOADS; ++i) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) odd_v = odd_v || not_finite<T>(vr[i][w]);
+        if (vcol * 8 < DP) *reinterpret_cast<u32x4*>(my_v + (i * RPI + vrow) * VSTRIDE + vcol * 16) = vr[i];
+      }
+      const bool ragged = __ballot(n < item.rows && limit < min(k0 + kBlock, item.key_end)) != 0;
+      const bool mend = ragged && __ballot(odd_v) != 0;
+
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int32_t at_key = i * 16 + quad * 4 + r;
+          if (k0 + at_key >= limit || !(present >> at_key & 1)) s[i][r] = -INFINITY;
+          top = fmaxf(top, s[i][r]);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float base = top == -INFINITY ? 0.f : top * a.scale;
+      const float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
+      u32x4 p;
+      float sum = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          const float x = exp2_of(__builtin_fmaf(s[i][r], a.scale, -base));
+          const float y = exp2_of(__builtin_fmaf(s[i][r + 1], a.scale, -base));
+          p[i * 2 + r / 2] = T::pack(x, y);
+          sum += x + y;
+        }
+      l = l * shrink + sum;
+      m = top;
+#pragma unroll
+      for (int d = 0; d < DTILES; ++d) {
+        const char* from = my_v + (quad * 4 + n / 4) * VSTRIDE + (d * 16 + n % 4 * 4) * 2;
+        typedef __attribute__((address_space(3))) s16x4* Lds;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 16 * VSTRIDE));
+        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+        u32x4 v = {x[0], x[1], y[0], y[1]};
+        if (mend)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v[w] = finite_part<T>(v[w]);
+        o[d] = T::mfma(v, p, o[d] * shrink);
+      }
+      if (mend) {
+        // infinities and NaN of V, left out above, go to the rows that see their keys
+        for (int32_t key = 0; key < kBlock; ++key) {
+          const int r = key & 3;
+          const uint32_t word = key < 16 ? (r < 2 ? p[0] : p[1]) : (r < 2 ? p[2] : p[3]);
+          const uint32_t got = __shfl(word, (key >> 2 & 3) * 16 + n);
+          const float weight = T::wide(r & 1 ? got >> 16 : got & 0xffffu);
+          if (k0 + key < limit && (present >> key & 1))
+#pragma unroll
+            for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t x = *reinterpret_cast<const uint16_t*>(my_v + key * VSTRIDE + (d * 16 + quad * 4 + e) * 2);
+                if ((x & T::kExponent) == T::kExponent) o[d][e] += weight * T::wide(x);
+              }
+        }
+      }
+    }
+    // the sum over the four quads' keys, then over the wavefronts
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (quad == 0) {
+      stats[wave][0][n] = m;
+      stats[wave][1][n] = l;
+    }
+    __syncthreads();
+    float all_m = -INFINITY, all_l = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all_m = fmaxf(all_m, stats[w][0][n]);
+    const float base = all_m == -INFINITY ? 0.f : all_m * a.scale;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all_l += stats[w][1][n] * exp2_of(stats[w][0][n] * a.scale - base);
+    const float part = exp2_of(m * a.scale - base) * (all_l == 0 ? 0.f : 1.f / all_l);
+    float* my_o = reinterpret_cast<float*>(my_v);
+#pragma unroll
+    for (int d = 0; d < DTILES; ++d)
+      *reinterpret_cast<f32x4*>(my_o + n * OSTRIDE + d * 16 + quad * 4) = o[d] * part;
+    if (wave == 0 && quad == 0 && n < item.rows) {
+      const float lse2 = all_l == 0 ? -INFINITY : base + __log2f(all_l);
+      if (item.slot >= 0) {
+        a.partial_lse[((int64_t)item.slot * a.kv_heads + h) * kTile + n] = lse2;
+      } else if (a.lse) {
+        const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
+        a.lse[(int64_t)(item.q_begin + i) * a.kv_heads * a.group + h * a.group + g] = lse2 * kLn2;
+      }
+    }
+    __syncthreads();
+    for (int32_t e = tid; e < kTile * (DP / 4); e += kThreads) {
+      const int32_t r = e / (DP / 4), d = e % (DP / 4) * 4;
+      if (r >= item.rows || d >= D) continue;
+      f32x4 x = {};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(v_lds[w]) + r * OSTRIDE + d);
+      if (item.slot >= 0) {
+        *reinterpret_cast<f32x4*>(a.partial + (((int64_t)item.slot * a.kv_heads + h) * kTile + r) * D + d) = x;
+      } else {
+        const int32_t row = item.row0 + r, i = row / a.group, g = row - i * a.group;
+        const u32x2 two = {T::pack(x[0], x[1]), T::pack(x[2], x[3])};
+        *reinterpret_cast<u32x2*>(a.out + (((int64_t)(item.q_begin + i) * a.kv_heads + h) * a.group + g) * D * 2 + d * 2) = two;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins a row's partials: weights exp2(lse_c - lse). A row without any is zero, its lse -inf. A wavefront per row, its
+// lanes over the columns.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
+  const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int32_t num_entries = a.l.header->entries, shared_chunks = a.l.header->shared_chunks;
+  const int32_t D = a.head_dim;
+  for (int32_t at = blockIdx.x; at < num_entries * a.kv_heads; at += gridDim.x) {
+    const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
+    const Entry e = a.l.entries[it];
+    const int32_t parts = e.chunks + (e.shared_row0 >= 0 ? shared_chunks : 0);
+    for (int32_t r = wave; r < e.rows; r += kWaves) {
+      const int32_t shared_row = e.shared_row0 + r;
+      const auto row_of = [&](int32_t c) {  // of part c
+        const bool own = c < e.chunks;
+        const int32_t slot = own ? e.slot + c : shared_row / kTile * shared_chunks + c - e.chunks;
+        return ((int64_t)slot * a.kv_heads + h) * kTile + (own ? r : shared_row % kTile);
+      };
+      float top = -INFINITY;
+      for (int32_t c = lane; c < parts; c += 64) top = fmaxf(top, a.partial_lse[row_of(c)]);
+      for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+      const float base = top == -INFINITY ? 0.f : top;
+      float total = 0;
+      for (int32_t c = lane; c < parts; c += 64) total += exp2_of(a.partial_lse[row_of(c)] - base);
+      for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+      const float inv = total == 0 ? 0.f : 1.f / total;
+      const int32_t row = e.row0 + r, i = row / a.group, g = row - i * a.group;
+      const int64_t out_row = ((int64_t)(e.q_begin + i) * a.kv_heads + h) * a.group + g;
+      if (a.lse && lane == 0) a.lse[out_row] = (total == 0 ? -INFINITY : base + __log2f(total)) * kLn2;
+      for (int32_t d = lane * 4; d < D; d += 256) {
+        f32x4 x = {};
+        for (int32_t c = 0; c < parts; ++c) {
+          const int64_t from = row_of(c);
+          const float weight = exp2_of(a.partial_lse[from] - base);
+          x += *reinterpret_cast<const f32x4*>(a.partial + from * D + d) * weight;
+        }
+        x *= inv;
+        const u32x2 two = {T::pack(x[0], x[1]), T::pack(x[2], x[3])};
+        *reinterpret_cast<u32x2*>(a.out + (out_row * D + d) * 2) = two;
+      }
+    }
+  }
+}
+
+int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+// The sizes that follow from the capacities
+struct Sizes {
+  int64_t target, max_items, max_entries, max_slots;
+};
+
+}  // namespace
+
+extern "C" {
+
+struct kvc_attention_plan {
+  const int32_t *qo_indptr, *kv_indices, *kv_indptr, *kv_last_page_len;
+  int64_t batch_size, num_tokens, num_kv_indices, num_heads, num_kv_heads, head_dim, page_size, shared_pages;
+  int dtype;
+  float scale;
+  Sizes n;
+  int64_t plan_bytes, workspace_bytes;
+  char* buffer;  // of kvc_attention_plan_build
+};
+
+}  // extern "C"
+
+namespace {
+
+// Items of a step: workgroups that fill the card four times, so that the last of them to end is a small part of it
+constexpr int64_t kWorkgroups = 1024;
+constexpr int32_t kMinChunk = 256;
+
+Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
+  Layout l;
+  int64_t at = 0;
+  const auto take = [&](int64_t n) {
+    char* q = buffer ? buffer + at : nullptr;
+    at += round_up(n, 256);
+    return q;
+  };
+  l.header = (Header*)take(sizeof(Header));
+  l.requests = (Request*)take(p.batch_size * sizeof(Request));
+  l.shares = (int32_t*)take(p.batch_size * 4);
+  l.offsets = (int32_t*)take(p.batch_size * 16);
+  l.limits = (int32_t*)take(p.num_tokens * 4);
+  l.shared_tokens = (int32_t*)take(p.num_tokens * 4);
+  l.items = (Item*)take(p.n.max_items * sizeof(Item));
+  l.entries = (Entry*)take(p.n.max_entries * sizeof(Entry));
+  if (bytes) *bytes = at;
+  return l;
+}
+
+// Row tiles are at most rows / 16 and one more for every request that has tokens; cut into items of a target-th of all
+// keys each, there are at most the target and one more for every tile. Without a shared prefix only tiles of more than one
+// item need a slot, which are at most twice the target.
+Sizes sizes_of(const kvc_attention_plan& p) {
+  Sizes n;
+  const int64_t group = p.num_kv_heads ? p.num_heads / p.num_kv_heads : 1;
+  const int64_t tiles = p.num_tokens * group / kTile + std::min(p.batch_size, p.num_tokens);
+  n.target = std::max<int64_t>(1, kWorkgroups / std::max<int64_t>(1, p.num_kv_heads));
+  const int64_t shared_tiles = p.shared_pages > 0 ? round_up(p.num_tokens * group, kTile) / kTile : 0;
+  n.max_items = n.target + tiles + (p.shared_pages > 0 ? n.target + shared_tiles : 0);
+  n.max_entries = tiles;
+  n.max_slots = p.shared_pages > 0 ? n.max_items : 2 * n.target;
+  return n;
+}
+
+template <typename T, int DP>
+void launch_rows(const AttendArgs& a, unsigned grid, hipStream_t s) {
+  kvc::launch((attend_rows_kernel<T, DP>), dim3(grid), dim3(kThreads), 0, s, a);
+}
+template <typename T>
+void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
+  const unsigned grid = (unsigned)std::min<int64_t>(p.n.max_items * p.num_kv_heads, 1 << 14);
+  if (p.head_dim <= 64) launch_rows<T, 64>(a, grid, s);
+  else if (p.head_dim <= 96) launch_rows<T, 96>(a, grid, s);
+  else if (p.head_dim <= 128) launch_rows<T, 128>(a, grid, s);
+  else launch_rows<T, 256>(a, grid, s);
+  const unsigned joins = (unsigned)std::min<int64_t>(p.n.max_entries * p.num_kv_heads, 2048);
+  kvc::launch((attend_join_kernel<T>), dim3(joins), dim3(kThreads), 0, s, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* kv_indptr,
+                              const int32_t* kv_last_page_len, int64_t batch_size, int64_t num_tokens,
+                              int64_t num_kv_indices, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                              int64_t page_size, int64_t shared_pages, float sm_scale, int dtype,
+                              kvc_attention_plan** out) {
+  constexpr const char* fn = "kvc_attention_plan_create";
+  if (!out) return fail(KVC_ERR_INVALID_ARG, "%s: null out", fn);
+  *out = nullptr;
+  if (dtype != KVC_DTYPE_BF16 && dtype != KVC_DTYPE_F16)
+    return fail(KVC_ERR_UNSUPPORTED, "%s: dtype %d (need bf16 or f16)", fn, dtype);
+  if (batch_size < 0 || num_tokens < 0 || num_kv_indices < 0 || shared_pages < 0)
+    return fail(KVC_ERR_INVALID_ARG, "%s: negative size", fn);
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
+    return fail(KVC_ERR_INVALID_ARG, "%s: %lld query heads are no multiple of %lld key heads", fn, (long long)num_heads,
+                (long long)num_kv_heads);
+  if (head_dim <= 0 || head_dim % 8 || head_dim > 256)
+    return fail(KVC_ERR_UNSUPPORTED, "%s: head_dim %lld (need a multiple of 8 up to 256)", fn, (long long)head_dim);
+  if (page_size <= 0 || page_size > (1 << 20))
+    return fail(KVC_ERR_INVALID_ARG, "%s: page_size %lld", fn, (long long)page_size);
+  if (!(sm_scale > 0) || !std::isfinite(sm_scale))
+    return fail(KVC_ERR_INVALID_ARG, "%s: the scale must be positive and finite", fn);
+  if (batch_size >= (1 << 24) || num_kv_indices >= (int64_t(1) << 31) || num_heads > 0xffff ||
+      num_tokens * num_heads >= (int64_t(1) << 30))
+    return fail(KVC_ERR_UNSUPPORTED, "%s: too many requests, pages, tokens or heads", fn);
+  if (batch_size > 0 && (!qo_indptr || !kv_indptr || !kv_last_page_len || (num_kv_indices > 0 && !kv_indices)))
+    return fail(KVC_ERR_INVALID_ARG, "%s: null pointer", fn);
+  // more pages than the tables hold are shared by no one
+  if (shared_pages > num_kv_indices || shared_pages * page_size > (1 << 30)) shared_pages = 0;
+  kvc_attention_plan* p = new (std::nothrow) kvc_attention_plan{
+      qo_indptr, kv_indices, kv_indptr, kv_last_page_len, batch_size, num_tokens, num_kv_indices, num_heads, num_kv_heads,
+      head_dim, page_size, shared_pages, dtype, sm_scale, {}, 0, 0, nullptr};
+  if (!p) return fail(KVC_ERR_HIP, "%s: out of host memory", fn);
+  p->n = sizes_of(*p);
+  layout_of(*p, nullptr, &p->plan_bytes);
+  p->workspace_bytes = round_up(p->n.max_slots * num_kv_heads * kTile * (head_dim + 1) * 4, 256);
+  *out = p;
+  return KVC_OK;
+}
+
+int64_t kvc_attention_plan_bytes(const kvc_attention_plan* plan) {
+  return plan ? plan->plan_bytes : (int64_t)fail(KVC_ERR_INVALID_ARG, "kvc_attention_plan_bytes: null plan");
+}
+int64_t kvc_attention_workspace_bytes(const kvc_attention_plan* plan) {
+  return plan ? plan->workspace_bytes : (int64_t)fail(KVC_ERR_INVALID_ARG, "kvc_attention_workspace_bytes: null plan");
+}
+
+int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buffer_bytes, void* stream) {
+  constexpr const char* fn = "kvc_attention_plan_build";
+  if (!plan) return fail(KVC_ERR_INVALID_ARG, "%s: null plan", fn);
+  if (!buffer || (uintptr_t)buffer % 256 || buffer_bytes < plan->plan_bytes)
+    return fail(KVC_ERR_STAGING, "%s: the plan needs %lld bytes, aligned to 256", fn, (long long)plan->plan_bytes);
+  plan->buffer = (char*)buffer;
+  if (plan->batch_size == 0 || plan->num_tokens == 0) return KVC_OK;
+  PlanArgs a{plan->qo_indptr, plan->kv_indices, plan->kv_indptr, plan->kv_last_page_len, (int32_t)plan->batch_size,
+             (int32_t)plan->num_tokens, (int32_t)plan->num_kv_indices, (int32_t)plan->page_size,
+             (int32_t)plan->shared_pages, (int32_t)(plan->num_heads / plan->num_kv_heads), (int32_t)plan->n.target,
+             kMinChunk, (int32_t)plan->n.max_items, (int32_t)plan->n.max_entries,
+             layout_of(*plan, plan->buffer, nullptr)};
+  hipStream_t s = (hipStream_t)stream;
+  kvc::launch(attend_requests_kernel, dim3((unsigned)plan->batch_size), dim3(256), 0, s, a);
+  kvc::launch(attend_schedule_kernel, dim3(1), dim3(1024), 0, s, a);
+  KVC_HIP(hipGetLastError());
+  return KVC_OK;
+}
+
+int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query, int64_t q_token_stride,
+                           const void* paged_kv_cache, int64_t page_stride, int64_t num_pages, void* out, float* lse,
+                           void* workspace, int64_t workspace_bytes, void* stream) {
+  constexpr const char* fn = "kvc_attention_plan_run";
+  if (!plan) return fail(KVC_ERR_INVALID_ARG, "%s: null plan", fn);
+  if (!plan->buffer) return fail(KVC_ERR_INVALID_ARG, "%s: the plan is not built", fn);
+  if (plan->batch_size == 0 || plan->num_tokens == 0) return KVC_OK;
+  const int64_t row = plan->num_kv_heads * plan->head_dim, page = 2 * plan->page_size * row;
+  if (!query || !out || !workspace || (num_pages > 0 && !paged_kv_cache))
+    return fail(KVC_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (num_pages < 0 || num_pages >= (int64_t(1) << 31) || page_stride < page || page_stride * 2 >= (int64_t(1) << 32))
+    return fail(KVC_ERR_INVALID_ARG, "%s: bad cache geometry", fn);
+  if (q_token_stride < plan->num_heads * plan->head_dim)
+    return fail(KVC_ERR_INVALID_ARG, "%s: token stride smaller than a row", fn);
+  if (((uintptr_t)query | (uintptr_t)paged_kv_cache | (uint64_t)q_token_stride * 2 | (uint64_t)page_stride * 2) % 16 ||
+      (uintptr_t)out % 8 || (uintptr_t)lse % 4 || (uintptr_t)workspace % 256)
+    return fail(KVC_ERR_INVALID_ARG, "%s: rows must be aligned to 16 bytes, the output to 8", fn);
+  if (workspace_bytes < plan->workspace_bytes)
+    return fail(KVC_ERR_STAGING, "%s: the workspace needs %lld bytes", fn, (long long)plan->workspace_bytes);
+  AttendArgs a{};
+  a.query = (const char*)query;
+  a.cache = (const char*)paged_kv_cache;
+  a.kv_indices = plan->kv_indices;
+  a.out = (char*)out;
+  a.lse = lse;
+  a.partial = (float*)workspace;
+  a.partial_lse = a.partial + plan->n.max_slots * plan->num_kv_heads * kTile * plan->head_dim;
+  a.q_stride = q_token_stride * 2;
+  a.page_stride = (uint32_t)(page_stride * 2);
+  a.row_stride = (uint32_t)(row * 2);
+  a.plane = (uint32_t)(plan->page_size * row * 2);
+  a.num_pages = (int32_t)num_pages;
+  a.page_size = (int32_t)plan->page_size;
+  a.page_shift = log2_exact(plan->page_size);
+  a.kv_heads = (int32_t)plan->num_kv_heads;
+  a.group = (int32_t)(plan->num_heads / plan->num_kv_heads);
+  a.head_dim = (int32_t)plan->head_dim;
+  a.scale = plan->scale * kLog2e;
+  a.l = layout_of(*plan, plan->buffer, nullptr);
+  if (plan->dtype == KVC_DTYPE_BF16) launch_attend<BF16>(a, *plan, (hipStream_t)stream);
+  else launch_attend<F16>(a, *plan, (hipStream_t)stream);
+  KVC_HIP(hipGetLastError());
+  return KVC_OK;
+}
+
+int kvc_attention_plan_destroy(kvc_attention_plan* plan) {
+  delete plan;
+  return KVC_OK;
+}
+
+}  // extern "C"
