@@ -517,6 +517,61 @@ int kvc_rotary_plan_resolve_slots(kvc_rotary_plan* plan, int64_t* slots, void* s
 int kvc_rotary_plan_set_slots(kvc_rotary_plan* plan, const int64_t* slots);
 
 /* ---------------------------------------------------------------------------
+ * The rotation with a norm of every query and key head in front, alone or with
+ * the K/V write: kvc_rotary_pos_emb and its forms, of
+ *   y = x * weight / sqrt(mean(x^2) + eps)      (over the head's head_dim lanes)
+ * in place of x for the Q heads (query_weight) and the K heads (key_weight); V is
+ * copied as it is. fp32 throughout, one rounding. Weights [head_dim] in the
+ * tensors' dtype, eps positive. All else as there: positions outside the table
+ * leave the token untouched, lanes beyond rotary_dim are normed and not rotated.
+ * query_out may be query's own rows and key_out key's; every other overlap of an
+ * output with an input or an output is refused (KVC_ERR_INVALID_ARG).
+ * kvc_rotary_plan_run_norm is kvc_rotary_plan_run with the layer's weights.
+ * No counterpart in the reference, whose models do not norm their heads; it runs
+ * where the rotation does (runtime/worker/llm_worker/models/llama.py:156-167). */
+int kvc_qk_norm_rotary_pos_emb(const void* query, const void* key, const void* query_weight,
+                               const void* key_weight, float eps, const void* positions,
+                               int pos_bytes, const void* cos_sin_cache, int64_t max_position,
+                               int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads,
+                               int64_t head_dim, int64_t rotary_dim, int64_t q_token_stride,
+                               int64_t k_token_stride, void* query_out, void* key_out,
+                               int64_t qo_token_stride, int64_t ko_token_stride, int dtype,
+                               void* stream);
+
+int kvc_qk_norm_rotary_pos_emb_and_cache(const void* query, const void* key, const void* value,
+                                         const void* query_weight, const void* key_weight, float eps,
+                                         const void* positions, int pos_bytes,
+                                         const void* cos_sin_cache, int64_t max_position,
+                                         int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads,
+                                         int64_t head_dim, int64_t rotary_dim,
+                                         int64_t q_token_stride, int64_t k_token_stride,
+                                         int64_t v_token_stride, void* query_out, void* key_out,
+                                         int64_t qo_token_stride, int64_t ko_token_stride,
+                                         void* key_cache, void* value_cache,
+                                         const void* slot_mapping, int slot_bytes,
+                                         int64_t block_size, int64_t cache_block_stride,
+                                         int64_t cache_slot_stride, int64_t num_cache_blocks,
+                                         int dtype, void* stream);
+
+int kvc_qk_norm_rotary_pos_emb_and_append_paged(
+    const void* query, const void* key, const void* value, const void* query_weight,
+    const void* key_weight, float eps, const int32_t* batch_indices, const int32_t* positions,
+    const void* cos_sin_cache, int64_t max_position, int64_t nnz, int64_t num_heads,
+    int64_t num_kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t q_token_stride,
+    int64_t k_token_stride, int64_t v_token_stride, void* query_out, void* key_out,
+    int64_t qo_token_stride, int64_t ko_token_stride, void* paged_kv_cache,
+    const int32_t* kv_indices, const int32_t* kv_indptr, int64_t batch_size,
+    int64_t num_kv_indices, int64_t page_size, int64_t page_stride, int64_t num_pages, int dtype,
+    void* stream);
+
+int kvc_rotary_plan_run_norm(const kvc_rotary_plan* plan, const void* query, const void* key,
+                             const void* value, const void* query_weight, const void* key_weight,
+                             float eps, int64_t q_token_stride, int64_t k_token_stride,
+                             int64_t v_token_stride, void* query_out, void* key_out,
+                             void* paged_kv_cache, int64_t page_stride, int64_t num_pages,
+                             void* stream);
+
+/* ---------------------------------------------------------------------------
  * Causal attention over the paged cache, for the queries of a step.
  * Stands where the reference calls BatchPrefillWithPagedKVCacheWrapper.run /
  * BatchDecodeWithPagedKVCacheWrapper.run behind the write

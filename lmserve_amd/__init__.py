@@ -6,7 +6,7 @@
     kv_worker   KVWorker (GPU <-> pinned host swap), Device, BlockMapping
     index_prep  host-side block-table / slot-mapping construction
     attention   causal attention over the paged cache, a shared prefix read once for the batch
-    rotary      rotary position embedding, alone or fused with the K/V write
+    rotary      rotary position embedding, alone or fused with the K/V write, with or without norms of the heads
     disk_tier   DiskTier (host <-> block file, native positional I/O)
     kv_pool     pool sizing, layer-sync handle and model-side hooks, hand-over to a second process
     kv_service  the KV worker as a process of its own (pool mapped from an IPC handle)
@@ -31,7 +31,8 @@ from .kv_pool import (CachePlan, KVWorkerHandle, KVWorkerParams, LayerSyncHooks,
 from .kv_service import serve_kv_worker
 from .kv_worker import (BlockMapping, BlockMappingEntry, Device, KVWorker, PinnedHostPool,
                         flatten_block_mappings)
-from .rotary import (PagedRotaryWritePlan, RotaryEmbedding, make_cos_sin_cache, rotary_pos_emb,
+from .rotary import (PagedRotaryWritePlan, RotaryEmbedding, make_cos_sin_cache, qk_norm_rotary_pos_emb,
+                     qk_norm_rotary_pos_emb_and_append_paged, qk_norm_rotary_pos_emb_and_cache, rotary_pos_emb,
                      rotary_pos_emb_and_append_paged, rotary_pos_emb_and_cache)
 from .paged import (BlockRuns, PagedKVWritePlan, append_paged_kv_cache, append_paged_kv_cache_layers,
                     build_write_index, get_batch_indices_positions, get_seq_lens, max_block_runs,
@@ -55,4 +56,5 @@ __all__ = [
     "build_write_index", "BlockRuns", "max_block_runs", "slot_block_runs", "write_block_runs_layers",
     "KVWriteStep",
     "PagedAttentionPlan", "paged_attention",
+    "qk_norm_rotary_pos_emb", "qk_norm_rotary_pos_emb_and_cache", "qk_norm_rotary_pos_emb_and_append_paged",
 ]

@@ -136,6 +136,17 @@ SIGNATURES = {
                                                     _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64,
                                                     _P, _P, _P, _I64, _I64, _I64, _I64, _I64, c_int,
                                                     _P]),
+    "kvc_qk_norm_rotary_pos_emb": (c_int, [_P, _P, _P, _P, c_float, _P, c_int, _P, _I64, _I64, _I64, _I64, _I64,
+                                           _I64, _I64, _I64, _P, _P, _I64, _I64, c_int, _P]),
+    "kvc_qk_norm_rotary_pos_emb_and_cache": (c_int, [_P, _P, _P, _P, _P, c_float, _P, c_int, _P, _I64, _I64, _I64,
+                                                     _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P,
+                                                     _P, c_int, _I64, _I64, _I64, _I64, c_int, _P]),
+    "kvc_qk_norm_rotary_pos_emb_and_append_paged": (c_int, [_P, _P, _P, _P, _P, c_float, _P, _P, _P, _I64, _I64,
+                                                            _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64,
+                                                            _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, c_int,
+                                                            _P]),
+    "kvc_rotary_plan_run_norm": (c_int, [_P, _P, _P, _P, _P, _P, c_float, _I64, _I64, _I64, _P, _P, _P, _I64, _I64,
+                                         _P]),
     "kvc_attention_plan_create": (c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, c_float,
                                           c_int, ctypes.POINTER(_P)]),
     "kvc_attention_plan_bytes": (_I64, [_P]),

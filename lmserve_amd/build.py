@@ -14,6 +14,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_ROOT = os.path.dirname(PKG_DIR)
 SOURCES = [os.path.join(PKG_DIR, "csrc", "kvcache.hip"),
            os.path.join(PKG_DIR, "csrc", "rope_cache.hip"),
+           os.path.join(PKG_DIR, "csrc", "qk_norm.hip"),
            os.path.join(PKG_DIR, "csrc", "attention.hip"),
            os.path.join(PKG_DIR, "csrc", "disk_tier.cpp"),
            os.path.join(PKG_DIR, "csrc", "host_rows.cpp")]

@@ -1287,6 +1287,29 @@ int kvc_rotary_plan_run(const kvc_rotary_plan* plan, const void* query, const vo
       plan->num_kv_indices, plan->page_size, page_stride, num_pages, plan->dtype, stream);
 }
 
+int kvc_rotary_plan_run_norm(const kvc_rotary_plan* plan, const void* query, const void* key, const void* value,
+                             const void* query_weight, const void* key_weight, float eps, int64_t q_token_stride,
+                             int64_t k_token_stride, int64_t v_token_stride, void* query_out, void* key_out,
+                             void* paged_kv_cache, int64_t page_stride, int64_t num_pages, void* stream) {
+  if (!plan) return fail(KVC_ERR_INVALID_ARG, "kvc_rotary_plan_run_norm: null plan");
+  const int64_t q_row = plan->num_heads * plan->head_dim, k_row = plan->num_kv_heads * plan->head_dim;
+  if (!plan->slots)
+    return kvc_qk_norm_rotary_pos_emb_and_append_paged(
+        query, key, value, query_weight, key_weight, eps, plan->batch_indices, plan->positions, plan->cos_sin_cache,
+        plan->max_position, plan->nnz, plan->num_heads, plan->num_kv_heads, plan->head_dim, plan->rotary_dim, q_token_stride,
+        k_token_stride, v_token_stride, query_out, key_out, q_row, k_row, paged_kv_cache, plan->kv_indices, plan->kv_indptr,
+        plan->batch_size, plan->num_kv_indices, plan->page_size, page_stride, num_pages, plan->dtype, stream);
+  if (page_stride < 2 * plan->page_size * k_row)
+    return fail(KVC_ERR_INVALID_ARG, "kvc_rotary_plan_run_norm: page_stride %lld < 2*page_size*H*D", (long long)page_stride);
+  const int E = plan->dtype == KVC_DTYPE_F32 ? 4 : 2;
+  char* vc = paged_kv_cache ? (char*)paged_kv_cache + plan->page_size * k_row * E : nullptr;
+  return kvc_qk_norm_rotary_pos_emb_and_cache(
+      query, key, value, query_weight, key_weight, eps, plan->positions, 4, plan->cos_sin_cache, plan->max_position, plan->nnz,
+      plan->num_heads, plan->num_kv_heads, plan->head_dim, plan->rotary_dim, q_token_stride, k_token_stride, v_token_stride,
+      query_out, key_out, q_row, k_row, paged_kv_cache, vc, plan->slots, 8, plan->page_size, page_stride, k_row, num_pages,
+      plan->dtype, stream);
+}
+
 int kvc_rotary_plan_run_layers(const kvc_rotary_plan* plan, int64_t num_layers, const kvc_rotary_layer* layers,
                                int64_t q_token_stride, int64_t k_token_stride, int64_t v_token_stride,
                                int64_t page_stride, int64_t num_pages, int* one_launch, void* stream) {

@@ -9,6 +9,9 @@ cache write that follows the rotation in the reference's attention layer
  runtime/worker/llm_worker/models/layers/attention.py:76-85), so K is read
 once and the write costs no launch of its own.
 
+The `qk_norm_` forms norm every query and key head first (root mean square, a weight
+per lane), in the same pass.
+
 Arithmetic: fp32 with one rounding to the tensors' dtype.
 """
 from __future__ import annotations
@@ -68,8 +71,8 @@ def _prep(query, key, positions, cos_sin_cache, head_dim):
     if key.dtype != query.dtype or cos_sin_cache.dtype != query.dtype:
         raise TypeError("query, key and cos_sin_cache must share one dtype")
     num_tokens = positions.shape[0]
-    q2 = query.reshape(num_tokens, -1)
-    k2 = key.reshape(num_tokens, -1)
+    q2 = query.reshape(num_tokens, -1) if num_tokens else query.flatten(1)
+    k2 = key.reshape(num_tokens, -1) if num_tokens else key.flatten(1)
     if q2.stride(-1) != 1:
         q2 = q2.contiguous()
     if k2.stride(-1) != 1:
@@ -223,6 +226,125 @@ def rotary_pos_emb_and_append_paged(query: torch.Tensor, key: torch.Tensor, valu
     return q_out.view(query.shape), (k_out.view(key.shape) if return_key else None)
 
 
+def _norm_weights(query_weight, key_weight, query, head_dim):
+    for t, n in ((query_weight, "query_weight"), (key_weight, "key_weight")):
+        _require_gpu(t, n)
+        if t.dtype != query.dtype or t.device != query.device:
+            raise TypeError(f"{n} must have the query's dtype and device")
+        if t.dim() != 1 or t.shape[0] != head_dim:
+            raise ValueError(f"{n} must be [head_dim]")
+    return query_weight.contiguous(), key_weight.contiguous()
+
+
+def _value_rows(value, cache, num_tokens, key, query, head_dim, name):
+    """The value's rows and the geometry of one layer of the pool."""
+    _require_gpu(value, "value")
+    _require_gpu(cache, name)
+    if value.dtype != query.dtype or cache.dtype != query.dtype:
+        raise TypeError(f"value and {name} must have the query's dtype")
+    if cache.dim() != 5 or cache.shape[1] != 2 or not _inner_contiguous(cache):
+        raise ValueError(f"{name} must be [num_blocks, 2, block_size, H, D] with contiguous blocks")
+    blocks, _, size, H, D = cache.shape
+    v2 = value.reshape(num_tokens, -1) if num_tokens else value.flatten(1)
+    if v2.stride(-1) != 1:
+        v2 = v2.contiguous()
+    if D != head_dim or key.shape[1] != H * D or v2.shape[1] != H * D:
+        raise ValueError("key/value rows do not match the cache's H*D")
+    return v2, blocks, size, H, cache.stride(0) if blocks > 1 else 2 * size * H * D
+
+
+def qk_norm_rotary_pos_emb(query: torch.Tensor, key: torch.Tensor, query_weight: torch.Tensor,
+                           key_weight: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor,
+                           head_dim: int, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`rotary_pos_emb` of heads that are normed first, in the same pass: every query and key head `x` becomes
+    `x * weight / sqrt(mean(x^2) + eps)`, the weights `[head_dim]` one for the queries and one for the keys,
+    in the tensors' dtype. Returns new tensors of the inputs' shapes."""
+    q2, k2, positions, pos_bytes, kd, T = _prep(query, key, positions, cos_sin_cache, head_dim)
+    qw, kw = _norm_weights(query_weight, key_weight, query, head_dim)
+    q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k2, memory_format=torch.contiguous_format)
+    if T > 0:
+        with _on_device_of(q2):
+            _lib.check(_lib.lib().kvc_qk_norm_rotary_pos_emb(
+                q2.data_ptr(), k2.data_ptr(), qw.data_ptr(), kw.data_ptr(), eps, positions.data_ptr(), pos_bytes,
+                cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], T, q2.shape[1] // head_dim, k2.shape[1] // head_dim,
+                head_dim, cos_sin_cache.shape[1] // 2, _tok_stride(q2), _tok_stride(k2), q_out.data_ptr(),
+                k_out.data_ptr(), q_out.shape[1], k_out.shape[1], kd, _stream_of(q2)))
+    return q_out.view(query.shape), k_out.view(key.shape)
+
+
+def qk_norm_rotary_pos_emb_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                                     query_weight: torch.Tensor, key_weight: torch.Tensor, positions: torch.Tensor,
+                                     cos_sin_cache: torch.Tensor, head_dim: int, kv_cache: torch.Tensor,
+                                     slot_mapping: torch.Tensor, eps: float = 1e-6, return_key: bool = True):
+    """`qk_norm_rotary_pos_emb` plus the slot-mapped write of the normed, rotated key and the value, as
+    `rotary_pos_emb_and_cache` writes them. Returns `(q_out, k_out)`; `k_out` is None with `return_key=False`."""
+    q2, k2, positions, pos_bytes, kd, T = _prep(query, key, positions, cos_sin_cache, head_dim)
+    qw, kw = _norm_weights(query_weight, key_weight, query, head_dim)
+    v2, nb, bs, H, stride = _value_rows(value, kv_cache, T, k2, query, head_dim, "kv_cache")
+    _require_gpu(slot_mapping, "slot_mapping")
+    if slot_mapping.shape[0] != T:
+        raise ValueError("slot_mapping length differs from the number of tokens")
+    slot_bytes = _SLOT_DTYPES.get(slot_mapping.dtype)
+    if slot_bytes is None:
+        slot_mapping, slot_bytes = slot_mapping.to(torch.int64), 8
+    if not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.contiguous()
+    if nb == 0:      # nothing to write into
+        q_out, k_out = qk_norm_rotary_pos_emb(query, key, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps)
+        return q_out, (k_out if return_key else None)
+    q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k2, memory_format=torch.contiguous_format) if return_key else None
+    if T > 0:
+        row = H * head_dim
+        with _on_device_of(q2):
+            _lib.check(_lib.lib().kvc_qk_norm_rotary_pos_emb_and_cache(
+                q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), qw.data_ptr(), kw.data_ptr(), eps, positions.data_ptr(),
+                pos_bytes, cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], T, q2.shape[1] // head_dim, H, head_dim,
+                cos_sin_cache.shape[1] // 2, _tok_stride(q2), _tok_stride(k2), _tok_stride(v2), q_out.data_ptr(),
+                k_out.data_ptr() if return_key else None, q_out.shape[1], row, kv_cache.data_ptr(),
+                kv_cache.data_ptr() + bs * row * kv_cache.element_size(), slot_mapping.data_ptr(), slot_bytes, bs, stride,
+                row, nb, kd, _stream_of(q2)))
+    return q_out.view(query.shape), (k_out.view(key.shape) if return_key else None)
+
+
+def qk_norm_rotary_pos_emb_and_append_paged(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                                            query_weight: torch.Tensor, key_weight: torch.Tensor,
+                                            batch_indices: torch.Tensor, positions: torch.Tensor,
+                                            cos_sin_cache: torch.Tensor, head_dim: int, paged_kv_cache: torch.Tensor,
+                                            kv_indices: torch.Tensor, kv_indptr: torch.Tensor,
+                                            kv_last_page_len: torch.Tensor, eps: float = 1e-6, return_key: bool = True):
+    """`qk_norm_rotary_pos_emb` plus `append_paged_kv_cache` of the normed, rotated key and the value in one launch;
+    `positions` (int32) is both the rotation position and the KV position of each token."""
+    q2, k2, positions, pos_bytes, kd, T = _prep(query, key, positions, cos_sin_cache, head_dim)
+    if pos_bytes != 4:
+        raise TypeError("positions must be int32 for page-table addressing")
+    qw, kw = _norm_weights(query_weight, key_weight, query, head_dim)
+    v2, pages, size, H, stride = _value_rows(value, paged_kv_cache, T, k2, query, head_dim, "paged_kv_cache")
+    for t, n in ((batch_indices, "batch_indices"), (kv_indices, "kv_indices"),
+                 (kv_indptr, "kv_indptr"), (kv_last_page_len, "kv_last_page_len")):
+        _require_gpu(t, n)
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise TypeError(f"{n} must be contiguous int32")
+    if batch_indices.numel() != T:
+        raise ValueError("batch_indices and positions differ in length")
+    if pages == 0:      # nothing to write into
+        q_out, k_out = qk_norm_rotary_pos_emb(query, key, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps)
+        return q_out, (k_out if return_key else None)
+    q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k2, memory_format=torch.contiguous_format) if return_key else None
+    if T > 0:
+        with _on_device_of(q2):
+            _lib.check(_lib.lib().kvc_qk_norm_rotary_pos_emb_and_append_paged(
+                q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), qw.data_ptr(), kw.data_ptr(), eps, batch_indices.data_ptr(),
+                positions.data_ptr(), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], T, q2.shape[1] // head_dim, H,
+                head_dim, cos_sin_cache.shape[1] // 2, _tok_stride(q2), _tok_stride(k2), _tok_stride(v2),
+                q_out.data_ptr(), k_out.data_ptr() if return_key else None, q_out.shape[1], H * head_dim,
+                paged_kv_cache.data_ptr(), kv_indices.data_ptr(), kv_indptr.data_ptr(), kv_indptr.numel() - 1,
+                kv_indices.numel(), size, stride, pages, kd, _stream_of(q2)))
+    return q_out.view(query.shape), (k_out.view(key.shape) if return_key else None)
+
+
 class PagedRotaryWritePlan:
     """`rotary_pos_emb_and_append_paged` with its per-step arguments checked ONCE.
 
@@ -321,20 +443,25 @@ class PagedRotaryWritePlan:
 
     def run(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
             paged_kv_cache: torch.Tensor, query_out: torch.Tensor = None,
-            key_out: torch.Tensor = None, return_key: bool = False):
+            key_out: torch.Tensor = None, return_key: bool = False, query_weight: torch.Tensor = None,
+            key_weight: torch.Tensor = None, eps: float = 1e-6):
         """One layer: rotates `query` and `key`, writes the rotated key and `value`
         into the pages. Returns `(query_out, key_out)`; `key_out` is None unless a
         buffer is given or `return_key` is set. Token-strided inputs (slices of a
         fused QKV projection) are read in place; the output buffers are contiguous.
-        Launches on the current stream of the plan's device, which must be the
+        With `query_weight` and `key_weight` (the layer's, `[head_dim]`) the heads are normed
+        first, as in `qk_norm_rotary_pos_emb`. Launches on the current stream of the plan's device, which must be the
         current device."""
+        normed = query_weight is not None
+        if normed != (key_weight is not None):
+            raise ValueError("query_weight and key_weight come together")
         if query_out is None:
             query_out = torch.empty((self.nnz, self.q_row), dtype=self.dtype, device=self.device)
         if key_out is None and return_key:
             key_out = torch.empty((self.nnz, self.kv_row), dtype=self.dtype, device=self.device)
         if self.nnz == 0:
             return query_out, key_out
-        fast = self._fast_run
+        fast = None if normed else self._fast_run
         if fast is not None:
             # layouts checked and pointers read in C++; 1 = not a layout it knows: fall through
             # to the checks below, which name what is wrong (or handle the rare case)
@@ -380,6 +507,14 @@ class PagedRotaryWritePlan:
                     and key_out.numel() == nnz * kv_row):
                 self._rows(key_out, kv_row, "key_out", dense=True)
             ko_ptr = key_out.data_ptr()
+        if normed:
+            query_weight, key_weight = _norm_weights(query_weight, key_weight, query, self.D)
+            _lib.check(_lib.lib().kvc_rotary_plan_run_norm(
+                self._plan, query.data_ptr(), key.data_ptr(), value.data_ptr(), query_weight.data_ptr(),
+                key_weight.data_ptr(), eps, q_stride, k_stride, v_stride, query_out.data_ptr(), ko_ptr,
+                paged_kv_cache.data_ptr(), st[0] if num_pages > 1 else self._dense_page, num_pages,
+                self._get_stream(self._dev_index)))
+            return query_out, key_out
         rc = self._run(self._plan, query.data_ptr(), key.data_ptr(), value.data_ptr(), q_stride,
                        k_stride, v_stride, query_out.data_ptr(), ko_ptr, paged_kv_cache.data_ptr(),
                        st[0] if num_pages > 1 else self._dense_page, num_pages,
