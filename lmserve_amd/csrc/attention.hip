@@ -331,6 +331,97 @@ __device__ __forceinline__ int64_t key_offset(const AttendArgs& a, int32_t table
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// How an item's keys are reached
+enum Reach : int {
+  kAnyPage,   // pages of any size: a lane looks up every key it loads
+  kGroups,    // pages of whole groups of 16 keys: one scalar address a group
+  kGroupsFull // and heads that fill the kernel's columns: no lane without a load
+};
+
+// The page ids of a wavefront's next 64 groups of 16 keys, one to a lane: looked up once in 32 blocks
+struct GroupIds {
+  int32_t page, off;  // -1: beyond the item's keys, or a page that the cache does not have
+  __device__ __forceinline__ void fetch(const AttendArgs& a, const Item& item, int32_t k0, int32_t lane) {
+    const int32_t key = k0 + (lane >> 1) * (kWaves * kBlock) + (lane & 1) * 16;
+    page = -1;
+    off = 0;
+    if (key < item.key_end) {
+      const int32_t p = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+      const int32_t id = a.kv_indices[item.table + p];
+      off = key - p * a.page_size;
+      page = id >= 0 && id < a.num_pages ? id : -1;
+    }
+  }
+};
+
+// A block of 32 keys in registers, as loaded
+template <int DP>
+struct Block {
+  static constexpr int KSTEPS = DP / 32;
+  static constexpr int LPR = DP <= 32 ? 4 : DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes to a row of V
+  static constexpr int RPI = 64 / LPR, VLOADS = kBlock / RPI;
+  u32x4 k[2][KSTEPS], v[VLOADS];
+  const char* rows[2];  // of the two groups of 16 keys, the same in all lanes
+
+  // Where the (it mod 32)-th block of those that `ids` were fetched for lies; which of its keys are there. Every address is
+  // inside a page of the cache; what is not the item's is cleared when it is used.
+  __device__ __forceinline__ uint32_t find(const AttendArgs& a, const Item& item, const char* heads, int32_t k0, int32_t it, const GroupIds& ids) {
+    uint32_t present = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int32_t page = __builtin_amdgcn_readlane(ids.page, (it & 31) * 2 + i);
+      const int32_t off = __builtin_amdgcn_readlane(ids.off, (it & 31) * 2 + i);
+      const int32_t left = item.key_end - k0 - i * 16;
+      if (page >= 0) present |= (left >= 16 ? 0xffffu : (1u << left) - 1u) << (i * 16);
+      rows[i] = heads + (int64_t)max(page, 0) * a.page_stride + (int64_t)off * a.row_stride;
+    }
+    return present;
+  }
+  template <Reach REACH>
+  __device__ __forceinline__ void load_k(const AttendArgs& a, const Item& item, const char* heads, int32_t k0, int32_t lane, uint32_t& present) {
+    const int32_t n = lane & 15, quad = lane >> 4, D = a.head_dim;
+    if constexpr (REACH == kAnyPage) present = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      bool have = true;
+      const char* row;
+      if constexpr (REACH == kAnyPage) {
+        const int64_t off = key_offset(a, item.table, k0 + i * 16 + n, item.key_end);
+        have = off >= 0;
+        present |= ((uint32_t)__ballot(have) & 0xffffu) << (i * 16);
+        row = heads + off + quad * 16;
+      } else {
+        row = rows[i] + (n * a.row_stride + quad * 16);
+      }
+#pragma unroll
+      for (int s = 0; s < KSTEPS; ++s) {
+        if (REACH != kGroupsFull) k[i][s] = u32x4{};
+        if (REACH == kGroupsFull || (have && s * 32 + quad * 8 < D)) k[i][s] = *reinterpret_cast<const u32x4*>(row + s * 64);
+      }
+    }
+  }
+  template <Reach REACH>
+  __device__ __forceinline__ void load_v(const AttendArgs& a, const Item& item, const char* heads, int32_t k0, int32_t lane) {
+    const int32_t vrow = lane / LPR, vcol = lane % LPR, D = a.head_dim;
+    const uint32_t at = a.plane + vrow * a.row_stride + vcol * 16;
+#pragma unroll
+    for (int i = 0; i < VLOADS; ++i) {
+      bool have = true;
+      const char* row;
+      if constexpr (REACH == kAnyPage) {
+        const int64_t off = key_offset(a, item.table, k0 + i * RPI + vrow, item.key_end);
+        have = off >= 0;
+        row = heads + a.plane + off + vcol * 16;
+      } else {
+        constexpr int HALF = VLOADS / 2;
+        row = rows[i / HALF] + (int64_t)(i % HALF * RPI) * a.row_stride + at;
+      }
+      if (REACH != kGroupsFull) v[i] = u32x4{};
+      if (REACH == kGroupsFull || (have && vcol * 8 < D)) v[i] = *reinterpret_cast<const u32x4*>(row);
+    }
+  }
+};
+
 // A workgroup per (item, key head); its wavefronts take blocks of 32 keys in turn, each with a maximum and a sum of its
 // own, joined at the end through LDS.
 //   S^T = K Q^T: the keys' rows are the matrix instruction's A operand as they lie in memory, 16 bytes a lane.
@@ -339,11 +430,127 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 // P is rounded to the storage type for the matrix instruction, each weight by at most half a step of itself, as the inputs
 // were; the sum l is of the weights before that, since lse is an output in 32 bits.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void attend_rows_kernel(AttendArgs a) {
-  constexpr int KSTEPS = DP / 32, DTILES = DP / 16;
-  constexpr int LPR = DP <= 32 ? 4 : DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // lanes to a row of V
-  constexpr int RPI = 64 / LPR, VLOADS = kBlock / RPI;
-  constexpr int VSTRIDE = DP * 2 + 32;           // rows 32 bytes apart in the banks: a transposing read takes 4 of them
+struct RowTile {
+  static constexpr int KSTEPS = DP / 32, DTILES = DP / 16;
+  static constexpr int VSTRIDE = DP * 2 + 32;  // rows 32 bytes apart in the banks: a transposing read takes 4 of them
+  typedef Block<DP> B;
+  u32x4 q[KSTEPS];
+  f32x4 o[DTILES];
+  float m, l;
+  int32_t limit;
+
+  // One block; `next` asks for the block after it, a half at a time, as soon as the registers are free
+  template <Reach REACH, typename Next>
+  __device__ __forceinline__ void take(const AttendArgs& a, const Item& item, B& b, uint32_t present, int32_t k0, char* my_v, int32_t lane,
+                                       const Next& next) {
+    const int32_t n = lane & 15, quad = lane >> 4, vrow = lane / B::LPR, vcol = lane % B::LPR;
+    f32x4 s[2] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k) s[i] = T::mfma(b.k[i][k], q[k], s[i]);
+    next(0);
+    const bool whole = present == 0xffffffffu;
+    if (REACH != kAnyPage && !whole)
+#pragma unroll
+      for (int i = 0; i < B::VLOADS; ++i)
+        if (!(present >> (i * B::RPI + vrow) & 1)) b.v[i] = u32x4{};
+    // does a row stop inside the block, and is there a value in it that 0 does not cancel?
+    const bool ragged = __ballot(n < item.rows && limit < min(k0 + kBlock, item.key_end)) != 0;
+    bool mend = false;
+    if (ragged) {
+      bool odd_v = false;
+#pragma unroll
+      for (int i = 0; i < B::VLOADS; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) odd_v = odd_v || not_finite<T>(b.v[i][w]);
+      mend = __ballot(odd_v) != 0;
+    }
+#pragma unroll
+    for (int i = 0; i < B::VLOADS; ++i)
+      if (B::LPR * 8 == DP || vcol * 8 < DP) *reinterpret_cast<u32x4*>(my_v + (i * B::RPI + vrow) * VSTRIDE + vcol * 16) = b.v[i];
+    next(1);
+    if (ragged || !whole)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int32_t at_key = i * 16 + quad * 4 + r;
+          if (k0 + at_key >= limit || !(present >> at_key & 1)) s[i][r] = -INFINITY;
+        }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float base = top == -INFINITY ? 0.f : top * a.scale;
+    float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
+    u32x4 p;
+    float sum = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float x = exp2_of(__builtin_fmaf(s[i][r], a.scale, -base));
+        const float y = exp2_of(__builtin_fmaf(s[i][r + 1], a.scale, -base));
+        p[i * 2 + r / 2] = T::pack(x, y);
+        sum += x + y;
+      }
+    l = l * shrink + sum;
+    m = top;
+    if (mend) {
+      // infinities and NaN of V go to the rows that see their keys, one by one, and are cleared for the product
+#pragma unroll
+      for (int d = 0; d < DTILES; ++d) o[d] *= shrink;
+      shrink = 1;
+#pragma unroll 1
+      for (int32_t key = 0; key < kBlock; ++key) {
+        const int r = key & 3;
+        const uint32_t word = key < 16 ? (r < 2 ? p[0] : p[1]) : (r < 2 ? p[2] : p[3]);
+        const uint32_t got = __shfl(word, (key >> 2 & 3) * 16 + n);
+        const float weight = T::wide(r & 1 ? got >> 16 : got & 0xffffu);
+        const bool sees = k0 + key < limit && (present >> key & 1);
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(my_v + key * VSTRIDE + (d * 16 + quad * 4) * 2);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t one = x[e / 2] >> (e % 2 * 16) & 0xffffu;
+            if (sees && (one & T::kExponent) == T::kExponent) o[d][e] += weight * T::wide(one);
+          }
+          asm volatile("" ::: "memory");  // one at a time: this path is to cost no registers
+        }
+      }
+#pragma unroll 1
+      for (int i = 0; i < B::VLOADS; ++i)
+        if (B::LPR * 8 == DP || vcol * 8 < DP) {
+          u32x4* mine = reinterpret_cast<u32x4*>(my_v + (i * B::RPI + vrow) * VSTRIDE + vcol * 16);
+          u32x4 x = *mine;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) x[w] = finite_part<T>(x[w]);
+          *mine = x;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DTILES; ++d) {
+      const char* from = my_v + (quad * 4 + n / 4) * VSTRIDE + (d * 16 + n % 4 * 4) * 2;
+      typedef __attribute__((address_space(3))) s16x4* Lds;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 16 * VSTRIDE));
+      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+      const u32x4 v = {x[0], x[1], y[0], y[1]};
+      o[d] = T::mfma(v, p, o[d] * shrink);
+    }
+  }
+};
+
+template <typename T, int DP, Reach REACH>
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs a) {
+  typedef RowTile<T, DP> Tile;
+  typedef Block<DP> B;
+  constexpr int KSTEPS = Tile::KSTEPS, DTILES = Tile::DTILES, VSTRIDE = Tile::VSTRIDE;
   constexpr int OSTRIDE = DP + 4;
   static_assert(kTile * OSTRIDE * 4 <= kBlock * VSTRIDE, "a wavefront's O takes the place of its V");
   __shared__ __attribute__((aligned(16))) char v_lds[kWaves][kBlock * VSTRIDE];
@@ -355,122 +562,54 @@ __global__ __launch_bounds__(kThreads) void attend_rows_kernel(AttendArgs a) {
     const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
     const Item item = a.l.items[it];
     const int32_t D = a.head_dim;
-
-    u32x4 q[KSTEPS] = {};
-    int32_t limit = 0;
+    Tile tile = {};
+    tile.m = -INFINITY;
     if (n < item.rows) {
       const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
       const int32_t token = item.q_begin >= 0 ? item.q_begin + i : a.l.shared_tokens[i];
-      limit = a.l.limits[token];
+      tile.limit = min(a.l.limits[token], item.key_end);
       const char* p = a.query + (int64_t)token * a.q_stride + ((int64_t)(h * a.group + g) * D + quad * 8) * 2;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k)
-        if (k * 32 + quad * 8 < D) q[k] = *reinterpret_cast<const u32x4*>(p + k * 64);
+        if (k * 32 + quad * 8 < D) tile.q[k] = *reinterpret_cast<const u32x4*>(p + k * 64);
     }
-    limit = min(limit, item.key_end);
-    float m = -INFINITY, l = 0;
-    f32x4 o[DTILES] = {};
-    const char* k_base = a.cache + (int64_t)h * D * 2;
+    const char* heads = a.cache + (int64_t)h * D * 2;
     char* my_v = v_lds[wave];
-    for (int32_t k0 = item.key_begin + wave * kBlock; k0 < item.key_end; k0 += kWaves * kBlock) {
-      u32x4 kr[2][KSTEPS] = {}, vr[VLOADS] = {};
-      bool have[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int64_t off = key_offset(a, item.table, k0 + i * 16 + n, item.key_end);
-        have[i] = off >= 0;
-        if (have[i])
-#pragma unroll
-          for (int k = 0; k < KSTEPS; ++k)
-            if (k * 32 + quad * 8 < D) kr[i][k] = *reinterpret_cast<const u32x4*>(k_base + off + k * 64 + quad * 16);
+    constexpr int32_t STEP = kWaves * kBlock;
+    int32_t k0 = item.key_begin + wave * kBlock;
+    if (k0 < item.key_end && a.num_pages > 0) {
+      GroupIds ids;
+      B block;
+      uint32_t present = 0;
+      if constexpr (REACH != kAnyPage) {
+        ids.fetch(a, item, k0, lane);
+        present = block.find(a, item, heads, k0, 0, ids);
       }
-      const int32_t vrow = lane / LPR, vcol = lane % LPR;
-#pragma unroll
-      for (int i = 0; i < VLOADS; ++i) {
-        const int64_t off = key_offset(a, item.table, k0 + i * RPI + vrow, item.key_end);
-        if (off >= 0 && vcol * 8 < D) vr[i] = *reinterpret_cast<const u32x4*>(k_base + a.plane + off + vcol * 16);
-      }
-      // which of the block's keys are there: bit n of half i
-      const uint32_t present = ((uint32_t)__ballot(have[0]) & 0xffffu) | (uint32_t)__ballot(have[1]) << 16;
-
-      f32x4 s[2] = {};
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int k = 0; k < KSTEPS; ++k) s[i] = T::mfma(kr[i][k], q[k], s[i]);
-      // does a row stop inside the block, and is there a value in it that 0 does not cancel?
-      bool odd_v = false;
-#pragma unroll
-      for (int i = 0; i < VLOADS; ++i) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) odd_v = odd_v || not_finite<T>(vr[i][w]);
-        if (vcol * 8 < DP) *reinterpret_cast<u32x4*>(my_v + (i * RPI + vrow) * VSTRIDE + vcol * 16) = vr[i];
-      }
-      const bool ragged = __ballot(n < item.rows && limit < min(k0 + kBlock, item.key_end)) != 0;
-      const bool mend = ragged && __ballot(odd_v) != 0;
-
-      float top = m;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int32_t at_key = i * 16 + quad * 4 + r;
-          if (k0 + at_key >= limit || !(present >> at_key & 1)) s[i][r] = -INFINITY;
-          top = fmaxf(top, s[i][r]);
-        }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float base = top == -INFINITY ? 0.f : top * a.scale;
-      const float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
-      u32x4 p;
-      float sum = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          const float x = exp2_of(__builtin_fmaf(s[i][r], a.scale, -base));
-          const float y = exp2_of(__builtin_fmaf(s[i][r + 1], a.scale, -base));
-          p[i * 2 + r / 2] = T::pack(x, y);
-          sum += x + y;
-        }
-      l = l * shrink + sum;
-      m = top;
-#pragma unroll
-      for (int d = 0; d < DTILES; ++d) {
-        const char* from = my_v + (quad * 4 + n / 4) * VSTRIDE + (d * 16 + n % 4 * 4) * 2;
-        typedef __attribute__((address_space(3))) s16x4* Lds;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 16 * VSTRIDE));
-        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-        u32x4 v = {x[0], x[1], y[0], y[1]};
-        if (mend)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) v[w] = finite_part<T>(v[w]);
-        o[d] = T::mfma(v, p, o[d] * shrink);
-      }
-      if (mend) {
-        // infinities and NaN of V, left out above, go to the rows that see their keys
-        for (int32_t key = 0; key < kBlock; ++key) {
-          const int r = key & 3;
-          const uint32_t word = key < 16 ? (r < 2 ? p[0] : p[1]) : (r < 2 ? p[2] : p[3]);
-          const uint32_t got = __shfl(word, (key >> 2 & 3) * 16 + n);
-          const float weight = T::wide(r & 1 ? got >> 16 : got & 0xffffu);
-          if (k0 + key < limit && (present >> key & 1))
-#pragma unroll
-            for (int d = 0; d < DTILES; ++d)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t x = *reinterpret_cast<const uint16_t*>(my_v + key * VSTRIDE + (d * 16 + quad * 4 + e) * 2);
-                if ((x & T::kExponent) == T::kExponent) o[d][e] += weight * T::wide(x);
-              }
-        }
+      block.template load_k<REACH>(a, item, heads, k0, lane, present);
+      block.template load_v<REACH>(a, item, heads, k0, lane);
+      for (int32_t i = 1;; ++i, k0 += STEP) {
+        const bool more = k0 + STEP < item.key_end;
+        uint32_t coming = 0;
+        if (REACH != kAnyPage && more && (i & 31) == 0) ids.fetch(a, item, k0 + STEP, lane);
+        tile.template take<REACH>(a, item, block, present, k0, my_v, lane, [&](int half) {
+          if (!more) return;
+          if (half == 0) {
+            if constexpr (REACH != kAnyPage) coming = block.find(a, item, heads, k0 + STEP, i, ids);
+            block.template load_k<REACH>(a, item, heads, k0 + STEP, lane, coming);
+          } else {
+            block.template load_v<REACH>(a, item, heads, k0 + STEP, lane);
+          }
+        });
+        if (!more) break;
+        present = coming;
       }
     }
     // the sum over the four quads' keys, then over the wavefronts
+    float l = tile.l;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (quad == 0) {
-      stats[wave][0][n] = m;
+      stats[wave][0][n] = tile.m;
       stats[wave][1][n] = l;
     }
     __syncthreads();
@@ -480,11 +619,11 @@ __global__ __launch_bounds__(kThreads) void attend_rows_kernel(AttendArgs a) {
     const float base = all_m == -INFINITY ? 0.f : all_m * a.scale;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) all_l += stats[w][1][n] * exp2_of(stats[w][0][n] * a.scale - base);
-    const float part = exp2_of(m * a.scale - base) * (all_l == 0 ? 0.f : 1.f / all_l);
+    const float part = exp2_of(tile.m * a.scale - base) * (all_l == 0 ? 0.f : 1.f / all_l);
     float* my_o = reinterpret_cast<float*>(my_v);
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
-      *reinterpret_cast<f32x4*>(my_o + n * OSTRIDE + d * 16 + quad * 4) = o[d] * part;
+      *reinterpret_cast<f32x4*>(my_o + n * OSTRIDE + d * 16 + quad * 4) = tile.o[d] * part;
     if (wave == 0 && quad == 0 && n < item.rows) {
       const float lse2 = all_l == 0 ? -INFINITY : base + __log2f(all_l);
       if (item.slot >= 0) {
@@ -623,7 +762,9 @@ Sizes sizes_of(const kvc_attention_plan& p) {
 
 template <typename T, int DP>
 void launch_rows(const AttendArgs& a, unsigned grid, hipStream_t s) {
-  kvc::launch((attend_rows_kernel<T, DP>), dim3(grid), dim3(kThreads), 0, s, a);
+  if (a.page_size % 16) kvc::launch((attend_rows_kernel<T, DP, kAnyPage>), dim3(grid), dim3(kThreads), 0, s, a);
+  else if (a.head_dim != DP) kvc::launch((attend_rows_kernel<T, DP, kGroups>), dim3(grid), dim3(kThreads), 0, s, a);
+  else kvc::launch((attend_rows_kernel<T, DP, kGroupsFull>), dim3(grid), dim3(kThreads), 0, s, a);
 }
 template <typename T>
 void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
