@@ -591,9 +591,10 @@ int kvc_rotary_plan_run_norm(const kvc_rotary_plan* plan, const void* query, con
  * statistics are fp32, the weights are rounded to the storage type for the
  * matrix instruction, the output once.
  *
- * shared_pages: the leading pages that the requests of the batch share (a
- * common prompt). They are read once for the rows of all requests whose block
- * table begins with the same pages as that of the first request with tokens and
+ * max_q_len: the most tokens that a request has, 0 if not known. It helps to choose
+ * kernels and is no limit. shared_pages: the leading pages that the requests of the batch share (a
+ * common prompt). They are read once for the rows of all requests of few tokens whose block
+ * table begins with the same pages as that of the first such request with
  * so many pages; a request that begins with others is computed by itself. The number
  * changes how the work is cut, not what is computed.
  *
@@ -614,8 +615,8 @@ int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indice
                               const int32_t* kv_indptr, const int32_t* kv_last_page_len,
                               int64_t batch_size, int64_t num_tokens, int64_t num_kv_indices,
                               int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
-                              int64_t page_size, int64_t shared_pages, float sm_scale, int dtype,
-                              kvc_attention_plan** out);
+                              int64_t page_size, int64_t max_q_len, int64_t shared_pages,
+                              float sm_scale, int dtype, kvc_attention_plan** out);
 int64_t kvc_attention_plan_bytes(const kvc_attention_plan* plan);
 int64_t kvc_attention_workspace_bytes(const kvc_attention_plan* plan);
 int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buffer_bytes,

@@ -147,7 +147,7 @@ SIGNATURES = {
                                                             _P]),
     "kvc_rotary_plan_run_norm": (c_int, [_P, _P, _P, _P, _P, _P, c_float, _I64, _I64, _I64, _P, _P, _P, _I64, _I64,
                                          _P]),
-    "kvc_attention_plan_create": (c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, c_float,
+    "kvc_attention_plan_create": (c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, c_float,
                                           c_int, ctypes.POINTER(_P)]),
     "kvc_attention_plan_bytes": (_I64, [_P]),
     "kvc_attention_workspace_bytes": (_I64, [_P]),

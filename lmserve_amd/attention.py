@@ -65,7 +65,7 @@ class PagedAttentionPlan:
         _lib.check(lib.kvc_attention_plan_create(
             self.qo_indptr.data_ptr(), self.kv_indices.data_ptr(), self.kv_indptr.data_ptr(),
             self.kv_last_page_len.data_ptr(), batch, self.num_tokens, self.kv_indices.numel(), self.Hq, self.H,
-            self.D, self.page_size, int(shared_pages), self.D ** -0.5 if sm_scale is None else float(sm_scale), kd,
+            self.D, self.page_size, int(max_q_len or 0), int(shared_pages), self.D ** -0.5 if sm_scale is None else float(sm_scale), kd,
             ctypes.byref(handle)))
         self._plan = handle.value
         self._destroy = lib.kvc_attention_plan_destroy

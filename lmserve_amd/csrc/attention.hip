@@ -29,13 +29,17 @@ using kvc::log2_exact;
 using kvc::u32x4;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kTile = 16;          // rows of an item
-constexpr int kBlock = 32;         // keys that a wavefront takes at once
+constexpr int kTile = 16;          // rows of a narrow item
+constexpr int kWide = 32 * kWaves; // rows of a wide item: 32 to a wavefront
+constexpr int kBlock = 32;         // keys that a wavefront takes at once of a narrow item
+constexpr int kStep = 64;          // keys that a workgroup takes at once of a wide item
+constexpr int kManyParts = 8;      // a row of more partials is joined by a workgroup
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -49,32 +53,34 @@ struct Item {  // 32 bytes
   int32_t slot;     // where its partial goes; -1: the only item of its rows
   int32_t pad;
 };
-struct Entry {  // 32 bytes: a row tile that is joined from partials (or has no keys at all)
+struct Entry {  // 32 bytes: rows of one tile that are joined from partials (or have no keys at all)
   int32_t q_begin, row0, rows, slot, chunks;
-  int32_t shared_row0;  // the tile's first row among those of the sharing requests, or -1
-  int32_t pad[2];
+  int32_t shared_row0;  // the first row among those of the sharing requests, or -1
+  int32_t wide, pad;
 };
 struct Header {
-  int32_t items, entries, shared_chunks, shared_tokens;
+  int32_t items[2];  // narrow, wide
+  int32_t entries, shared_chunks, shared_wide;
 };
 
 struct Layout {  // the plan's device buffer
   Header* header;
   Request* requests;
   int32_t* shares;         // [B] 1: its leading pages are the shared ones
-  int32_t* offsets;        // [B][4] first item, slot, entry, shared token
+  int32_t* offsets;        // [B][4] first item and slot of its kind, entry, shared token
   int32_t* limits;         // [T] keys that a token sees
   int32_t* shared_tokens;  // [T]
-  Item* items;
+  Item* items[2];
   Entry* entries;
 };
 
 struct PlanArgs {
   const int32_t *qo_indptr, *kv_indices, *kv_indptr, *kv_last_page_len;
   int32_t batch_size, num_tokens, num_kv_indices, page_size, shared_pages, group;
-  int32_t target;      // items that a step is cut into, about
-  int32_t min_chunk;   // keys
-  int32_t max_items, max_entries;
+  int32_t narrow_rows, narrow_shared_rows;  // the most rows of a request, and of all sharing ones, for narrow items
+  int32_t target[2];     // items that a step is cut into, about
+  int32_t min_chunk[2];  // keys
+  int32_t max_items[2], max_entries;
   Layout l;
 };
 
@@ -93,7 +99,7 @@ __device__ __forceinline__ Table tokens_of(const PlanArgs& a, int32_t b) {
 }
 
 // A workgroup per request: its lengths, its tokens' limits, and whether it begins with the shared pages. Which pages these
-// are is what the first request with tokens and that many pages holds; a request that holds others is a request by itself,
+// are is what the first request with few tokens and that many pages holds; a request that holds others is a request by itself,
 // so that the number of shared pages changes how the work is cut and never the result.
 __global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
   __shared__ int32_t first, differ;
@@ -106,7 +112,8 @@ __global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
     const int32_t lim = len - q.pages + j + 1;
     a.l.limits[q.begin + j] = lim > 0 ? lim : 0;
   }
-  bool shares = a.shared_pages > 0 && q.pages > 0 && t.pages >= a.shared_pages;
+  // (of the requests of many rows none: they read a key for 128 rows as it is)
+  bool shares = a.shared_pages > 0 && q.pages > 0 && q.pages * a.group <= a.narrow_rows && t.pages >= a.shared_pages;
   if (shares) {
     if (tid == 0) {
       first = b;
@@ -115,7 +122,8 @@ __global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
     __syncthreads();
     for (int32_t c0 = 0; c0 < b; c0 += 256) {
       const int32_t c = c0 + tid;
-      if (c < b && tokens_of(a, c).pages > 0 && table_of(a, c).pages >= a.shared_pages) atomicMin(&first, c);
+      const int32_t n = c < b ? tokens_of(a, c).pages : 0;
+      if (n > 0 && n * a.group <= a.narrow_rows && table_of(a, c).pages >= a.shared_pages) atomicMin(&first, c);
       __syncthreads();
       const bool found = first < b;
       __syncthreads();  // everyone has looked before someone lowers it further
@@ -136,129 +144,147 @@ __global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
 }
 
 struct Counts {
-  int32_t v[4];  // items, slots, entries, shared tokens
+  int32_t v[6];  // items and slots of either kind, entries, shared tokens
 };
 __device__ __forceinline__ int32_t ceil_div(int32_t x, int32_t y) { return (x + y - 1) / y; }
 
+// Rows of an entry: one of many parts is by itself
+__device__ __forceinline__ int32_t joined_rows(int32_t parts) { return parts > kManyParts ? 1 : kTile; }
+
 struct Cut {
-  int32_t tiles, chunks, begin;  // row tiles, key ranges of each, first key of its own
+  int32_t tiles, chunks, begin, tile;  // row tiles, key ranges of each, first key of its own, rows of a tile
+  bool wide;
 };
-__device__ __forceinline__ Cut cut_of(const PlanArgs& a, const Request& r, bool shares, int32_t chunk) {
+__device__ __forceinline__ Cut cut_of(const PlanArgs& a, const Request& r, bool shares, int32_t narrow_chunk, int32_t wide_chunk) {
   Cut c;
+  c.wide = r.n * a.group > a.narrow_rows;
+  c.tile = c.wide ? kWide : kTile;
   c.begin = shares ? min(a.shared_pages * a.page_size, r.len) : 0;
-  c.tiles = ceil_div(r.n * a.group, kTile);
-  c.chunks = ceil_div(r.len - c.begin, chunk);
+  c.tiles = ceil_div(r.n * a.group, c.tile);
+  c.chunks = ceil_div(r.len - c.begin, c.wide ? wide_chunk : narrow_chunk);
   return c;
 }
+__device__ __forceinline__ int32_t round_up(int32_t x, int32_t to) { return ceil_div(x, to) * to; }
 
 // One workgroup: the keys of an item, from all the work there is; how many items, slots and entries come before each
 // request's, by a scan; the lists. A request of few tokens is one tile and takes a few lines of its own, so a wavefront
 // does a request.
 __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
-  __shared__ int64_t total_work, total_shared;
-  __shared__ int32_t wave_sums[16][4], carry[4], some_request;
+  __shared__ unsigned long long total_work[2], total_shared;
+  __shared__ int32_t wave_sums[16][6], carry[6], some_request;
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) {
-    total_work = total_shared = 0;
+    total_work[0] = total_work[1] = total_shared = 0;
     some_request = INT32_MAX;
   }
   __syncthreads();
-  int64_t work = 0, shared = 0;
   for (int32_t b = tid; b < a.batch_size; b += 1024) {
     const Request r = a.l.requests[b];
     const bool sh = a.l.shares[b];
-    const Cut c = cut_of(a, r, sh, 1 << 30);
-    work += (int64_t)c.tiles * (r.len - c.begin);
+    const Cut c = cut_of(a, r, sh, 1 << 30, 1 << 30);
+    if (c.tiles) atomicAdd(&total_work[c.wide], (unsigned long long)((int64_t)c.tiles * (r.len - c.begin)));
     if (sh) {
-      shared += r.n;
+      atomicAdd(&total_shared, (unsigned long long)r.n);
       atomicMin(&some_request, b);
     }
   }
-  atomicAdd((unsigned long long*)&total_work, (unsigned long long)work);
-  atomicAdd((unsigned long long*)&total_shared, (unsigned long long)shared);
   __syncthreads();
-  const int32_t shared_tokens = (int32_t)total_shared;
-  const int32_t shared_len = a.shared_pages * a.page_size;
-  const int32_t shared_tiles = ceil_div(shared_tokens * a.group, kTile);
-  const int64_t all = total_work + (int64_t)shared_tiles * shared_len;
-  int64_t per = (all + a.target - 1) / a.target;
-  per = (per + kBlock - 1) / kBlock * kBlock;
-  const int32_t chunk = (int32_t)(per < a.min_chunk ? a.min_chunk : per < (1 << 30) ? per : 1 << 30);
-  const int32_t shared_chunks = shared_tokens ? ceil_div(shared_len, chunk) : 0;
+  const int32_t shared_rows = (int32_t)total_shared * a.group, shared_len = a.shared_pages * a.page_size;
+  const bool shared_wide = shared_rows > a.narrow_shared_rows;
+  const int32_t shared_tile = shared_wide ? kWide : kTile, shared_tiles = ceil_div(shared_rows, shared_tile);
+  int32_t chunk[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int64_t work = (int64_t)total_work[k] + (shared_wide == (k == 1) ? (int64_t)shared_tiles * shared_len : 0);
+    const int64_t per = (work + a.target[k] - 1) / a.target[k];
+    chunk[k] = round_up((int32_t)(per < a.min_chunk[k] ? a.min_chunk[k] : per < (1 << 30) ? per : 1 << 30), kStep);
+  }
+  const int32_t shared_chunks = shared_rows ? ceil_div(shared_len, chunk[shared_wide]) : 0;
   const int32_t shared_items = shared_tiles * shared_chunks;
-  if (tid < 4) carry[tid] = tid < 2 ? shared_items : 0;
+  if (tid < 6) carry[tid] = tid < 4 && tid / 2 == shared_wide ? shared_items : 0;
   __syncthreads();
   for (int32_t b0 = 0; b0 < a.batch_size; b0 += 1024) {
     const int32_t b = b0 + tid;
     Counts n = {};
+    bool wide = false;
     if (b < a.batch_size) {
       const Request r = a.l.requests[b];
       const bool sh = a.l.shares[b];
-      const Cut c = cut_of(a, r, sh, chunk);
-      n.v[0] = c.tiles * c.chunks;
-      n.v[1] = sh || c.chunks > 1 ? n.v[0] : 0;
-      n.v[2] = sh || c.chunks != 1 ? c.tiles : 0;
-      n.v[3] = sh ? r.n : 0;
+      const Cut c = cut_of(a, r, sh, chunk[0], chunk[1]);
+      wide = c.wide;
+      const int32_t items = c.tiles * c.chunks, slots = sh || c.chunks > 1 ? items : 0;
+      n.v[0] = wide ? 0 : items;
+      n.v[1] = wide ? 0 : slots;
+      n.v[2] = wide ? items : 0;
+      n.v[3] = wide ? slots : 0;
+      n.v[4] = sh || c.chunks != 1 ? ceil_div(r.n * a.group, joined_rows(c.chunks + (sh ? shared_chunks : 0))) : 0;
+      n.v[5] = sh ? r.n : 0;
     }
     Counts before = n;  // inclusive, then exclusive
     for (int d = 1; d < 64; d <<= 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 6; ++i) {
         const int32_t x = __shfl_up(before.v[i], d);
         if (lane >= d) before.v[i] += x;
       }
     if (lane == 63)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) wave_sums[wave][i] = before.v[i];
+      for (int i = 0; i < 6; ++i) wave_sums[wave][i] = before.v[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 6; ++i) {
       int32_t base = carry[i];
       for (int w = 0; w < wave; ++w) base += wave_sums[w][i];
       before.v[i] += base - n.v[i];
     }
-    if (b < a.batch_size) *reinterpret_cast<int4*>(a.l.offsets + 4 * b) = *reinterpret_cast<const int4*>(before.v);
+    if (b < a.batch_size)
+      *reinterpret_cast<int4*>(a.l.offsets + 4 * b) =
+          make_int4(wide ? before.v[2] : before.v[0], wide ? before.v[3] : before.v[1], before.v[4], before.v[5]);
     __syncthreads();
     if (tid == 1023)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) carry[i] = before.v[i] + n.v[i];
+      for (int i = 0; i < 6; ++i) carry[i] = before.v[i] + n.v[i];
     __syncthreads();
   }
-  if (tid == 0) *a.l.header = {min(carry[0], a.max_items), min(carry[2], a.max_entries), shared_chunks, shared_tokens};
+  if (tid == 0)
+    *a.l.header = {{min(carry[0], a.max_items[0]), min(carry[2], a.max_items[1])}, min(carry[4], a.max_entries), shared_chunks, shared_wide};
 
   for (int32_t b = wave; b < a.batch_size; b += 16) {
     const Request r = a.l.requests[b];
     const bool sh = a.l.shares[b];
-    const Cut c = cut_of(a, r, sh, chunk);
+    const Cut c = cut_of(a, r, sh, chunk[0], chunk[1]);
     const int4 first = *reinterpret_cast<const int4*>(a.l.offsets + 4 * b);
     const int32_t rows = r.n * a.group;
     const bool partial = sh || c.chunks > 1;
+    Item* const items = c.wide ? a.l.items[1] : a.l.items[0];
+    const int32_t max_items = c.wide ? a.max_items[1] : a.max_items[0], unit = c.wide ? kStep : kBlock;
     for (int32_t i = lane; i < c.tiles * c.chunks; i += 64) {
       const int32_t tile = i / c.chunks, part = i - tile * c.chunks;
-      const int32_t row0 = tile * kTile, last_row = min(row0 + kTile, rows) - 1;
+      const int32_t row0 = tile * c.tile, last_row = min(row0 + c.tile, rows) - 1;
       const int32_t end = clamp(r.len - r.n + last_row / a.group + 1, c.begin, r.len);  // keys that the tile's last token sees
-      const int32_t each = (ceil_div(end - c.begin, c.chunks) + kBlock - 1) / kBlock * kBlock;
+      const int32_t each = round_up(ceil_div(end - c.begin, c.chunks), unit);
       const int32_t from = min(c.begin + part * each, end), to = min(from + each, end);
-      if (first.x + i < a.max_items)
-        a.l.items[first.x + i] = {r.q_begin, row0, last_row + 1 - row0, r.table, from, to, partial ? first.y + i : -1, 0};
+      if (first.x + i < max_items)
+        items[first.x + i] = {r.q_begin, row0, last_row + 1 - row0, r.table, from, to, partial ? first.y + i : -1, 0};
     }
-    if (sh || c.chunks != 1)
-      for (int32_t i = lane; i < c.tiles; i += 64) {
-        const int32_t row0 = i * kTile;
+    if (sh || c.chunks != 1) {
+      const int32_t each = joined_rows(c.chunks + (sh ? shared_chunks : 0));  // (divides a tile)
+      for (int32_t row0 = lane * each, i = lane; row0 < rows; row0 += 64 * each, i += 64)
         if (first.z + i < a.max_entries)
-          a.l.entries[first.z + i] = {r.q_begin, row0, min(kTile, rows - row0), first.y + i * c.chunks, c.chunks,
-                                      sh ? first.w * a.group + row0 : -1, {}};
-      }
+          a.l.entries[first.z + i] = {r.q_begin, row0, min(each, rows - row0), first.y + row0 / c.tile * c.chunks, c.chunks,
+                                      sh ? first.w * a.group + row0 : -1, c.wide, 0};
+    }
     if (sh)
       for (int32_t i = lane; i < r.n; i += 64) a.l.shared_tokens[first.w + i] = r.q_begin + i;
   }
   if (shared_items) {
     const int32_t table = a.l.requests[some_request].table;
-    const int32_t each = (ceil_div(shared_len, shared_chunks) + kBlock - 1) / kBlock * kBlock;
-    for (int32_t i = tid; i < shared_items && i < a.max_items; i += 1024) {
-      const int32_t tile = i / shared_chunks, part = i - tile * shared_chunks, row0 = tile * kTile;
+    const int32_t each = round_up(ceil_div(shared_len, shared_chunks), shared_wide ? kStep : kBlock);
+    Item* const items = shared_wide ? a.l.items[1] : a.l.items[0];
+    for (int32_t i = tid; i < shared_items && i < a.max_items[shared_wide]; i += 1024) {
+      const int32_t tile = i / shared_chunks, part = i - tile * shared_chunks, row0 = tile * shared_tile;
       const int32_t from = min(part * each, shared_len);
-      a.l.items[i] = {-1, row0, min(kTile, shared_tokens * a.group - row0), table, from, min(from + each, shared_len), i, 0};
+      items[i] = {-1, row0, min(shared_tile, shared_rows - row0), table, from, min(from + each, shared_len), i, 0};
     }
   }
 }
@@ -268,6 +294,9 @@ struct BF16 {
   typedef __bf16 V8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -282,6 +311,9 @@ struct F16 {
   typedef _Float16 V8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -298,10 +330,23 @@ template <typename T>
 __device__ __forceinline__ bool not_finite(uint32_t two) {
   return (two & T::kExponent) == T::kExponent || (two >> 16 & T::kExponent) == T::kExponent;
 }
+// The infinities and NaN among 4 values, 0 for the others
 template <typename T>
-__device__ __forceinline__ uint32_t finite_part(uint32_t two) {
-  return ((two & T::kExponent) == T::kExponent ? 0 : two & 0xffffu) |
-         ((two >> 16 & T::kExponent) == T::kExponent ? 0 : two & 0xffff0000u);
+__device__ __forceinline__ f32x4 infinite_part(u32x2 four) {
+  f32x4 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t one = four[e / 2] >> (e % 2 * 16) & 0xffffu;
+    x[e] = (one & T::kExponent) == T::kExponent ? T::wide(one) : 0.f;
+  }
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 finite_part(u32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = ((v[i] & T::kExponent) == T::kExponent ? 0 : v[i] & 0xffffu) | ((v[i] >> 16 & T::kExponent) == T::kExponent ? 0 : v[i] & 0xffff0000u);
+  return v;
 }
 
 struct AttendArgs {
@@ -310,8 +355,8 @@ struct AttendArgs {
   const int32_t* kv_indices;
   char* out;
   float* lse;              // may be null
-  float* partial;          // [slots][kv heads][kTile][head_dim]
-  float* partial_lse;      // [slots][kv heads][kTile], to base 2
+  float* partial[2];       // narrow, wide: [slots][kv heads][rows of a tile][head_dim]
+  float* partial_lse[2];   // [slots][kv heads][rows of a tile], to base 2
   int64_t q_stride;        // bytes
   uint32_t page_stride, row_stride, plane;  // bytes: page to page, key to key in a page, K to V
   int32_t num_pages, page_size, page_shift;
@@ -438,6 +483,7 @@ struct RowTile {
   f32x4 o[DTILES];
   float m, l;
   int32_t limit;
+  int32_t odd_from;  // the first block whose infinities and NaN of V were left out
 
   // One block; `next` asks for the block after it, a half at a time, as soon as the registers are free
   template <Reach REACH, typename Next>
@@ -457,27 +503,32 @@ struct RowTile {
         if (!(present >> (i * B::RPI + vrow) & 1)) b.v[i] = u32x4{};
     // does a row stop inside the block, and is there a value in it that 0 does not cancel?
     const bool ragged = __ballot(n < item.rows && limit < min(k0 + kBlock, item.key_end)) != 0;
-    bool mend = false;
     if (ragged) {
       bool odd_v = false;
 #pragma unroll
       for (int i = 0; i < B::VLOADS; ++i)
 #pragma unroll
         for (int w = 0; w < 4; ++w) odd_v = odd_v || not_finite<T>(b.v[i][w]);
-      mend = __ballot(odd_v) != 0;
+      if (__ballot(odd_v)) {
+        odd_from = min(odd_from, k0);
+#pragma unroll
+        for (int i = 0; i < B::VLOADS; ++i) b.v[i] = finite_part<T>(b.v[i]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < B::VLOADS; ++i)
       if (B::LPR * 8 == DP || vcol * 8 < DP) *reinterpret_cast<u32x4*>(my_v + (i * B::RPI + vrow) * VSTRIDE + vcol * 16) = b.v[i];
     next(1);
-    if (ragged || !whole)
+    if (ragged || !whole) {
+      // the keys that the row sees, bit x for key x + 4 quad, so that a lane's are at fixed bits
+      const int32_t left = clamp(limit - k0, 0, kBlock);
+      const uint32_t sees = (left ? 0xffffffffu >> (kBlock - left) & present : 0) >> quad * 4;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int32_t at_key = i * 16 + quad * 4 + r;
-          if (k0 + at_key >= limit || !(present >> at_key & 1)) s[i][r] = -INFINITY;
-        }
+        for (int r = 0; r < 4; ++r)
+          if (!(sees >> (i * 16 + r) & 1)) s[i][r] = -INFINITY;
+    }
     float top = m;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -486,7 +537,7 @@ struct RowTile {
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     const float base = top == -INFINITY ? 0.f : top * a.scale;
-    float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
+    const float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
     u32x4 p;
     float sum = 0;
 #pragma unroll
@@ -500,39 +551,6 @@ struct RowTile {
       }
     l = l * shrink + sum;
     m = top;
-    if (mend) {
-      // infinities and NaN of V go to the rows that see their keys, one by one, and are cleared for the product
-#pragma unroll
-      for (int d = 0; d < DTILES; ++d) o[d] *= shrink;
-      shrink = 1;
-#pragma unroll 1
-      for (int32_t key = 0; key < kBlock; ++key) {
-        const int r = key & 3;
-        const uint32_t word = key < 16 ? (r < 2 ? p[0] : p[1]) : (r < 2 ? p[2] : p[3]);
-        const uint32_t got = __shfl(word, (key >> 2 & 3) * 16 + n);
-        const float weight = T::wide(r & 1 ? got >> 16 : got & 0xffffu);
-        const bool sees = k0 + key < limit && (present >> key & 1);
-#pragma unroll
-        for (int d = 0; d < DTILES; ++d) {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(my_v + key * VSTRIDE + (d * 16 + quad * 4) * 2);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t one = x[e / 2] >> (e % 2 * 16) & 0xffffu;
-            if (sees && (one & T::kExponent) == T::kExponent) o[d][e] += weight * T::wide(one);
-          }
-          asm volatile("" ::: "memory");  // one at a time: this path is to cost no registers
-        }
-      }
-#pragma unroll 1
-      for (int i = 0; i < B::VLOADS; ++i)
-        if (B::LPR * 8 == DP || vcol * 8 < DP) {
-          u32x4* mine = reinterpret_cast<u32x4*>(my_v + (i * B::RPI + vrow) * VSTRIDE + vcol * 16);
-          u32x4 x = *mine;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) x[w] = finite_part<T>(x[w]);
-          *mine = x;
-        }
-    }
 #pragma unroll
     for (int d = 0; d < DTILES; ++d) {
       const char* from = my_v + (quad * 4 + n / 4) * VSTRIDE + (d * 16 + n % 4 * 4) * 2;
@@ -557,13 +575,14 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void at
   __shared__ float stats[kWaves][2][kTile];
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t n = lane & 15, quad = lane >> 4;
-  const int32_t num_items = a.l.header->items;
+  const int32_t num_items = a.l.header->items[0];
   for (int32_t at = blockIdx.x; at < num_items * a.kv_heads; at += gridDim.x) {
     const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
-    const Item item = a.l.items[it];
+    const Item item = a.l.items[0][it];
     const int32_t D = a.head_dim;
     Tile tile = {};
     tile.m = -INFINITY;
+    tile.odd_from = INT32_MAX;
     if (n < item.rows) {
       const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
       const int32_t token = item.q_begin >= 0 ? item.q_begin + i : a.l.shared_tokens[i];
@@ -604,6 +623,22 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void at
         present = coming;
       }
     }
+    // infinities and NaN of V that were left out, where rows stop, go to the rows that see their keys. (A weight is taken for
+    // 1: what it scales is infinite. The opaque zero keeps the compiler from working on this ahead.)
+    if (tile.odd_from < item.key_end) {
+      int32_t zero = 0;
+      asm volatile("" : "+v"(zero));
+      for (int32_t b0 = tile.odd_from; b0 < item.key_end; b0 += STEP)
+#pragma unroll 1
+        for (int32_t key = b0; key < min(b0 + kBlock, item.key_end); ++key) {
+          const int64_t off = key_offset(a, item.table, key, item.key_end);
+          if (off < 0 || key >= tile.limit) continue;
+          const char* row = heads + a.plane + off + quad * 8 + zero;
+#pragma unroll
+          for (int d = 0; d < DTILES; ++d)
+            if (d * 16 + quad * 4 < D) tile.o[d] += infinite_part<T>(*reinterpret_cast<const u32x2*>(row + d * 32));
+        }
+    }
     // the sum over the four quads' keys, then over the wavefronts
     float l = tile.l;
     l += __shfl_xor(l, 16);
@@ -627,7 +662,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void at
     if (wave == 0 && quad == 0 && n < item.rows) {
       const float lse2 = all_l == 0 ? -INFINITY : base + __log2f(all_l);
       if (item.slot >= 0) {
-        a.partial_lse[((int64_t)item.slot * a.kv_heads + h) * kTile + n] = lse2;
+        a.partial_lse[0][((int64_t)item.slot * a.kv_heads + h) * kTile + n] = lse2;
       } else if (a.lse) {
         const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
         a.lse[(int64_t)(item.q_begin + i) * a.kv_heads * a.group + h * a.group + g] = lse2 * kLn2;
@@ -641,7 +676,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void at
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(v_lds[w]) + r * OSTRIDE + d);
       if (item.slot >= 0) {
-        *reinterpret_cast<f32x4*>(a.partial + (((int64_t)item.slot * a.kv_heads + h) * kTile + r) * D + d) = x;
+        *reinterpret_cast<f32x4*>(a.partial[0] + (((int64_t)item.slot * a.kv_heads + h) * kTile + r) * D + d) = x;
       } else {
         const int32_t row = item.row0 + r, i = row / a.group, g = row - i * a.group;
         const u32x2 two = {T::pack(x[0], x[1]), T::pack(x[2], x[3])};
@@ -652,45 +687,348 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void at
   }
 }
 
-// Joins a row's partials: weights exp2(lse_c - lse). A row without any is zero, its lse -inf. A wavefront per row, its
-// lanes over the columns.
+// A workgroup per (item of up to 128 rows, key head): 32 rows to a wavefront, 64 keys at a time, staged in LDS for all four.
+// The next step's loads are under way in registers while one is worked on; the buffers alternate, so that a step has one
+// barrier. S^T and O^T as above, in 32 x 32 pieces: a lane holds one row and, of 32 keys, those with bit 2 as its own
+// half (lane / 32). K rows are 16 bytes apart in the banks (a lane reads 16 bytes of a row of its own), V rows 32.
+// The maximum that the weights are taken against grows only when a row's has outgrown it by 2^8: until then the larger weights
+// (below 2^8) and sums say the same, and the rescaling of O, 64 registers at 128 columns, is left out of nearly every step.
+template <typename T, int DP, Reach REACH>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_tiles_kernel(AttendArgs a) {
+  constexpr int KSTEPS = DP / 16, DTILES = DP / 32;
+  constexpr int KSTRIDE = DP * 2 + 16, VSTRIDE = DP * 2 + 32;
+  constexpr int LPR = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes to a row
+  constexpr int RPW = 64 / LPR, ROUNDS = kStep / (RPW * kWaves);
+  constexpr float kOutgrown = 8;
+  __shared__ __attribute__((aligned(16))) char k_lds[2][kStep * KSTRIDE];
+  __shared__ __attribute__((aligned(16))) char v_lds[2][kStep * VSTRIDE];
+  __shared__ int32_t leasts[kWaves], left_out;
+  const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int32_t n = lane & 31, hi = lane >> 5, lrow = lane / LPR, lcol = lane % LPR;
+  const int32_t num_items = a.l.header->items[1];
+  const int32_t D = a.head_dim;
+  for (int32_t at = blockIdx.x; at < num_items * a.kv_heads; at += gridDim.x) {
+    const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
+    const Item item = a.l.items[1][it];
+    const char* const heads = a.cache + (int64_t)h * D * 2;
+    const int32_t my_row = wave * 32 + n;
+    u32x4 q[KSTEPS] = {};
+    int32_t limit = 0, token = 0, g = 0;
+    if (my_row < item.rows) {
+      const int32_t row = item.row0 + my_row, i = row / a.group;
+      g = row - i * a.group;
+      token = item.q_begin >= 0 ? item.q_begin + i : a.l.shared_tokens[i];
+      limit = min(a.l.limits[token], item.key_end);
+      const char* p = a.query + (int64_t)token * a.q_stride + ((int64_t)(h * a.group + g) * D + hi * 8) * 2;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k)
+        if (REACH == kGroupsFull || k * 16 + hi * 8 < D) q[k] = *reinterpret_cast<const u32x4*>(p + k * 32);
+    }
+    // the wavefront's first and last limits (rows that are not there have none)
+    int32_t least = my_row < item.rows ? limit : INT32_MAX, most = limit;
+    for (int d = 16; d; d >>= 1) {
+      least = min(least, __shfl_xor(least, d));
+      most = max(most, __shfl_xor(most, d));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    if (lane == 0) leasts[wave] = least;
+    if (tid == 0) left_out = 0;
+    __syncthreads();
+    const int32_t tile_least = min(min(leasts[0], leasts[1]), min(leasts[2], leasts[3]));
+    f32x16 o[DTILES] = {};
+    float m = -INFINITY, l = 0;
+    u32x4 kr[ROUNDS], vr[ROUNDS];
+    int32_t id_page = -1, id_off = 0;
+    // the keys of a step from k0 on, on their way; which are there
+    const auto fetch = [&](int32_t k0, int32_t step) -> uint64_t {
+      uint64_t present = 0;
+      if constexpr (REACH == kAnyPage) {
+        present = __ballot(key_offset(a, item.table, k0 + lane, item.key_end) >= 0);
+      } else if ((step & 15) == 0) {
+        const int32_t key = k0 + lane * 16;
+        id_page = -1;
+        if (key < item.key_end) {
+          const int32_t p = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+          const int32_t id = a.kv_indices[item.table + p];
+          id_off = key - p * a.page_size;
+          if (id >= 0 && id < a.num_pages) id_page = id;
+        }
+      }
+      if constexpr (REACH != kAnyPage)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int32_t left = item.key_end - k0 - i * 16;
+          if (__builtin_amdgcn_readlane(id_page, (step & 15) * 4 + i) >= 0)
+            present |= (uint64_t)(left >= 16 ? 0xffffu : (1u << left) - 1u) << (i * 16);
+        }
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) {
+        const int32_t row0 = i * RPW * kWaves + wave * RPW;
+        const char* from;
+        bool have = lcol * 8 < D;
+        if constexpr (REACH == kAnyPage) {
+          const int64_t off = key_offset(a, item.table, k0 + row0 + lrow, item.key_end);
+          have = have && off >= 0;
+          from = heads + off + lcol * 16;
+        } else {
+          const int32_t group = (step & 15) * 4 + row0 / 16;
+          const int32_t page = __builtin_amdgcn_readlane(id_page, group), off = __builtin_amdgcn_readlane(id_off, group);
+          from = heads + (int64_t)max(page, 0) * a.page_stride + (int64_t)(page < 0 ? 0 : off + row0 % 16) * a.row_stride +
+                 (lrow * a.row_stride + lcol * 16);
+        }
+        if (REACH != kGroupsFull) kr[i] = vr[i] = u32x4{};
+        if (REACH == kGroupsFull || have) {
+          kr[i] = *reinterpret_cast<const u32x4*>(from);
+          vr[i] = *reinterpret_cast<const u32x4*>(from + a.plane);
+        }
+      }
+      return present;
+    };
+    // those keys into LDS; V of keys that are not there is cleared, which K's need not be: their scores are masked
+    const auto stage = [&](int buf, int32_t k0, uint64_t present) {
+      if (REACH != kAnyPage && ~present)
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i)
+          if (!(present >> (i * RPW * kWaves + wave * RPW + lrow) & 1)) vr[i] = u32x4{};
+      if (k0 + kStep > tile_least) {  // a row stops in this step: are there values that 0 does not cancel?
+        bool odd_v = false;
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) odd_v = odd_v || not_finite<T>(vr[i][w]);
+        if (__ballot(odd_v)) {
+          left_out = 1;
+#pragma unroll
+          for (int i = 0; i < ROUNDS; ++i) vr[i] = finite_part<T>(vr[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) {
+        const int32_t row = i * RPW * kWaves + wave * RPW + lrow;
+        if (LPR * 8 == DP || lcol * 8 < DP) {
+          *reinterpret_cast<u32x4*>(k_lds[buf] + row * KSTRIDE + lcol * 16) = kr[i];
+          *reinterpret_cast<u32x4*>(v_lds[buf] + row * VSTRIDE + lcol * 16) = vr[i];
+        }
+      }
+    };
+    const auto work = [&](int buf, int32_t k0, uint64_t present) {
+      // pieces of K and V come from LDS a group ahead of the products that take them, and no further: registers
+      f32x16 s[2] = {};
+      constexpr int GROUPS = 2 * KSTEPS / 4;
+      const char* const k_from = k_lds[buf] + n * KSTRIDE + hi * 16;
+      const auto k_piece = [&](int i) { return *reinterpret_cast<const u32x4*>(k_from + i / KSTEPS * 32 * KSTRIDE + i % KSTEPS * 32); };
+      u32x4 piece[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) piece[0][i] = k_piece(i);
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        if (j + 1 < GROUPS)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) piece[(j + 1) % 2][i] = k_piece(j * 4 + 4 + i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[(j * 4 + i) / KSTEPS] = T::mfma(piece[j % 2][i], q[(j * 4 + i) % KSTEPS], s[(j * 4 + i) / KSTEPS]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const bool ragged = least < k0 + kStep;
+      if (ragged || ~present) {
+        // the keys that the row sees, bit x for key x + 4 hi, so that a lane's are at fixed bits
+        const int32_t left = clamp(limit - k0, 0, kStep);
+        const uint64_t sees = (left ? ~uint64_t(0) >> (kStep - left) & present : 0) >> hi * 4;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t bits = (uint32_t)(sees >> t * 32);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!(bits >> (r / 4 * 8 + r % 4) & 1)) s[t][r] = -INFINITY;
+        }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (__ballot(top * a.scale > m * a.scale + kOutgrown)) {
+        const float grown = fmaxf(m, top), base = grown == -INFINITY ? 0.f : grown * a.scale;
+        const float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d) o[d] *= shrink;
+        l *= shrink;
+        m = grown;
+      }
+      const float base = m == -INFINITY ? 0.f : m * a.scale;
+      uint32_t p[2][8];
+      float sum = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float x = exp2_of(__builtin_fmaf(s[t][r], a.scale, -base));
+          const float y = exp2_of(__builtin_fmaf(s[t][r + 1], a.scale, -base));
+          p[t][r / 2] = T::pack(x, y);
+          sum += x + y;
+        }
+      l += sum;
+      // 16 keys at a time; the lane's are 4 hi..4 hi + 3 and 8 + 4 hi..8 + 4 hi + 3 of them
+      const char* const v_from = v_lds[buf] + (hi * 4 + (n & 15) / 4) * VSTRIDE + ((n >> 4) * 16 + n % 4 * 4) * 2;
+      const auto v_piece = [&](int u, int d) {
+        typedef __attribute__((address_space(3))) s16x4* Lds;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v_from + u * 16 * VSTRIDE + d * 64));
+        const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v_from + (u * 16 + 8) * VSTRIDE + d * 64));
+        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, up);
+        return u32x4{x[0], x[1], y[0], y[1]};
+      };
+      constexpr int AT_ONCE = DTILES < 4 ? DTILES : 4, PARTS = 4 * DTILES / AT_ONCE;
+      static_assert(4 * DTILES % AT_ONCE == 0, "groups of pieces");
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) piece[0][i] = v_piece(i / DTILES, i % DTILES);
+#pragma unroll
+      for (int j = 0; j < PARTS; ++j) {
+        if (j + 1 < PARTS)
+#pragma unroll
+          for (int i = 0; i < AT_ONCE; ++i) {
+            const int x = (j + 1) * AT_ONCE + i;
+            piece[(j + 1) % 2][i] = v_piece(x / DTILES, x % DTILES);
+          }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          const int x = j * AT_ONCE + i;
+          const uint32_t* w = p[x / DTILES / 2] + x / DTILES % 2 * 4;
+          o[x % DTILES] = T::mfma(piece[j % 2][i], u32x4{w[0], w[1], w[2], w[3]}, o[x % DTILES]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    const int32_t steps = a.num_pages > 0 ? (item.key_end - item.key_begin + kStep - 1) / kStep : 0;
+    uint64_t present = 0;
+    if (steps > 0) {
+      present = fetch(item.key_begin, 0);
+      stage(0, item.key_begin, present);
+    }
+    for (int32_t i = 0; i < steps; ++i) {
+      const int32_t k0 = item.key_begin + i * kStep;
+      __syncthreads();  // the step is staged, and the other buffer has been read
+      const uint64_t now = present;
+      if (i + 1 < steps) present = fetch(k0 + kStep, i + 1);
+      if (most > k0) work(i & 1, k0, now);
+      if (i + 1 < steps) stage(i + 1 & 1, k0 + kStep, present);
+    }
+    __syncthreads();  // (left_out is complete, and the buffers are free)
+    if (left_out) {  // as above
+      int32_t zero = 0;
+      asm volatile("" : "+v"(zero));
+      const int32_t from = item.key_begin + max(tile_least - item.key_begin, 0) / kStep * kStep;
+#pragma unroll 1
+      for (int32_t key = from; key < item.key_end; ++key) {
+        const int64_t off = key_offset(a, item.table, key, item.key_end);
+        if (off < 0 || key >= limit) continue;
+        const char* row = heads + a.plane + off + hi * 8 + zero;
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (d * 32 + i * 8 + hi * 4 < D) {
+              const f32x4 x = infinite_part<T>(*reinterpret_cast<const u32x2*>(row + d * 64 + i * 16));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][i * 4 + e] += x[e];
+            }
+      }
+    }
+    l += __shfl_xor(l, 32);
+    const float base = m == -INFINITY ? 0.f : m * a.scale;
+    const float inv = l == 0 ? 0.f : 1.f / l, lse2 = l == 0 ? -INFINITY : base + __log2f(l);
+    if (my_row < item.rows) {
+      if (item.slot >= 0) {
+        const int64_t row = ((int64_t)item.slot * a.kv_heads + h) * kWide + my_row;
+        if (hi == 0) a.partial_lse[1][row] = lse2;
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int32_t c = d * 32 + i * 8 + hi * 4;
+            if (REACH != kGroupsFull && c >= D) continue;
+            *reinterpret_cast<f32x4*>(a.partial[1] + row * D + c) =
+                f32x4{o[d][i * 4] * inv, o[d][i * 4 + 1] * inv, o[d][i * 4 + 2] * inv, o[d][i * 4 + 3] * inv};
+          }
+      } else {
+        const int64_t row = ((int64_t)token * a.kv_heads + h) * a.group + g;
+        if (a.lse && hi == 0) a.lse[row] = lse2 * kLn2;
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int32_t c = d * 32 + i * 8 + hi * 4;
+            if (REACH != kGroupsFull && c >= D) continue;
+            *reinterpret_cast<u32x2*>(a.out + (row * D + c) * 2) =
+                u32x2{T::pack(o[d][i * 4] * inv, o[d][i * 4 + 1] * inv), T::pack(o[d][i * 4 + 2] * inv, o[d][i * 4 + 3] * inv)};
+          }
+      }
+    }
+    __syncthreads();  // before the next item
+  }
+}
+
+// Joins a row's partials: weights exp2(lse_c - lse). A row without any is zero, its lse -inf. An entry of several rows,
+// of few parts each, takes a wavefront a row; one of a single row of many parts a workgroup, the parts over the eight halves
+// of its wavefronts.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
-  const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ f32x4 sums[8][64];
+  const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = threadIdx.x >> 5, column = threadIdx.x & 31;
   const int32_t num_entries = a.l.header->entries, shared_chunks = a.l.header->shared_chunks;
+  const bool shared_wide = a.l.header->shared_wide;
   const int32_t D = a.head_dim;
   for (int32_t at = blockIdx.x; at < num_entries * a.kv_heads; at += gridDim.x) {
     const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
     const Entry e = a.l.entries[it];
     const int32_t parts = e.chunks + (e.shared_row0 >= 0 ? shared_chunks : 0);
-    for (int32_t r = wave; r < e.rows; r += kWaves) {
-      const int32_t shared_row = e.shared_row0 + r;
+    const bool many = parts > kManyParts;
+    const int32_t own_tile = e.wide ? kWide : kTile, shared_tile = shared_wide ? kWide : kTile;
+    for (int32_t r = many ? 0 : wave; r < e.rows; r += many ? 1 : kWaves) {
+      const int32_t row = e.row0 + r, in_tile = row % own_tile;
+      const int32_t shared_row = e.shared_row0 + r, shared_slot = shared_row / shared_tile * shared_chunks - e.chunks;
       const auto row_of = [&](int32_t c) {  // of part c
-        const bool own = c < e.chunks;
-        const int32_t slot = own ? e.slot + c : shared_row / kTile * shared_chunks + c - e.chunks;
-        return ((int64_t)slot * a.kv_heads + h) * kTile + (own ? r : shared_row % kTile);
+        return c < e.chunks ? ((int64_t)(e.slot + c) * a.kv_heads + h) * own_tile + in_tile
+                            : ((int64_t)(shared_slot + c) * a.kv_heads + h) * shared_tile + shared_row % shared_tile;
       };
+      const auto lse_of = [&](int32_t c) { return a.partial_lse[c < e.chunks ? e.wide : shared_wide][row_of(c)]; };
       float top = -INFINITY;
-      for (int32_t c = lane; c < parts; c += 64) top = fmaxf(top, a.partial_lse[row_of(c)]);
+      for (int32_t c = lane; c < parts; c += 64) top = fmaxf(top, lse_of(c));
       for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
       const float base = top == -INFINITY ? 0.f : top;
       float total = 0;
-      for (int32_t c = lane; c < parts; c += 64) total += exp2_of(a.partial_lse[row_of(c)] - base);
+      for (int32_t c = lane; c < parts; c += 64) total += exp2_of(lse_of(c) - base);
       for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
       const float inv = total == 0 ? 0.f : 1.f / total;
-      const int32_t row = e.row0 + r, i = row / a.group, g = row - i * a.group;
+      const int32_t i = row / a.group, g = row - i * a.group;
       const int64_t out_row = ((int64_t)(e.q_begin + i) * a.kv_heads + h) * a.group + g;
-      if (a.lse && lane == 0) a.lse[out_row] = (total == 0 ? -INFINITY : base + __log2f(total)) * kLn2;
-      for (int32_t d = lane * 4; d < D; d += 256) {
-        f32x4 x = {};
-        for (int32_t c = 0; c < parts; ++c) {
-          const int64_t from = row_of(c);
-          const float weight = exp2_of(a.partial_lse[from] - base);
-          x += *reinterpret_cast<const f32x4*>(a.partial + from * D + d) * weight;
-        }
+      if (a.lse && (many ? threadIdx.x : lane) == 0) a.lse[out_row] = (total == 0 ? -INFINITY : base + __log2f(total)) * kLn2;
+      const auto put = [&](int32_t d, f32x4 x) {
         x *= inv;
-        const u32x2 two = {T::pack(x[0], x[1]), T::pack(x[2], x[3])};
-        *reinterpret_cast<u32x2*>(a.out + (out_row * D + d) * 2) = two;
+        *reinterpret_cast<u32x2*>(a.out + (out_row * D + d) * 2) = u32x2{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
+      };
+      const auto sum_of = [&](int32_t d, int32_t from, int32_t step) {
+        f32x4 x = {};
+#pragma unroll 4
+        for (int32_t c = from; c < parts; c += step) {
+          const float weight = exp2_of(lse_of(c) - base);
+          x += *reinterpret_cast<const f32x4*>(a.partial[c < e.chunks ? e.wide : shared_wide] + row_of(c) * D + d) * weight;
+        }
+        return x;
+      };
+      if (!many) {
+        for (int32_t d = lane * 4; d < D; d += 256) put(d, sum_of(d, 0, 1));
+      } else {
+        for (int32_t d = column; d < D / 4; d += 32) sums[half][d] = sum_of(d * 4, half, 8);
+        __syncthreads();
+        for (int32_t d = threadIdx.x; d < D / 4; d += kThreads) {
+          f32x4 x = {};
+#pragma unroll
+          for (int w = 0; w < 8; ++w) x += sums[w][d];
+          put(d * 4, x);
+        }
+        __syncthreads();
       }
     }
   }
@@ -698,9 +1036,10 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// The sizes that follow from the capacities
+// The sizes that follow from the capacities: of narrow and of wide items
 struct Sizes {
-  int64_t target, max_items, max_entries, max_slots;
+  int64_t target[2], max_items[2], max_slots[2], max_entries;
+  bool wide;  // are there wide items at all?
 };
 
 }  // namespace
@@ -710,6 +1049,7 @@ extern "C" {
 struct kvc_attention_plan {
   const int32_t *qo_indptr, *kv_indices, *kv_indptr, *kv_last_page_len;
   int64_t batch_size, num_tokens, num_kv_indices, num_heads, num_kv_heads, head_dim, page_size, shared_pages;
+  int64_t narrow_rows;
   int dtype;
   float scale;
   Sizes n;
@@ -721,9 +1061,11 @@ struct kvc_attention_plan {
 
 namespace {
 
-// Items of a step: workgroups that fill the card four times, so that the last of them to end is a small part of it
-constexpr int64_t kWorkgroups = 1024;
-constexpr int32_t kMinChunk = 256;
+// Workgroups that a step's items of a kind make, about: enough that the last to end is a small part of the time
+constexpr int64_t kWorkgroups[2] = {1024, 512};
+constexpr int32_t kMinChunk[2] = {256, 512};  // keys
+constexpr int64_t kNarrowRows = 32;           // of a request; with more it is cut into wide items
+constexpr int64_t kNarrowSharedRows = 64;     // of all sharing requests
 
 Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
   Layout l;
@@ -739,40 +1081,49 @@ Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
   l.offsets = (int32_t*)take(p.batch_size * 16);
   l.limits = (int32_t*)take(p.num_tokens * 4);
   l.shared_tokens = (int32_t*)take(p.num_tokens * 4);
-  l.items = (Item*)take(p.n.max_items * sizeof(Item));
+  for (int k = 0; k < 2; ++k) l.items[k] = (Item*)take(p.n.max_items[k] * sizeof(Item));
   l.entries = (Entry*)take(p.n.max_entries * sizeof(Entry));
   if (bytes) *bytes = at;
   return l;
 }
 
-// Row tiles are at most rows / 16 and one more for every request that has tokens; cut into items of a target-th of all
-// keys each, there are at most the target and one more for every tile. Without a shared prefix only tiles of more than one
-// item need a slot, which are at most twice the target.
+// Row tiles are at most rows / tile and one more for every request that has tokens; cut into items of a target-th of all
+// keys each, there are at most the target and one more for every tile, those of the shared prefix among them. Without a shared
+// prefix only tiles of more than one item need slots, which are at most twice the target.
 Sizes sizes_of(const kvc_attention_plan& p) {
   Sizes n;
-  const int64_t group = p.num_kv_heads ? p.num_heads / p.num_kv_heads : 1;
-  const int64_t tiles = p.num_tokens * group / kTile + std::min(p.batch_size, p.num_tokens);
-  n.target = std::max<int64_t>(1, kWorkgroups / std::max<int64_t>(1, p.num_kv_heads));
-  const int64_t shared_tiles = p.shared_pages > 0 ? round_up(p.num_tokens * group, kTile) / kTile : 0;
-  n.max_items = n.target + tiles + (p.shared_pages > 0 ? n.target + shared_tiles : 0);
-  n.max_entries = tiles;
-  n.max_slots = p.shared_pages > 0 ? n.max_items : 2 * n.target;
+  const int64_t rows = p.num_tokens * (p.num_heads / p.num_kv_heads);
+  n.wide = rows > p.narrow_rows || (p.shared_pages > 0 && rows > kNarrowSharedRows);
+  for (int k = 0; k < 2; ++k) {
+    const int64_t tile = k ? kWide : kTile, tiles = rows / tile + std::min(p.batch_size, p.num_tokens);
+    n.target[k] = std::max<int64_t>(1, kWorkgroups[k] / p.num_kv_heads);
+    n.max_items[k] = k && !n.wide ? 0 : n.target[k] + tiles + (p.shared_pages > 0 ? rows / tile + 1 : 0);
+    n.max_slots[k] = k && !n.wide ? 0 : p.shared_pages > 0 ? n.max_items[k] : 2 * n.target[k];
+  }
+  n.max_entries = rows;
   return n;
 }
 
 template <typename T, int DP>
-void launch_rows(const AttendArgs& a, unsigned grid, hipStream_t s) {
-  if (a.page_size % 16) kvc::launch((attend_rows_kernel<T, DP, kAnyPage>), dim3(grid), dim3(kThreads), 0, s, a);
-  else if (a.head_dim != DP) kvc::launch((attend_rows_kernel<T, DP, kGroups>), dim3(grid), dim3(kThreads), 0, s, a);
-  else kvc::launch((attend_rows_kernel<T, DP, kGroupsFull>), dim3(grid), dim3(kThreads), 0, s, a);
+void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
+  const dim3 block(kThreads);
+  // (a workgroup takes further items where there are more than the grid has places for)
+  const auto grid = [&](int64_t items) { return dim3((unsigned)std::min<int64_t>(items * p.num_kv_heads, 1 << 14)); };
+  const bool any = a.page_size % 16 != 0, full = a.head_dim == DP;
+  if (any) kvc::launch((attend_rows_kernel<T, DP, kAnyPage>), grid(p.n.max_items[0]), block, 0, s, a);
+  else if (!full) kvc::launch((attend_rows_kernel<T, DP, kGroups>), grid(p.n.max_items[0]), block, 0, s, a);
+  else kvc::launch((attend_rows_kernel<T, DP, kGroupsFull>), grid(p.n.max_items[0]), block, 0, s, a);
+  if (!p.n.wide) return;
+  if (any) kvc::launch((attend_tiles_kernel<T, DP, kAnyPage>), grid(p.n.max_items[1]), block, 0, s, a);
+  else if (!full) kvc::launch((attend_tiles_kernel<T, DP, kGroups>), grid(p.n.max_items[1]), block, 0, s, a);
+  else kvc::launch((attend_tiles_kernel<T, DP, kGroupsFull>), grid(p.n.max_items[1]), block, 0, s, a);
 }
 template <typename T>
 void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
-  const unsigned grid = (unsigned)std::min<int64_t>(p.n.max_items * p.num_kv_heads, 1 << 14);
-  if (p.head_dim <= 64) launch_rows<T, 64>(a, grid, s);
-  else if (p.head_dim <= 96) launch_rows<T, 96>(a, grid, s);
-  else if (p.head_dim <= 128) launch_rows<T, 128>(a, grid, s);
-  else launch_rows<T, 256>(a, grid, s);
+  if (p.head_dim <= 64) launch_attend<T, 64>(a, p, s);
+  else if (p.head_dim <= 96) launch_attend<T, 96>(a, p, s);
+  else if (p.head_dim <= 128) launch_attend<T, 128>(a, p, s);
+  else launch_attend<T, 256>(a, p, s);
   const unsigned joins = (unsigned)std::min<int64_t>(p.n.max_entries * p.num_kv_heads, 2048);
   kvc::launch((attend_join_kernel<T>), dim3(joins), dim3(kThreads), 0, s, a);
 }
@@ -784,14 +1135,14 @@ extern "C" {
 int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* kv_indptr,
                               const int32_t* kv_last_page_len, int64_t batch_size, int64_t num_tokens,
                               int64_t num_kv_indices, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
-                              int64_t page_size, int64_t shared_pages, float sm_scale, int dtype,
+                              int64_t page_size, int64_t max_q_len, int64_t shared_pages, float sm_scale, int dtype,
                               kvc_attention_plan** out) {
   constexpr const char* fn = "kvc_attention_plan_create";
   if (!out) return fail(KVC_ERR_INVALID_ARG, "%s: null out", fn);
   *out = nullptr;
   if (dtype != KVC_DTYPE_BF16 && dtype != KVC_DTYPE_F16)
     return fail(KVC_ERR_UNSUPPORTED, "%s: dtype %d (need bf16 or f16)", fn, dtype);
-  if (batch_size < 0 || num_tokens < 0 || num_kv_indices < 0 || shared_pages < 0)
+  if (batch_size < 0 || num_tokens < 0 || num_kv_indices < 0 || shared_pages < 0 || max_q_len < 0)
     return fail(KVC_ERR_INVALID_ARG, "%s: negative size", fn);
   if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads)
     return fail(KVC_ERR_INVALID_ARG, "%s: %lld query heads are no multiple of %lld key heads", fn, (long long)num_heads,
@@ -811,11 +1162,14 @@ int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indice
   if (shared_pages > num_kv_indices || shared_pages * page_size > (1 << 30)) shared_pages = 0;
   kvc_attention_plan* p = new (std::nothrow) kvc_attention_plan{
       qo_indptr, kv_indices, kv_indptr, kv_last_page_len, batch_size, num_tokens, num_kv_indices, num_heads, num_kv_heads,
-      head_dim, page_size, shared_pages, dtype, sm_scale, {}, 0, 0, nullptr};
+      head_dim, page_size, shared_pages, kNarrowRows, dtype, sm_scale, {}, 0, 0, nullptr};
   if (!p) return fail(KVC_ERR_HIP, "%s: out of host memory", fn);
+  // said to have few tokens each: every request in narrow items, whatever it has, and no launch for the others
+  if (max_q_len > 0 && max_q_len * (num_heads / num_kv_heads) <= kNarrowRows) p->narrow_rows = INT32_MAX;
   p->n = sizes_of(*p);
   layout_of(*p, nullptr, &p->plan_bytes);
-  p->workspace_bytes = round_up(p->n.max_slots * num_kv_heads * kTile * (head_dim + 1) * 4, 256);
+  for (int k = 0; k < 2; ++k) p->workspace_bytes += p->n.max_slots[k] * num_kv_heads * (k ? kWide : kTile) * (head_dim + 1) * 4;
+  p->workspace_bytes = round_up(std::max<int64_t>(p->workspace_bytes, 1), 256);
   *out = p;
   return KVC_OK;
 }
@@ -836,8 +1190,9 @@ int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buf
   if (plan->batch_size == 0 || plan->num_tokens == 0) return KVC_OK;
   PlanArgs a{plan->qo_indptr, plan->kv_indices, plan->kv_indptr, plan->kv_last_page_len, (int32_t)plan->batch_size,
              (int32_t)plan->num_tokens, (int32_t)plan->num_kv_indices, (int32_t)plan->page_size,
-             (int32_t)plan->shared_pages, (int32_t)(plan->num_heads / plan->num_kv_heads), (int32_t)plan->n.target,
-             kMinChunk, (int32_t)plan->n.max_items, (int32_t)plan->n.max_entries,
+             (int32_t)plan->shared_pages, (int32_t)(plan->num_heads / plan->num_kv_heads), (int32_t)plan->narrow_rows,
+             (int32_t)kNarrowSharedRows, {(int32_t)plan->n.target[0], (int32_t)plan->n.target[1]}, {kMinChunk[0], kMinChunk[1]},
+             {(int32_t)plan->n.max_items[0], (int32_t)plan->n.max_items[1]}, (int32_t)plan->n.max_entries,
              layout_of(*plan, plan->buffer, nullptr)};
   hipStream_t s = (hipStream_t)stream;
   kvc::launch(attend_requests_kernel, dim3((unsigned)plan->batch_size), dim3(256), 0, s, a);
@@ -871,8 +1226,16 @@ int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query, in
   a.kv_indices = plan->kv_indices;
   a.out = (char*)out;
   a.lse = lse;
-  a.partial = (float*)workspace;
-  a.partial_lse = a.partial + plan->n.max_slots * plan->num_kv_heads * kTile * plan->head_dim;
+  float* at = (float*)workspace;
+  for (int k = 0; k < 2; ++k) {
+    const int64_t rows = plan->n.max_slots[k] * plan->num_kv_heads * (k ? kWide : kTile);
+    a.partial[k] = at;
+    at += rows * plan->head_dim;
+  }
+  for (int k = 0; k < 2; ++k) {
+    a.partial_lse[k] = at;
+    at += plan->n.max_slots[k] * plan->num_kv_heads * (k ? kWide : kTile);
+  }
   a.q_stride = q_token_stride * 2;
   a.page_stride = (uint32_t)(page_stride * 2);
   a.row_stride = (uint32_t)(row * 2);
