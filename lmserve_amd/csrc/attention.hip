@@ -39,47 +39,68 @@ constexpr int kTile = 16;          // rows of a narrow item
 constexpr int kWide = 32 * kWaves; // rows of a wide item: 32 to a wavefront
 constexpr int kBlock = 32;         // keys that a wavefront takes at once of a narrow item
 constexpr int kStep = 64;          // keys that a workgroup takes at once of a wide item
-constexpr int kManyParts = 8;      // a row of more partials is joined by a workgroup
+constexpr int kAhead = 3;          // pieces of a wide item's K and V that are read from LDS ahead of their product
+constexpr int kMaxGroups = 1024;    // workgroups of a key head
+// In keys: what a narrow tile costs beside its own, a workgroup's least share, the least part of a tile
+__device__ constexpr int kTileWork = 64, kMinShare = 512, kMinPart = 256;
+// the least range of a wide tile; what an item costs beside its keys, and what one that leaves a partial does
+__device__ constexpr int kMinChunk = 512, kWideTileWork = 128, kWidePartWork = 384;
+constexpr int kManyParts = 16;     // a row of more partials is joined by a workgroup
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // ---- the step's layout ---------------------------------------------------------------------------------------------
+// Row tiles are of 16 rows (narrow, of requests of few rows) or of 128 (wide), each over the keys that its last row sees.
+//   Narrow tiles lie end to end on a line of work, measured in keys, that is cut into as many equal shares as there are
+//   workgroups for a key head: a workgroup takes the pieces of tiles in its share, so that every one has the same work
+//   whatever the lengths are. Of a share only the first and the last piece can be parts of a tile. A cut that would leave
+//   a sliver moves to the tile's end.
+//   Wide tiles of a request read the same keys: they are cut at the same keys, and the tiles of one range of keys are
+//   neighbours in the list and run on one XCD, whose L2 the range then comes to once. (Shares of a line put them at
+//   different keys: 2048 new tokens behind contexts of 1024 to 32768 took 1638 us, 900 in this order.)
+// A part of a tile leaves its rows' unfinished result in a slot of the workspace, and the parts are joined at the end.
 struct Request {  // 16 bytes
   int32_t q_begin, n, len, table;  // first token, tokens, keys, first entry of its block table
 };
-struct Item {  // 32 bytes
+struct Item {  // 32 bytes: a tile or a part of one
   int32_t q_begin;  // first token of the request; -1: the rows of all sharing requests, through shared_tokens
   int32_t row0, rows, table, key_begin, key_end;
-  int32_t slot;     // where its partial goes; -1: the only item of its rows
+  int32_t slot;     // of its partial; -1: the whole tile
   int32_t pad;
 };
-struct Entry {  // 32 bytes: rows of one tile that are joined from partials (or have no keys at all)
-  int32_t q_begin, row0, rows, slot, chunks;
+struct Parts {  // 16 bytes: of a tile: the slot of the first, and of the c-th further one next + c * step
+  int32_t slot, next, step, count;
+};
+struct Entry {  // 32 bytes: rows of one tile that are joined from partials
+  int32_t q_begin, row0;
+  int16_t rows, many;   // (a single one, of many parts)
   int32_t shared_row0;  // the first row among those of the sharing requests, or -1
-  int32_t wide, pad;
+  Parts parts;
+};
+struct Range {
+  int32_t begin, end;
 };
 struct Header {
-  int32_t items[2];  // narrow, wide
-  int32_t entries, shared_chunks, shared_wide;
+  int32_t wide_items, narrow_entries, wide_entries, shared_wide;  // (narrow entries from the front, wide ones from the back)
 };
 
 struct Layout {  // the plan's device buffer
   Header* header;
   Request* requests;
   int32_t* shares;         // [B] 1: its leading pages are the shared ones
-  int32_t* offsets;        // [B][4] first item and slot of its kind, entry, shared token
   int32_t* limits;         // [T] keys that a token sees
   int32_t* shared_tokens;  // [T]
-  Item* items[2];
+  Range* ranges;           // [groups] narrow items of a workgroup
+  Item* items[2];          // narrow: tile t's part in workgroup w at t + w: those of a workgroup lie side by side
+  Parts* shared_parts;     // of the tiles of the sharing requests' rows
   Entry* entries;
 };
 
 struct PlanArgs {
   const int32_t *qo_indptr, *kv_indices, *kv_indptr, *kv_last_page_len;
   int32_t batch_size, num_tokens, num_kv_indices, page_size, shared_pages, group;
-  int32_t narrow_rows, narrow_shared_rows;  // the most rows of a request, and of all sharing ones, for narrow items
-  int32_t target[2];     // items that a step is cut into, about
-  int32_t min_chunk[2];  // keys
+  int32_t narrow_rows, narrow_shared_rows;  // the most rows of a request, and of all sharing ones, for narrow tiles
+  int32_t groups, residents;                // of a key head: workgroups for narrow tiles, wide tiles on the card at a time
   int32_t max_items[2], max_entries;
   Layout l;
 };
@@ -143,150 +164,267 @@ __global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
   }
 }
 
-struct Counts {
-  int32_t v[6];  // items and slots of either kind, entries, shared tokens
-};
 __device__ __forceinline__ int32_t ceil_div(int32_t x, int32_t y) { return (x + y - 1) / y; }
 
+// A request's tiles
+struct Tiles {
+  int64_t at;               // narrow: where the first begins on the line of work
+  int32_t q_begin, n, len, table;
+  int32_t begin;            // first key of its own
+  int32_t tiles, first;     // and the first's place in its list
+  int32_t first_slot;       // wide
+  int32_t shared_token0;    // its first token among the sharing ones, or -1
+  bool wide;
+  __device__ __forceinline__ int32_t rows_of_tile() const { return wide ? kWide : kTile; }
+  // Work of the narrow tiles before the i-th: each sees tile / group keys more than the one before, and costs something by itself
+  __device__ __forceinline__ int64_t before(int64_t i, int32_t group) const {
+    const int32_t keys = min(len, len - n + ceil_div(kTile, group)) - begin;
+    return i * ((keys > 0 ? keys : 0) + kTileWork) + i * (i - 1) / 2 * kTile / group;
+  }
+  // Ranges of keys that wide tiles are cut into where none is to be longer than `chunk`
+  __device__ __forceinline__ int32_t chunks(int32_t chunk) const { return max(ceil_div(len, chunk), 1); }
+};
+__device__ __forceinline__ Tiles tiles_of(const PlanArgs& a, int32_t b) {
+  const Request r = a.l.requests[b];
+  Tiles t = {};
+  t.q_begin = r.q_begin;
+  t.n = r.n;
+  t.len = r.len;
+  t.table = r.table;
+  t.wide = r.n * a.group > a.narrow_rows;
+  t.shared_token0 = a.l.shares[b] ? 0 : -1;
+  t.begin = a.l.shares[b] ? min(a.shared_pages * a.page_size, r.len) : 0;
+  t.tiles = ceil_div(r.n * a.group, t.rows_of_tile());
+  return t;
+}
+
+// The parts of a narrow tile at `at`, `work` long, when the line is cut every `share`
+struct Cuts {
+  int32_t group, count;  // the first part's workgroup, and how many parts there are
+};
+__device__ __forceinline__ Cuts cuts_of(const PlanArgs& a, int64_t at, int64_t work, int64_t share) {
+  const int64_t sliver = min(share / 2, (int64_t)kMinPart);
+  // (the line may end within a sliver of the last share's end)
+  const int64_t first = min((at + sliver - 1) / share, (int64_t)a.groups - 1), last = (at + work - sliver) / share;
+  return {(int32_t)first, (int32_t)(last > first ? last - first : 0) + 1};
+}
 // Rows of an entry: one of many parts is by itself
 __device__ __forceinline__ int32_t joined_rows(int32_t parts) { return parts > kManyParts ? 1 : kTile; }
-
-struct Cut {
-  int32_t tiles, chunks, begin, tile;  // row tiles, key ranges of each, first key of its own, rows of a tile
-  bool wide;
-};
-__device__ __forceinline__ Cut cut_of(const PlanArgs& a, const Request& r, bool shares, int32_t narrow_chunk, int32_t wide_chunk) {
-  Cut c;
-  c.wide = r.n * a.group > a.narrow_rows;
-  c.tile = c.wide ? kWide : kTile;
-  c.begin = shares ? min(a.shared_pages * a.page_size, r.len) : 0;
-  c.tiles = ceil_div(r.n * a.group, c.tile);
-  c.chunks = ceil_div(r.len - c.begin, c.wide ? wide_chunk : narrow_chunk);
-  return c;
-}
 __device__ __forceinline__ int32_t round_up(int32_t x, int32_t to) { return ceil_div(x, to) * to; }
 
-// One workgroup: the keys of an item, from all the work there is; how many items, slots and entries come before each
-// request's, by a scan; the lists. A request of few tokens is one tile and takes a few lines of its own, so a wavefront
-// does a request.
+// One workgroup: the share and the wide tiles' ranges, from all the work there is; where each request's tiles begin, by a scan;
+// the lists.
 __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
-  __shared__ unsigned long long total_work[2], total_shared;
-  __shared__ int32_t wave_sums[16][6], carry[6], some_request;
+  constexpr int SUMS = 4;  // narrow tiles, wide items, wide slots, sharing tokens
+  __shared__ unsigned long long narrow_work, wide_work, best;
+  __shared__ int64_t wave_work[16], carry_work;
+  __shared__ int32_t wave_sums[16][SUMS], carry[SUMS], shared_tokens, some_request, narrow_entries, wide_entries, longest;
+  __shared__ int32_t first_item[kMaxGroups], last_item[kMaxGroups];
+  __shared__ Tiles cached[1024];
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid == 0) {
-    total_work[0] = total_work[1] = total_shared = 0;
+    narrow_work = wide_work = 0;
+    best = ~0ull;
+    shared_tokens = narrow_entries = wide_entries = longest = 0;
     some_request = INT32_MAX;
+  }
+  for (int32_t w = tid; w < a.groups; w += 1024) {
+    first_item[w] = INT32_MAX;
+    last_item[w] = -1;
   }
   __syncthreads();
   for (int32_t b = tid; b < a.batch_size; b += 1024) {
-    const Request r = a.l.requests[b];
-    const bool sh = a.l.shares[b];
-    const Cut c = cut_of(a, r, sh, 1 << 30, 1 << 30);
-    if (c.tiles) atomicAdd(&total_work[c.wide], (unsigned long long)((int64_t)c.tiles * (r.len - c.begin)));
-    if (sh) {
-      atomicAdd(&total_shared, (unsigned long long)r.n);
+    const Tiles t = tiles_of(a, b);
+    if (t.tiles && !t.wide) atomicAdd(&narrow_work, (unsigned long long)t.before(t.tiles, a.group));
+    if (t.wide) {
+      atomicAdd(&wide_work, (unsigned long long)t.tiles * t.len);
+      atomicMax(&longest, t.len);
+    }
+    if (t.shared_token0 >= 0) {
+      atomicAdd(&shared_tokens, t.n);
       atomicMin(&some_request, b);
     }
   }
   __syncthreads();
-  const int32_t shared_rows = (int32_t)total_shared * a.group, shared_len = a.shared_pages * a.page_size;
+  const int32_t shared_rows = shared_tokens * a.group, shared_len = a.shared_pages * a.page_size;
   const bool shared_wide = shared_rows > a.narrow_shared_rows;
   const int32_t shared_tile = shared_wide ? kWide : kTile, shared_tiles = ceil_div(shared_rows, shared_tile);
-  int32_t chunk[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int64_t work = (int64_t)total_work[k] + (shared_wide == (k == 1) ? (int64_t)shared_tiles * shared_len : 0);
-    const int64_t per = (work + a.target[k] - 1) / a.target[k];
-    chunk[k] = round_up((int32_t)(per < a.min_chunk[k] ? a.min_chunk[k] : per < (1 << 30) ? per : 1 << 30), kStep);
+  const int64_t shared_work = shared_len + kTileWork;  // of a narrow tile
+  const int64_t share = max(((int64_t)narrow_work + (shared_wide ? 0 : shared_tiles * shared_work) + a.groups - 1) / a.groups, (int64_t)kMinShare);
+
+  // The wide tiles' ranges: of lengths that make from a 16th of a round of the card to 4 of them, the one that ends soonest.
+  // Every round lasts as long as a range, and what an item costs beside its keys, more so where it leaves a partial.
+  int32_t chunk = 1 << 30;
+  const int64_t all_wide = (int64_t)wide_work + (shared_wide ? (int64_t)shared_tiles * shared_len : 0);
+  if (all_wide) {
+    const int32_t most = max(longest, shared_wide ? shared_len : 0);
+    const auto chunk_of = [&](int32_t x) {
+      const int64_t keys = (all_wide * 16 + (int64_t)a.residents * (x + 1) - 1) / ((int64_t)a.residents * (x + 1));
+      return round_up((int32_t)(keys < kMinChunk ? kMinChunk : keys < (1 << 30) ? keys : 1 << 30), kStep);
+    };
+    for (int32_t x = wave; x < 64; x += 16) {
+      const int32_t keys = chunk_of(x);
+      int32_t items = 0;
+      for (int32_t b = lane; b < a.batch_size; b += 64) {
+        const Tiles t = tiles_of(a, b);
+        if (t.wide) items += t.tiles * t.chunks(keys);
+      }
+      for (int d = 32; d; d >>= 1) items += __shfl_xor(items, d);
+      if (shared_wide) items += shared_tiles * ceil_div(shared_len, keys);
+      const int64_t each = min(keys, most) + (keys < most ? kWidePartWork : kWideTileWork);
+      const int64_t cost = (int64_t)ceil_div(items, a.residents) * each;
+      if (lane == 0) atomicMin(&best, (unsigned long long)cost << 8 | (unsigned)x);
+    }
+    __syncthreads();
+    chunk = chunk_of((int32_t)(best & 255));
   }
-  const int32_t shared_chunks = shared_rows ? ceil_div(shared_len, chunk[shared_wide]) : 0;
-  const int32_t shared_items = shared_tiles * shared_chunks;
-  if (tid < 6) carry[tid] = tid < 4 && tid / 2 == shared_wide ? shared_items : 0;
+  const int32_t shared_chunks = shared_rows && shared_wide ? ceil_div(shared_len, chunk) : 0, shared_items = shared_tiles * shared_chunks;
+  if (tid == 0) {
+    carry_work = shared_wide ? 0 : shared_tiles * shared_work;
+    carry[0] = shared_wide ? 0 : shared_tiles;
+    carry[1] = carry[2] = shared_items;
+    carry[3] = 0;
+  }
   __syncthreads();
+
+  // a narrow item, and whose it is
+  const auto put = [&](int32_t tile, int32_t group, const Item& item) {
+    const int32_t at = tile + group;
+    if (at >= a.max_items[0] || group >= a.groups) return;
+    a.l.items[0][at] = item;
+    atomicMin(&first_item[group], at);
+    atomicMax(&last_item[group], at);
+  };
+  // the first key of a narrow tile's c-th part: the share of its work before the cut, in whole blocks
+  const auto cut_key = [&](int64_t at, int64_t work, const Cuts& p, int32_t c, int32_t begin, int32_t end) {
+    if (c == 0) return begin;
+    if (c == p.count) return end;
+    const int64_t before = ((int64_t)(p.group + c) * share - at) * (end - begin) / work;
+    return begin + min((int32_t)((before + kStep / 2) / kStep * kStep), end - begin);
+  };
+
+  if (shared_rows) {
+    const int32_t table = a.l.requests[some_request].table;
+    const int32_t each = shared_wide ? round_up(ceil_div(shared_len, shared_chunks), kStep) : 0;
+    for (int32_t i = tid; i < shared_tiles; i += 1024) {
+      const int32_t row0 = i * shared_tile, rows = min(shared_tile, shared_rows - row0);
+      if (shared_wide) {
+        a.l.shared_parts[i] = {i, i, shared_tiles, ceil_div(shared_len, each)};
+      } else {
+        const Cuts p = cuts_of(a, i * shared_work, shared_work, share);
+        a.l.shared_parts[i] = {2 * a.groups + i, 2 * p.group, 2, p.count};
+        for (int32_t c = 0; c < p.count; ++c)
+          put(i, p.group + c,
+              {-1, row0, rows, table, cut_key(i * shared_work, shared_work, p, c, 0, shared_len),
+               cut_key(i * shared_work, shared_work, p, c + 1, 0, shared_len), c ? 2 * (p.group + c) : 2 * a.groups + i, 0});
+      }
+    }
+    for (int32_t i = tid; i < shared_items && i < a.max_items[1]; i += 1024) {
+      const int32_t c = i / shared_tiles, row0 = (i - c * shared_tiles) * kWide, from = min(c * each, shared_len);
+      a.l.items[1][i] = {-1, row0, min(kWide, shared_rows - row0), table, from, min(from + each, shared_len), i, 0};
+    }
+  }
+
   for (int32_t b0 = 0; b0 < a.batch_size; b0 += 1024) {
     const int32_t b = b0 + tid;
-    Counts n = {};
-    bool wide = false;
-    if (b < a.batch_size) {
-      const Request r = a.l.requests[b];
-      const bool sh = a.l.shares[b];
-      const Cut c = cut_of(a, r, sh, chunk[0], chunk[1]);
-      wide = c.wide;
-      const int32_t items = c.tiles * c.chunks, slots = sh || c.chunks > 1 ? items : 0;
-      n.v[0] = wide ? 0 : items;
-      n.v[1] = wide ? 0 : slots;
-      n.v[2] = wide ? items : 0;
-      n.v[3] = wide ? slots : 0;
-      n.v[4] = sh || c.chunks != 1 ? ceil_div(r.n * a.group, joined_rows(c.chunks + (sh ? shared_chunks : 0))) : 0;
-      n.v[5] = sh ? r.n : 0;
-    }
-    Counts before = n;  // inclusive, then exclusive
-    for (int d = 1; d < 64; d <<= 1)
+    Tiles t = {};
+    t.shared_token0 = -1;
+    if (b < a.batch_size) t = tiles_of(a, b);
+    const int32_t chunks = t.wide ? t.chunks(chunk) : 0;
+    const int64_t work = t.tiles && !t.wide ? t.before(t.tiles, a.group) : 0;
+    const int32_t sums[SUMS] = {t.wide ? 0 : t.tiles, t.tiles * chunks, chunks > 1 ? t.tiles * chunks : 0, t.shared_token0 >= 0 ? t.n : 0};
+    int64_t work_to = work;  // inclusive
+    int32_t sums_to[SUMS] = {sums[0], sums[1], sums[2], sums[3]};
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t x = __shfl_up((long long)work_to, d);
+      if (lane >= d) work_to += x;
 #pragma unroll
-      for (int i = 0; i < 6; ++i) {
-        const int32_t x = __shfl_up(before.v[i], d);
-        if (lane >= d) before.v[i] += x;
+      for (int i = 0; i < SUMS; ++i) {
+        const int32_t y = __shfl_up(sums_to[i], d);
+        if (lane >= d) sums_to[i] += y;
       }
-    if (lane == 63)
-#pragma unroll
-      for (int i = 0; i < 6; ++i) wave_sums[wave][i] = before.v[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 6; ++i) {
-      int32_t base = carry[i];
-      for (int w = 0; w < wave; ++w) base += wave_sums[w][i];
-      before.v[i] += base - n.v[i];
     }
-    if (b < a.batch_size)
-      *reinterpret_cast<int4*>(a.l.offsets + 4 * b) =
-          make_int4(wide ? before.v[2] : before.v[0], wide ? before.v[3] : before.v[1], before.v[4], before.v[5]);
+    if (lane == 63) {
+      wave_work[wave] = work_to;
+      for (int i = 0; i < SUMS; ++i) wave_sums[wave][i] = sums_to[i];
+    }
     __syncthreads();
-    if (tid == 1023)
+    work_to += carry_work;
+    for (int w = 0; w < wave; ++w) work_to += wave_work[w];
 #pragma unroll
-      for (int i = 0; i < 6; ++i) carry[i] = before.v[i] + n.v[i];
+    for (int i = 0; i < SUMS; ++i) {
+      sums_to[i] += carry[i];
+      for (int w = 0; w < wave; ++w) sums_to[i] += wave_sums[w][i];
+    }
+    t.at = work_to - work;
+    t.first = t.wide ? sums_to[1] - sums[1] : sums_to[0] - sums[0];
+    t.first_slot = sums_to[2] - sums[2];
+    if (t.shared_token0 >= 0) t.shared_token0 = sums_to[3] - sums[3];
+    cached[tid] = t;
     __syncthreads();
-  }
-  if (tid == 0)
-    *a.l.header = {{min(carry[0], a.max_items[0]), min(carry[2], a.max_items[1])}, min(carry[4], a.max_entries), shared_chunks, shared_wide};
+    if (tid == 1023) {
+      carry_work = work_to;
+      for (int i = 0; i < SUMS; ++i) carry[i] = sums_to[i];
+    }
 
-  for (int32_t b = wave; b < a.batch_size; b += 16) {
-    const Request r = a.l.requests[b];
-    const bool sh = a.l.shares[b];
-    const Cut c = cut_of(a, r, sh, chunk[0], chunk[1]);
-    const int4 first = *reinterpret_cast<const int4*>(a.l.offsets + 4 * b);
-    const int32_t rows = r.n * a.group;
-    const bool partial = sh || c.chunks > 1;
-    Item* const items = c.wide ? a.l.items[1] : a.l.items[0];
-    const int32_t max_items = c.wide ? a.max_items[1] : a.max_items[0], unit = c.wide ? kStep : kBlock;
-    for (int32_t i = lane; i < c.tiles * c.chunks; i += 64) {
-      const int32_t tile = i / c.chunks, part = i - tile * c.chunks;
-      const int32_t row0 = tile * c.tile, last_row = min(row0 + c.tile, rows) - 1;
-      const int32_t end = clamp(r.len - r.n + last_row / a.group + 1, c.begin, r.len);  // keys that the tile's last token sees
-      const int32_t each = round_up(ceil_div(end - c.begin, c.chunks), unit);
-      const int32_t from = min(c.begin + part * each, end), to = min(from + each, end);
-      if (first.x + i < max_items)
-        items[first.x + i] = {r.q_begin, row0, last_row + 1 - row0, r.table, from, to, partial ? first.y + i : -1, 0};
+    // A request to a wavefront, its lanes over the tiles, or over the parts where there are few tiles
+    for (int32_t x = wave; x < min(1024, a.batch_size - b0); x += 16) {
+      const Tiles r = cached[x];
+      const int32_t rows = r.n * a.group;
+      const bool sh = r.shared_token0 >= 0;
+      // keys that the tile's last token sees
+      const auto end_of = [&](int32_t last_row) { return clamp(r.len - r.n + last_row / a.group + 1, r.begin, r.len); };
+      if (r.wide) {
+        const int32_t parts = r.chunks(chunk), each = round_up(max(ceil_div(r.len, parts), 1), kStep);
+        for (int32_t i = lane; i < r.tiles * parts; i += 64) {
+          const int32_t c = i / r.tiles, row0 = (i - c * r.tiles) * kWide, last_row = min(row0 + kWide, rows) - 1;
+          const int32_t end = end_of(last_row), from = min(c * each, end), to = min(from + each, end);
+          // (a range that a tile sees nothing of is an item without rows)
+          if (r.first + i < a.max_items[1])
+            a.l.items[1][r.first + i] = {r.q_begin, row0, c && from == to ? 0 : last_row + 1 - row0, r.table, from, to,
+                                         end > each ? r.first_slot + i : -1, 0};
+        }
+        if (parts > 1)
+          for (int32_t i = lane; i < r.tiles; i += 64) {
+            const int32_t row0 = i * kWide, count = ceil_div(end_of(min(row0 + kWide, rows) - 1), each);
+            if (count < 2) continue;
+            const int32_t lines = joined_rows(count), tile_rows = min(kWide, rows - row0);
+            int32_t to = a.max_entries - 1 - atomicAdd(&wide_entries, ceil_div(tile_rows, lines));
+            for (int32_t e = 0; e < tile_rows && to >= 0; e += lines)
+              a.l.entries[to--] = {r.q_begin, row0 + e, (int16_t)min(lines, tile_rows - e), lines == 1, -1,
+                                   {r.first_slot + i, r.first_slot + i, r.tiles, count}};
+          }
+        continue;
+      }
+      const bool by_parts = r.tiles < 8;
+      for (int32_t i = by_parts ? 0 : lane; i < r.tiles; i += by_parts ? 1 : 64) {
+        const int64_t at = r.at + r.before(i, a.group), tile_work = r.before(i + 1, a.group) - r.before(i, a.group);
+        const Cuts p = cuts_of(a, at, tile_work, share);
+        const int32_t row0 = i * kTile, last_row = min(row0 + kTile, rows) - 1, end = end_of(last_row);
+        const int32_t slot = sh ? 2 * a.groups + r.first + i : p.count > 1 ? 2 * p.group + 1 : -1;
+        for (int32_t c = by_parts ? lane : 0; c < p.count; c += by_parts ? 64 : 1)
+          put(r.first + i, p.group + c,
+              {r.q_begin, row0, last_row + 1 - row0, r.table, cut_key(at, tile_work, p, c, r.begin, end),
+               cut_key(at, tile_work, p, c + 1, r.begin, end), c ? 2 * (p.group + c) : slot, 0});
+        if (slot >= 0 && (!by_parts || lane == 0)) {
+          int32_t parts = p.count;
+          if (sh && shared_wide) parts += shared_chunks;
+          else if (sh) parts += cuts_of(a, (r.shared_token0 * a.group + row0) / kTile * shared_work, shared_work, share).count;
+          const int32_t lines = joined_rows(parts), tile_rows = last_row + 1 - row0;
+          int32_t to = atomicAdd(&narrow_entries, ceil_div(tile_rows, lines));
+          for (int32_t e = 0; e < tile_rows && to < a.max_entries; e += lines)
+            a.l.entries[to++] = {r.q_begin, row0 + e, (int16_t)min(lines, tile_rows - e), lines == 1, sh ? r.shared_token0 * a.group + row0 + e : -1,
+                                 {slot, 2 * p.group, 2, p.count}};
+        }
+      }
+      if (sh)
+        for (int32_t i = lane; i < r.n; i += 64) a.l.shared_tokens[r.shared_token0 + i] = r.q_begin + i;
     }
-    if (sh || c.chunks != 1) {
-      const int32_t each = joined_rows(c.chunks + (sh ? shared_chunks : 0));  // (divides a tile)
-      for (int32_t row0 = lane * each, i = lane; row0 < rows; row0 += 64 * each, i += 64)
-        if (first.z + i < a.max_entries)
-          a.l.entries[first.z + i] = {r.q_begin, row0, min(each, rows - row0), first.y + row0 / c.tile * c.chunks, c.chunks,
-                                      sh ? first.w * a.group + row0 : -1, c.wide, 0};
-    }
-    if (sh)
-      for (int32_t i = lane; i < r.n; i += 64) a.l.shared_tokens[first.w + i] = r.q_begin + i;
+    __syncthreads();
   }
-  if (shared_items) {
-    const int32_t table = a.l.requests[some_request].table;
-    const int32_t each = round_up(ceil_div(shared_len, shared_chunks), shared_wide ? kStep : kBlock);
-    Item* const items = shared_wide ? a.l.items[1] : a.l.items[0];
-    for (int32_t i = tid; i < shared_items && i < a.max_items[shared_wide]; i += 1024) {
-      const int32_t tile = i / shared_chunks, part = i - tile * shared_chunks, row0 = tile * shared_tile;
-      const int32_t from = min(part * each, shared_len);
-      items[i] = {-1, row0, min(shared_tile, shared_rows - row0), table, from, min(from + each, shared_len), i, 0};
-    }
-  }
+  if (tid == 0) *a.l.header = {min(carry[1], a.max_items[1]), min(narrow_entries, a.max_entries), min(wide_entries, a.max_entries), shared_wide};
+  for (int32_t w = tid; w < a.groups; w += 1024)
+    a.l.ranges[w] = last_item[w] < 0 ? Range{0, 0} : Range{first_item[w], last_item[w] + 1};
 }
 
 // ---- storage types -------------------------------------------------------------------------------------------------
@@ -361,6 +499,8 @@ struct AttendArgs {
   uint32_t page_stride, row_stride, plane;  // bytes: page to page, key to key in a page, K to V
   int32_t num_pages, page_size, page_shift;
   int32_t kv_heads, group, head_dim;
+  int32_t narrow_groups, wide_groups;  // workgroups, of all key heads
+  int32_t max_entries;
   float scale;             // times log2(e)
   Layout l;
 };
@@ -564,22 +704,22 @@ struct RowTile {
   }
 };
 
+template <typename T, int DP>
+constexpr int narrow_lds() { return kWaves * kBlock * RowTile<T, DP>::VSTRIDE + kWaves * 2 * kTile * 4; }
+
 template <typename T, int DP, Reach REACH>
-__global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs a) {
+__device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& item, int32_t h, char* lds) {
   typedef RowTile<T, DP> Tile;
   typedef Block<DP> B;
   constexpr int KSTEPS = Tile::KSTEPS, DTILES = Tile::DTILES, VSTRIDE = Tile::VSTRIDE;
   constexpr int OSTRIDE = DP + 4;
   static_assert(kTile * OSTRIDE * 4 <= kBlock * VSTRIDE, "a wavefront's O takes the place of its V");
-  __shared__ __attribute__((aligned(16))) char v_lds[kWaves][kBlock * VSTRIDE];
-  __shared__ float stats[kWaves][2][kTile];
+  typedef float Stats[2][kTile];
+  Stats* const stats = reinterpret_cast<Stats*>(lds + kWaves * kBlock * VSTRIDE);
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t n = lane & 15, quad = lane >> 4;
-  const int32_t num_items = a.l.header->items[0];
-  for (int32_t at = blockIdx.x; at < num_items * a.kv_heads; at += gridDim.x) {
-    const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
-    const Item item = a.l.items[0][it];
-    const int32_t D = a.head_dim;
+  const int32_t D = a.head_dim;
+  {
     Tile tile = {};
     tile.m = -INFINITY;
     tile.odd_from = INT32_MAX;
@@ -593,7 +733,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void at
         if (k * 32 + quad * 8 < D) tile.q[k] = *reinterpret_cast<const u32x4*>(p + k * 64);
     }
     const char* heads = a.cache + (int64_t)h * D * 2;
-    char* my_v = v_lds[wave];
+    char* const my_v = lds + wave * (kBlock * VSTRIDE);
     constexpr int32_t STEP = kWaves * kBlock;
     int32_t k0 = item.key_begin + wave * kBlock;
     if (k0 < item.key_end && a.num_pages > 0) {
@@ -674,7 +814,8 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void at
       if (r >= item.rows || d >= D) continue;
       f32x4 x = {};
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(v_lds[w]) + r * OSTRIDE + d);
+      for (int w = 0; w < kWaves; ++w)
+        x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(lds + w * (kBlock * VSTRIDE)) + r * OSTRIDE + d);
       if (item.slot >= 0) {
         *reinterpret_cast<f32x4*>(a.partial[0] + (((int64_t)item.slot * a.kv_heads + h) * kTile + r) * D + d) = x;
       } else {
@@ -693,23 +834,26 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void at
 // half (lane / 32). K rows are 16 bytes apart in the banks (a lane reads 16 bytes of a row of its own), V rows 32.
 // The maximum that the weights are taken against grows only when a row's has outgrown it by 2^8: until then the larger weights
 // (below 2^8) and sums say the same, and the rescaling of O, 64 registers at 128 columns, is left out of nearly every step.
+template <int DP>
+constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16 + DP * 2 + 32) + (kWaves + 1) * 4; }
+
 template <typename T, int DP, Reach REACH>
-__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_tiles_kernel(AttendArgs a) {
+__device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item, int32_t h, char* lds) {
   constexpr int KSTEPS = DP / 16, DTILES = DP / 32;
   constexpr int KSTRIDE = DP * 2 + 16, VSTRIDE = DP * 2 + 32;
   constexpr int LPR = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes to a row
   constexpr int RPW = 64 / LPR, ROUNDS = kStep / (RPW * kWaves);
   constexpr float kOutgrown = 8;
-  __shared__ __attribute__((aligned(16))) char k_lds[2][kStep * KSTRIDE];
-  __shared__ __attribute__((aligned(16))) char v_lds[2][kStep * VSTRIDE];
-  __shared__ int32_t leasts[kWaves], left_out;
+  typedef char KStep[kStep * KSTRIDE];
+  typedef char VStep[kStep * VSTRIDE];
+  KStep* const k_lds = reinterpret_cast<KStep*>(lds);
+  VStep* const v_lds = reinterpret_cast<VStep*>(lds + 2 * sizeof(KStep));
+  int32_t* const leasts = reinterpret_cast<int32_t*>(lds + 2 * sizeof(KStep) + 2 * sizeof(VStep));
+  int32_t& left_out = leasts[kWaves];
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t n = lane & 31, hi = lane >> 5, lrow = lane / LPR, lcol = lane % LPR;
-  const int32_t num_items = a.l.header->items[1];
   const int32_t D = a.head_dim;
-  for (int32_t at = blockIdx.x; at < num_items * a.kv_heads; at += gridDim.x) {
-    const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
-    const Item item = a.l.items[1][it];
+  {
     const char* const heads = a.cache + (int64_t)h * D * 2;
     const int32_t my_row = wave * 32 + n;
     u32x4 q[KSTEPS] = {};
@@ -812,43 +956,31 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_tiles_kern
         }
       }
     };
-    const auto work = [&](int buf, int32_t k0, uint64_t present) {
-      // pieces of K and V come from LDS a group ahead of the products that take them, and no further: registers
-      f32x16 s[2] = {};
-      constexpr int GROUPS = 2 * KSTEPS / 4;
-      const char* const k_from = k_lds[buf] + n * KSTRIDE + hi * 16;
-      const auto k_piece = [&](int i) { return *reinterpret_cast<const u32x4*>(k_from + i / KSTEPS * 32 * KSTRIDE + i % KSTEPS * 32); };
-      u32x4 piece[2][4];
+    // 32 keys of a staged step: their scores,
+    const auto scores = [&](int buf, int half) {
+      f32x16 s = {};
+      const char* from = k_lds[buf] + (half * 32 + n) * KSTRIDE + hi * 16;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) piece[0][i] = k_piece(i);
-#pragma unroll
-      for (int j = 0; j < GROUPS; ++j) {
-        if (j + 1 < GROUPS)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) piece[(j + 1) % 2][i] = k_piece(j * 4 + 4 + i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[(j * 4 + i) / KSTEPS] = T::mfma(piece[j % 2][i], q[(j * 4 + i) % KSTEPS], s[(j * 4 + i) / KSTEPS]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      const bool ragged = least < k0 + kStep;
-      if (ragged || ~present) {
+      for (int k = 0; k < KSTEPS; ++k) s = T::mfma(*reinterpret_cast<const u32x4*>(from + k * 32), q[k], s);
+      return s;
+    };
+    // those of keys that the row does not see taken out, and the row's highest
+    const auto highest = [&](f32x16& s, int32_t k0, uint32_t present) {
+      if (least < k0 + 32 || ~present) {
         // the keys that the row sees, bit x for key x + 4 hi, so that a lane's are at fixed bits
-        const int32_t left = clamp(limit - k0, 0, kStep);
-        const uint64_t sees = (left ? ~uint64_t(0) >> (kStep - left) & present : 0) >> hi * 4;
+        const int32_t left = clamp(limit - k0, 0, 32);
+        const uint32_t sees = (left ? 0xffffffffu >> (32 - left) & present : 0) >> hi * 4;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t bits = (uint32_t)(sees >> t * 32);
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!(bits >> (r / 4 * 8 + r % 4) & 1)) s[t][r] = -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r)
+          if (!(sees >> (r / 4 * 8 + r % 4) & 1)) s[r] = -INFINITY;
       }
-      float top = s[0][0];
+      float top = s[0];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-      top = fmaxf(top, __shfl_xor(top, 32));
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+      return fmaxf(top, __shfl_xor(top, 32));
+    };
+    // a maximum that has been outgrown
+    const auto grow = [&](float top) {
       if (__ballot(top * a.scale > m * a.scale + kOutgrown)) {
         const float grown = fmaxf(m, top), base = grown == -INFINITY ? 0.f : grown * a.scale;
         const float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
@@ -857,62 +989,89 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_tiles_kern
         l *= shrink;
         m = grown;
       }
+    };
+    // their weights from the scores, while the scores of the 32 keys behind them are on the matrix unit; then the product
+    // with V. 16 keys at a time, of which the lane's are 4 hi..4 hi + 3 and 8 + 4 hi..8 + 4 hi + 3.
+    const auto take = [&](const f32x16& s, int buf, int half, int next_buf, int next_half) {
       const float base = m == -INFINITY ? 0.f : m * a.scale;
-      uint32_t p[2][8];
-      float sum = 0;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float x = exp2_of(__builtin_fmaf(s[t][r], a.scale, -base));
-          const float y = exp2_of(__builtin_fmaf(s[t][r + 1], a.scale, -base));
-          p[t][r / 2] = T::pack(x, y);
-          sum += x + y;
-        }
-      l += sum;
-      // 16 keys at a time; the lane's are 4 hi..4 hi + 3 and 8 + 4 hi..8 + 4 hi + 3 of them
-      const char* const v_from = v_lds[buf] + (hi * 4 + (n & 15) / 4) * VSTRIDE + ((n >> 4) * 16 + n % 4 * 4) * 2;
-      const auto v_piece = [&](int u, int d) {
+      uint32_t p[8];
+      float sum[2] = {};
+      f32x16 next = {};
+      u32x4 piece[kAhead + 1];
+      const char* const k_from = k_lds[next_buf] + (next_half * 32 + n) * KSTRIDE + hi * 16;
+      const char* const v_from = v_lds[buf] + (half * 32 + hi * 4 + (n & 15) / 4) * VSTRIDE + ((n >> 4) * 16 + n % 4 * 4) * 2;
+      const auto k_piece = [&](int k) { return *reinterpret_cast<const u32x4*>(k_from + k * 32); };
+      const auto v_piece = [&](int j) {
         typedef __attribute__((address_space(3))) s16x4* Lds;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v_from + u * 16 * VSTRIDE + d * 64));
-        const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(v_from + (u * 16 + 8) * VSTRIDE + d * 64));
+        const char* from = v_from + j / DTILES * 16 * VSTRIDE + j % DTILES * 64;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from));
+        const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 8 * VSTRIDE));
         const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, up);
         return u32x4{x[0], x[1], y[0], y[1]};
       };
-      constexpr int AT_ONCE = DTILES < 4 ? DTILES : 4, PARTS = 4 * DTILES / AT_ONCE;
-      static_assert(4 * DTILES % AT_ONCE == 0, "groups of pieces");
+      // The order is written out, a product with what goes on beside it to a line: pieces of K and then of V from LDS for the
+      // products kAhead further on, and a share of the weights.
+      constexpr int PIECES = KSTEPS + 2 * DTILES;
+      const auto ask = [&](int j) {
+        if (j < PIECES) piece[j % (kAhead + 1)] = j < KSTEPS ? k_piece(j) : v_piece(j - KSTEPS);
+      };
 #pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) piece[0][i] = v_piece(i / DTILES, i % DTILES);
+      for (int j = 0; j < kAhead; ++j) ask(j);
 #pragma unroll
-      for (int j = 0; j < PARTS; ++j) {
-        if (j + 1 < PARTS)
+      for (int k = 0; k < KSTEPS; ++k) {
+        ask(k + kAhead);
+        next = T::mfma(piece[k % (kAhead + 1)], q[k], next);
 #pragma unroll
-          for (int i = 0; i < AT_ONCE; ++i) {
-            const int x = (j + 1) * AT_ONCE + i;
-            piece[(j + 1) % 2][i] = v_piece(x / DTILES, x % DTILES);
-          }
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-          const int x = j * AT_ONCE + i;
-          const uint32_t* w = p[x / DTILES / 2] + x / DTILES % 2 * 4;
-          o[x % DTILES] = T::mfma(piece[j % 2][i], u32x4{w[0], w[1], w[2], w[3]}, o[x % DTILES]);
+        for (int r = k * 8 / KSTEPS * 2; r < (k + 1) * 8 / KSTEPS * 2; r += 2) {
+          const float x = exp2_of(__builtin_fmaf(s[r], a.scale, -base));
+          const float y = exp2_of(__builtin_fmaf(s[r + 1], a.scale, -base));
+          p[r / 2] = T::pack(x, y);
+          sum[0] += x;
+          sum[1] += y;
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int j = 0; j < 2 * DTILES; ++j) {
+        const int u = j / DTILES * 4;
+        ask(KSTEPS + j + kAhead);
+        o[j % DTILES] = T::mfma(piece[(KSTEPS + j) % (kAhead + 1)], u32x4{p[u], p[u + 1], p[u + 2], p[u + 3]}, o[j % DTILES]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      l += sum[0] + sum[1];
+      return next;
     };
     const int32_t steps = a.num_pages > 0 ? (item.key_end - item.key_begin + kStep - 1) / kStep : 0;
-    uint64_t present = 0;
     if (steps > 0) {
-      present = fetch(item.key_begin, 0);
-      stage(0, item.key_begin, present);
-    }
-    for (int32_t i = 0; i < steps; ++i) {
-      const int32_t k0 = item.key_begin + i * kStep;
-      __syncthreads();  // the step is staged, and the other buffer has been read
-      const uint64_t now = present;
-      if (i + 1 < steps) present = fetch(k0 + kStep, i + 1);
-      if (most > k0) work(i & 1, k0, now);
-      if (i + 1 < steps) stage(i + 1 & 1, k0 + kStep, present);
+      int32_t k0 = item.key_begin;
+      uint64_t present = fetch(k0, 0), coming = 0;
+      stage(0, k0, present);
+      if (steps > 1) coming = fetch(k0 + kStep, 1);
+      __syncthreads();
+      f32x16 s = scores(0, 0);
+      float top = highest(s, k0, (uint32_t)present);
+      for (int32_t i = 0; i < steps; ++i, k0 += kStep) {
+        const int buf = i & 1;
+        uint64_t then = 0;
+        __syncthreads();  // the other buffer has been read
+        if (i + 1 < steps) {
+          stage(buf ^ 1, k0 + kStep, coming);
+          if (i + 2 < steps) then = fetch(k0 + 2 * kStep, i + 2);
+        }
+        if (most > k0) {
+          grow(top);
+          s = take(s, buf, 0, buf, 1);
+          top = highest(s, k0 + 32, (uint32_t)(present >> 32));
+        }
+        __syncthreads();  // the next step is staged
+        if (most > k0 + 32) {
+          grow(top);
+          s = take(s, buf, 1, buf ^ 1, 0);  // (after the last step: whatever is there, and no use of it)
+          top = highest(s, k0 + kStep, (uint32_t)coming);
+        }
+        present = coming;
+        coming = then;
+      }
     }
     __syncthreads();  // (left_out is complete, and the buffers are free)
     if (left_out) {  // as above
@@ -969,41 +1128,91 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_tiles_kern
   }
 }
 
-// Joins a row's partials: weights exp2(lse_c - lse). A row without any is zero, its lse -inf. An entry of several rows,
-// of few parts each, takes a wavefront a row; one of a single row of many parts a workgroup, the parts over the eight halves
-// of its wavefronts.
+// A workgroup of a key head takes its share's items one after the other
+template <typename T, int DP, Reach REACH>
+__device__ __forceinline__ void narrow_share(const AttendArgs& a, int32_t at, char* lds) {
+  const int32_t group = at / a.kv_heads, h = at - group * a.kv_heads;
+  const Range range = a.l.ranges[group];
+  for (int32_t i = range.begin; i < range.end; ++i) narrow_item<T, DP, REACH>(a, a.l.items[0][i], h, lds);
+}
+template <typename T, int DP, Reach REACH>
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[narrow_lds<T, DP>()];
+  narrow_share<T, DP, REACH>(a, blockIdx.x, lds);
+}
+
+// Steps that may have wide tiles: both kinds in one launch, side by side on the card, as the narrow ones wait for memory and
+// the wide ones for the matrix units. 32 workgroups of a kind in turn: they are dealt to the 8 XCDs and there to 4 shader
+// engines in rotation (8 in turn put all wide ones on half of the engines: 1200 us for 680). The wide items, of one key head
+// after the other, are dealt to the XCDs in eight runs, so that items that read the same keys share an L2.
+template <typename T, int DP, Reach REACH>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_step_kernel(AttendArgs a) {
+  constexpr int LDS = wide_lds<DP>() > narrow_lds<T, DP>() ? wide_lds<DP>() : narrow_lds<T, DP>();
+  __shared__ __attribute__((aligned(16))) char lds[LDS];
+  const int32_t narrow = a.narrow_groups, both = min(narrow, a.wide_groups) & ~31;
+  int32_t at = blockIdx.x;
+  bool is_wide;
+  if (at < 2 * both) {
+    is_wide = (at & 32) == 0;
+    at = (at >> 6) * 32 + (at & 31);
+  } else {
+    at -= both;  // what is left of either, the wide first
+    is_wide = at < a.wide_groups;
+    if (!is_wide) at = at - a.wide_groups + both;
+  }
+  if (!is_wide) {
+    narrow_share<T, DP, REACH>(a, at, lds);
+    return;
+  }
+  const int32_t items = a.l.header->wide_items, all = items * a.kv_heads, run = (all + 7) / 8;
+  for (int32_t i = at >> 3; i < run; i += a.wide_groups >> 3) {
+    const int32_t x = (at & 7) * run + i;
+    if (x >= all) break;
+    const int32_t h = x / items;
+    const Item item = a.l.items[1][x - h * items];
+    if (item.rows) wide_item<T, DP, REACH>(a, item, h, lds);
+  }
+}
+
+// Joins a row's partials: weights exp2(lse_c - lse). An entry of several rows, of few parts each, takes half a wavefront a row,
+// its lanes over the columns; one of a single row of many parts a workgroup, the parts over the eight halves.
+// Bound by the chain of loads (entry, lse, partials) at few rows, by the partials' bytes at many.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kThreads, 6) void attend_join_kernel(AttendArgs a) {
   __shared__ f32x4 sums[8][64];
-  const int32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = threadIdx.x >> 5, column = threadIdx.x & 31;
-  const int32_t num_entries = a.l.header->entries, shared_chunks = a.l.header->shared_chunks;
-  const bool shared_wide = a.l.header->shared_wide;
-  const int32_t D = a.head_dim;
-  for (int32_t at = blockIdx.x; at < num_entries * a.kv_heads; at += gridDim.x) {
+  const int32_t half = threadIdx.x >> 5, column = threadIdx.x & 31;
+  const Header head = *a.l.header;
+  const bool shared_wide = head.shared_wide;
+  const int32_t D = a.head_dim, entries = head.narrow_entries + head.wide_entries;
+  for (int32_t at = blockIdx.x; at < entries * a.kv_heads; at += gridDim.x) {
     const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
-    const Entry e = a.l.entries[it];
-    const int32_t parts = e.chunks + (e.shared_row0 >= 0 ? shared_chunks : 0);
-    const bool many = parts > kManyParts;
-    const int32_t own_tile = e.wide ? kWide : kTile, shared_tile = shared_wide ? kWide : kTile;
-    for (int32_t r = many ? 0 : wave; r < e.rows; r += many ? 1 : kWaves) {
-      const int32_t row = e.row0 + r, in_tile = row % own_tile;
-      const int32_t shared_row = e.shared_row0 + r, shared_slot = shared_row / shared_tile * shared_chunks - e.chunks;
-      const auto row_of = [&](int32_t c) {  // of part c
-        return c < e.chunks ? ((int64_t)(e.slot + c) * a.kv_heads + h) * own_tile + in_tile
-                            : ((int64_t)(shared_slot + c) * a.kv_heads + h) * shared_tile + shared_row % shared_tile;
+    const bool wide = it >= head.narrow_entries;
+    const Entry e = a.l.entries[wide ? a.max_entries - 1 - (it - head.narrow_entries) : it];
+    const int32_t own_tile = wide ? kWide : kTile, shared_tile = shared_wide ? kWide : kTile;
+    const float* const own_lse = a.partial_lse[wide], * const shared_lse = a.partial_lse[shared_wide];
+    const float* const own_o = a.partial[wide], * const shared_o = a.partial[shared_wide];
+    const bool many = e.many;
+    for (int32_t r = many ? 0 : half; r < e.rows; r += 8) {
+      const int32_t row = e.row0 + r, shared_row = e.shared_row0 + r;
+      const Parts sh = e.shared_row0 >= 0 ? a.l.shared_parts[shared_row / shared_tile] : Parts{};
+      const int32_t own = e.parts.count, parts = own + sh.count;
+      const auto row_of = [&](int32_t c) -> int64_t {  // of part c
+        if (c < own) return ((int64_t)(c ? e.parts.next + c * e.parts.step : e.parts.slot) * a.kv_heads + h) * own_tile + row % own_tile;
+        c -= own;
+        return ((int64_t)(c ? sh.next + c * sh.step : sh.slot) * a.kv_heads + h) * shared_tile + shared_row % shared_tile;
       };
-      const auto lse_of = [&](int32_t c) { return a.partial_lse[c < e.chunks ? e.wide : shared_wide][row_of(c)]; };
+      const auto lse_of = [&](int32_t c) { return (c < own ? own_lse : shared_lse)[row_of(c)]; };
       float top = -INFINITY;
-      for (int32_t c = lane; c < parts; c += 64) top = fmaxf(top, lse_of(c));
-      for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+      for (int32_t c = column; c < parts; c += 32) top = fmaxf(top, lse_of(c));
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
       const float base = top == -INFINITY ? 0.f : top;
       float total = 0;
-      for (int32_t c = lane; c < parts; c += 64) total += exp2_of(lse_of(c) - base);
-      for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+      for (int32_t c = column; c < parts; c += 32) total += exp2_of(lse_of(c) - base);
+      for (int d = 16; d; d >>= 1) total += __shfl_xor(total, d);
       const float inv = total == 0 ? 0.f : 1.f / total;
       const int32_t i = row / a.group, g = row - i * a.group;
       const int64_t out_row = ((int64_t)(e.q_begin + i) * a.kv_heads + h) * a.group + g;
-      if (a.lse && (many ? threadIdx.x : lane) == 0) a.lse[out_row] = (total == 0 ? -INFINITY : base + __log2f(total)) * kLn2;
+      if (a.lse && column == 0 && (!many || half == 0)) a.lse[out_row] = (total == 0 ? -INFINITY : base + __log2f(total)) * kLn2;
       const auto put = [&](int32_t d, f32x4 x) {
         x *= inv;
         *reinterpret_cast<u32x2*>(a.out + (out_row * D + d) * 2) = u32x2{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
@@ -1011,14 +1220,12 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(AttendArgs a) {
       const auto sum_of = [&](int32_t d, int32_t from, int32_t step) {
         f32x4 x = {};
 #pragma unroll 4
-        for (int32_t c = from; c < parts; c += step) {
-          const float weight = exp2_of(lse_of(c) - base);
-          x += *reinterpret_cast<const f32x4*>(a.partial[c < e.chunks ? e.wide : shared_wide] + row_of(c) * D + d) * weight;
-        }
+        for (int32_t c = from; c < parts; c += step)
+          x += *reinterpret_cast<const f32x4*>((c < own ? own_o : shared_o) + row_of(c) * D + d) * exp2_of(lse_of(c) - base);
         return x;
       };
       if (!many) {
-        for (int32_t d = lane * 4; d < D; d += 256) put(d, sum_of(d, 0, 1));
+        for (int32_t d = column * 4; d < D; d += 128) put(d, sum_of(d, 0, 1));
       } else {
         for (int32_t d = column; d < D / 4; d += 32) sums[half][d] = sum_of(d * 4, half, 8);
         __syncthreads();
@@ -1038,8 +1245,8 @@ int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
 // The sizes that follow from the capacities: of narrow and of wide items
 struct Sizes {
-  int64_t target[2], max_items[2], max_slots[2], max_entries;
-  bool wide;  // are there wide items at all?
+  int64_t groups, residents, max_items[2], max_slots[2], max_shared_tiles, max_entries;
+  bool wide, join;  // can there be wide tiles, or any that are joined?
 };
 
 }  // namespace
@@ -1061,10 +1268,10 @@ struct kvc_attention_plan {
 
 namespace {
 
-// Workgroups that a step's items of a kind make, about: enough that the last to end is a small part of the time
-constexpr int64_t kWorkgroups[2] = {1024, 512};
-constexpr int32_t kMinChunk[2] = {256, 512};  // keys
-constexpr int64_t kNarrowRows = 32;           // of a request; with more it is cut into wide items
+constexpr int64_t kNarrowGroups = 1024;       // workgroups of a launch for narrow tiles
+constexpr int64_t kResidents = 512;           // wide items on the card at a time
+constexpr int64_t kMaxRounds = 4;             // of them in a step, where a range of keys is longer than the least
+constexpr int64_t kNarrowRows = 32;           // of a request; with more it is cut into wide tiles
 constexpr int64_t kNarrowSharedRows = 64;     // of all sharing requests
 
 Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
@@ -1078,45 +1285,54 @@ Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
   l.header = (Header*)take(sizeof(Header));
   l.requests = (Request*)take(p.batch_size * sizeof(Request));
   l.shares = (int32_t*)take(p.batch_size * 4);
-  l.offsets = (int32_t*)take(p.batch_size * 16);
   l.limits = (int32_t*)take(p.num_tokens * 4);
   l.shared_tokens = (int32_t*)take(p.num_tokens * 4);
+  l.ranges = (Range*)take(p.n.groups * sizeof(Range));
   for (int k = 0; k < 2; ++k) l.items[k] = (Item*)take(p.n.max_items[k] * sizeof(Item));
+  l.shared_parts = (Parts*)take(p.n.max_shared_tiles * sizeof(Parts));
   l.entries = (Entry*)take(p.n.max_entries * sizeof(Entry));
   if (bytes) *bytes = at;
   return l;
 }
 
-// Row tiles are at most rows / tile and one more for every request that has tokens; cut into items of a target-th of all
-// keys each, there are at most the target and one more for every tile, those of the shared prefix among them. Without a shared
-// prefix only tiles of more than one item need slots, which are at most twice the target.
+// Row tiles are at most rows / tile and one more for every request that has tokens, and those of the shared prefix. A narrow
+// tile's part in a workgroup has place tile + workgroup in the list; two parts of a workgroup need slots, and, where a prefix is
+// shared, every tile's first part. Wide tiles cut into ranges of at least the rounds' share of all keys make at most
+// the rounds' items and one more a tile; those of two ranges or more, which need slots, at most twice the rounds' items.
 Sizes sizes_of(const kvc_attention_plan& p) {
   Sizes n;
   const int64_t rows = p.num_tokens * (p.num_heads / p.num_kv_heads);
-  n.wide = rows > p.narrow_rows || (p.shared_pages > 0 && rows > kNarrowSharedRows);
-  for (int k = 0; k < 2; ++k) {
-    const int64_t tile = k ? kWide : kTile, tiles = rows / tile + std::min(p.batch_size, p.num_tokens);
-    n.target[k] = std::max<int64_t>(1, kWorkgroups[k] / p.num_kv_heads);
-    n.max_items[k] = k && !n.wide ? 0 : n.target[k] + tiles + (p.shared_pages > 0 ? rows / tile + 1 : 0);
-    n.max_slots[k] = k && !n.wide ? 0 : p.shared_pages > 0 ? n.max_items[k] : 2 * n.target[k];
-  }
-  n.max_entries = rows;
+  const bool shared = p.shared_pages > 0;
+  n.wide = rows > p.narrow_rows || (shared && rows > kNarrowSharedRows);
+  n.groups = std::min<int64_t>(kMaxGroups, std::max<int64_t>(1, kNarrowGroups / p.num_kv_heads));
+  n.residents = std::max<int64_t>(1, kResidents / p.num_kv_heads);
+  const auto shared_tiles = [&](int64_t tile) { return shared ? rows / tile + 1 : 0; };
+  const auto tiles = [&](int64_t tile) { return rows / tile + std::min(p.batch_size, p.num_tokens) + shared_tiles(tile); };
+  n.max_items[0] = tiles(kTile) + n.groups;
+  n.max_slots[0] = 2 * n.groups + (shared ? tiles(kTile) : 0);
+  n.max_items[1] = n.wide ? tiles(kWide) + kMaxRounds * n.residents : 0;
+  n.max_slots[1] = n.wide ? 2 * kMaxRounds * n.residents + shared_tiles(kWide) : 0;
+  n.max_shared_tiles = shared_tiles(kTile);
+  // (a narrow tile that is shorter than two of the least parts is never cut, a wide one that is no longer than the least range)
+  const int64_t keys = p.num_kv_indices * p.page_size;
+  n.join = shared || keys + kTileWork + kTile + 2 >= 2 * std::min(kMinShare / 2, kMinPart) || (n.wide && keys > kMinChunk);
+  n.max_entries = n.join ? rows : 0;
   return n;
 }
 
 template <typename T, int DP>
 void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
-  const dim3 block(kThreads);
-  // (a workgroup takes further items where there are more than the grid has places for)
-  const auto grid = [&](int64_t items) { return dim3((unsigned)std::min<int64_t>(items * p.num_kv_heads, 1 << 14)); };
+  const dim3 block(kThreads), grid((unsigned)(a.narrow_groups + a.wide_groups));
   const bool any = a.page_size % 16 != 0, full = a.head_dim == DP;
-  if (any) kvc::launch((attend_rows_kernel<T, DP, kAnyPage>), grid(p.n.max_items[0]), block, 0, s, a);
-  else if (!full) kvc::launch((attend_rows_kernel<T, DP, kGroups>), grid(p.n.max_items[0]), block, 0, s, a);
-  else kvc::launch((attend_rows_kernel<T, DP, kGroupsFull>), grid(p.n.max_items[0]), block, 0, s, a);
-  if (!p.n.wide) return;
-  if (any) kvc::launch((attend_tiles_kernel<T, DP, kAnyPage>), grid(p.n.max_items[1]), block, 0, s, a);
-  else if (!full) kvc::launch((attend_tiles_kernel<T, DP, kGroups>), grid(p.n.max_items[1]), block, 0, s, a);
-  else kvc::launch((attend_tiles_kernel<T, DP, kGroupsFull>), grid(p.n.max_items[1]), block, 0, s, a);
+  if (p.n.wide) {
+    if (any) kvc::launch((attend_step_kernel<T, DP, kAnyPage>), grid, block, 0, s, a);
+    else if (!full) kvc::launch((attend_step_kernel<T, DP, kGroups>), grid, block, 0, s, a);
+    else kvc::launch((attend_step_kernel<T, DP, kGroupsFull>), grid, block, 0, s, a);
+  } else {
+    if (any) kvc::launch((attend_rows_kernel<T, DP, kAnyPage>), grid, block, 0, s, a);
+    else if (!full) kvc::launch((attend_rows_kernel<T, DP, kGroups>), grid, block, 0, s, a);
+    else kvc::launch((attend_rows_kernel<T, DP, kGroupsFull>), grid, block, 0, s, a);
+  }
 }
 template <typename T>
 void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
@@ -1124,7 +1340,8 @@ void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t
   else if (p.head_dim <= 96) launch_attend<T, 96>(a, p, s);
   else if (p.head_dim <= 128) launch_attend<T, 128>(a, p, s);
   else launch_attend<T, 256>(a, p, s);
-  const unsigned joins = (unsigned)std::min<int64_t>(p.n.max_entries * p.num_kv_heads, 2048);
+  if (!p.n.join) return;
+  const unsigned joins = (unsigned)std::min<int64_t>(p.n.max_entries * p.num_kv_heads, 4096);
   kvc::launch((attend_join_kernel<T>), dim3(joins), dim3(kThreads), 0, s, a);
 }
 
@@ -1191,7 +1408,7 @@ int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buf
   PlanArgs a{plan->qo_indptr, plan->kv_indices, plan->kv_indptr, plan->kv_last_page_len, (int32_t)plan->batch_size,
              (int32_t)plan->num_tokens, (int32_t)plan->num_kv_indices, (int32_t)plan->page_size,
              (int32_t)plan->shared_pages, (int32_t)(plan->num_heads / plan->num_kv_heads), (int32_t)plan->narrow_rows,
-             (int32_t)kNarrowSharedRows, {(int32_t)plan->n.target[0], (int32_t)plan->n.target[1]}, {kMinChunk[0], kMinChunk[1]},
+             (int32_t)kNarrowSharedRows, (int32_t)plan->n.groups, (int32_t)plan->n.residents,
              {(int32_t)plan->n.max_items[0], (int32_t)plan->n.max_items[1]}, (int32_t)plan->n.max_entries,
              layout_of(*plan, plan->buffer, nullptr)};
   hipStream_t s = (hipStream_t)stream;
@@ -1246,6 +1463,10 @@ int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query, in
   a.kv_heads = (int32_t)plan->num_kv_heads;
   a.group = (int32_t)(plan->num_heads / plan->num_kv_heads);
   a.head_dim = (int32_t)plan->head_dim;
+  a.narrow_groups = (int32_t)(plan->n.groups * plan->num_kv_heads);
+  // (a workgroup takes further items where there are more than these)
+  a.wide_groups = (int32_t)round_up(std::min<int64_t>(plan->n.max_items[1] * plan->num_kv_heads, 4096), 8);
+  a.max_entries = (int32_t)plan->n.max_entries;
   a.scale = plan->scale * kLog2e;
   a.l = layout_of(*plan, plan->buffer, nullptr);
   if (plan->dtype == KVC_DTYPE_BF16) launch_attend<BF16>(a, *plan, (hipStream_t)stream);
