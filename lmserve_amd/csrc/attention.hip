@@ -39,6 +39,7 @@ constexpr int kTile = 16;          // rows of a narrow item
 constexpr int kWide = 32 * kWaves; // rows of a wide item: 32 to a wavefront
 constexpr int kBlock = 32;         // keys that a wavefront takes at once of a narrow item
 constexpr int kStep = 64;          // keys that a workgroup takes at once of a wide item
+constexpr int kVPad = 64;          // bytes between a wide item's rows of V in LDS
 constexpr int kAhead = 3;          // pieces of a wide item's K and V that are read from LDS ahead of their product
 constexpr int kMaxGroups = 1024;    // workgroups of a key head
 // In keys: what a narrow tile costs beside its own, a workgroup's least share, the least part of a tile
@@ -835,12 +836,12 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
 // The maximum that the weights are taken against grows only when a row's has outgrown it by 2^8: until then the larger weights
 // (below 2^8) and sums say the same, and the rescaling of O, 64 registers at 128 columns, is left out of nearly every step.
 template <int DP>
-constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16 + DP * 2 + 32) + (kWaves + 1) * 4; }
+constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16 + DP * 2 + kVPad) + (kWaves + 1) * 4; }
 
 template <typename T, int DP, Reach REACH>
 __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item, int32_t h, char* lds) {
   constexpr int KSTEPS = DP / 16, DTILES = DP / 32;
-  constexpr int KSTRIDE = DP * 2 + 16, VSTRIDE = DP * 2 + 32;
+  constexpr int KSTRIDE = DP * 2 + 16, VSTRIDE = DP * 2 + kVPad;
   constexpr int LPR = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes to a row
   constexpr int RPW = 64 / LPR, ROUNDS = kStep / (RPW * kWaves);
   constexpr float kOutgrown = 8;
@@ -868,69 +869,81 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
       for (int k = 0; k < KSTEPS; ++k)
         if (REACH == kGroupsFull || k * 16 + hi * 8 < D) q[k] = *reinterpret_cast<const u32x4*>(p + k * 32);
     }
-    // the wavefront's first and last limits (rows that are not there have none)
-    int32_t least = my_row < item.rows ? limit : INT32_MAX, most = limit;
-    for (int d = 16; d; d >>= 1) {
-      least = min(least, __shfl_xor(least, d));
-      most = max(most, __shfl_xor(most, d));
-    }
+    // the wavefront's first limit (rows that are not there have none)
+    int32_t least = my_row < item.rows ? limit : INT32_MAX;
+    for (int d = 16; d; d >>= 1) least = min(least, __shfl_xor(least, d));
     least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
     if (lane == 0) leasts[wave] = least;
     if (tid == 0) left_out = 0;
     __syncthreads();
     const int32_t tile_least = min(min(leasts[0], leasts[1]), min(leasts[2], leasts[3]));
     f32x16 o[DTILES] = {};
-    float m = -INFINITY, l = 0;
+    float base = -INFINITY, l = 0;  // weights are exp2(score * scale - base)
     u32x4 kr[ROUNDS], vr[ROUNDS];
     int32_t id_page = -1, id_off = 0;
-    // the keys of a step from k0 on, on their way; which are there
-    const auto fetch = [&](int32_t k0, int32_t step) -> uint64_t {
+    // where a round's rows of a step lie (one row of every LPR lanes), or null where there is none to read
+    const auto row_of = [&](int32_t k0, int32_t step, int i) -> const char* {
+      const int32_t row0 = i * RPW * kWaves + wave * RPW;
+      if constexpr (REACH == kAnyPage) {
+        const int64_t off = key_offset(a, item.table, k0 + row0 + lrow, item.key_end);
+        return off < 0 || lcol * 8 >= D ? nullptr : heads + off + lcol * 16;
+      } else {
+        const int32_t group = (step & 15) * 4 + row0 / 16;
+        const int32_t page = __builtin_amdgcn_readlane(id_page, group), off = __builtin_amdgcn_readlane(id_off, group);
+        if (REACH == kGroups && lcol * 8 >= D) return nullptr;
+        return heads + (int64_t)max(page, 0) * a.page_stride + (int64_t)(page < 0 ? 0 : off + row0 % 16) * a.row_stride +
+               (lrow * a.row_stride + lcol * 16);
+      }
+    };
+    // K of the step from k0 on, on its way; which of the keys are there
+    const auto fetch_k = [&](int32_t k0, int32_t step) -> uint64_t {
       uint64_t present = 0;
       if constexpr (REACH == kAnyPage) {
         present = __ballot(key_offset(a, item.table, k0 + lane, item.key_end) >= 0);
-      } else if ((step & 15) == 0) {
-        const int32_t key = k0 + lane * 16;
-        id_page = -1;
-        if (key < item.key_end) {
-          const int32_t p = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
-          const int32_t id = a.kv_indices[item.table + p];
-          id_off = key - p * a.page_size;
-          if (id >= 0 && id < a.num_pages) id_page = id;
+      } else {
+        if ((step & 15) == 0) {  // the page ids of 16 steps, one to a lane
+          const int32_t key = k0 + lane * 16;
+          id_page = -1;
+          if (key < item.key_end) {
+            const int32_t p = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+            const int32_t id = a.kv_indices[item.table + p];
+            id_off = key - p * a.page_size;
+            if (id >= 0 && id < a.num_pages) id_page = id;
+          }
         }
-      }
-      if constexpr (REACH != kAnyPage)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int32_t left = item.key_end - k0 - i * 16;
           if (__builtin_amdgcn_readlane(id_page, (step & 15) * 4 + i) >= 0)
             present |= (uint64_t)(left >= 16 ? 0xffffu : (1u << left) - 1u) << (i * 16);
         }
+      }
 #pragma unroll
       for (int i = 0; i < ROUNDS; ++i) {
-        const int32_t row0 = i * RPW * kWaves + wave * RPW;
-        const char* from;
-        bool have = lcol * 8 < D;
-        if constexpr (REACH == kAnyPage) {
-          const int64_t off = key_offset(a, item.table, k0 + row0 + lrow, item.key_end);
-          have = have && off >= 0;
-          from = heads + off + lcol * 16;
-        } else {
-          const int32_t group = (step & 15) * 4 + row0 / 16;
-          const int32_t page = __builtin_amdgcn_readlane(id_page, group), off = __builtin_amdgcn_readlane(id_off, group);
-          from = heads + (int64_t)max(page, 0) * a.page_stride + (int64_t)(page < 0 ? 0 : off + row0 % 16) * a.row_stride +
-                 (lrow * a.row_stride + lcol * 16);
-        }
-        if (REACH != kGroupsFull) kr[i] = vr[i] = u32x4{};
-        if (REACH == kGroupsFull || have) {
-          kr[i] = *reinterpret_cast<const u32x4*>(from);
-          vr[i] = *reinterpret_cast<const u32x4*>(from + a.plane);
-        }
+        const char* from = row_of(k0, step, i);
+        if (REACH != kGroupsFull) kr[i] = u32x4{};
+        if (REACH == kGroupsFull || from) kr[i] = *reinterpret_cast<const u32x4*>(from);
       }
       return present;
     };
-    // those keys into LDS; V of keys that are not there is cleared, which K's need not be: their scores are masked
-    const auto stage = [&](int buf, int32_t k0, uint64_t present) {
+    // V of the same step, after its K
+    const auto fetch_v = [&](int32_t k0, int32_t step) {
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) {
+        const char* from = row_of(k0, step, i);
+        if (REACH != kGroupsFull) vr[i] = u32x4{};
+        if (REACH == kGroupsFull || from) vr[i] = *reinterpret_cast<const u32x4*>(from + a.plane);
+      }
+    };
+    // The columns beyond head_dim are zeros, and V of keys that are not there is cleared, which K's need not be: their scores
+    // are masked.
+    const auto stage_k = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i)
+        if (LPR * 8 == DP || lcol * 8 < DP)
+          *reinterpret_cast<u32x4*>(k_lds[buf] + (i * RPW * kWaves + wave * RPW + lrow) * KSTRIDE + lcol * 16) = kr[i];
+    };
+    const auto stage_v = [&](int buf, int32_t k0, uint64_t present) {
       if (REACH != kAnyPage && ~present)
 #pragma unroll
         for (int i = 0; i < ROUNDS; ++i)
@@ -948,24 +961,33 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
         }
       }
 #pragma unroll
-      for (int i = 0; i < ROUNDS; ++i) {
-        const int32_t row = i * RPW * kWaves + wave * RPW + lrow;
-        if (LPR * 8 == DP || lcol * 8 < DP) {
-          *reinterpret_cast<u32x4*>(k_lds[buf] + row * KSTRIDE + lcol * 16) = kr[i];
-          *reinterpret_cast<u32x4*>(v_lds[buf] + row * VSTRIDE + lcol * 16) = vr[i];
-        }
-      }
+      for (int i = 0; i < ROUNDS; ++i)
+        if (LPR * 8 == DP || lcol * 8 < DP)
+          *reinterpret_cast<u32x4*>(v_lds[buf] + (i * RPW * kWaves + wave * RPW + lrow) * VSTRIDE + lcol * 16) = vr[i];
     };
-    // 32 keys of a staged step: their scores,
-    const auto scores = [&](int buf, int half) {
-      f32x16 s = {};
-      const char* from = k_lds[buf] + (half * 32 + n) * KSTRIDE + hi * 16;
+
+    // Pieces from LDS: 16 columns of K of 32 keys (a half of a step), 32 columns of V of 16 of them, of which the lane's are
+    // 4 hi..4 hi + 3 and 8 + 4 hi..8 + 4 hi + 3.
+    const auto k_piece = [&](int buf, int half, int j) {
+      return *reinterpret_cast<const u32x4*>(k_lds[buf] + (half * 32 + n) * KSTRIDE + hi * 16 + j * 32);
+    };
+    const auto v_piece = [&](int buf, int half, int j) {
+      typedef __attribute__((address_space(3))) s16x4* Lds;
+      const char* from = v_lds[buf] + (half * 32 + hi * 4 + (n & 15) / 4) * VSTRIDE + ((n >> 4) * 16 + n % 4 * 4) * 2 +
+                         j / DTILES * 16 * VSTRIDE + j % DTILES * 64;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from));
+      const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 8 * VSTRIDE));
+      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, up);
+      return u32x4{x[0], x[1], y[0], y[1]};
+    };
+    // the row's highest score of 32 keys, those of keys that it does not see taken out
+    const auto highest = [&](f32x16& s) {
+      float top = s[0];
 #pragma unroll
-      for (int k = 0; k < KSTEPS; ++k) s = T::mfma(*reinterpret_cast<const u32x4*>(from + k * 32), q[k], s);
-      return s;
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+      return top;
     };
-    // those of keys that the row does not see taken out, and the row's highest
-    const auto highest = [&](f32x16& s, int32_t k0, uint32_t present) {
+    const auto mask = [&](f32x16& s, float top, int32_t k0, uint32_t present) {
       if (least < k0 + 32 || ~present) {
         // the keys that the row sees, bit x for key x + 4 hi, so that a lane's are at fixed bits
         const int32_t left = clamp(limit - k0, 0, 32);
@@ -973,104 +995,109 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (!(sees >> (r / 4 * 8 + r % 4) & 1)) s[r] = -INFINITY;
+        top = highest(s);
       }
-      float top = s[0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
       return fmaxf(top, __shfl_xor(top, 32));
     };
-    // a maximum that has been outgrown
-    const auto grow = [&](float top) {
-      if (__ballot(top * a.scale > m * a.scale + kOutgrown)) {
-        const float grown = fmaxf(m, top), base = grown == -INFINITY ? 0.f : grown * a.scale;
-        const float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
+    // A base that has been outgrown. It is a whole number, so that what was made with the old one, the weights that wait
+    // for their product among it, is scaled exactly.
+    const auto grow = [&](float top, uint32_t* waiting) {
+      if (__ballot(top * a.scale > base + kOutgrown)) {
+        const float grown = fmaxf(base, __builtin_ceilf(top * a.scale));
+        const float shrink = exp2_of(base - (grown == -INFINITY ? 0.f : grown));  // 0 from -inf
 #pragma unroll
         for (int d = 0; d < DTILES; ++d) o[d] *= shrink;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) waiting[i] = T::pack(T::wide(waiting[i] & 0xffffu) * shrink, T::wide(waiting[i] >> 16) * shrink);
         l *= shrink;
-        m = grown;
+        base = grown;
       }
     };
-    // their weights from the scores, while the scores of the 32 keys behind them are on the matrix unit; then the product
-    // with V. 16 keys at a time, of which the lane's are 4 hi..4 hi + 3 and 8 + 4 hi..8 + 4 hi + 3.
-    const auto take = [&](const f32x16& s, int buf, int half, int next_buf, int next_half) {
-      const float base = m == -INFINITY ? 0.f : m * a.scale;
-      uint32_t p[8];
-      float sum[2] = {};
-      f32x16 next = {};
-      u32x4 piece[kAhead + 1];
-      const char* const k_from = k_lds[next_buf] + (next_half * 32 + n) * KSTRIDE + hi * 16;
-      const char* const v_from = v_lds[buf] + (half * 32 + hi * 4 + (n & 15) / 4) * VSTRIDE + ((n >> 4) * 16 + n % 4 * 4) * 2;
-      const auto k_piece = [&](int k) { return *reinterpret_cast<const u32x4*>(k_from + k * 32); };
-      const auto v_piece = [&](int j) {
-        typedef __attribute__((address_space(3))) s16x4* Lds;
-        const char* from = v_from + j / DTILES * 16 * VSTRIDE + j % DTILES * 64;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from));
-        const s16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + 8 * VSTRIDE));
-        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, up);
-        return u32x4{x[0], x[1], y[0], y[1]};
-      };
-      // The order is written out, a product with what goes on beside it to a line: pieces of K and then of V from LDS for the
-      // products kAhead further on, and a share of the weights.
+    // 32 keys: their weights from the scores s, while the scores of the keys behind them and the product of the weights
+    // before them, that waited, with V are on the matrix unit. The order is written out, a product with what goes on beside
+    // it to a line: pieces from LDS for the products kAhead further on, half a pair of weights, the next scores' maximum.
+    const auto take = [&](const f32x16& s, uint32_t* p, f32x16& next, float& top, int next_buf, int next_half, const uint32_t* waiting,
+                          int v_buf, int v_half) {
       constexpr int PIECES = KSTEPS + 2 * DTILES;
+      const float minus = base == -INFINITY ? 0.f : -base;
+      float sum[2] = {}, x = 0;
+      u32x4 piece[kAhead + 1];
+      next = f32x16{};
       const auto ask = [&](int j) {
-        if (j < PIECES) piece[j % (kAhead + 1)] = j < KSTEPS ? k_piece(j) : v_piece(j - KSTEPS);
+        if (j < PIECES) piece[j % (kAhead + 1)] = j < KSTEPS ? k_piece(next_buf, next_half, j) : v_piece(v_buf, v_half, j - KSTEPS);
       };
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) ask(j);
 #pragma unroll
-      for (int k = 0; k < KSTEPS; ++k) {
-        ask(k + kAhead);
-        next = T::mfma(piece[k % (kAhead + 1)], q[k], next);
-#pragma unroll
-        for (int r = k * 8 / KSTEPS * 2; r < (k + 1) * 8 / KSTEPS * 2; r += 2) {
-          const float x = exp2_of(__builtin_fmaf(s[r], a.scale, -base));
-          const float y = exp2_of(__builtin_fmaf(s[r + 1], a.scale, -base));
-          p[r / 2] = T::pack(x, y);
-          sum[0] += x;
-          sum[1] += y;
+      for (int j = 0; j < PIECES; ++j) {
+        ask(j + kAhead);
+        if (j < KSTEPS) {
+          next = T::mfma(piece[j % (kAhead + 1)], q[j], next);
+        } else {
+          const int v = j - KSTEPS;
+          const uint32_t* w = waiting + v / DTILES * 4;
+          o[v % DTILES] = T::mfma(piece[j % (kAhead + 1)], u32x4{w[0], w[1], w[2], w[3]}, o[v % DTILES]);
         }
-        __builtin_amdgcn_sched_barrier(0);
-      }
 #pragma unroll
-      for (int j = 0; j < 2 * DTILES; ++j) {
-        const int u = j / DTILES * 4;
-        ask(KSTEPS + j + kAhead);
-        o[j % DTILES] = T::mfma(piece[(KSTEPS + j) % (kAhead + 1)], u32x4{p[u], p[u + 1], p[u + 2], p[u + 3]}, o[j % DTILES]);
+        for (int r = j * 16 / PIECES; r < (j + 1) * 16 / PIECES; ++r) {
+          const float y = exp2_of(__builtin_fmaf(s[r], a.scale, minus));
+          sum[r % 2] += y;
+          if (r % 2) p[r / 2] = T::pack(x, y);
+          x = y;
+          asm volatile("" : "+v"(x), "+v"(sum[r % 2]));  // here, and not where it is used
+          if (r % 2) asm volatile("" : "+v"(p[r / 2]));
+        }
+        if (j == PIECES - 1) top = highest(next);
         __builtin_amdgcn_sched_barrier(0);
       }
       l += sum[0] + sum[1];
-      return next;
     };
     const int32_t steps = a.num_pages > 0 ? (item.key_end - item.key_begin + kStep - 1) / kStep : 0;
     if (steps > 0) {
       int32_t k0 = item.key_begin;
-      uint64_t present = fetch(k0, 0), coming = 0;
-      stage(0, k0, present);
-      if (steps > 1) coming = fetch(k0 + kStep, 1);
+      // nothing waits for the first product: zeros, in V as well
+      uint32_t p0[8], p1[8] = {};
+      for (int32_t i = tid * 16; i < 32 * VSTRIDE; i += kThreads * 16) *reinterpret_cast<u32x4*>(v_lds[1] + 32 * VSTRIDE + i) = u32x4{};
+      uint64_t present = fetch_k(k0, 0), coming = 0;
+      fetch_v(k0, 0);
+      stage_k(0);
+      stage_v(0, k0, present);
+      if (steps > 1) {
+        coming = fetch_k(k0 + kStep, 1);
+        fetch_v(k0 + kStep, 1);
+      }
       __syncthreads();
-      f32x16 s = scores(0, 0);
-      float top = highest(s, k0, (uint32_t)present);
+      f32x16 s0 = {}, s1;
+#pragma unroll
+      for (int j = 0; j < KSTEPS; ++j) s0 = T::mfma(k_piece(0, 0, j), q[j], s0);
+      float top = mask(s0, highest(s0), k0, (uint32_t)present);
       for (int32_t i = 0; i < steps; ++i, k0 += kStep) {
         const int buf = i & 1;
         uint64_t then = 0;
-        __syncthreads();  // the other buffer has been read
+        __syncthreads();  // the other buffer's K has been read, this one's V is there
         if (i + 1 < steps) {
-          stage(buf ^ 1, k0 + kStep, coming);
-          if (i + 2 < steps) then = fetch(k0 + 2 * kStep, i + 2);
+          stage_k(buf ^ 1);
+          if (i + 2 < steps) then = fetch_k(k0 + 2 * kStep, i + 2);
         }
-        if (most > k0) {
-          grow(top);
-          s = take(s, buf, 0, buf, 1);
-          top = highest(s, k0 + 32, (uint32_t)(present >> 32));
+        grow(top, p1);
+        take(s0, p0, s1, top, buf, 1, p1, buf ^ 1, 1);
+        top = mask(s1, top, k0 + 32, (uint32_t)(present >> 32));
+        __syncthreads();  // the other buffer's V has been read, its K is there
+        if (i + 1 < steps) {
+          stage_v(buf ^ 1, k0 + kStep, coming);
+          if (i + 2 < steps) fetch_v(k0 + 2 * kStep, i + 2);
         }
-        __syncthreads();  // the next step is staged
-        if (most > k0 + 32) {
-          grow(top);
-          s = take(s, buf, 1, buf ^ 1, 0);  // (after the last step: whatever is there, and no use of it)
-          top = highest(s, k0 + kStep, (uint32_t)coming);
-        }
+        grow(top, p0);
+        take(s1, p1, s0, top, buf ^ 1, 0, p0, buf, 0);  // (after the last step: whatever is there, and no use of it)
+        top = mask(s0, top, k0 + kStep, (uint32_t)coming);
         present = coming;
         coming = then;
+      }
+      // the last weights' product
+#pragma unroll
+      for (int j = 0; j < 2 * DTILES; ++j) {
+        const uint32_t* w = p1 + j / DTILES * 4;
+        o[j % DTILES] = T::mfma(v_piece((steps - 1) & 1, 1, j), u32x4{w[0], w[1], w[2], w[3]}, o[j % DTILES]);
       }
     }
     __syncthreads();  // (left_out is complete, and the buffers are free)
@@ -1095,7 +1122,6 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
       }
     }
     l += __shfl_xor(l, 32);
-    const float base = m == -INFINITY ? 0.f : m * a.scale;
     const float inv = l == 0 ? 0.f : 1.f / l, lse2 = l == 0 ? -INFINITY : base + __log2f(l);
     if (my_row < item.rows) {
       if (item.slot >= 0) {
