@@ -18,6 +18,8 @@ from .cache_ops import _on_device_of, _require_gpu, _stream_of
 from .paged import _i32
 from .rotary import _DTYPES
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
 
 class PagedAttentionPlan:
     """Attention of a step's queries, its index arguments handed over ONCE.
@@ -72,6 +74,10 @@ class PagedAttentionPlan:
         self._buffer = torch.empty(lib.kvc_attention_plan_bytes(self._plan), dtype=torch.uint8, device=self.device)
         self._workspace_bytes = lib.kvc_attention_workspace_bytes(self._plan)
         self._stream = _stream_of(self._buffer)      # whose allocator the buffer is from
+        self._dev_index = self.device.index
+        fast = _lib.fast()
+        self._fast_run = fast.attention_plan_run if fast else None
+        self._dtype_code = fast.scalar_type_code(torch.empty(0, dtype=dtype)) if fast else -1
         self.build()
 
     def __del__(self):
@@ -92,6 +98,17 @@ class PagedAttentionPlan:
         Returns `out` in the query's shape, with `return_lse` also the fp32 `[num_tokens, Hq]` logarithms of the
         softmax sums. `out` / `lse` may be contiguous buffers of the caller's; without one, rows
         behind the last request are not initialised. Launches on the current stream of the plan's device."""
+        fast = self._fast_run
+        if fast is not None and lse is None:
+            # layouts checked and tensors allocated in C++; 1 = not a layout it knows: the checks below name what is wrong
+            stream = _raw_stream(self._dev_index)
+            if stream == self._stream:
+                got = fast(self._plan, self.num_tokens, self.Hq, self.H, self.D, self.page_size, self._dtype_code,
+                           self._dev_index, query, paged_kv_cache, out, return_lse, stream)
+                if type(got) is not int:
+                    return got
+                if got < 0:
+                    _lib.check(got)
         for t, n in ((query, "query"), (paged_kv_cache, "paged_kv_cache")):
             _require_gpu(t, n)
             if t.dtype != self.dtype or t.device != self.device:
@@ -143,6 +160,17 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: torch.Tensor, qo_indptr
                     out: Optional[torch.Tensor] = None, return_lse: bool = False, kv_layout: str = "NHD"):
     """`PagedAttentionPlan` made and run once: attention of one layer with index tensors that
     serve no other (a model's layers share a plan). Arguments and results are the plan's."""
+    fast = _lib.fast_entry("paged_attention")
+    if fast is not None and kv_layout == "NHD" and isinstance(paged_kv_cache, torch.Tensor) and paged_kv_cache.is_cuda:
+        # common layouts: checked and launched from C++ (1 = not one of them: fall through)
+        dev = paged_kv_cache.device.index
+        got = fast(query, paged_kv_cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len or 0, shared_pages,
+                   (paged_kv_cache.shape[-1] or 1) ** -0.5 if sm_scale is None else sm_scale, out, return_lse, dev,
+                   _raw_stream(dev))
+        if type(got) is not int:
+            return got
+        if got < 0:
+            _lib.check(got)
     for t, n in ((query, "query"), (paged_kv_cache, "paged_kv_cache")):
         _require_gpu(t, n)
     if paged_kv_cache.dim() != 5 or paged_kv_cache.shape[1] != 2:

@@ -44,7 +44,7 @@
 namespace {
 
 constexpr long NOT_FAST = 1;
-constexpr long kInterface = 2;  // changes with the names or arguments of the functions below; _lib.py checks it
+constexpr long kInterface = 3;  // changes with the names or arguments of the functions below; _lib.py checks it
 
 bool as_ptr(PyObject* o, void** out) {
   if (o == Py_None) {
@@ -372,6 +372,267 @@ PyObject* fast_rotary_append_paged(PyObject*, PyObject* const* args, Py_ssize_t 
       cs->sizes()[1] / 2, qs, ks, vs, qo->data_ptr(), ko ? ko->data_ptr() : nullptr, qw, row, c->data_ptr(),
       (const int32_t*)ind->data_ptr(), (const int32_t*)ptr->data_ptr(), ptr->sizes()[0] - 1,
       ind->sizes()[0], page_size, ps, num_pages, kd, stream));
+}
+
+bool as_f32(PyObject* o, float* out) {
+  const double d = PyFloat_AsDouble(o);
+  *out = (float)d;
+  return !(d == -1.0 && PyErr_Occurred());
+}
+
+// a norm's weight: [head_dim], dense
+bool head_weight(const at::Tensor& w, int64_t dim, at::ScalarType type, int device) {
+  return w.is_cuda() && w.device().index() == device && w.scalar_type() == type && w.dim() == 1 && w.sizes()[0] == dim &&
+         (dim <= 1 || w.strides()[0] == 1);
+}
+
+// (query_out, key_out or None)
+PyObject* rotated(at::Tensor&& qo, at::Tensor&& ko) {
+  PyObject* k = nullptr;
+  if (ko.defined()) {
+    k = THPVariable_Wrap(std::move(ko));
+  } else {
+    k = Py_None;
+    Py_INCREF(k);
+  }
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(qo)), k);
+}
+
+/* qk_norm(query, key, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps, device, stream
+ *         [, value, cache, return_key, slots | batch_indices, kv_indices, kv_indptr, kv_last_page_len])
+ * -> 1, a negative kvc_status, or (query_out, key_out | None): kvc_qk_norm_rotary_pos_emb, _and_cache or
+ * _and_append_paged into new dense tensors */
+PyObject* fast_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10 && nargs != 14 && nargs != 17) {
+    PyErr_SetString(PyExc_TypeError, "qk_norm takes 10, 14 or 17 arguments");
+    return nullptr;
+  }
+  int64_t head_dim, device;
+  float eps;
+  void* stream;
+  if (!as_i64(args[6], &head_dim) || !as_f32(args[7], &eps) || !as_i64(args[8], &device) || !as_ptr(args[9], &stream)) return nullptr;
+  const at::Tensor* t[6];
+  for (int i = 0; i < 6; ++i)
+    if (!(t[i] = tensor_of(args[i]))) return PyLong_FromLong(NOT_FAST);
+  const at::Tensor &q = *t[0], &k = *t[1], &qw = *t[2], &kw = *t[3], &pos = *t[4], &cs = *t[5];
+  const int dev = (int)device;
+  const at::ScalarType type = q.scalar_type();
+  const int kd = kvc_dtype_of(type);
+  if (kd < 0 || head_dim <= 0 || !on_current_device(dev) || !cos_sin_table(cs, type, dev) || !head_weight(qw, head_dim, type, dev) ||
+      !head_weight(kw, head_dim, type, dev))
+    return PyLong_FromLong(NOT_FAST);
+  const bool pos64 = pos.scalar_type() == at::kLong;
+  if (!index_array(pos, dev, pos64 ? at::kLong : at::kInt)) return PyLong_FromLong(NOT_FAST);
+  const int64_t n = pos.sizes()[0];
+  int64_t q_width, qs, k_width, ks;
+  if (n == 0 || !token_rows(q, n, type, dev, &q_width, &qs) || !token_rows(k, n, type, dev, &k_width, &ks) || q_width % head_dim ||
+      k_width % head_dim)
+    return PyLong_FromLong(NOT_FAST);
+  const at::Tensor *v = nullptr, *c = nullptr, *x[4] = {};
+  int return_key = 1, slot_bytes = 8;
+  int64_t v_width, vs = 0, page_size = 0, num_pages = 0, stride = 0;
+  if (nargs > 10) {
+    v = tensor_of(args[10]);
+    c = tensor_of(args[11]);
+    return_key = PyObject_IsTrue(args[12]);
+    if (return_key < 0) return nullptr;
+    for (int i = 0; i < nargs - 13; ++i)
+      if (!(x[i] = tensor_of(args[13 + i]))) return PyLong_FromLong(NOT_FAST);
+    if (!v || !c || c->dim() != 5 || !token_rows(*v, n, type, dev, &v_width, &vs) || v_width != k_width) return PyLong_FromLong(NOT_FAST);
+    page_size = c->sizes()[2];
+    stride = page_stride(*c, page_size, k_width / head_dim, head_dim, (int)type, dev, &num_pages);
+    if (stride < 0) return PyLong_FromLong(NOT_FAST);
+    if (nargs == 14) {
+      slot_bytes = x[0]->scalar_type() == at::kLong ? 8 : 4;
+      if (!index_array(*x[0], dev, slot_bytes == 8 ? at::kLong : at::kInt) || x[0]->sizes()[0] != n) return PyLong_FromLong(NOT_FAST);
+    } else {
+      for (int i = 0; i < 4; ++i)
+        if (!index_array(*x[i], dev, at::kInt)) return PyLong_FromLong(NOT_FAST);
+      if (pos64 || x[0]->sizes()[0] != n || x[2]->sizes()[0] < 1) return PyLong_FromLong(NOT_FAST);
+    }
+  }
+  at::Tensor qo, ko;
+  {
+    pybind11::gil_scoped_release no_lock;  // the allocator may wait
+    qo = dense_like(q);
+    if (return_key) ko = dense_like(k);
+  }
+  void* const ko_data = return_key ? ko.data_ptr() : nullptr;
+  const int64_t hq = q_width / head_dim, hk = k_width / head_dim, rd = cs.sizes()[1] / 2, mp = cs.sizes()[0];
+  int rc;
+  if (nargs == 10) {
+    rc = kvc_qk_norm_rotary_pos_emb(q.data_ptr(), k.data_ptr(), qw.data_ptr(), kw.data_ptr(), eps, pos.data_ptr(), pos64 ? 8 : 4,
+                                    cs.data_ptr(), mp, n, hq, hk, head_dim, rd, qs, ks, qo.data_ptr(), ko_data, q_width, k_width,
+                                    kd, stream);
+  } else if (nargs == 14) {
+    char* kc = (char*)c->data_ptr();
+    rc = kvc_qk_norm_rotary_pos_emb_and_cache(
+        q.data_ptr(), k.data_ptr(), v->data_ptr(), qw.data_ptr(), kw.data_ptr(), eps, pos.data_ptr(), pos64 ? 8 : 4, cs.data_ptr(),
+        mp, n, hq, hk, head_dim, rd, qs, ks, vs, qo.data_ptr(), ko_data, q_width, k_width, kc,
+        kc + page_size * k_width * (int64_t)c->element_size(), x[0]->data_ptr(), slot_bytes, page_size, stride, k_width, num_pages,
+        kd, stream);
+  } else {
+    rc = kvc_qk_norm_rotary_pos_emb_and_append_paged(
+        q.data_ptr(), k.data_ptr(), v->data_ptr(), qw.data_ptr(), kw.data_ptr(), eps, (const int32_t*)x[0]->data_ptr(),
+        (const int32_t*)pos.data_ptr(), cs.data_ptr(), mp, n, hq, hk, head_dim, rd, qs, ks, vs, qo.data_ptr(), ko_data, q_width,
+        k_width, c->data_ptr(), (const int32_t*)x[1]->data_ptr(), (const int32_t*)x[2]->data_ptr(), x[2]->sizes()[0] - 1,
+        x[1]->sizes()[0], page_size, stride, num_pages, kd, stream);
+  }
+  if (rc < 0) return PyLong_FromLong(rc);
+  return rotated(std::move(qo), std::move(ko));
+  END_HANDLE_TH_ERRORS
+}
+
+/* rotary_plan_run_norm(plan, nnz, q_heads, heads, dim, page_size, dtype, device, query, key, value, query_out | None,
+ *                      key_out | None, return_key, cache, query_weight, key_weight, eps, stream)
+ * -> 1, a negative kvc_status, or (query_out, key_out | None): kvc_rotary_plan_run_norm on tensors */
+PyObject* fast_rotary_plan_run_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  void *plan, *stream;
+  int64_t nnz, q_heads, heads, dim, page_size, dtype, device;
+  float eps;
+  if (nargs != 19) {
+    PyErr_SetString(PyExc_TypeError, "rotary_plan_run_norm takes 19 arguments");
+    return nullptr;
+  }
+  const int return_key = PyObject_IsTrue(args[13]);
+  if (!as_ptr(args[0], &plan) || !as_i64(args[1], &nnz) || !as_i64(args[2], &q_heads) || !as_i64(args[3], &heads) ||
+      !as_i64(args[4], &dim) || !as_i64(args[5], &page_size) || !as_i64(args[6], &dtype) || !as_i64(args[7], &device) ||
+      return_key < 0 || !as_f32(args[17], &eps) || !as_ptr(args[18], &stream))
+    return nullptr;
+  const at::Tensor *q = tensor_of(args[8]), *k = tensor_of(args[9]), *v = tensor_of(args[10]), *c = tensor_of(args[14]),
+                   *qw = tensor_of(args[15]), *kw = tensor_of(args[16]);
+  const at::Tensor* qo = args[11] == Py_None ? nullptr : tensor_of(args[11]);
+  const at::Tensor* ko = args[12] == Py_None ? nullptr : tensor_of(args[12]);
+  if (!q || !k || !v || !c || !qw || !kw || (args[11] != Py_None && !qo) || (args[12] != Py_None && !ko)) return PyLong_FromLong(NOT_FAST);
+  const int64_t q_row = q_heads * dim, kv_row = heads * dim;
+  const int dt = (int)dtype, dev = (int)device;
+  const at::ScalarType type = (at::ScalarType)dt;
+  if (!on_current_device(dev)) return PyLong_FromLong(NOT_FAST);
+  const int64_t qs = row_stride(*q, nnz, q_row, dt, dev), ks = row_stride(*k, nnz, kv_row, dt, dev),
+                vs = row_stride(*v, nnz, kv_row, dt, dev);
+  if (qs < 0 || ks < 0 || vs < 0 || !head_weight(*qw, dim, type, dev) || !head_weight(*kw, dim, type, dev) ||
+      (qo && row_stride(*qo, nnz, q_row, dt, dev) != q_row) || (ko && row_stride(*ko, nnz, kv_row, dt, dev) != kv_row))
+    return PyLong_FromLong(NOT_FAST);
+  int64_t num_pages = 0;
+  const int64_t ps = page_stride(*c, page_size, heads, dim, dt, dev, &num_pages);
+  if (ps < 0 || nnz == 0) return PyLong_FromLong(NOT_FAST);
+  at::Tensor q_out, k_out;
+  {
+    pybind11::gil_scoped_release no_lock;  // the allocator may wait
+    const auto rows = [&](int64_t width) { return at::empty({nnz, width}, at::TensorOptions().dtype(type).device(q->device())); };
+    q_out = qo ? *qo : rows(q_row);
+    if (ko) k_out = *ko;
+    else if (return_key) k_out = rows(kv_row);
+  }
+  const int rc = kvc_rotary_plan_run_norm((const kvc_rotary_plan*)plan, q->data_ptr(), k->data_ptr(), v->data_ptr(), qw->data_ptr(),
+                                          kw->data_ptr(), eps, qs, ks, vs, q_out.data_ptr(),
+                                          k_out.defined() ? k_out.data_ptr() : nullptr, c->data_ptr(), ps, num_pages, stream);
+  if (rc < 0) return PyLong_FromLong(rc);
+  return rotated(std::move(q_out), std::move(k_out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A plan's run into new tensors (or `given`): out, or (out, lse)
+PyObject* attend(const kvc_attention_plan* plan, const at::Tensor& q, int64_t q_stride, int64_t tokens, int64_t q_heads, int64_t dim,
+                 const at::Tensor& c, int64_t pages, int64_t stride, const at::Tensor* given, bool with_lse, void* stream) {
+  at::Tensor out, lse, work;
+  {
+    pybind11::gil_scoped_release no_lock;  // the allocator may wait
+    out = given ? *given : dense_like(q);
+    const auto on_device = at::TensorOptions().device(q.device());
+    if (with_lse) lse = at::empty({tokens, q_heads}, on_device.dtype(at::kFloat));
+    work = at::empty({kvc_attention_workspace_bytes(plan)}, on_device.dtype(at::kByte));
+  }
+  const int rc = kvc_attention_plan_run(plan, q.data_ptr(), q_stride, c.data_ptr(), stride, pages, out.data_ptr(),
+                                        with_lse ? lse.data_ptr<float>() : nullptr, work.data_ptr(), work.numel(), stream);
+  if (rc < 0) return PyLong_FromLong(rc);
+  if (!with_lse) return THPVariable_Wrap(std::move(out));
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
+}
+
+/* attention_plan_run(plan, tokens, q_heads, heads, dim, page_size, dtype, device, query, cache, out | None, return_lse, stream)
+ * -> 1, a negative kvc_status, out or (out, lse): kvc_attention_plan_run on tensors */
+PyObject* fast_attention_plan_run(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  void *plan, *stream;
+  int64_t tokens, q_heads, heads, dim, page_size, dtype, device;
+  if (nargs != 13) {
+    PyErr_SetString(PyExc_TypeError, "attention_plan_run takes 13 arguments");
+    return nullptr;
+  }
+  const int with_lse = PyObject_IsTrue(args[11]);
+  if (!as_ptr(args[0], &plan) || !as_i64(args[1], &tokens) || !as_i64(args[2], &q_heads) || !as_i64(args[3], &heads) ||
+      !as_i64(args[4], &dim) || !as_i64(args[5], &page_size) || !as_i64(args[6], &dtype) || !as_i64(args[7], &device) ||
+      with_lse < 0 || !as_ptr(args[12], &stream))
+    return nullptr;
+  const at::Tensor *q = tensor_of(args[8]), *c = tensor_of(args[9]);
+  const at::Tensor* given = args[10] == Py_None ? nullptr : tensor_of(args[10]);
+  if (!q || !c || (args[10] != Py_None && !given) || tokens == 0 || !on_current_device((int)device)) return PyLong_FromLong(NOT_FAST);
+  const int64_t row = q_heads * dim, qs = row_stride(*q, tokens, row, (int)dtype, (int)device);
+  int64_t pages = 0;
+  const int64_t ps = page_stride(*c, page_size, heads, dim, (int)dtype, (int)device, &pages);
+  if (qs < 0 || ps < 0 || (q->dim() == 3 && q->sizes()[2] != dim) || qs % 8 || (uintptr_t)q->data_ptr() % 16 ||
+      (given && (row_stride(*given, tokens, row, (int)dtype, (int)device) != row)))
+    return PyLong_FromLong(NOT_FAST);
+  return attend((const kvc_attention_plan*)plan, *q, qs, tokens, q_heads, dim, *c, pages, ps, given, with_lse, stream);
+  END_HANDLE_TH_ERRORS
+}
+
+/* paged_attention(query, cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len, shared_pages, sm_scale,
+ *                 out | None, return_lse, device, stream) -> 1, a negative kvc_status, out or (out, lse): a plan made, built,
+ * run once and given back (through the interpreter 27 us a call, so 15 for one request) */
+PyObject* fast_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  int64_t max_q_len, shared_pages, device;
+  float scale;
+  void* stream;
+  if (nargs != 13) {
+    PyErr_SetString(PyExc_TypeError, "paged_attention takes 13 arguments");
+    return nullptr;
+  }
+  const int with_lse = PyObject_IsTrue(args[10]);
+  if (!as_i64(args[6], &max_q_len) || !as_i64(args[7], &shared_pages) || !as_f32(args[8], &scale) || with_lse < 0 ||
+      !as_i64(args[11], &device) || !as_ptr(args[12], &stream))
+    return nullptr;
+  const at::Tensor* t[6];
+  for (int i = 0; i < 6; ++i)
+    if (!(t[i] = tensor_of(args[i]))) return PyLong_FromLong(NOT_FAST);
+  const at::Tensor &q = *t[0], &c = *t[1], &qo = *t[2], &ind = *t[3], &ptr = *t[4], &last = *t[5];
+  const at::Tensor* given = args[9] == Py_None ? nullptr : tensor_of(args[9]);
+  const int dev = (int)device;
+  if ((args[9] != Py_None && !given) || !on_current_device(dev) || c.dim() != 5 || (q.dim() != 2 && q.dim() != 3))
+    return PyLong_FromLong(NOT_FAST);
+  for (int i = 2; i < 6; ++i)
+    if (!index_array(*t[i], dev, at::kInt)) return PyLong_FromLong(NOT_FAST);
+  const at::ScalarType type = q.scalar_type();
+  const int64_t batch = last.sizes()[0], tokens = q.sizes()[0], page_size = c.sizes()[2], heads = c.sizes()[3], dim = c.sizes()[4];
+  const int64_t row = q.dim() == 3 ? q.sizes()[1] * q.sizes()[2] : q.sizes()[1];
+  int64_t pages = 0;
+  const int64_t qs = row_stride(q, tokens, row, (int)type, dev), ps = page_stride(c, page_size, heads, dim, (int)type, dev, &pages);
+  if (kvc_dtype_of(type) < 0 || tokens == 0 || qs < 0 || ps < 0 || dim == 0 || row % dim || (q.dim() == 3 && q.sizes()[2] != dim) ||
+      qo.sizes()[0] != batch + 1 || ptr.sizes()[0] != batch + 1 || qs % 8 || (uintptr_t)q.data_ptr() % 16 ||
+      (given && row_stride(*given, tokens, row, (int)type, dev) != row))
+    return PyLong_FromLong(NOT_FAST);
+  kvc_attention_plan* plan = nullptr;
+  int rc = kvc_attention_plan_create((const int32_t*)qo.data_ptr(), (const int32_t*)ind.data_ptr(), (const int32_t*)ptr.data_ptr(),
+                                     (const int32_t*)last.data_ptr(), batch, tokens, ind.sizes()[0], row / dim, heads, dim, page_size,
+                                     max_q_len, shared_pages, scale, kvc_dtype_of(type), &plan);
+  if (rc < 0) return PyLong_FromLong(rc);
+  struct Owner {
+    kvc_attention_plan* p;
+    ~Owner() { kvc_attention_plan_destroy(p); }
+  } owner{plan};
+  at::Tensor buffer;
+  {
+    pybind11::gil_scoped_release no_lock;  // the allocator may wait
+    buffer = at::empty({kvc_attention_plan_bytes(plan)}, at::TensorOptions().dtype(at::kByte).device(q.device()));
+  }
+  rc = kvc_attention_plan_build(plan, buffer.data_ptr(), buffer.numel(), stream);
+  if (rc < 0) return PyLong_FromLong(rc);
+  return attend(plan, q, qs, tokens, row / dim, dim, c, pages, ps, given, with_lse, stream);
+  END_HANDLE_TH_ERRORS
 }
 
 // ---- a step's requests, read where the scheduler's objects lie ---------------------------
@@ -823,6 +1084,14 @@ PyMethodDef methods[] = {
      "kvc_rotary_pos_emb on tensors; 0, 1 = not the fast layout, or a negative kvc_status."},
     {"rotary_append_paged", (PyCFunction)(void (*)(void))fast_rotary_append_paged, METH_FASTCALL,
      "kvc_rotary_pos_emb_and_append_paged on tensors; 0, 1 = not the fast layout, or a negative kvc_status."},
+    {"qk_norm", (PyCFunction)(void (*)(void))fast_qk_norm, METH_FASTCALL,
+     "kvc_qk_norm_rotary_pos_emb and its forms on tensors; the outputs, 1 = not the fast layout, or a negative kvc_status."},
+    {"rotary_plan_run_norm", (PyCFunction)(void (*)(void))fast_rotary_plan_run_norm, METH_FASTCALL,
+     "kvc_rotary_plan_run_norm on tensors; the outputs, 1 = not the fast layout, or a negative kvc_status."},
+    {"attention_plan_run", (PyCFunction)(void (*)(void))fast_attention_plan_run, METH_FASTCALL,
+     "kvc_attention_plan_run on tensors; the outputs, 1 = not the fast layout, or a negative kvc_status."},
+    {"paged_attention", (PyCFunction)(void (*)(void))fast_paged_attention, METH_FASTCALL,
+     "An attention plan made and run once; the outputs, 1 = not the fast layout, or a negative kvc_status."},
     {"build_index", (PyCFunction)(void (*)(void))fast_build_index, METH_FASTCALL,
      "Requests -> the step's index tensors, one launch; 1 = not what it reads, or a negative kvc_status."},
     {"host_index", (PyCFunction)(void (*)(void))fast_host_index, METH_FASTCALL,

@@ -259,6 +259,15 @@ def qk_norm_rotary_pos_emb(query: torch.Tensor, key: torch.Tensor, query_weight:
     """`rotary_pos_emb` of heads that are normed first, in the same pass: every query and key head `x` becomes
     `x * weight / sqrt(mean(x^2) + eps)`, the weights `[head_dim]` one for the queries and one for the keys,
     in the tensors' dtype. Returns new tensors of the inputs' shapes."""
+    fast = _fast_entry("qk_norm")
+    if fast is not None and isinstance(query, torch.Tensor) and query.is_cuda:
+        # common layouts: checked and launched from C++ (1 = not one of them: fall through)
+        dev = query.device.index
+        got = fast(query, key, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps, dev, _raw_stream(dev))
+        if type(got) is tuple:
+            return got
+        if got < 0:
+            _lib.check(got)
     q2, k2, positions, pos_bytes, kd, T = _prep(query, key, positions, cos_sin_cache, head_dim)
     qw, kw = _norm_weights(query_weight, key_weight, query, head_dim)
     q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
@@ -279,6 +288,15 @@ def qk_norm_rotary_pos_emb_and_cache(query: torch.Tensor, key: torch.Tensor, val
                                      slot_mapping: torch.Tensor, eps: float = 1e-6, return_key: bool = True):
     """`qk_norm_rotary_pos_emb` plus the slot-mapped write of the normed, rotated key and the value, as
     `rotary_pos_emb_and_cache` writes them. Returns `(q_out, k_out)`; `k_out` is None with `return_key=False`."""
+    fast = _fast_entry("qk_norm")
+    if fast is not None and isinstance(query, torch.Tensor) and query.is_cuda:
+        dev = query.device.index
+        got = fast(query, key, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps, dev, _raw_stream(dev),
+                   value, kv_cache, return_key, slot_mapping)
+        if type(got) is tuple:
+            return got
+        if got < 0:
+            _lib.check(got)
     q2, k2, positions, pos_bytes, kd, T = _prep(query, key, positions, cos_sin_cache, head_dim)
     qw, kw = _norm_weights(query_weight, key_weight, query, head_dim)
     v2, nb, bs, H, stride = _value_rows(value, kv_cache, T, k2, query, head_dim, "kv_cache")
@@ -316,6 +334,15 @@ def qk_norm_rotary_pos_emb_and_append_paged(query: torch.Tensor, key: torch.Tens
                                             kv_last_page_len: torch.Tensor, eps: float = 1e-6, return_key: bool = True):
     """`qk_norm_rotary_pos_emb` plus `append_paged_kv_cache` of the normed, rotated key and the value in one launch;
     `positions` (int32) is both the rotation position and the KV position of each token."""
+    fast = _fast_entry("qk_norm")
+    if fast is not None and isinstance(query, torch.Tensor) and query.is_cuda:
+        dev = query.device.index
+        got = fast(query, key, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps, dev, _raw_stream(dev),
+                   value, paged_kv_cache, return_key, batch_indices, kv_indices, kv_indptr, kv_last_page_len)
+        if type(got) is tuple:
+            return got
+        if got < 0:
+            _lib.check(got)
     q2, k2, positions, pos_bytes, kd, T = _prep(query, key, positions, cos_sin_cache, head_dim)
     if pos_bytes != 4:
         raise TypeError("positions must be int32 for page-table addressing")
@@ -413,6 +440,7 @@ class PagedRotaryWritePlan:
                     torch._C._cuda_getCurrentRawStream(self.device.index)))
         fast = _lib.fast()
         self._fast_run = fast.rotary_plan_run if fast else None
+        self._fast_run_norm = fast.rotary_plan_run_norm if fast else None
         self._dtype_code = fast.scalar_type_code(cos_sin_cache) if fast else -1
         self._run = lib.kvc_rotary_plan_run
         self._destroy = lib.kvc_rotary_plan_destroy
@@ -453,7 +481,18 @@ class PagedRotaryWritePlan:
         first, as in `qk_norm_rotary_pos_emb`. Launches on the current stream of the plan's device, which must be the
         current device."""
         normed = query_weight is not None
-        if normed != (key_weight is not None):
+        if normed:
+            if key_weight is None:
+                raise ValueError("query_weight and key_weight come together")
+            if self._fast_run_norm is not None:
+                got = self._fast_run_norm(self._plan, self.nnz, self.Hq, self.H, self.D, self.page_size, self._dtype_code,
+                                          self._dev_index, query, key, value, query_out, key_out, return_key,
+                                          paged_kv_cache, query_weight, key_weight, eps, self._get_stream(self._dev_index))
+                if type(got) is tuple:
+                    return got
+                if got < 0:
+                    _lib.check(got)
+        elif key_weight is not None:
             raise ValueError("query_weight and key_weight come together")
         if query_out is None:
             query_out = torch.empty((self.nnz, self.q_row), dtype=self.dtype, device=self.device)
