@@ -60,14 +60,11 @@ constexpr float kLog2e = 1.44269504088896340736f;
 //   neighbours in the list and run on one XCD, whose L2 the range then comes to once. (Shares of a line put them at
 //   different keys: 2048 new tokens behind contexts of 1024 to 32768 took 1638 us, 900 in this order.)
 // A part of a tile leaves its rows' unfinished result in a slot of the workspace, and the parts are joined at the end.
-struct Request {  // 16 bytes
-  int32_t q_begin, n, len, table;  // first token, tokens, keys, first entry of its block table
-};
 struct Item {  // 32 bytes: a tile or a part of one
   int32_t q_begin;  // first token of the request; -1: the rows of all sharing requests, through shared_tokens
   int32_t row0, rows, table, key_begin, key_end;
   int32_t slot;     // of its partial; -1: the whole tile
-  int32_t pad;
+  int32_t limit;    // keys that the request's first token sees, each further one a key more (less than 1: none)
 };
 struct Parts {  // 16 bytes: of a tile: the slot of the first, and of the c-th further one next + c * step
   int32_t slot, next, step, count;
@@ -87,10 +84,8 @@ struct Header {
 
 struct Layout {  // the plan's device buffer
   Header* header;
-  Request* requests;
   int32_t* shares;         // [B] 1: its leading pages are the shared ones
-  int32_t* limits;         // [T] keys that a token sees
-  int32_t* shared_tokens;  // [T]
+  int2* shared_tokens;     // [T] token, and the keys it sees
   Range* ranges;           // [groups] narrow items of a workgroup
   Item* items[2];          // narrow: tile t's part in workgroup w at t + w: those of a workgroup lie side by side
   Parts* shared_parts;     // of the tiles of the sharing requests' rows
@@ -120,22 +115,24 @@ __device__ __forceinline__ Table tokens_of(const PlanArgs& a, int32_t b) {
   return {begin, clamp(a.qo_indptr[b + 1], begin, a.num_tokens) - begin};
 }
 
-// A workgroup per request: its lengths, its tokens' limits, and whether it begins with the shared pages. Which pages these
-// are is what the first request with few tokens and that many pages holds; a request that holds others is a request by itself,
-// so that the number of shared pages changes how the work is cut and never the result.
-__global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
+__device__ __forceinline__ int32_t keys_of(const PlanArgs& a, int32_t b, int32_t pages) {
+  if (!pages) return 0;
+  const int64_t keys = (int64_t)(pages - 1) * a.page_size + clamp(a.kv_last_page_len[b], 0, a.page_size);
+  return (int32_t)(keys < INT32_MAX - kStep ? keys : INT32_MAX - kStep);
+}
+
+// A workgroup per request: does it begin with the shared pages? Which pages these are is what the first request with few
+// tokens and that many pages holds; a request that holds others is a request by itself, so that the number of shared
+// pages changes how the work is cut and never the result. (Of the requests of many rows none share: they read a key for 128
+// rows as it is.)
+__device__ __forceinline__ bool may_share(const PlanArgs& a, int32_t b) {
+  const int32_t n = tokens_of(a, b).pages;
+  return n > 0 && n * a.group <= a.narrow_rows && table_of(a, b).pages >= a.shared_pages;
+}
+__global__ __launch_bounds__(256) void attend_shares_kernel(PlanArgs a) {
   __shared__ int32_t first, differ;
   const int32_t b = blockIdx.x, tid = threadIdx.x;
-  const Table q = tokens_of(a, b), t = table_of(a, b);
-  const int64_t room = (int64_t)t.pages * a.page_size;
-  const int64_t want = t.pages ? room - a.page_size + clamp(a.kv_last_page_len[b], 0, a.page_size) : 0;
-  const int32_t len = (int32_t)(want < INT32_MAX - 64 ? want : INT32_MAX - 64);
-  for (int32_t j = tid; j < q.pages; j += 256) {
-    const int32_t lim = len - q.pages + j + 1;
-    a.l.limits[q.begin + j] = lim > 0 ? lim : 0;
-  }
-  // (of the requests of many rows none: they read a key for 128 rows as it is)
-  bool shares = a.shared_pages > 0 && q.pages > 0 && q.pages * a.group <= a.narrow_rows && t.pages >= a.shared_pages;
+  bool shares = may_share(a, b);
   if (shares) {
     if (tid == 0) {
       first = b;
@@ -143,15 +140,13 @@ __global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
     }
     __syncthreads();
     for (int32_t c0 = 0; c0 < b; c0 += 256) {
-      const int32_t c = c0 + tid;
-      const int32_t n = c < b ? tokens_of(a, c).pages : 0;
-      if (n > 0 && n * a.group <= a.narrow_rows && table_of(a, c).pages >= a.shared_pages) atomicMin(&first, c);
+      if (c0 + tid < b && may_share(a, c0 + tid)) atomicMin(&first, c0 + tid);
       __syncthreads();
       const bool found = first < b;
       __syncthreads();  // everyone has looked before someone lowers it further
       if (found) break;
     }
-    const int32_t* mine = a.kv_indices + t.begin;
+    const int32_t* mine = a.kv_indices + table_of(a, b).begin;
     const int32_t* theirs = a.kv_indices + table_of(a, first).begin;
     bool other = false;
     for (int32_t i = tid; i < a.shared_pages; i += 256) other = other || mine[i] != theirs[i];
@@ -159,43 +154,43 @@ __global__ __launch_bounds__(256) void attend_requests_kernel(PlanArgs a) {
     __syncthreads();
     shares = !differ;
   }
-  if (tid == 0) {
-    a.l.requests[b] = {q.begin, q.pages, len, t.begin};
-    a.l.shares[b] = shares;
-  }
+  if (tid == 0) a.l.shares[b] = shares;
 }
 
-__device__ __forceinline__ int32_t ceil_div(int32_t x, int32_t y) { return (x + y - 1) / y; }
+__device__ __forceinline__ int32_t ceil_div(int32_t x, int32_t y) { return (int32_t)(((uint32_t)x + (uint32_t)y - 1) / (uint32_t)y); }
+__device__ __forceinline__ int32_t round_up(int32_t x, int32_t to) { return ceil_div(x, to) * to; }
 
 // A request's tiles
 struct Tiles {
-  int64_t at;               // narrow: where the first begins on the line of work
+  uint32_t at;              // narrow: where the first begins on the line of work, in units
   int32_t q_begin, n, len, table;
   int32_t begin;            // first key of its own
   int32_t tiles, first;     // and the first's place in its list
   int32_t first_slot;       // wide
   int32_t shared_token0;    // its first token among the sharing ones, or -1
-  bool wide;
+  int32_t wide;
   __device__ __forceinline__ int32_t rows_of_tile() const { return wide ? kWide : kTile; }
   // Work of the narrow tiles before the i-th: each sees tile / group keys more than the one before, and costs something by itself
-  __device__ __forceinline__ int64_t before(int64_t i, int32_t group) const {
+  __device__ __forceinline__ int64_t before(int32_t i, int32_t group) const {
     const int32_t keys = min(len, len - n + ceil_div(kTile, group)) - begin;
-    return i * ((keys > 0 ? keys : 0) + kTileWork) + i * (i - 1) / 2 * kTile / group;
+    const int64_t more = i < 2 ? 0 : (int64_t)i * (i - 1) / 2 * kTile / group;
+    return (int64_t)i * ((keys > 0 ? keys : 0) + kTileWork) + more;
   }
   // Ranges of keys that wide tiles are cut into where none is to be longer than `chunk`
   __device__ __forceinline__ int32_t chunks(int32_t chunk) const { return max(ceil_div(len, chunk), 1); }
 };
 __device__ __forceinline__ Tiles tiles_of(const PlanArgs& a, int32_t b) {
-  const Request r = a.l.requests[b];
+  const Table q = tokens_of(a, b), table = table_of(a, b);
   Tiles t = {};
-  t.q_begin = r.q_begin;
-  t.n = r.n;
-  t.len = r.len;
-  t.table = r.table;
-  t.wide = r.n * a.group > a.narrow_rows;
-  t.shared_token0 = a.l.shares[b] ? 0 : -1;
-  t.begin = a.l.shares[b] ? min(a.shared_pages * a.page_size, r.len) : 0;
-  t.tiles = ceil_div(r.n * a.group, t.rows_of_tile());
+  t.q_begin = q.begin;
+  t.n = q.pages;
+  t.len = keys_of(a, b, table.pages);
+  t.table = table.begin;
+  t.wide = t.n * a.group > a.narrow_rows;
+  const bool shares = a.shared_pages > 0 && a.l.shares[b];
+  t.shared_token0 = shares ? 0 : -1;
+  t.begin = shares ? min(a.shared_pages * a.page_size, t.len) : 0;
+  t.tiles = ceil_div(t.n * a.group, t.rows_of_tile());
   return t;
 }
 
@@ -203,30 +198,34 @@ __device__ __forceinline__ Tiles tiles_of(const PlanArgs& a, int32_t b) {
 struct Cuts {
   int32_t group, count;  // the first part's workgroup, and how many parts there are
 };
-__device__ __forceinline__ Cuts cuts_of(const PlanArgs& a, int64_t at, int64_t work, int64_t share) {
-  const int64_t sliver = min(share / 2, (int64_t)kMinPart);
+__device__ __forceinline__ Cuts cuts_of(const PlanArgs& a, uint32_t at, uint32_t work, uint32_t share, uint32_t sliver) {
   // (the line may end within a sliver of the last share's end)
-  const int64_t first = min((at + sliver - 1) / share, (int64_t)a.groups - 1), last = (at + work - sliver) / share;
-  return {(int32_t)first, (int32_t)(last > first ? last - first : 0) + 1};
+  const int32_t first = min((int32_t)((at + sliver - 1) / share), a.groups - 1);
+  const int32_t last = at + work < sliver ? 0 : (int32_t)((at + work - sliver) / share);
+  return {first, (last > first ? last - first : 0) + 1};
 }
 // Rows of an entry: one of many parts is by itself
 __device__ __forceinline__ int32_t joined_rows(int32_t parts) { return parts > kManyParts ? 1 : kTile; }
-__device__ __forceinline__ int32_t round_up(int32_t x, int32_t to) { return ceil_div(x, to) * to; }
 
 // One workgroup: the share and the wide tiles' ranges, from all the work there is; where each request's tiles begin, by a scan;
-// the lists.
+// the lists. The line of work is measured in units of as many keys as let it end below 2^30. A thread does a request of
+// few items, a wavefront one of many.
 __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
-  constexpr int SUMS = 4;  // narrow tiles, wide items, wide slots, sharing tokens
+  constexpr int SUMS = 5;  // narrow work, narrow tiles, wide items, wide slots, sharing tokens
+  constexpr int kFew = 4;  // items of a request that its thread does
   __shared__ unsigned long long narrow_work, wide_work, best;
-  __shared__ int64_t wave_work[16], carry_work;
-  __shared__ int32_t wave_sums[16][SUMS], carry[SUMS], shared_tokens, some_request, narrow_entries, wide_entries, longest;
+  __shared__ int32_t wave_sums[16][SUMS], carry[SUMS], shared_tokens, some_request, entries[2], longest, num_wide, num_long;
   __shared__ int32_t first_item[kMaxGroups], last_item[kMaxGroups];
-  __shared__ Tiles cached[1024];
+  __shared__ int2 wide_tiles[1024];  // tiles and keys of wide requests (as many as there is room for)
+  __shared__ Tiles long_requests[1024];
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Tiles mine = {};
+  mine.shared_token0 = -1;
+  if (tid < a.batch_size) mine = tiles_of(a, tid);
   if (tid == 0) {
     narrow_work = wide_work = 0;
     best = ~0ull;
-    shared_tokens = narrow_entries = wide_entries = longest = 0;
+    shared_tokens = entries[0] = entries[1] = longest = num_wide = 0;
     some_request = INT32_MAX;
   }
   for (int32_t w = tid; w < a.groups; w += 1024) {
@@ -235,11 +234,13 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
   }
   __syncthreads();
   for (int32_t b = tid; b < a.batch_size; b += 1024) {
-    const Tiles t = tiles_of(a, b);
+    const Tiles t = b < 1024 ? mine : tiles_of(a, b);
     if (t.tiles && !t.wide) atomicAdd(&narrow_work, (unsigned long long)t.before(t.tiles, a.group));
     if (t.wide) {
       atomicAdd(&wide_work, (unsigned long long)t.tiles * t.len);
       atomicMax(&longest, t.len);
+      const int32_t at = atomicAdd(&num_wide, 1);
+      if (at < 1024) wide_tiles[at] = make_int2(t.tiles, t.len);
     }
     if (t.shared_token0 >= 0) {
       atomicAdd(&shared_tokens, t.n);
@@ -250,26 +251,27 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
   const int32_t shared_rows = shared_tokens * a.group, shared_len = a.shared_pages * a.page_size;
   const bool shared_wide = shared_rows > a.narrow_shared_rows;
   const int32_t shared_tile = shared_wide ? kWide : kTile, shared_tiles = ceil_div(shared_rows, shared_tile);
-  const int64_t shared_work = shared_len + kTileWork;  // of a narrow tile
-  const int64_t share = max(((int64_t)narrow_work + (shared_wide ? 0 : shared_tiles * shared_work) + a.groups - 1) / a.groups, (int64_t)kMinShare);
+  const int64_t all_narrow = (int64_t)narrow_work + (shared_wide ? 0 : shared_tiles * ((int64_t)shared_len + kTileWork));
+  const int32_t unit = max(0, 34 - (int32_t)__clzll((unsigned long long)all_narrow + 1));  // log2 of the keys of a unit
+  const uint32_t shared_work = (uint32_t)(((int64_t)shared_len + kTileWork) >> unit);      // of a narrow tile
+  // (rounding down tile by tile, the line is no longer than this)
+  const uint32_t share = max(ceil_div((int32_t)(all_narrow >> unit), a.groups), max(kMinShare >> unit, 1));
+  const uint32_t sliver = max(min(share / 2, (uint32_t)(kMinPart >> unit)), 1u);
 
   // The wide tiles' ranges: of lengths that make from a 16th of a round of the card to 4 of them, the one that ends soonest.
   // Every round lasts as long as a range, and what an item costs beside its keys, more so where it leaves a partial.
   int32_t chunk = 1 << 30;
   const int64_t all_wide = (int64_t)wide_work + (shared_wide ? (int64_t)shared_tiles * shared_len : 0);
   if (all_wide) {
-    const int32_t most = max(longest, shared_wide ? shared_len : 0);
+    const int32_t most = max(longest, shared_wide ? shared_len : 0), listed = min(num_wide, 1024);
     const auto chunk_of = [&](int32_t x) {
-      const int64_t keys = (all_wide * 16 + (int64_t)a.residents * (x + 1) - 1) / ((int64_t)a.residents * (x + 1));
+      const double keys = __builtin_ceil((double)all_wide * 16 / ((double)a.residents * (x + 1)));
       return round_up((int32_t)(keys < kMinChunk ? kMinChunk : keys < (1 << 30) ? keys : 1 << 30), kStep);
     };
     for (int32_t x = wave; x < 64; x += 16) {
       const int32_t keys = chunk_of(x);
       int32_t items = 0;
-      for (int32_t b = lane; b < a.batch_size; b += 64) {
-        const Tiles t = tiles_of(a, b);
-        if (t.wide) items += t.tiles * t.chunks(keys);
-      }
+      for (int32_t i = lane; i < listed; i += 64) items += wide_tiles[i].x * max(ceil_div(wide_tiles[i].y, keys), 1);
       for (int d = 32; d; d >>= 1) items += __shfl_xor(items, d);
       if (shared_wide) items += shared_tiles * ceil_div(shared_len, keys);
       const int64_t each = min(keys, most) + (keys < most ? kWidePartWork : kWideTileWork);
@@ -281,10 +283,10 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
   }
   const int32_t shared_chunks = shared_rows && shared_wide ? ceil_div(shared_len, chunk) : 0, shared_items = shared_tiles * shared_chunks;
   if (tid == 0) {
-    carry_work = shared_wide ? 0 : shared_tiles * shared_work;
-    carry[0] = shared_wide ? 0 : shared_tiles;
-    carry[1] = carry[2] = shared_items;
-    carry[3] = 0;
+    carry[0] = shared_wide ? 0 : shared_tiles * shared_work;
+    carry[1] = shared_wide ? 0 : shared_tiles;
+    carry[2] = carry[3] = shared_items;
+    carry[4] = 0;
   }
   __syncthreads();
 
@@ -297,22 +299,22 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     atomicMax(&last_item[group], at);
   };
   // the first key of a narrow tile's c-th part: the share of its work before the cut, in whole blocks
-  const auto cut_key = [&](int64_t at, int64_t work, const Cuts& p, int32_t c, int32_t begin, int32_t end) {
+  const auto cut_key = [&](uint32_t at, uint32_t work, const Cuts& p, int32_t c, int32_t begin, int32_t end) {
     if (c == 0) return begin;
     if (c == p.count) return end;
-    const int64_t before = ((int64_t)(p.group + c) * share - at) * (end - begin) / work;
-    return begin + min((int32_t)((before + kStep / 2) / kStep * kStep), end - begin);
+    const double before = (double)((uint64_t)(p.group + c) * share - at) * (end - begin) / work;
+    return begin + clamp(((int32_t)before + kStep / 2) / kStep * kStep, 0, end - begin);
   };
 
   if (shared_rows) {
-    const int32_t table = a.l.requests[some_request].table;
+    const int32_t table = table_of(a, some_request).begin;
     const int32_t each = shared_wide ? round_up(ceil_div(shared_len, shared_chunks), kStep) : 0;
     for (int32_t i = tid; i < shared_tiles; i += 1024) {
       const int32_t row0 = i * shared_tile, rows = min(shared_tile, shared_rows - row0);
       if (shared_wide) {
         a.l.shared_parts[i] = {i, i, shared_tiles, ceil_div(shared_len, each)};
       } else {
-        const Cuts p = cuts_of(a, i * shared_work, shared_work, share);
+        const Cuts p = cuts_of(a, i * shared_work, shared_work, share, sliver);
         a.l.shared_parts[i] = {2 * a.groups + i, 2 * p.group, 2, p.count};
         for (int32_t c = 0; c < p.count; ++c)
           put(i, p.group + c,
@@ -326,104 +328,103 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     }
   }
 
-  for (int32_t b0 = 0; b0 < a.batch_size; b0 += 1024) {
-    const int32_t b = b0 + tid;
-    Tiles t = {};
-    t.shared_token0 = -1;
-    if (b < a.batch_size) t = tiles_of(a, b);
-    const int32_t chunks = t.wide ? t.chunks(chunk) : 0;
-    const int64_t work = t.tiles && !t.wide ? t.before(t.tiles, a.group) : 0;
-    const int32_t sums[SUMS] = {t.wide ? 0 : t.tiles, t.tiles * chunks, chunks > 1 ? t.tiles * chunks : 0, t.shared_token0 >= 0 ? t.n : 0};
-    int64_t work_to = work;  // inclusive
-    int32_t sums_to[SUMS] = {sums[0], sums[1], sums[2], sums[3]};
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t x = __shfl_up((long long)work_to, d);
-      if (lane >= d) work_to += x;
-#pragma unroll
-      for (int i = 0; i < SUMS; ++i) {
-        const int32_t y = __shfl_up(sums_to[i], d);
-        if (lane >= d) sums_to[i] += y;
+  // A request's lists, by `lanes` lanes over its tiles, or over the parts where there are few tiles
+  const auto lay_out = [&](const Tiles& r, int32_t lane, int32_t lanes) {
+    const int32_t rows = r.n * a.group, limit = r.len - r.n + 1;
+    const bool sh = r.shared_token0 >= 0;
+    // keys that a tile's last row sees
+    const auto end_of = [&](int32_t last_row) { return clamp(limit + last_row / a.group, r.begin, r.len); };
+    if (r.wide) {
+      const int32_t parts = r.chunks(chunk), each = round_up(max(ceil_div(r.len, parts), 1), kStep);
+      for (int32_t i = lane; i < r.tiles * parts; i += lanes) {
+        const int32_t c = i / r.tiles, row0 = (i - c * r.tiles) * kWide, last_row = min(row0 + kWide, rows) - 1;
+        const int32_t end = end_of(last_row), from = min(c * each, end), to = min(from + each, end);
+        // (a range that a tile sees nothing of is an item without rows)
+        if (r.first + i < a.max_items[1])
+          a.l.items[1][r.first + i] = {r.q_begin, row0, c && from == to ? 0 : last_row + 1 - row0, r.table, from, to,
+                                       end > each ? r.first_slot + i : -1, limit};
+      }
+      if (parts > 1)
+        for (int32_t i = lane; i < r.tiles; i += lanes) {
+          const int32_t row0 = i * kWide, count = ceil_div(end_of(min(row0 + kWide, rows) - 1), each);
+          if (count < 2) continue;
+          const int32_t lines = joined_rows(count), tile_rows = min(kWide, rows - row0);
+          int32_t to = a.max_entries - 1 - atomicAdd(&entries[1], ceil_div(tile_rows, lines));
+          for (int32_t e = 0; e < tile_rows && to >= 0; e += lines)
+            a.l.entries[to--] = {r.q_begin, row0 + e, (int16_t)min(lines, tile_rows - e), lines == 1, -1,
+                                 {r.first_slot + i, r.first_slot + i, r.tiles, count}};
+        }
+      return;
+    }
+    const bool by_parts = r.tiles < 8;
+    for (int32_t i = by_parts ? 0 : lane; i < r.tiles; i += by_parts ? 1 : lanes) {
+      const uint32_t before = (uint32_t)(r.before(i, a.group) >> unit), at = r.at + before;
+      const uint32_t tile_work = (uint32_t)(r.before(i + 1, a.group) >> unit) - before;
+      const Cuts p = cuts_of(a, at, tile_work, share, sliver);
+      const int32_t row0 = i * kTile, last_row = min(row0 + kTile, rows) - 1, end = end_of(last_row);
+      const int32_t slot = sh ? 2 * a.groups + r.first + i : p.count > 1 ? 2 * p.group + 1 : -1;
+      for (int32_t c = by_parts ? lane : 0; c < p.count; c += by_parts ? lanes : 1)
+        put(r.first + i, p.group + c,
+            {r.q_begin, row0, last_row + 1 - row0, r.table, cut_key(at, tile_work, p, c, r.begin, end),
+             cut_key(at, tile_work, p, c + 1, r.begin, end), c ? 2 * (p.group + c) : slot, limit});
+      if (slot >= 0 && (!by_parts || lane == 0)) {
+        int32_t parts = p.count;
+        if (sh && shared_wide) parts += shared_chunks;
+        else if (sh) parts += cuts_of(a, (r.shared_token0 * a.group + row0) / kTile * shared_work, shared_work, share, sliver).count;
+        const int32_t lines = joined_rows(parts), tile_rows = last_row + 1 - row0;
+        int32_t to = atomicAdd(&entries[0], ceil_div(tile_rows, lines));
+        for (int32_t e = 0; e < tile_rows && to < a.max_entries; e += lines)
+          a.l.entries[to++] = {r.q_begin, row0 + e, (int16_t)min(lines, tile_rows - e), lines == 1,
+                               sh ? r.shared_token0 * a.group + row0 + e : -1, {slot, 2 * p.group, 2, p.count}};
       }
     }
-    if (lane == 63) {
-      wave_work[wave] = work_to;
-      for (int i = 0; i < SUMS; ++i) wave_sums[wave][i] = sums_to[i];
+    if (sh)
+      for (int32_t i = lane; i < r.n; i += lanes) a.l.shared_tokens[r.shared_token0 + i] = make_int2(r.q_begin + i, limit + i);
+  };
+
+  for (int32_t b0 = 0; b0 < a.batch_size; b0 += 1024) {
+    Tiles t = mine;
+    if (b0) {
+      t = {};
+      t.shared_token0 = -1;
+      if (b0 + tid < a.batch_size) t = tiles_of(a, b0 + tid);
     }
+    const int32_t chunks = t.wide ? t.chunks(chunk) : 0;
+    const int32_t sums[SUMS] = {t.tiles && !t.wide ? (int32_t)(t.before(t.tiles, a.group) >> unit) : 0, t.wide ? 0 : t.tiles,
+                                t.tiles * chunks, chunks > 1 ? t.tiles * chunks : 0, t.shared_token0 >= 0 ? t.n : 0};
+    int32_t sums_to[SUMS];  // inclusive
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i) {
+      sums_to[i] = sums[i];
+      for (int d = 1; d < 64; d <<= 1) {
+        const int32_t x = __shfl_up(sums_to[i], d);
+        if (lane >= d) sums_to[i] += x;
+      }
+      if (lane == 63) wave_sums[wave][i] = sums_to[i];
+    }
+    if (tid == 0) num_long = 0;
     __syncthreads();
-    work_to += carry_work;
-    for (int w = 0; w < wave; ++w) work_to += wave_work[w];
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) {
       sums_to[i] += carry[i];
       for (int w = 0; w < wave; ++w) sums_to[i] += wave_sums[w][i];
     }
-    t.at = work_to - work;
-    t.first = t.wide ? sums_to[1] - sums[1] : sums_to[0] - sums[0];
-    t.first_slot = sums_to[2] - sums[2];
-    if (t.shared_token0 >= 0) t.shared_token0 = sums_to[3] - sums[3];
-    cached[tid] = t;
+    t.at = sums_to[0] - sums[0];
+    t.first = t.wide ? sums_to[2] - sums[2] : sums_to[1] - sums[1];
+    t.first_slot = sums_to[3] - sums[3];
+    if (t.shared_token0 >= 0) t.shared_token0 = sums_to[4] - sums[4];
+    if (t.tiles) {
+      if (!t.wide && t.tiles == 1 && cuts_of(a, t.at, sums[0], share, sliver).count <= kFew) lay_out(t, 0, 1);
+      else long_requests[atomicAdd(&num_long, 1)] = t;
+    }
     __syncthreads();
-    if (tid == 1023) {
-      carry_work = work_to;
+    if (tid == 1023)
       for (int i = 0; i < SUMS; ++i) carry[i] = sums_to[i];
-    }
-
-    // A request to a wavefront, its lanes over the tiles, or over the parts where there are few tiles
-    for (int32_t x = wave; x < min(1024, a.batch_size - b0); x += 16) {
-      const Tiles r = cached[x];
-      const int32_t rows = r.n * a.group;
-      const bool sh = r.shared_token0 >= 0;
-      // keys that the tile's last token sees
-      const auto end_of = [&](int32_t last_row) { return clamp(r.len - r.n + last_row / a.group + 1, r.begin, r.len); };
-      if (r.wide) {
-        const int32_t parts = r.chunks(chunk), each = round_up(max(ceil_div(r.len, parts), 1), kStep);
-        for (int32_t i = lane; i < r.tiles * parts; i += 64) {
-          const int32_t c = i / r.tiles, row0 = (i - c * r.tiles) * kWide, last_row = min(row0 + kWide, rows) - 1;
-          const int32_t end = end_of(last_row), from = min(c * each, end), to = min(from + each, end);
-          // (a range that a tile sees nothing of is an item without rows)
-          if (r.first + i < a.max_items[1])
-            a.l.items[1][r.first + i] = {r.q_begin, row0, c && from == to ? 0 : last_row + 1 - row0, r.table, from, to,
-                                         end > each ? r.first_slot + i : -1, 0};
-        }
-        if (parts > 1)
-          for (int32_t i = lane; i < r.tiles; i += 64) {
-            const int32_t row0 = i * kWide, count = ceil_div(end_of(min(row0 + kWide, rows) - 1), each);
-            if (count < 2) continue;
-            const int32_t lines = joined_rows(count), tile_rows = min(kWide, rows - row0);
-            int32_t to = a.max_entries - 1 - atomicAdd(&wide_entries, ceil_div(tile_rows, lines));
-            for (int32_t e = 0; e < tile_rows && to >= 0; e += lines)
-              a.l.entries[to--] = {r.q_begin, row0 + e, (int16_t)min(lines, tile_rows - e), lines == 1, -1,
-                                   {r.first_slot + i, r.first_slot + i, r.tiles, count}};
-          }
-        continue;
-      }
-      const bool by_parts = r.tiles < 8;
-      for (int32_t i = by_parts ? 0 : lane; i < r.tiles; i += by_parts ? 1 : 64) {
-        const int64_t at = r.at + r.before(i, a.group), tile_work = r.before(i + 1, a.group) - r.before(i, a.group);
-        const Cuts p = cuts_of(a, at, tile_work, share);
-        const int32_t row0 = i * kTile, last_row = min(row0 + kTile, rows) - 1, end = end_of(last_row);
-        const int32_t slot = sh ? 2 * a.groups + r.first + i : p.count > 1 ? 2 * p.group + 1 : -1;
-        for (int32_t c = by_parts ? lane : 0; c < p.count; c += by_parts ? 64 : 1)
-          put(r.first + i, p.group + c,
-              {r.q_begin, row0, last_row + 1 - row0, r.table, cut_key(at, tile_work, p, c, r.begin, end),
-               cut_key(at, tile_work, p, c + 1, r.begin, end), c ? 2 * (p.group + c) : slot, 0});
-        if (slot >= 0 && (!by_parts || lane == 0)) {
-          int32_t parts = p.count;
-          if (sh && shared_wide) parts += shared_chunks;
-          else if (sh) parts += cuts_of(a, (r.shared_token0 * a.group + row0) / kTile * shared_work, shared_work, share).count;
-          const int32_t lines = joined_rows(parts), tile_rows = last_row + 1 - row0;
-          int32_t to = atomicAdd(&narrow_entries, ceil_div(tile_rows, lines));
-          for (int32_t e = 0; e < tile_rows && to < a.max_entries; e += lines)
-            a.l.entries[to++] = {r.q_begin, row0 + e, (int16_t)min(lines, tile_rows - e), lines == 1, sh ? r.shared_token0 * a.group + row0 + e : -1,
-                                 {slot, 2 * p.group, 2, p.count}};
-        }
-      }
-      if (sh)
-        for (int32_t i = lane; i < r.n; i += 64) a.l.shared_tokens[r.shared_token0 + i] = r.q_begin + i;
-    }
+    for (int32_t x = wave; x < num_long; x += 16) lay_out(long_requests[x], lane, 64);
     __syncthreads();
   }
-  if (tid == 0) *a.l.header = {min(carry[1], a.max_items[1]), min(narrow_entries, a.max_entries), min(wide_entries, a.max_entries), shared_wide};
+  if (tid == 0)
+    *a.l.header = {min(carry[2], a.max_items[1]), min(entries[0], a.max_entries), min(entries[1], a.max_entries), shared_wide};
   for (int32_t w = tid; w < a.groups; w += 1024)
     a.l.ranges[w] = last_item[w] < 0 ? Range{0, 0} : Range{first_item[w], last_item[w] + 1};
 }
@@ -726,8 +727,9 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
     tile.odd_from = INT32_MAX;
     if (n < item.rows) {
       const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
-      const int32_t token = item.q_begin >= 0 ? item.q_begin + i : a.l.shared_tokens[i];
-      tile.limit = min(a.l.limits[token], item.key_end);
+      const int2 x = item.q_begin >= 0 ? make_int2(item.q_begin + i, item.limit + i) : a.l.shared_tokens[i];
+      const int32_t token = x.x;
+      tile.limit = clamp(x.y, 0, item.key_end);
       const char* p = a.query + (int64_t)token * a.q_stride + ((int64_t)(h * a.group + g) * D + quad * 8) * 2;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k)
@@ -862,8 +864,9 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
     if (my_row < item.rows) {
       const int32_t row = item.row0 + my_row, i = row / a.group;
       g = row - i * a.group;
-      token = item.q_begin >= 0 ? item.q_begin + i : a.l.shared_tokens[i];
-      limit = min(a.l.limits[token], item.key_end);
+      const int2 x = item.q_begin >= 0 ? make_int2(item.q_begin + i, item.limit + i) : a.l.shared_tokens[i];
+      token = x.x;
+      limit = clamp(x.y, 0, item.key_end);
       const char* p = a.query + (int64_t)token * a.q_stride + ((int64_t)(h * a.group + g) * D + hi * 8) * 2;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k)
@@ -1309,10 +1312,8 @@ Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
     return q;
   };
   l.header = (Header*)take(sizeof(Header));
-  l.requests = (Request*)take(p.batch_size * sizeof(Request));
-  l.shares = (int32_t*)take(p.batch_size * 4);
-  l.limits = (int32_t*)take(p.num_tokens * 4);
-  l.shared_tokens = (int32_t*)take(p.num_tokens * 4);
+  l.shares = (int32_t*)take(p.shared_pages > 0 ? p.batch_size * 4 : 0);
+  l.shared_tokens = (int2*)take(p.shared_pages > 0 ? p.num_tokens * 8 : 0);
   l.ranges = (Range*)take(p.n.groups * sizeof(Range));
   for (int k = 0; k < 2; ++k) l.items[k] = (Item*)take(p.n.max_items[k] * sizeof(Item));
   l.shared_parts = (Parts*)take(p.n.max_shared_tiles * sizeof(Parts));
@@ -1438,7 +1439,7 @@ int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buf
              {(int32_t)plan->n.max_items[0], (int32_t)plan->n.max_items[1]}, (int32_t)plan->n.max_entries,
              layout_of(*plan, plan->buffer, nullptr)};
   hipStream_t s = (hipStream_t)stream;
-  kvc::launch(attend_requests_kernel, dim3((unsigned)plan->batch_size), dim3(256), 0, s, a);
+  if (plan->shared_pages > 0) kvc::launch(attend_shares_kernel, dim3((unsigned)plan->batch_size), dim3(256), 0, s, a);
   kvc::launch(attend_schedule_kernel, dim3(1), dim3(1024), 0, s, a);
   KVC_HIP(hipGetLastError());
   return KVC_OK;
