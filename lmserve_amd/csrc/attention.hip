@@ -42,8 +42,10 @@ constexpr int kStep = 64;          // keys that a workgroup takes at once of a w
 constexpr int kVPad = 64;          // bytes between a wide item's rows of V in LDS
 constexpr int kAhead = 3;          // pieces of a wide item's K and V that are read from LDS ahead of their product
 constexpr int kMaxGroups = 1024;    // workgroups of a key head
-// In keys: what a narrow tile costs beside its own, a workgroup's least share, the least part of a tile
-__device__ constexpr int kTileWork = 64, kMinShare = 512, kMinPart = 256;
+// In keys: what a narrow tile costs beside its own, a workgroup's least share, the least part of a tile. With the least
+// share there are workgroups to spare, and a part is half of it: a short tile in one piece is done sooner than cut
+// and joined (900 keys of one request: 17.4 us whole, 18.6 to 19.7 in two to four). Behind a shared prefix every tile is joined.
+__device__ constexpr int kTileWork = 64, kMinShare = 1024, kMinSharedShare = 256, kMinPart = 256;
 // the least range of a wide tile; what an item costs beside its keys, and what one that leaves a partial does
 __device__ constexpr int kMinChunk = 512, kWideTileWork = 128, kWidePartWork = 384;
 constexpr int kManyParts = 16;     // a row of more partials is joined by a workgroup
@@ -255,8 +257,9 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
   const int32_t unit = max(0, 34 - (int32_t)__clzll((unsigned long long)all_narrow + 1));  // log2 of the keys of a unit
   const uint32_t shared_work = (uint32_t)(((int64_t)shared_len + kTileWork) >> unit);      // of a narrow tile
   // (rounding down tile by tile, the line is no longer than this)
-  const uint32_t share = max(ceil_div((int32_t)(all_narrow >> unit), a.groups), max(kMinShare >> unit, 1));
-  const uint32_t sliver = max(min(share / 2, (uint32_t)(kMinPart >> unit)), 1u);
+  const uint32_t least = max((shared_rows ? kMinSharedShare : kMinShare) >> unit, 1);
+  const uint32_t share = max((uint32_t)ceil_div((int32_t)(all_narrow >> unit), a.groups), least);
+  const uint32_t sliver = max(share <= least ? share / 2 : min(share / 2, (uint32_t)(kMinPart >> unit)), 1u);
 
   // The wide tiles' ranges: of lengths that make from a 16th of a round of the card to 4 of them, the one that ends soonest.
   // Every round lasts as long as a range, and what an item costs beside its keys, more so where it leaves a partial.
@@ -541,6 +544,12 @@ struct GroupIds {
   }
 };
 
+template <bool NT>
+__device__ __forceinline__ u32x4 ld16(const char* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  else return *reinterpret_cast<const u32x4*>(p);
+}
+
 // A block of 32 keys in registers, as loaded
 template <int DP>
 struct Block {
@@ -564,7 +573,7 @@ struct Block {
     }
     return present;
   }
-  template <Reach REACH>
+  template <Reach REACH, bool NT>
   __device__ __forceinline__ void load_k(const AttendArgs& a, const Item& item, const char* heads, int32_t k0, int32_t lane, uint32_t& present) {
     const int32_t n = lane & 15, quad = lane >> 4, D = a.head_dim;
     if constexpr (REACH == kAnyPage) present = 0;
@@ -583,11 +592,11 @@ struct Block {
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
         if (REACH != kGroupsFull) k[i][s] = u32x4{};
-        if (REACH == kGroupsFull || (have && s * 32 + quad * 8 < D)) k[i][s] = *reinterpret_cast<const u32x4*>(row + s * 64);
+        if (REACH == kGroupsFull || (have && s * 32 + quad * 8 < D)) k[i][s] = ld16<NT>(row + s * 64);
       }
     }
   }
-  template <Reach REACH>
+  template <Reach REACH, bool NT>
   __device__ __forceinline__ void load_v(const AttendArgs& a, const Item& item, const char* heads, int32_t k0, int32_t lane) {
     const int32_t vrow = lane / LPR, vcol = lane % LPR, D = a.head_dim;
     const uint32_t at = a.plane + vrow * a.row_stride + vcol * 16;
@@ -604,7 +613,7 @@ struct Block {
         row = rows[i / HALF] + (int64_t)(i % HALF * RPI) * a.row_stride + at;
       }
       if (REACH != kGroupsFull) v[i] = u32x4{};
-      if (REACH == kGroupsFull || (have && vcol * 8 < D)) v[i] = *reinterpret_cast<const u32x4*>(row);
+      if (REACH == kGroupsFull || (have && vcol * 8 < D)) v[i] = ld16<NT>(row);
     }
   }
 };
@@ -709,7 +718,7 @@ struct RowTile {
 template <typename T, int DP>
 constexpr int narrow_lds() { return kWaves * kBlock * RowTile<T, DP>::VSTRIDE + kWaves * 2 * kTile * 4; }
 
-template <typename T, int DP, Reach REACH>
+template <typename T, int DP, Reach REACH, bool NT>
 __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& item, int32_t h, char* lds) {
   typedef RowTile<T, DP> Tile;
   typedef Block<DP> B;
@@ -747,8 +756,8 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
         ids.fetch(a, item, k0, lane);
         present = block.find(a, item, heads, k0, 0, ids);
       }
-      block.template load_k<REACH>(a, item, heads, k0, lane, present);
-      block.template load_v<REACH>(a, item, heads, k0, lane);
+      block.template load_k<REACH, NT>(a, item, heads, k0, lane, present);
+      block.template load_v<REACH, NT>(a, item, heads, k0, lane);
       for (int32_t i = 1;; ++i, k0 += STEP) {
         const bool more = k0 + STEP < item.key_end;
         uint32_t coming = 0;
@@ -757,9 +766,9 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
           if (!more) return;
           if (half == 0) {
             if constexpr (REACH != kAnyPage) coming = block.find(a, item, heads, k0 + STEP, i, ids);
-            block.template load_k<REACH>(a, item, heads, k0 + STEP, lane, coming);
+            block.template load_k<REACH, NT>(a, item, heads, k0 + STEP, lane, coming);
           } else {
-            block.template load_v<REACH>(a, item, heads, k0 + STEP, lane);
+            block.template load_v<REACH, NT>(a, item, heads, k0 + STEP, lane);
           }
         });
         if (!more) break;
@@ -1158,16 +1167,18 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
 }
 
 // A workgroup of a key head takes its share's items one after the other
-template <typename T, int DP, Reach REACH>
+template <typename T, int DP, Reach REACH, bool NT>
 __device__ __forceinline__ void narrow_share(const AttendArgs& a, int32_t at, char* lds) {
   const int32_t group = at / a.kv_heads, h = at - group * a.kv_heads;
   const Range range = a.l.ranges[group];
-  for (int32_t i = range.begin; i < range.end; ++i) narrow_item<T, DP, REACH>(a, a.l.items[0][i], h, lds);
+  for (int32_t i = range.begin; i < range.end; ++i) narrow_item<T, DP, REACH, NT>(a, a.l.items[0][i], h, lds);
 }
-template <typename T, int DP, Reach REACH>
-__global__ __launch_bounds__(kThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void attend_rows_kernel(AttendArgs a) {
+// As many workgroups as are on the card at once, by their registers. NT: keys by non-temporal loads, see launch_attend.
+constexpr int narrow_residents(int dp) { return dp <= 64 ? 4 : dp <= 128 ? 2 : 1; }  // of a CU
+template <typename T, int DP, Reach REACH, bool NT = false>
+__global__ __launch_bounds__(kThreads, narrow_residents(DP)) void attend_rows_kernel(AttendArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[narrow_lds<T, DP>()];
-  narrow_share<T, DP, REACH>(a, blockIdx.x, lds);
+  narrow_share<T, DP, REACH, NT>(a, blockIdx.x, lds);
 }
 
 // Steps that may have wide tiles: both kinds in one launch, side by side on the card, as the narrow ones wait for memory and
@@ -1190,7 +1201,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_step_kerne
     if (!is_wide) at = at - a.wide_groups + both;
   }
   if (!is_wide) {
-    narrow_share<T, DP, REACH>(a, at, lds);
+    narrow_share<T, DP, REACH, false>(a, at, lds);
     return;
   }
   const int32_t items = a.l.header->wide_items, all = items * a.kv_heads, run = (all + 7) / 8;
@@ -1297,11 +1308,11 @@ struct kvc_attention_plan {
 
 namespace {
 
-constexpr int64_t kNarrowGroups = 1024;       // workgroups of a launch for narrow tiles
+constexpr int64_t kStepGroups = 1024;         // workgroups for narrow tiles of a launch that has wide ones as well
 constexpr int64_t kResidents = 512;           // wide items on the card at a time
 constexpr int64_t kMaxRounds = 4;             // of them in a step, where a range of keys is longer than the least
 constexpr int64_t kNarrowRows = 32;           // of a request; with more it is cut into wide tiles
-constexpr int64_t kNarrowSharedRows = 64;     // of all sharing requests
+constexpr int64_t kNarrowSharedRows = 128;    // of all sharing requests
 
 Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
   Layout l;
@@ -1331,7 +1342,8 @@ Sizes sizes_of(const kvc_attention_plan& p) {
   const int64_t rows = p.num_tokens * (p.num_heads / p.num_kv_heads);
   const bool shared = p.shared_pages > 0;
   n.wide = rows > p.narrow_rows || (shared && rows > kNarrowSharedRows);
-  n.groups = std::min<int64_t>(kMaxGroups, std::max<int64_t>(1, kNarrowGroups / p.num_kv_heads));
+  const int64_t groups = n.wide ? kStepGroups : 256 * narrow_residents((int)p.head_dim);
+  n.groups = std::min<int64_t>(kMaxGroups, std::max<int64_t>(1, groups / p.num_kv_heads));
   n.residents = std::max<int64_t>(1, kResidents / p.num_kv_heads);
   const auto shared_tiles = [&](int64_t tile) { return shared ? rows / tile + 1 : 0; };
   const auto tiles = [&](int64_t tile) { return rows / tile + std::min(p.batch_size, p.num_tokens) + shared_tiles(tile); };
@@ -1340,9 +1352,10 @@ Sizes sizes_of(const kvc_attention_plan& p) {
   n.max_items[1] = n.wide ? tiles(kWide) + kMaxRounds * n.residents : 0;
   n.max_slots[1] = n.wide ? 2 * kMaxRounds * n.residents + shared_tiles(kWide) : 0;
   n.max_shared_tiles = shared_tiles(kTile);
-  // (a narrow tile that is shorter than two of the least parts is never cut, a wide one that is no longer than the least range)
-  const int64_t keys = p.num_kv_indices * p.page_size;
-  n.join = shared || keys + kTileWork + kTile + 2 >= 2 * std::min(kMinShare / 2, kMinPart) || (n.wide && keys > kMinChunk);
+  // (where the shares are the least there are, a narrow tile that is no longer is never cut; nor is a wide one that is no
+  // longer than the least range)
+  const int64_t keys = p.num_kv_indices * p.page_size, work = keys + tiles(kTile) * (kTileWork + kTile + 2);
+  n.join = shared || work > kMinShare * n.groups || keys + kTileWork + kTile + 2 >= kMinShare || (n.wide && keys > kMinChunk);
   n.max_entries = n.join ? rows : 0;
   return n;
 }
@@ -1351,6 +1364,10 @@ template <typename T, int DP>
 void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
   const dim3 block(kThreads), grid((unsigned)(a.narrow_groups + a.wide_groups));
   const bool any = a.page_size % 16 != 0, full = a.head_dim == DP;
+  // Keys that no cache holds, and that are read once, by non-temporal loads (decode of 256 requests, 2.2 GB: 421 and 406 us;
+  // one of 131001 keys, 0.5 GB: 108 and 103; behind a shared prompt, 0.27 GB of which 16 MB are read again and again, 126
+  // and 130)
+  const bool nt = p.shared_pages == 0 && p.num_kv_indices * 2 * p.page_size * p.num_kv_heads * p.head_dim * 2 >= (int64_t(256) << 20);
   if (p.n.wide) {
     if (any) kvc::launch((attend_step_kernel<T, DP, kAnyPage>), grid, block, 0, s, a);
     else if (!full) kvc::launch((attend_step_kernel<T, DP, kGroups>), grid, block, 0, s, a);
@@ -1358,6 +1375,7 @@ void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t
   } else {
     if (any) kvc::launch((attend_rows_kernel<T, DP, kAnyPage>), grid, block, 0, s, a);
     else if (!full) kvc::launch((attend_rows_kernel<T, DP, kGroups>), grid, block, 0, s, a);
+    else if (nt) kvc::launch((attend_rows_kernel<T, DP, kGroupsFull, true>), grid, block, 0, s, a);
     else kvc::launch((attend_rows_kernel<T, DP, kGroupsFull>), grid, block, 0, s, a);
   }
 }
