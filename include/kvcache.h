@@ -607,8 +607,9 @@ int kvc_rotary_plan_run_norm(const kvc_rotary_plan* plan, const void* query, con
  * (kvc_attention_workspace_bytes, aligned to 256): runs that may overlap need a workspace each.
  * query [num_tokens, num_heads*head_dim] with a token stride in elements,
  * rows and pages aligned to 16 bytes; out [num_tokens, num_heads*head_dim]
- * contiguous; lse fp32 [num_tokens, num_heads] or NULL. dtype bf16 or f16;
- * head_dim a multiple of 8 up to 256. */
+ * contiguous; lse fp32 [num_tokens, num_heads] or NULL. `out` may be the query
+ * itself (its rows contiguous); any other overlap of what is written with what is read is refused.
+ * dtype bf16 or f16; head_dim a multiple of 8 up to 256. */
 typedef struct kvc_attention_plan kvc_attention_plan;
 
 int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indices,

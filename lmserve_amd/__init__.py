@@ -12,7 +12,8 @@
     kv_service  the KV worker as a process of its own (pool mapped from an IPC handle)
     streams     the streams of the KV worker and of a recording, held by no one else
     step_graph  KVWriteStep: fixed-capacity index buffers and plans, so that a step's index build
-                and per-layer writes can be recorded once into a hipGraph and replayed for later steps
+                and per-layer writes (and the attention behind them) can be recorded once into a
+                hipGraph and replayed for later steps
 
 Every operator runs a hand-written HIP kernel from libkvcache.so through the
 C ABI of include/kvcache.h; the disk tier is host-side file I/O in the same
@@ -24,7 +25,7 @@ from .cache_ops import (check_block_maps, copy_blocks, fill_key_cache, flatten_b
                         gather_blocks, reshape_and_cache, reshape_and_cache_layers, scatter_blocks,
                         swap_in, swap_out)
 from .disk_tier import DiskTier
-from .index_prep import (InferInput, KVIndexInputs, make_kv_index_inputs, to_device,
+from .index_prep import (InferInput, KVIndexInputs, common_prefix_pages, make_kv_index_inputs, to_device,
                          to_device_one_launch)
 from .kv_pool import (CachePlan, KVWorkerHandle, KVWorkerParams, LayerSyncHooks,
                       allocate_kv_caches, make_kv_worker_params, open_kv_worker_params, plan_cache)
@@ -55,6 +56,6 @@ __all__ = [
     "InferInput", "KVIndexInputs", "make_kv_index_inputs", "to_device", "to_device_one_launch",
     "build_write_index", "BlockRuns", "max_block_runs", "slot_block_runs", "write_block_runs_layers",
     "KVWriteStep",
-    "PagedAttentionPlan", "paged_attention",
+    "PagedAttentionPlan", "paged_attention", "common_prefix_pages",
     "qk_norm_rotary_pos_emb", "qk_norm_rotary_pos_emb_and_cache", "qk_norm_rotary_pos_emb_and_append_paged",
 ]

@@ -88,6 +88,8 @@ class PagedAttentionPlan:
     def build(self) -> None:
         """Lay out the step that the index buffers hold (two small launches on the current stream)."""
         with _on_device_of(self._buffer):
+            if _stream_of(self._buffer) != self._stream:
+                self._buffer.record_stream(torch.cuda.current_stream())
             _lib.check(_lib.lib().kvc_attention_plan_build(self._plan, self._buffer.data_ptr(), self._buffer.numel(),
                                                            _stream_of(self._buffer)))
 
@@ -96,7 +98,8 @@ class PagedAttentionPlan:
         """One layer: `query [num_tokens, Hq, D]` (or `[num_tokens, Hq*D]`; rows may be slices
         of a fused projection) over `paged_kv_cache [num_pages, 2, page_size, H, D]`.
         Returns `out` in the query's shape, with `return_lse` also the fp32 `[num_tokens, Hq]` logarithms of the
-        softmax sums. `out` / `lse` may be contiguous buffers of the caller's; without one, rows
+        softmax sums. `out` / `lse` may be contiguous buffers of the caller's (`out` the query itself, but no other
+        memory that is read); without one, rows
         behind the last request are not initialised. Launches on the current stream of the plan's device."""
         fast = self._fast_run
         if fast is not None and lse is None:

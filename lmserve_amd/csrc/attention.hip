@@ -1472,7 +1472,6 @@ int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query, in
                            void* workspace, int64_t workspace_bytes, void* stream) {
   constexpr const char* fn = "kvc_attention_plan_run";
   if (!plan) return fail(KVC_ERR_INVALID_ARG, "%s: null plan", fn);
-  if (!plan->buffer) return fail(KVC_ERR_INVALID_ARG, "%s: the plan is not built", fn);
   if (plan->batch_size == 0 || plan->num_tokens == 0) return KVC_OK;
   const int64_t row = plan->num_kv_heads * plan->head_dim, page = 2 * plan->page_size * row;
   if (!query || !out || !workspace || (num_pages > 0 && !paged_kv_cache))
@@ -1486,6 +1485,22 @@ int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query, in
     return fail(KVC_ERR_INVALID_ARG, "%s: rows must be aligned to 16 bytes, the output to 8", fn);
   if (workspace_bytes < plan->workspace_bytes)
     return fail(KVC_ERR_STAGING, "%s: the workspace needs %lld bytes", fn, (long long)plan->workspace_bytes);
+  if (!plan->buffer) return fail(KVC_ERR_INVALID_ARG, "%s: the plan is not built", fn);
+  // A row of the query is read before the same row of the output is written, and by no one else afterwards; nothing else that
+  // is read or written may share memory with the output
+  const auto meet = [](const void* x, int64_t n, const void* y, int64_t m) {
+    return x && y && (uintptr_t)x < (uintptr_t)y + (uint64_t)m && (uintptr_t)y < (uintptr_t)x + (uint64_t)n;
+  };
+  const int64_t q_row = plan->num_heads * plan->head_dim * 2, out_bytes = plan->num_tokens * q_row;
+  const int64_t q_bytes = (plan->num_tokens - 1) * q_token_stride * 2 + q_row, lse_bytes = plan->num_tokens * plan->num_heads * 4;
+  const int64_t cache_bytes = num_pages > 0 ? (num_pages - 1) * page_stride * 2 + page * 2 : 0;
+  const bool in_place = out == query && (plan->num_tokens == 1 || q_token_stride * 2 == q_row);
+  if ((!in_place && meet(out, out_bytes, query, q_bytes)) || meet(out, out_bytes, paged_kv_cache, cache_bytes) ||
+      meet(lse, lse_bytes, query, q_bytes) || meet(lse, lse_bytes, paged_kv_cache, cache_bytes) ||
+      meet(lse, lse_bytes, out, out_bytes) || meet(workspace, plan->workspace_bytes, query, q_bytes) ||
+      meet(workspace, plan->workspace_bytes, paged_kv_cache, cache_bytes) || meet(workspace, plan->workspace_bytes, out, out_bytes) ||
+      meet(workspace, plan->workspace_bytes, lse, lse_bytes) || meet(workspace, plan->workspace_bytes, plan->buffer, plan->plan_bytes))
+    return fail(KVC_ERR_INVALID_ARG, "%s: what is written overlaps what is read (the output may be the query itself)", fn);
   AttendArgs a{};
   a.query = (const char*)query;
   a.cache = (const char*)paged_kv_cache;

@@ -122,6 +122,22 @@ def make_kv_index_inputs(inputs: Sequence[InferInput], page_size: int) -> KVInde
     )
 
 
+def common_prefix_pages(tables: Sequence[Sequence[int]]) -> int:
+    """The leading pages that all block tables (`block_ids` of the requests) have in common: the `shared_pages`
+    of an attention plan, which reads them once for all requests that begin with them. The plan's shared pages
+    are the first such request's, so the tables of a step's prefill chunks, which share none, can be left out."""
+    tables = list(tables)
+    if not tables:
+        return 0
+    n = min(len(t) for t in tables)
+    first = np.asarray(tables[0][:n])
+    for t in tables[1:]:
+        differ = np.flatnonzero(np.asarray(t[:n]) != first[:n])
+        if differ.size:
+            n = int(differ[0])
+    return n
+
+
 @dataclass
 class DeviceKVIndexInputs:
     """Device tensors in the shape of the reference's `InputParams`
