@@ -1,4 +1,4 @@
-"""A whole step's K/V write as ONE recordable sequence: index build + every layer.
+"""A whole step's K/V write, and the attention that reads it, as ONE recordable sequence: index build + every layer.
 
 The reference rebuilds its index tensors on the host for every step and uploads
 them piecewise (`ModelWorker._make_inputs`,
@@ -16,11 +16,14 @@ depend on a host scalar of the step it was recorded for:
   entries beyond the step's tokens are -1);
 * the per-layer writes run through a plan over those buffers that addresses
   the cache by the slot mapping the index build writes, sized for
-  `max_tokens`; tokens with slot -1 are skipped.
+  `max_tokens`; tokens with slot -1 are skipped;
+* the attention's work is laid out on the device behind the index build, by
+  kernels launched for the capacities; rows beyond the step's tokens are left
+  as they were.
 
 `KVWriteStep` owns those buffers and plans. `set_requests` (or `set_arrays`)
 packs a step on the host and uploads it with one copy; `build_index` and
-`append` / `rotate_and_append` are the launches, eager or under stream capture.
+`append` / `rotate_and_append` / `attend` are the launches, eager or under stream capture.
 """
 from __future__ import annotations
 
@@ -31,6 +34,7 @@ import numpy as np
 import torch
 
 from . import _lib, streams
+from .attention import PagedAttentionPlan
 from .index_prep import InferInput
 from .paged import BlockRuns, PagedKVWritePlan, build_write_index, max_block_runs
 from .rotary import PagedRotaryWritePlan
@@ -46,12 +50,19 @@ class KVWriteStep:
     cos_sin_cache, num_heads: when given, `rotate_and_append` is available (the
       rotation fused with the write, one launch per layer).
     with_runs: also have the index build emit the step's block runs (`self.runs`).
+    with_attention: `attend` is available (needs `num_heads`), and the index build lays out its work;
+      shared_pages, sm_scale and max_q_len are `PagedAttentionPlan`'s, for all steps to come.
+
+    The buffers hold one step: the sequences recorded from one object run one after another.
     """
 
     def __init__(self, num_kv_heads: int, head_dim: int, page_size: int, dtype: torch.dtype, device,
                  max_requests: int, max_tokens: int, max_block_ids: int,
                  cos_sin_cache: Optional[torch.Tensor] = None, num_heads: int = 0,
-                 with_runs: bool = False):
+                 with_runs: bool = False, with_attention: bool = False, shared_pages: int = 0,
+                 sm_scale: Optional[float] = None, max_q_len: Optional[int] = None):
+        if with_attention and num_heads < 1:
+            raise ValueError("with_attention needs num_heads")
         self.device = torch.device(device)
         self.page_size = int(page_size)
         self.max_requests, self.max_tokens, self.max_block_ids = int(max_requests), int(max_tokens), int(max_block_ids)
@@ -92,6 +103,12 @@ class KVWriteStep:
                                                     self.kv_indptr, self.kv_last_page_len, cos_sin_cache,
                                                     num_heads, num_kv_heads, head_dim, page_size,
                                                     slots=self.slot_mapping)
+        self.attention_plan = None
+        if with_attention:
+            self.attention_plan = PagedAttentionPlan(self.cu_seqlens_q, self.kv_indices, self.kv_indptr,
+                                                     self.kv_last_page_len, num_heads, num_kv_heads, head_dim, page_size,
+                                                     dtype, T, max_q_len=max_q_len, shared_pages=shared_pages,
+                                                     sm_scale=sm_scale)
         self.num_tokens = 0       # of the step last packed (host-side knowledge)
         self.num_requests = 0
 
@@ -162,31 +179,68 @@ class KVWriteStep:
     # ------------------------------------------------------------------ launches
     def build_index(self) -> None:
         """One launch on the current stream: every index tensor of the step that
-        the buffers hold, written in place."""
+        the buffers hold, written in place. With attention two more lay out its work."""
         build_write_index(self.input_lens, self.context_lens, self.num_blocks, self.kv_indices,
                           self.page_size, self.max_tokens, out=self._out)
+        if self.attention_plan is not None:
+            self.attention_plan.build()
 
     def append(self, key: torch.Tensor, value: torch.Tensor, paged_kv_cache: torch.Tensor) -> None:
         """One layer's write; `key` / `value` hold `max_tokens` rows, of which the
         step's first `num_tokens` are written."""
         self.plan.append(key, value, paged_kv_cache)
 
-    def rotate_and_append(self, query, key, value, paged_kv_cache, query_out=None, key_out=None):
+    def rotate_and_append(self, query, key, value, paged_kv_cache, query_out=None, key_out=None,
+                          query_weight=None, key_weight=None, eps: float = 1e-6):
+        """One layer's rotation and write; with the layer's `query_weight` and `key_weight` its heads are normed first."""
         if self.rotary_plan is None:
             raise ValueError("this step was made without a cos/sin table")
-        return self.rotary_plan.run(query, key, value, paged_kv_cache, query_out=query_out, key_out=key_out)
+        return self.rotary_plan.run(query, key, value, paged_kv_cache, query_out=query_out, key_out=key_out,
+                                    query_weight=query_weight, key_weight=key_weight, eps=eps)
+
+    def attend(self, query, paged_kv_cache, out=None, return_lse: bool = False, lse=None):
+        """One layer's attention of `query [max_tokens, num_heads, D]` over what the cache holds, the
+        step's own tokens among it once they are written. Rows beyond the step's tokens are left as they were."""
+        if self.attention_plan is None:
+            raise ValueError("this step was made without attention")
+        return self.attention_plan.run(query, paged_kv_cache, out=out, return_lse=return_lse, lse=lse)
 
     def capture(self, keys: Sequence[torch.Tensor], values: Sequence[torch.Tensor],
                 caches: Sequence[torch.Tensor], queries: Optional[Sequence[torch.Tensor]] = None,
-                query_outs: Optional[Sequence[torch.Tensor]] = None) -> "torch.cuda.CUDAGraph":
+                query_outs: Optional[Sequence[torch.Tensor]] = None,
+                norm_weights: Optional[Sequence] = None, eps: float = 1e-6,
+                attention_outs: Optional[Sequence[torch.Tensor]] = None) -> "torch.cuda.CUDAGraph":
         """Record `build_index` and every layer's write into a hipGraph. The tensors
         are the fixed buffers the model writes its projections into before every
         replay (`max_tokens` rows each). With `queries` the fused rotation runs in
         place of the plain write, and with `query_outs` as well as one launch for all
-        layers whose buffers allow it (`PagedRotaryWritePlan.run_layers`). One eager
+        layers whose buffers allow it (`PagedRotaryWritePlan.run_layers`). `norm_weights`,
+        the layers' `(query_weight, key_weight)`, norm the heads before their rotation, a launch
+        to a layer. With `attention_outs` every layer's attention follows its write, of
+        `query_outs` where these are rotated and of `queries` where the step has no cos/sin table. One eager
         pass runs first (outside the capture)."""
+        if norm_weights is not None and queries is None:
+            raise ValueError("norm_weights need queries")
+        if attention_outs is not None:
+            if self.attention_plan is None:
+                raise ValueError("this step was made without attention")
+            if queries is None or (self.rotary_plan is not None and query_outs is None):
+                raise ValueError("attention_outs need queries, and query_outs where they are rotated")
+
         def body():
             self.build_index()
+            if attention_outs is not None or norm_weights is not None:
+                for l, (k, v, c) in enumerate(zip(keys, values, caches)):
+                    q = queries[l]
+                    if self.rotary_plan is None and norm_weights is None:
+                        self.append(k, v, c)
+                    else:
+                        qw, kw = norm_weights[l] if norm_weights is not None else (None, None)
+                        q, _ = self.rotate_and_append(q, k, v, c, query_out=query_outs[l] if query_outs is not None else None,
+                                                      query_weight=qw, key_weight=kw, eps=eps)
+                    if attention_outs is not None:
+                        self.attend(q, c, out=attention_outs[l])
+                return
             if queries is not None and query_outs is not None and self.rotary_plan is not None:
                 n = min(len(keys), len(values), len(caches))
                 self.rotary_plan.run_layers([queries[l] for l in range(n)], keys[:n], values[:n], caches[:n],
