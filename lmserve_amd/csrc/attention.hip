@@ -17,6 +17,7 @@
 #include <cmath>
 #include <cstdint>
 #include <new>
+#include <type_traits>
 
 #include "common.h"
 #include "device.h"
@@ -48,6 +49,7 @@ constexpr int kMaxGroups = 1024;    // workgroups of a key head
 __device__ constexpr int kTileWork = 64, kMinShare = 1024, kMinSharedShare = 256, kMinPart = 256;
 // the least range of a wide tile; what an item costs beside its keys, and what one that leaves a partial does
 __device__ constexpr int kMinChunk = 512, kWideTileWork = 128, kWidePartWork = 384;
+constexpr int32_t kMaxKeys = INT32_MAX - 8192;  // of a request: a key that is looked up ahead stays below 2^31
 constexpr int kManyParts = 16;     // a row of more partials is joined by a workgroup
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -120,7 +122,7 @@ __device__ __forceinline__ Table tokens_of(const PlanArgs& a, int32_t b) {
 __device__ __forceinline__ int32_t keys_of(const PlanArgs& a, int32_t b, int32_t pages) {
   if (!pages) return 0;
   const int64_t keys = (int64_t)(pages - 1) * a.page_size + clamp(a.kv_last_page_len[b], 0, a.page_size);
-  return (int32_t)(keys < INT32_MAX - kStep ? keys : INT32_MAX - kStep);
+  return (int32_t)(keys < kMaxKeys ? keys : kMaxKeys);
 }
 
 // A workgroup per request: does it begin with the shared pages? Which pages these are is what the first request with few
@@ -472,11 +474,18 @@ struct F16 {
   }
   static constexpr uint32_t kExponent = 0x7c00u;
 };
-// Two 16-bit values side by side: is one infinite or not a number?
+// Is an infinity or NaN among the 16-bit values that were taken in? (The largest exponent of either half.)
 template <typename T>
-__device__ __forceinline__ bool not_finite(uint32_t two) {
-  return (two & T::kExponent) == T::kExponent || (two >> 16 & T::kExponent) == T::kExponent;
-}
+struct Oddities {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 top = {};
+  __device__ __forceinline__ void take(u32x4 v) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[w] & (T::kExponent << 16 | T::kExponent)));
+  }
+  __device__ __forceinline__ bool any() const { return max((uint32_t)top[0], (uint32_t)top[1]) == T::kExponent; }
+};
 // The infinities and NaN among 4 values, 0 for the others
 template <typename T>
 __device__ __forceinline__ f32x4 infinite_part(u32x2 four) {
@@ -521,6 +530,16 @@ __device__ __forceinline__ int64_t key_offset(const AttendArgs& a, int32_t table
   const int32_t page = a.kv_indices[table + p];
   if (page < 0 || page >= a.num_pages) return -1;
   return (int64_t)page * a.page_stride + (int64_t)(key - p * a.page_size) * a.row_stride;
+}
+
+// The larger of a lane's value and that of the lane 32 (16) further on or before, without LDS
+__device__ __forceinline__ float max_across32(float x) {
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float max_across16(float x) {
+  const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
 }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -659,12 +678,10 @@ struct RowTile {
     // does a row stop inside the block, and is there a value in it that 0 does not cancel?
     const bool ragged = __ballot(n < item.rows && limit < min(k0 + kBlock, item.key_end)) != 0;
     if (ragged) {
-      bool odd_v = false;
+      Oddities<T> odd;
 #pragma unroll
-      for (int i = 0; i < B::VLOADS; ++i)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) odd_v = odd_v || not_finite<T>(b.v[i][w]);
-      if (__ballot(odd_v)) {
+      for (int i = 0; i < B::VLOADS; ++i) odd.take(b.v[i]);
+      if (__ballot(odd.any())) {
         odd_from = min(odd_from, k0);
 #pragma unroll
         for (int i = 0; i < B::VLOADS; ++i) b.v[i] = finite_part<T>(b.v[i]);
@@ -689,8 +706,7 @@ struct RowTile {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = max_across32(max_across16(top));
     const float base = top == -INFINITY ? 0.f : top * a.scale;
     const float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
     u32x4 p;
@@ -896,57 +912,71 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
     f32x16 o[DTILES] = {};
     float base = -INFINITY, l = 0;  // weights are exp2(score * scale - base)
     u32x4 kr[ROUNDS], vr[ROUNDS];
-    int32_t id_page = -1, id_off = 0;
-    // where a round's rows of a step lie (one row of every LPR lanes), or null where there is none to read
-    const auto row_of = [&](int32_t k0, int32_t step, int i) -> const char* {
-      const int32_t row0 = i * RPW * kWaves + wave * RPW;
+    uint32_t group_lo = 0, group_hi = 0;  // where the groups of 16 keys of 16 windows lie, one to a lane
+    uint64_t groups = 0;                  // and which of them are there
+    // Keys come in windows of 64: window w begins 32 before the item's 64 w-th key, so that what a step reads, K of the 64
+    // keys from its own 32nd on and V of the 64 keys up to its own 32nd, are the windows w + 1 and w.
+    const auto window = [&](int32_t w) { return item.key_begin + w * kStep - kStep / 2; };
+    const auto offset_of = [&](int32_t key) { return key < item.key_begin ? -1 : key_offset(a, item.table, key, item.key_end); };
+    int64_t place[ROUNDS];  // of the rows of the window that K was last asked of, by round (the same in all lanes)
+    // where a round's rows lie (one row of every LPR lanes), or null where there is none to read
+    const auto row_of = [&](int32_t w, int i) -> const char* {
       if constexpr (REACH == kAnyPage) {
-        const int64_t off = key_offset(a, item.table, k0 + row0 + lrow, item.key_end);
+        const int64_t off = offset_of(window(w) + i * RPW * kWaves + wave * RPW + lrow);
         return off < 0 || lcol * 8 >= D ? nullptr : heads + off + lcol * 16;
       } else {
-        const int32_t group = (step & 15) * 4 + row0 / 16;
-        const int32_t page = __builtin_amdgcn_readlane(id_page, group), off = __builtin_amdgcn_readlane(id_off, group);
         if (REACH == kGroups && lcol * 8 >= D) return nullptr;
-        return heads + (int64_t)max(page, 0) * a.page_stride + (int64_t)(page < 0 ? 0 : off + row0 % 16) * a.row_stride +
-               (lrow * a.row_stride + lcol * 16);
+        return heads + place[i] + (lrow * a.row_stride + lcol * 16);
       }
     };
-    // K of the step from k0 on, on its way; which of the keys are there
-    const auto fetch_k = [&](int32_t k0, int32_t step) -> uint64_t {
+    // K of a window, on its way; which of the keys are there
+    const auto fetch_k = [&](int32_t w) -> uint64_t {
       uint64_t present = 0;
+      const int32_t first = window(w);
       if constexpr (REACH == kAnyPage) {
-        present = __ballot(key_offset(a, item.table, k0 + lane, item.key_end) >= 0);
+        present = __ballot(offset_of(first + lane) >= 0);
       } else {
-        if ((step & 15) == 0) {  // the page ids of 16 steps, one to a lane
-          const int32_t key = k0 + lane * 16;
-          id_page = -1;
-          if (key < item.key_end) {
+        if ((w & 15) == 0) {
+          const int32_t key = first + lane * 16;
+          uint64_t at = 0;  // (of what is not there: the cache's first page)
+          bool have = false;
+          if (key >= item.key_begin && key < item.key_end) {
             const int32_t p = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
             const int32_t id = a.kv_indices[item.table + p];
-            id_off = key - p * a.page_size;
-            if (id >= 0 && id < a.num_pages) id_page = id;
+            have = id >= 0 && id < a.num_pages;
+            if (have) at = (uint64_t)(uint32_t)id * a.page_stride + (uint64_t)(uint32_t)(key - p * a.page_size) * a.row_stride;
           }
+          group_lo = (uint32_t)at;
+          group_hi = (uint32_t)(at >> 32);
+          groups = __ballot(have);
+        }
+        const uint32_t four = (uint32_t)(groups >> (w & 15) * 4) & 15, left = (uint32_t)(item.key_end - first);
+        present = ~(uint64_t)0;
+        if (four != 15 || left < kStep) {
+          present = 0;
+          for (int i = 0; i < 4; ++i) present |= (uint64_t)(four >> i & 1 ? 0xffffu : 0) << (i * 16);
+          if (left < kStep) present &= ((uint64_t)1 << left) - 1;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int32_t left = item.key_end - k0 - i * 16;
-          if (__builtin_amdgcn_readlane(id_page, (step & 15) * 4 + i) >= 0)
-            present |= (uint64_t)(left >= 16 ? 0xffffu : (1u << left) - 1u) << (i * 16);
+        for (int i = 0; i < ROUNDS; ++i) {
+          const int32_t row0 = i * RPW * kWaves + wave * RPW, group = (w & 15) * 4 + row0 / 16;
+          place[i] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(group_hi, group) << 32 |
+                               (uint32_t)__builtin_amdgcn_readlane(group_lo, group)) + (uint32_t)(row0 % 16) * a.row_stride;
         }
       }
 #pragma unroll
       for (int i = 0; i < ROUNDS; ++i) {
-        const char* from = row_of(k0, step, i);
+        const char* from = row_of(w, i);
         if (REACH != kGroupsFull) kr[i] = u32x4{};
         if (REACH == kGroupsFull || from) kr[i] = *reinterpret_cast<const u32x4*>(from);
       }
       return present;
     };
-    // V of the same step, after its K
-    const auto fetch_v = [&](int32_t k0, int32_t step) {
+    // V of the window that K was last asked of
+    const auto fetch_v = [&](int32_t w) {
 #pragma unroll
       for (int i = 0; i < ROUNDS; ++i) {
-        const char* from = row_of(k0, step, i);
+        const char* from = row_of(w, i);
         if (REACH != kGroupsFull) vr[i] = u32x4{};
         if (REACH == kGroupsFull || from) vr[i] = *reinterpret_cast<const u32x4*>(from + a.plane);
       }
@@ -959,18 +989,16 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
         if (LPR * 8 == DP || lcol * 8 < DP)
           *reinterpret_cast<u32x4*>(k_lds[buf] + (i * RPW * kWaves + wave * RPW + lrow) * KSTRIDE + lcol * 16) = kr[i];
     };
-    const auto stage_v = [&](int buf, int32_t k0, uint64_t present) {
+    const auto stage_v = [&](int buf, int32_t w, uint64_t present) {
       if (REACH != kAnyPage && ~present)
 #pragma unroll
         for (int i = 0; i < ROUNDS; ++i)
           if (!(present >> (i * RPW * kWaves + wave * RPW + lrow) & 1)) vr[i] = u32x4{};
-      if (k0 + kStep > tile_least) {  // a row stops in this step: are there values that 0 does not cancel?
-        bool odd_v = false;
+      if (window(w) + kStep > tile_least) {  // a row stops in it: are there values that 0 does not cancel?
+        Oddities<T> odd;
 #pragma unroll
-        for (int i = 0; i < ROUNDS; ++i)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) odd_v = odd_v || not_finite<T>(vr[i][w]);
-        if (__ballot(odd_v)) {
+        for (int i = 0; i < ROUNDS; ++i) odd.take(vr[i]);
+        if (__ballot(odd.any())) {
           left_out = 1;
 #pragma unroll
           for (int i = 0; i < ROUNDS; ++i) vr[i] = finite_part<T>(vr[i]);
@@ -1013,7 +1041,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
           if (!(sees >> (r / 4 * 8 + r % 4) & 1)) s[r] = -INFINITY;
         top = highest(s);
       }
-      return fmaxf(top, __shfl_xor(top, 32));
+      return max_across32(top);
     };
     // A base that has been outgrown. It is a whole number, so that what was made with the old one, the weights that wait
     // for their product among it, is scaled exactly.
@@ -1032,18 +1060,20 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
     // 32 keys: their weights from the scores s, while the scores of the keys behind them and the product of the weights
     // before them, that waited, with V are on the matrix unit. The order is written out, a product with what goes on beside
     // it to a line: pieces from LDS for the products kAhead further on, half a pair of weights, the next scores' maximum.
-    const auto take = [&](const f32x16& s, uint32_t* p, f32x16& next, float& top, int next_buf, int next_half, const uint32_t* waiting,
-                          int v_buf, int v_half) {
-      constexpr int PIECES = KSTEPS + 2 * DTILES;
+    const auto take = [&](const f32x16& s, uint32_t* p, f32x16& next, float& top, const uint32_t* waiting, int buf, auto which,
+                          u32x4* piece) {
+      constexpr int PIECES = KSTEPS + 2 * DTILES, HALF = decltype(which)::value;
+      static_assert(PIECES % (kAhead + 1) == 0, "the second half's first pieces are asked for at the end of the first's");
       const float minus = base == -INFINITY ? 0.f : -base;
       float sum[2] = {}, x = 0;
-      u32x4 piece[kAhead + 1];
       next = f32x16{};
       const auto ask = [&](int j) {
-        if (j < PIECES) piece[j % (kAhead + 1)] = j < KSTEPS ? k_piece(next_buf, next_half, j) : v_piece(v_buf, v_half, j - KSTEPS);
+        if (j < PIECES) piece[j % (kAhead + 1)] = j < KSTEPS ? k_piece(buf, HALF, j) : v_piece(buf, HALF, j - KSTEPS);
+        else if (HALF == 0) piece[j % (kAhead + 1)] = k_piece(buf, 1, j - PIECES);
       };
+      if (HALF == 0)
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) ask(j);
+        for (int j = 0; j < kAhead; ++j) ask(j);
 #pragma unroll
       for (int j = 0; j < PIECES; ++j) {
         ask(j + kAhead);
@@ -1071,56 +1101,54 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
     const int32_t steps = a.num_pages > 0 ? (item.key_end - item.key_begin + kStep - 1) / kStep : 0;
     if (steps > 0) {
       int32_t k0 = item.key_begin;
-      // nothing waits for the first product: zeros, in V as well
+      // nothing waits for the first product: zeros, and V of the keys before the first is cleared
       uint32_t p0[8], p1[8] = {};
-      for (int32_t i = tid * 16; i < 32 * VSTRIDE; i += kThreads * 16) *reinterpret_cast<u32x4*>(v_lds[1] + 32 * VSTRIDE + i) = u32x4{};
-      uint64_t present = fetch_k(k0, 0), coming = 0;
-      fetch_v(k0, 0);
+      uint64_t before = fetch_k(0);
+      fetch_v(0);
+      stage_k(1);
+      stage_v(0, 0, before);
+      uint64_t present = fetch_k(1), coming = 0, then = 0;  // of the windows i + 1, i + 2, i + 3
+      fetch_v(1);
       stage_k(0);
-      stage_v(0, k0, present);
-      if (steps > 1) {
-        coming = fetch_k(k0 + kStep, 1);
-        fetch_v(k0 + kStep, 1);
-      }
+      if (steps > 1) coming = fetch_k(2);
       __syncthreads();
       f32x16 s0 = {}, s1;
 #pragma unroll
-      for (int j = 0; j < KSTEPS; ++j) s0 = T::mfma(k_piece(0, 0, j), q[j], s0);
-      float top = mask(s0, highest(s0), k0, (uint32_t)present);
+      for (int j = 0; j < KSTEPS; ++j) s0 = T::mfma(k_piece(1, 1, j), q[j], s0);
+      float top = mask(s0, highest(s0), k0, (uint32_t)(before >> 32));
       for (int32_t i = 0; i < steps; ++i, k0 += kStep) {
         const int buf = i & 1;
-        uint64_t then = 0;
-        __syncthreads();  // the other buffer's K has been read, this one's V is there
+        u32x4 piece[kAhead + 1];
+        __syncthreads();  // this step's windows are there, the last step's have been read
+        stage_v(buf ^ 1, i + 1, present);
         if (i + 1 < steps) {
           stage_k(buf ^ 1);
-          if (i + 2 < steps) then = fetch_k(k0 + 2 * kStep, i + 2);
+          fetch_v(i + 2);
+          if (i + 2 < steps) then = fetch_k(i + 3);
         }
         grow(top, p1);
-        take(s0, p0, s1, top, buf, 1, p1, buf ^ 1, 1);
-        top = mask(s1, top, k0 + 32, (uint32_t)(present >> 32));
-        __syncthreads();  // the other buffer's V has been read, its K is there
-        if (i + 1 < steps) {
-          stage_v(buf ^ 1, k0 + kStep, coming);
-          if (i + 2 < steps) fetch_v(k0 + 2 * kStep, i + 2);
-        }
+        take(s0, p0, s1, top, p1, buf, std::integral_constant<int, 0>{}, piece);
+        top = mask(s1, top, k0 + 32, (uint32_t)present);
         grow(top, p0);
-        take(s1, p1, s0, top, buf ^ 1, 0, p0, buf, 0);  // (after the last step: whatever is there, and no use of it)
-        top = mask(s0, top, k0 + kStep, (uint32_t)coming);
+        take(s1, p1, s0, top, p0, buf, std::integral_constant<int, 1>{}, piece);  // (after the last step: scores of keys that are not there)
+        top = mask(s0, top, k0 + kStep, (uint32_t)(present >> 32));
         present = coming;
         coming = then;
+        then = 0;
       }
+      __syncthreads();
       // the last weights' product
 #pragma unroll
       for (int j = 0; j < 2 * DTILES; ++j) {
         const uint32_t* w = p1 + j / DTILES * 4;
-        o[j % DTILES] = T::mfma(v_piece((steps - 1) & 1, 1, j), u32x4{w[0], w[1], w[2], w[3]}, o[j % DTILES]);
+        o[j % DTILES] = T::mfma(v_piece(steps & 1, 0, j), u32x4{w[0], w[1], w[2], w[3]}, o[j % DTILES]);
       }
     }
     __syncthreads();  // (left_out is complete, and the buffers are free)
     if (left_out) {  // as above
       int32_t zero = 0;
       asm volatile("" : "+v"(zero));
-      const int32_t from = item.key_begin + max(tile_least - item.key_begin, 0) / kStep * kStep;
+      const int32_t from = item.key_begin + max((max(tile_least - item.key_begin, 0) + kStep / 2) / kStep * kStep - kStep / 2, 0);
 #pragma unroll 1
       for (int32_t key = from; key < item.key_end; ++key) {
         const int64_t off = key_offset(a, item.table, key, item.key_end);
