@@ -861,11 +861,14 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
 }
 
 // A workgroup per (item of up to 128 rows, key head): 32 rows to a wavefront, 64 keys at a time, staged in LDS for all four.
-// The next step's loads are under way in registers while one is worked on; the buffers alternate, so that a step has one
-// barrier. S^T and O^T as above, in 32 x 32 pieces: a lane holds one row and, of 32 keys, those with bit 2 as its own
-// half (lane / 32). K rows are 16 bytes apart in the banks (a lane reads 16 bytes of a row of its own), V rows 32.
+// The next step's loads are under way in registers while one is worked on; the buffers alternate, and K runs half a step
+// ahead of V, as their products do, so that a step has one barrier. S^T and O^T as above, in 32 x 32 pieces: a lane holds one
+// row and, of 32 keys, those with bit 2 as its own half (lane / 32). K rows are 16 bytes apart in the banks (a lane reads 16
+// bytes of a row of its own), V rows 64.
 // The maximum that the weights are taken against grows only when a row's has outgrown it by 2^8: until then the larger weights
 // (below 2^8) and sums say the same, and the rescaling of O, 64 registers at 128 columns, is left out of nearly every step.
+// Bound by the instructions that two wavefronts a SIMD can have under way: the matrix unit is busy for 41 % of the cycles
+// (2048 new tokens behind 14 to 30 thousand keys, 7 query heads to a key head of 128: 900 TFLOP/s with the joins).
 template <int DP>
 constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16 + DP * 2 + kVPad) + (kWaves + 1) * 4; }
 
@@ -1065,8 +1068,17 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
       constexpr int PIECES = KSTEPS + 2 * DTILES, HALF = decltype(which)::value;
       static_assert(PIECES % (kAhead + 1) == 0, "the second half's first pieces are asked for at the end of the first's");
       const float minus = base == -INFINITY ? 0.f : -base;
-      float sum[2] = {}, x = 0;
+      float sum[2] = {}, weight[3] = {};
       next = f32x16{};
+      // a weight is used behind the next one's exponential, whose result the adder would wait for
+      const auto add = [&](int r) {
+        sum[r % 2] += weight[r % 3];
+        asm volatile("" : "+v"(sum[r % 2]));
+        if (r % 2) {
+          p[r / 2] = T::pack(weight[(r + 2) % 3], weight[r % 3]);
+          asm volatile("" : "+v"(p[r / 2]));
+        }
+      };
       const auto ask = [&](int j) {
         if (j < PIECES) piece[j % (kAhead + 1)] = j < KSTEPS ? k_piece(buf, HALF, j) : v_piece(buf, HALF, j - KSTEPS);
         else if (HALF == 0) piece[j % (kAhead + 1)] = k_piece(buf, 1, j - PIECES);
@@ -1086,16 +1098,15 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
         }
 #pragma unroll
         for (int r = j * 16 / PIECES; r < (j + 1) * 16 / PIECES; ++r) {
-          const float y = exp2_of(__builtin_fmaf(s[r], a.scale, minus));
-          sum[r % 2] += y;
-          if (r % 2) p[r / 2] = T::pack(x, y);
-          x = y;
-          asm volatile("" : "+v"(x), "+v"(sum[r % 2]));  // here, and not where it is used
-          if (r % 2) asm volatile("" : "+v"(p[r / 2]));
+          float y = exp2_of(__builtin_fmaf(s[r], a.scale, minus));
+          asm volatile("" : "+v"(y));  // here, and not where it is used
+          weight[r % 3] = y;
+          if (r) add(r - 1);
         }
         if (j == PIECES - 1) top = highest(next);
         __builtin_amdgcn_sched_barrier(0);
       }
+      add(15);
       l += sum[0] + sum[1];
     };
     const int32_t steps = a.num_pages > 0 ? (item.key_end - item.key_begin + kStep - 1) / kStep : 0;
@@ -1126,12 +1137,15 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
           fetch_v(i + 2);
           if (i + 2 < steps) then = fetch_k(i + 3);
         }
+        // before the other workgroup's wavefronts that stage (2048 new tokens 817 us without, 796 so)
+        __builtin_amdgcn_s_setprio(1);
         grow(top, p1);
         take(s0, p0, s1, top, p1, buf, std::integral_constant<int, 0>{}, piece);
         top = mask(s1, top, k0 + 32, (uint32_t)present);
         grow(top, p0);
         take(s1, p1, s0, top, p0, buf, std::integral_constant<int, 1>{}, piece);  // (after the last step: scores of keys that are not there)
         top = mask(s0, top, k0 + kStep, (uint32_t)(present >> 32));
+        __builtin_amdgcn_s_setprio(0);
         present = coming;
         coming = then;
         then = 0;
