@@ -61,8 +61,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 //   whatever the lengths are. Of a share only the first and the last piece can be parts of a tile. A cut that would leave
 //   a sliver moves to the tile's end.
 //   Wide tiles of a request read the same keys: they are cut at the same keys, and the tiles of one range of keys are
-//   neighbours in the list and run on one XCD, whose L2 the range then comes to once. (Shares of a line put them at
-//   different keys: 2048 new tokens behind contexts of 1024 to 32768 took 1638 us, 900 in this order.)
+//   neighbours in the list and run on one XCD, whose L2 the range then comes to once (2048 new
+//   tokens behind 13 to 30 thousand keys 834 us; the tiles dealt to all XCDs in turn 854).
 // A part of a tile leaves its rows' unfinished result in a slot of the workspace, and the parts are joined at the end.
 struct Item {  // 32 bytes: a tile or a part of one
   int32_t q_begin;  // first token of the request; -1: the rows of all sharing requests, through shared_tokens
@@ -868,7 +868,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
 // The maximum that the weights are taken against grows only when a row's has outgrown it by 2^8: until then the larger weights
 // (below 2^8) and sums say the same, and the rescaling of O, 64 registers at 128 columns, is left out of nearly every step.
 // Bound by the instructions that two wavefronts a SIMD can have under way: the matrix unit is busy for 41 % of the cycles
-// (2048 new tokens behind 14 to 30 thousand keys, 7 query heads to a key head of 128: 900 TFLOP/s with the joins).
+// (2048 new tokens behind 13 to 30 thousand keys, 7 query heads to a key head of 128: 740 us, 965 TFLOP/s).
 template <int DP>
 constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16 + DP * 2 + kVPad) + (kWaves + 1) * 4; }
 
@@ -1229,7 +1229,7 @@ __global__ __launch_bounds__(kThreads, narrow_residents(DP)) void attend_rows_ke
 
 // Steps that may have wide tiles: both kinds in one launch, side by side on the card, as the narrow ones wait for memory and
 // the wide ones for the matrix units. 32 workgroups of a kind in turn: they are dealt to the 8 XCDs and there to 4 shader
-// engines in rotation (8 in turn put all wide ones on half of the engines: 1200 us for 680). The wide items, of one key head
+// engines in rotation (8 in turn put all wide ones on half of the engines: 2048 new tokens 1218 us, 917 so). The wide items, of one key head
 // after the other, are dealt to the XCDs in eight runs, so that items that read the same keys share an L2.
 template <typename T, int DP, Reach REACH>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_step_kernel(AttendArgs a) {

@@ -582,7 +582,7 @@ PyObject* fast_attention_plan_run(PyObject*, PyObject* const* args, Py_ssize_t n
 
 /* paged_attention(query, cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len, shared_pages, sm_scale,
  *                 out | None, return_lse, device, stream) -> 1, a negative kvc_status, out or (out, lse): a plan made, built,
- * run once and given back (through the interpreter 27 us a call, so 15 for one request) */
+ * run once and given back (one request's call through the interpreter 27 us, so the 17 that its two kernels take) */
 PyObject* fast_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   int64_t max_q_len, shared_pages, device;
