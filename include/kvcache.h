@@ -1,7 +1,8 @@
 /*
  * kvcache.h -- C ABI of libkvcache, the MI355X (gfx950) paged KV-cache
  * data-movement library: slot-mapped and page-table K/V write (alone or fused
- * with the rotary embedding), block copy, block gather/scatter between the HBM
+ * with the rotary embedding and the norms of query and key heads), the causal
+ * attention that reads the pages, block copy, block gather/scatter between the HBM
  * pool and a pinned host pool, the index preparation of a step, and the
  * host <-> disk tier of the block cache.
  *
@@ -585,7 +586,8 @@ int kvc_rotary_plan_run_norm(const kvc_rotary_plan* plan, const void* query, con
  * x / (num_heads / num_kv_heads):
  *   out = softmax(sm_scale * q.k) v,  lse = log(sum exp(sm_scale * q.k)).
  * A row without keys (also: one whose every score is -inf) is zero, its lse
- * -inf. A page outside [0, num_pages) has no keys. What lies behind a request's
+ * -inf. A page outside [0, num_pages) has no keys; nor has a request more than
+ * 2^31 - 8193. What lies behind a request's
  * last key, or is masked, does not reach the result, infinities and NaN included.
  * Rows behind qo_indptr[batch_size] are left as they were. Sums and softmax
  * statistics are fp32, the weights are rounded to the storage type for the
