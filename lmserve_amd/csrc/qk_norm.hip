@@ -147,9 +147,8 @@ __device__ __forceinline__ u32x4 ld16_any(const char* p) { return *reinterpret_c
 
 // Rows of aligned 16-byte vectors. W lanes to a head.
 // Bound by HBM where tokens are many: 16384 of (32 + 2 x 8) heads of 128 in bf16, 0.71 GB, take 119 us (5.95 TB/s); few of them
-// by the launch and loads one behind the other, position, then cos/sin: one token 2.6 us, 256 tokens 3.8. Outputs are stored past the caches, which hold them no longer than the
-// launch: 119 us against 134 (2048 tokens: 8.2 against 9.7); inputs by non-temporal loads as well 119.
-template <typename T, Addressing ADDR, bool FAST, int W>
+// by the launch and loads one behind the other, position, then cos/sin: one token 2.6 us, 256 tokens 3.8.
+template <typename T, Addressing ADDR, bool FAST, int W, bool PAST>
 __global__ __launch_bounds__(256) void norm_rotate_kernel(NormArgs a) {
   constexpr int N = Vec<T>::kN, E = T::kBytes;
   const int64_t t = blockIdx.x;
@@ -208,8 +207,14 @@ __global__ __launch_bounds__(256) void norm_rotate_kernel(NormArgs a) {
     x1 = Vec<T>::narrow(x[1]);
   }
   const auto put = [&](char* row) {
-    __builtin_nontemporal_store(x0, reinterpret_cast<u32x4*>(row + head_off + v0 * 16));
-    if (both) __builtin_nontemporal_store(x1, reinterpret_cast<u32x4*>(row + head_off + v1 * 16));
+    u32x4 *to0 = reinterpret_cast<u32x4*>(row + head_off + v0 * 16), *to1 = reinterpret_cast<u32x4*>(row + head_off + v1 * 16);
+    if constexpr (PAST) {
+      __builtin_nontemporal_store(x0, to0);
+      if (both) __builtin_nontemporal_store(x1, to1);
+    } else {
+      *to0 = x0;
+      if (both) *to1 = x1;
+    }
   };
   if (is_q) put(a.query_out + t * a.qo_token_stride);
   else if (!is_v && a.key_out) put(a.key_out + t * a.ko_token_stride);
@@ -267,16 +272,16 @@ __global__ __launch_bounds__(256) void norm_rotate_element_kernel(NormArgs a) {
   }
 }
 
-template <typename T, Addressing ADDR, bool FAST>
+template <typename T, Addressing ADDR, bool FAST, bool PAST>
 void launch_vector(const NormArgs& a, int lanes, dim3 grid, dim3 block, hipStream_t s) {
   switch (lanes) {
-    case 1: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 1>), grid, block, 0, s, a); break;
-    case 2: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 2>), grid, block, 0, s, a); break;
-    case 4: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 4>), grid, block, 0, s, a); break;
-    case 8: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 8>), grid, block, 0, s, a); break;
-    case 16: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 16>), grid, block, 0, s, a); break;
-    case 32: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 32>), grid, block, 0, s, a); break;
-    default: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 64>), grid, block, 0, s, a); break;
+    case 1: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 1, PAST>), grid, block, 0, s, a); break;
+    case 2: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 2, PAST>), grid, block, 0, s, a); break;
+    case 4: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 4, PAST>), grid, block, 0, s, a); break;
+    case 8: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 8, PAST>), grid, block, 0, s, a); break;
+    case 16: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 16, PAST>), grid, block, 0, s, a); break;
+    case 32: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 32, PAST>), grid, block, 0, s, a); break;
+    default: kvc::launch((norm_rotate_kernel<T, ADDR, FAST, 64, PAST>), grid, block, 0, s, a); break;
   }
 }
 
@@ -287,6 +292,12 @@ void launch_norm(const NormArgs& a, bool vector, int64_t tokens, hipStream_t s) 
     kvc::launch((norm_rotate_element_kernel<T, ADDR>), dim3((unsigned)tokens, (unsigned)((heads + 3) / 4)), dim3(256), 0, s, a);
     return;
   }
+  // Outputs past the caches where the last-level one would not hold them till they are read, and where they are few (what is
+  // written ends the launch later than the stores do). With the attention that reads them behind it, a layer of 32 + 2 x 8
+  // heads of 128 takes, plain and past the caches: 256 tokens (3 MB) 135 and 132 us, 2048 (25 MB) 46.6 and 47.3, 8192 (101 MB) 162
+  // and 169, 16384 (201 MB) 328 and 330; the launch by itself 2048 tokens 9.7 and 8.1, 16384 134 and 119 (loads too: 119).
+  const int64_t written = tokens * heads * a.head_dim * T::kBytes;
+  const bool past = written < (int64_t(8) << 20) || written >= (int64_t(128) << 20);
   int lanes = 1;
   while (2 * lanes < a.vecs) lanes *= 2;
   const int64_t all = (int64_t)heads * lanes;
@@ -294,8 +305,9 @@ void launch_norm(const NormArgs& a, bool vector, int64_t tokens, hipStream_t s) 
   const unsigned threads = (unsigned)std::min<int64_t>(256, (all + 63) / 64 * 64);
   const dim3 grid((unsigned)tokens, (unsigned)((all + threads - 1) / threads)), block(threads);
   const bool fast = a.pos_bytes == 4 && (ADDR == kNoCache || a.bs_shift >= 0) && (ADDR != kSlots || a.slot_bytes == 8);
-  if (fast) launch_vector<T, ADDR, true>(a, lanes, grid, block, s);
-  else launch_vector<T, ADDR, false>(a, lanes, grid, block, s);
+  if (!fast) launch_vector<T, ADDR, false, false>(a, lanes, grid, block, s);
+  else if (past) launch_vector<T, ADDR, true, true>(a, lanes, grid, block, s);
+  else launch_vector<T, ADDR, true, false>(a, lanes, grid, block, s);
 }
 
 template <typename T>
