@@ -868,7 +868,8 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
 // The maximum that the weights are taken against grows only when a row's has outgrown it by 2^8: until then the larger weights
 // (below 2^8) and sums say the same, and the rescaling of O, 64 registers at 128 columns, is left out of nearly every step.
 // Bound by the instructions that two wavefronts a SIMD can have under way: the matrix unit is busy for 41 % of the cycles
-// (2048 new tokens behind 13 to 30 thousand keys, 7 query heads to a key head of 128: 740 us, 965 TFLOP/s).
+// (2048 new tokens behind 13 to 30 thousand keys, 7 query heads to a key head of 128: 740 to 830 us as the clock is, up to 965
+// TFLOP/s).
 template <int DP>
 constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16 + DP * 2 + kVPad) + (kWaves + 1) * 4; }
 
