@@ -37,8 +37,8 @@ class PagedAttentionPlan:
 
     The step's work is laid out on the device at construction, by two small launches on the current
     stream; `build()` does it again after the index buffers were written for another step, and can
-    be recorded with the runs into a hipGraph. Runs must be ordered after it. The plan keeps references to
-    the index tensors. Every run takes a workspace of its own from torch's allocator, so runs on
+    be recorded with the runs into a hipGraph (keep the plan while that is replayed). Runs must be ordered after it. The
+    plan keeps references to the index tensors; a step whose `qo_indptr` or `kv_indptr` decreases is not computed. Every run takes a workspace of its own from torch's allocator, so runs on
     different streams do not meet.
     """
 

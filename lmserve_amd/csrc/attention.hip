@@ -218,9 +218,9 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
   constexpr int SUMS = 5;  // narrow work, narrow tiles, wide items, wide slots, sharing tokens
   constexpr int kFew = 4;  // items of a request that its thread does
   __shared__ unsigned long long narrow_work, wide_work, best;
-  __shared__ int32_t wave_sums[16][SUMS], carry[SUMS], shared_tokens, some_request, entries[2], longest, num_wide, num_long;
+  __shared__ int32_t wave_sums[16][SUMS], carry[SUMS], shared_tokens, some_request, entries[2], longest, num_long, out_of_order;
   __shared__ int32_t first_item[kMaxGroups], last_item[kMaxGroups];
-  __shared__ int2 wide_tiles[1024];  // tiles and keys of wide requests (as many as there is room for)
+  __shared__ int2 wide_tiles[1024];  // tiles and keys of those of the first requests that are wide
   __shared__ Tiles long_requests[1024];
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Tiles mine = {};
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
   if (tid == 0) {
     narrow_work = wide_work = 0;
     best = ~0ull;
-    shared_tokens = entries[0] = entries[1] = longest = num_wide = 0;
+    shared_tokens = entries[0] = entries[1] = longest = out_of_order = 0;
     some_request = INT32_MAX;
   }
   for (int32_t w = tid; w < a.groups; w += 1024) {
@@ -237,14 +237,14 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     last_item[w] = -1;
   }
   __syncthreads();
+  wide_tiles[tid] = mine.wide ? make_int2(mine.tiles, mine.len) : make_int2(0, 0);
   for (int32_t b = tid; b < a.batch_size; b += 1024) {
     const Tiles t = b < 1024 ? mine : tiles_of(a, b);
+    if (a.qo_indptr[b] > a.qo_indptr[b + 1] || a.kv_indptr[b] > a.kv_indptr[b + 1]) out_of_order = 1;
     if (t.tiles && !t.wide) atomicAdd(&narrow_work, (unsigned long long)t.before(t.tiles, a.group));
     if (t.wide) {
       atomicAdd(&wide_work, (unsigned long long)t.tiles * t.len);
       atomicMax(&longest, t.len);
-      const int32_t at = atomicAdd(&num_wide, 1);
-      if (at < 1024) wide_tiles[at] = make_int2(t.tiles, t.len);
     }
     if (t.shared_token0 >= 0) {
       atomicAdd(&shared_tokens, t.n);
@@ -252,6 +252,12 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     }
   }
   __syncthreads();
+  // Requests that are to have the same rows or pages: the lists' sizes hold for those that have their own. Nothing is done.
+  if (out_of_order) {
+    if (tid == 0) *a.l.header = {};
+    for (int32_t w = tid; w < a.groups; w += 1024) a.l.ranges[w] = Range{0, 0};
+    return;
+  }
   const int32_t shared_rows = shared_tokens * a.group, shared_len = a.shared_pages * a.page_size;
   const bool shared_wide = shared_rows > a.narrow_shared_rows;
   const int32_t shared_tile = shared_wide ? kWide : kTile, shared_tiles = ceil_div(shared_rows, shared_tile);
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
   int32_t chunk = 1 << 30;
   const int64_t all_wide = (int64_t)wide_work + (shared_wide ? (int64_t)shared_tiles * shared_len : 0);
   if (all_wide) {
-    const int32_t most = max(longest, shared_wide ? shared_len : 0), listed = min(num_wide, 1024);
+    const int32_t most = max(longest, shared_wide ? shared_len : 0), listed = min(a.batch_size, 1024);
     const auto chunk_of = [&](int32_t x) {
       const double keys = __builtin_ceil((double)all_wide * 16 / ((double)a.residents * (x + 1)));
       return round_up((int32_t)(keys < kMinChunk ? kMinChunk : keys < (1 << 30) ? keys : 1 << 30), kStep);
@@ -279,7 +285,7 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     for (int32_t x = wave; x < 64; x += 16) {
       const int32_t keys = chunk_of(x);
       int32_t items = 0;
-      for (int32_t i = lane; i < listed; i += 64) items += wide_tiles[i].x * max(ceil_div(wide_tiles[i].y, keys), 1);
+      for (int32_t i = lane; i < listed; i += 64) if (wide_tiles[i].x) items += wide_tiles[i].x * max(ceil_div(wide_tiles[i].y, keys), 1);
       for (int d = 32; d; d >>= 1) items += __shfl_xor(items, d);
       if (shared_wide) items += shared_tiles * ceil_div(shared_len, keys);
       const int64_t each = min(keys, most) + (keys < most ? kWidePartWork : kWideTileWork);
