@@ -50,6 +50,13 @@ __device__ constexpr int kTileWork = 64, kMinShare = 1024, kMinSharedShare = 256
 // the least range of a wide tile; what an item costs beside its keys, and what one that leaves a partial does
 __device__ constexpr int kMinChunk = 512, kWideTileWork = 128, kWidePartWork = 384;
 constexpr int32_t kMaxKeys = INT32_MAX - 8192;  // of a request: a key that is looked up ahead stays below 2^31
+// The rows of all sharing requests are wide tiles where they are more than kNarrowSharedRows, or more than a narrow tile and
+// rows times keys above kNarrowWork: 96 rows over 4096 keys 26.8 us wide and 33.6 narrow, 128 rows 28.6 and 40.7, 64 rows
+// 26 either way; 91 rows over 2000 keys 24.7 and 20.8, 104 over 1024 18.1 and 15.7.
+__host__ __device__ constexpr bool wide_prefix(int64_t rows, int64_t keys) {
+  constexpr int64_t kNarrowSharedRows = 128, kNarrowWork = 1 << 18;
+  return rows > kNarrowSharedRows || (rows > kTile && rows * keys > kNarrowWork);
+}
 constexpr int kManyParts = 16;     // a row of more partials is joined by a workgroup
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -99,7 +106,7 @@ struct Layout {  // the plan's device buffer
 struct PlanArgs {
   const int32_t *qo_indptr, *kv_indices, *kv_indptr, *kv_last_page_len;
   int32_t batch_size, num_tokens, num_kv_indices, page_size, shared_pages, group;
-  int32_t narrow_rows, narrow_shared_rows;  // the most rows of a request, and of all sharing ones, for narrow tiles
+  int32_t narrow_rows;                      // the most rows of a request for narrow tiles
   int32_t groups, residents;                // of a key head: workgroups for narrow tiles, wide tiles on the card at a time
   int32_t max_items[2], max_entries;
   Layout l;
@@ -259,7 +266,7 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     return;
   }
   const int32_t shared_rows = shared_tokens * a.group, shared_len = a.shared_pages * a.page_size;
-  const bool shared_wide = shared_rows > a.narrow_shared_rows;
+  const bool shared_wide = wide_prefix(shared_rows, shared_len);
   const int32_t shared_tile = shared_wide ? kWide : kTile, shared_tiles = ceil_div(shared_rows, shared_tile);
   const int64_t all_narrow = (int64_t)narrow_work + (shared_wide ? 0 : shared_tiles * ((int64_t)shared_len + kTileWork));
   const int32_t unit = max(0, 34 - (int32_t)__clzll((unsigned long long)all_narrow + 1));  // log2 of the keys of a unit
@@ -1364,8 +1371,11 @@ namespace {
 constexpr int64_t kStepGroups = 1024;         // workgroups for narrow tiles of a launch that has wide ones as well
 constexpr int64_t kResidents = 512;           // wide items on the card at a time
 constexpr int64_t kMaxRounds = 4;             // of them in a step, where a range of keys is longer than the least
-constexpr int64_t kNarrowRows = 32;           // of a request; with more it is cut into wide tiles
-constexpr int64_t kNarrowSharedRows = 128;    // of all sharing requests
+// The most rows of a request for narrow tiles, with more it is cut into wide ones: one narrow tile where there is work to
+// fill the card, that is, where all rows together, over the requests' average of keys, make more than kMuchWork, else two. 32 rows
+// each: 64 requests of 2000 keys 125 us wide and 132 in two narrow tiles, 256 of 600 172 and 221, one of 16000 32 and 40, of
+// 131000 131 and 190; one of 2000 24.8 and 23.0, four of 20 rows and 900 keys 23.1 and 17.5. (48 rows, 64 requests: 127 and 258.)
+constexpr int64_t kNarrowRows = 32, kMuchWork = 1 << 18;
 
 Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
   Layout l;
@@ -1394,7 +1404,7 @@ Sizes sizes_of(const kvc_attention_plan& p) {
   Sizes n;
   const int64_t rows = p.num_tokens * (p.num_heads / p.num_kv_heads);
   const bool shared = p.shared_pages > 0;
-  n.wide = rows > p.narrow_rows || (shared && rows > kNarrowSharedRows);
+  n.wide = rows > p.narrow_rows || (shared && wide_prefix(rows, p.shared_pages * p.page_size));
   const int64_t groups = n.wide ? kStepGroups : 256 * narrow_residents((int)p.head_dim);
   n.groups = std::min<int64_t>(kMaxGroups, std::max<int64_t>(1, groups / p.num_kv_heads));
   n.residents = std::max<int64_t>(1, kResidents / p.num_kv_heads);
@@ -1479,8 +1489,10 @@ int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indice
       qo_indptr, kv_indices, kv_indptr, kv_last_page_len, batch_size, num_tokens, num_kv_indices, num_heads, num_kv_heads,
       head_dim, page_size, shared_pages, kNarrowRows, dtype, sm_scale, {}, 0, 0, nullptr};
   if (!p) return fail(KVC_ERR_HIP, "%s: out of host memory", fn);
+  const int64_t rows = num_tokens * (num_heads / num_kv_heads), keys = num_kv_indices * page_size / std::max<int64_t>(batch_size, 1);
+  if ((double)rows * (double)keys > (double)kMuchWork) p->narrow_rows = kTile;
   // said to have few tokens each: every request in narrow items, whatever it has, and no launch for the others
-  if (max_q_len > 0 && max_q_len * (num_heads / num_kv_heads) <= kNarrowRows) p->narrow_rows = INT32_MAX;
+  if (max_q_len > 0 && max_q_len * (num_heads / num_kv_heads) <= p->narrow_rows) p->narrow_rows = INT32_MAX;
   p->n = sizes_of(*p);
   layout_of(*p, nullptr, &p->plan_bytes);
   for (int k = 0; k < 2; ++k) p->workspace_bytes += p->n.max_slots[k] * num_kv_heads * (k ? kWide : kTile) * (head_dim + 1) * 4;
@@ -1506,7 +1518,7 @@ int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buf
   PlanArgs a{plan->qo_indptr, plan->kv_indices, plan->kv_indptr, plan->kv_last_page_len, (int32_t)plan->batch_size,
              (int32_t)plan->num_tokens, (int32_t)plan->num_kv_indices, (int32_t)plan->page_size,
              (int32_t)plan->shared_pages, (int32_t)(plan->num_heads / plan->num_kv_heads), (int32_t)plan->narrow_rows,
-             (int32_t)kNarrowSharedRows, (int32_t)plan->n.groups, (int32_t)plan->n.residents,
+             (int32_t)plan->n.groups, (int32_t)plan->n.residents,
              {(int32_t)plan->n.max_items[0], (int32_t)plan->n.max_items[1]}, (int32_t)plan->n.max_entries,
              layout_of(*plan, plan->buffer, nullptr)};
   hipStream_t s = (hipStream_t)stream;
