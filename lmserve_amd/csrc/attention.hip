@@ -1415,10 +1415,14 @@ Sizes sizes_of(const kvc_attention_plan& p) {
   n.max_items[1] = n.wide ? tiles(kWide) + kMaxRounds * n.residents : 0;
   n.max_slots[1] = n.wide ? 2 * kMaxRounds * n.residents + shared_tiles(kWide) : 0;
   n.max_shared_tiles = shared_tiles(kTile);
-  // (where the shares are the least there are, a narrow tile that is no longer is never cut; nor is a wide one that is no
-  // longer than the least range)
-  const int64_t keys = p.num_kv_indices * p.page_size, work = keys + tiles(kTile) * (kTileWork + kTile + 2);
-  n.join = shared || work > kMinShare * n.groups || keys + kTileWork + kTile + 2 >= kMinShare || (n.wide && keys > kMinChunk);
+  // Where no tile can be cut none is joined. Narrow ones are cut where the line of work is longer than all shares of the least length,
+  // or a tile as long as one. The line counts a request's keys once a tile (Tiles::before), or its tokens where they are more than
+  // its keys; a request has as many tiles as `narrow_rows` allow, all of them where a hint made every request narrow. Wide
+  // ones are cut where a request has more keys than the least range.
+  const int64_t group = p.num_heads / p.num_kv_heads, keys = p.num_kv_indices * p.page_size, each = kTileWork + kTile + 2;
+  const int64_t request_rows = std::min(rows, p.narrow_rows), request_tokens = request_rows / group;
+  const int64_t line = (request_rows + kTile - 1) / kTile * (keys + p.num_tokens) + tiles(kTile) * each;
+  n.join = shared || line > kMinShare * n.groups || std::max(keys, request_tokens) + each >= kMinShare || (n.wide && keys > kMinChunk);
   n.max_entries = n.join ? rows : 0;
   return n;
 }

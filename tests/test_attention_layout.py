@@ -1,0 +1,100 @@
+"""The attention plan's capacities against the work that its layout can make of a step, without a GPU: what is cut must have
+somewhere to be joined. The rules of the line of work are restated here."""
+import ctypes
+import random
+
+import pytest
+
+from lmserve_amd import _lib
+
+TILE, TILE_WORK, MIN_SHARE, MIN_PART, MAX_GROUPS = 16, 64, 1024, 256, 1024
+
+
+def ceil(a, b):
+    return -(-a // b)
+
+
+def plan_bytes(lens, hq, hk, d, page, max_q, pages=None, tokens=None):
+    tokens = sum(n for n, _ in lens) if tokens is None else tokens
+    pages = sum(ceil(k, page) for _, k in lens) if pages is None else pages
+    h = ctypes.c_void_p()
+    L = _lib.lib()
+    assert L.kvc_attention_plan_create(4096, 8192, 12288, 16384, len(lens), tokens, pages, hq, hk, d, page, max_q, 0, d ** -0.5, 0,
+                                       ctypes.byref(h)) == _lib.KVC_OK
+    got = L.kvc_attention_plan_bytes(h)
+    L.kvc_attention_plan_destroy(h)
+    return got
+
+
+def narrow_rows(lens, hq, hk, page, max_q, pages=None):
+    rows = sum(n for n, _ in lens) * (hq // hk)
+    pages = sum(ceil(k, page) for _, k in lens) if pages is None else pages
+    most = 16 if rows * (pages * page // len(lens)) > 1 << 18 else 32
+    return 1 << 31 if 0 < max_q * (hq // hk) <= most else most
+
+
+def parts_of_narrow_tiles(lens, hq, hk, d, most):
+    """How many parts every narrow tile of a step is cut into, its tiles end to end on the line of work."""
+    group = hq // hk
+    wide = sum(n for n, _ in lens) * group > most
+    groups = max(1, min(MAX_GROUPS, (1024 if wide else 256 * (4 if d <= 64 else 2 if d <= 128 else 1)) // hk))
+    tiles = []
+    for n, k in lens:
+        if n == 0 or n * group > most:
+            continue
+
+        def before(i):
+            first = max(0, min(k, k - n + ceil(TILE, group)))
+            return i * (first + TILE_WORK) + (i * (i - 1) // 2 * TILE // group if i >= 2 else 0)
+        tiles += [before(i + 1) - before(i) for i in range(ceil(n * group, TILE))]
+    share = max(ceil(sum(tiles), groups), MIN_SHARE)
+    sliver = share // 2 if share <= MIN_SHARE else min(share // 2, MIN_PART)
+    at, parts = 0, []
+    for work in tiles:
+        first = min((at + sliver - 1) // share, groups - 1)
+        last = 0 if at + work < sliver else (at + work - sliver) // share
+        parts.append(max(last - first, 0) + 1)
+        at += work
+    return parts
+
+
+def check(lens, hq, hk, d, page, max_q):
+    """Where a tile is cut, the plan has room for its rows' entries: it is as large as one whose requests could have keys enough."""
+    most = narrow_rows(lens, hq, hk, page, max_q)
+    cut = max(parts_of_narrow_tiles(lens, hq, hk, d, most), default=1) > 1
+    if cut:
+        long = ceil(942, page)
+        if narrow_rows(lens, hq, hk, page, max_q, long) != most:
+            return False      # (other tiles with more keys: nothing to compare with)
+        assert plan_bytes(lens, hq, hk, d, page, max_q) == plan_bytes(lens, hq, hk, d, page, max_q, pages=long), lens
+    return cut
+
+
+@pytest.mark.parametrize("lens,hq,hk,d,max_q", [
+    ([(900, 900)], 32, 8, 128, 1), ([(600, 900)], 32, 8, 128, 1), ([(700, 700)], 32, 32, 256, 1), ([(900, 900)], 16, 2, 256, 2),
+    ([(20, 704), (20, 224)], 128, 128, 256, 20), ([(1500, 100)], 8, 8, 128, 1), ([(3000, 0)], 2, 1, 64, 1)])
+def test_tiles_that_are_cut_are_joined(lens, hq, hk, d, max_q):
+    assert check(lens, hq, hk, d, 16, max_q)
+
+
+def test_tiles_that_are_cut_are_joined_in_steps_as_they_come():
+    rng, cuts = random.Random(5), 0
+    for _ in range(4000):
+        hk = rng.choice([1, 2, 8, 32, 128, 512])
+        hq, d, page = hk * rng.choice([1, 2, 4, 7]), rng.choice([64, 128, 256]), rng.choice([1, 16, 20])
+        left, lens = rng.randint(0, 941), []
+        for _ in range(rng.randint(1, 8)):
+            k = rng.randint(0, left)
+            left -= k
+            lens.append((rng.choice([0, 1, 3, 20, 200, 1500]) if rng.random() < .5 else min(k, rng.choice([1, 5, 20, 900])), k))
+        cuts += check(lens, hq, hk, d, page, rng.choice([0, 1, 4, 20]))
+    assert cuts > 200
+
+
+def test_small_steps_need_no_join():
+    """What cannot be cut has no entries: a decode step of short requests and a chunk of few tokens are one launch."""
+    for lens, hq, hk, max_q in (([(1, 200)] * 4, 32, 8, 1), ([(1, 900)], 32, 8, 1), ([(1, 16)] * 50, 32, 8, 1), ([(4, 100)] * 4, 32, 8, 4)):
+        rows = sum(n for n, _ in lens) * (hq // hk)
+        long = ceil(1100, 16)
+        assert narrow_rows(lens, hq, hk, 16, max_q, long) == narrow_rows(lens, hq, hk, 16, max_q)
+        assert plan_bytes(lens, hq, hk, 128, 16, max_q, pages=long) - plan_bytes(lens, hq, hk, 128, 16, max_q) == ceil(rows * 32, 256) * 256
