@@ -468,6 +468,7 @@ struct BF16 {
   }
   static __device__ __forceinline__ float wide(uint32_t half) { return __uint_as_float(half << 16); }
   static constexpr uint32_t kExponent = 0x7f80u;
+  static constexpr float kScaledUp = 0;
 };
 struct F16 {
   typedef _Float16 V8 __attribute__((ext_vector_type(8)));
@@ -486,6 +487,9 @@ struct F16 {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)half);
   }
   static constexpr uint32_t kExponent = 0x7c00u;
+  // log2 of what weights are scaled up by, so that small ones, of which there may be many, are numbers of the type: a weight of 1 is
+  // then 2^14 in a narrow tile, and one of kOutgrown, 2^8, is 2^15 in a wide tile. Both keep a step of the type below its largest.
+  static constexpr float kScaledUp = 14;
 };
 // Is an infinity or NaN among the 16-bit values that were taken in? (The largest exponent of either half.)
 template <typename T>
@@ -660,7 +664,8 @@ struct Block {
 //   O^T = V^T P^T: a lane's 8 probabilities, of keys 4q..4q+3 and 16+4q..16+4q+3 (q = lane / 16), are the B operand as S^T
 //   left them; the A operand wants the same keys of one column of V, which the transposing LDS read gives.
 // P is rounded to the storage type for the matrix instruction, each weight by at most half a step of itself, as the inputs
-// were; the sum l is of the weights before that, since lse is an output in 32 bits.
+// were (in f16 from 2^-28 of the largest on; smaller ones by at most 2^-39 of it); the sum l is of the weights before that, since
+// lse is an output in 32 bits.
 template <typename T, int DP>
 struct RowTile {
   static constexpr int KSTEPS = DP / 32, DTILES = DP / 16;
@@ -668,7 +673,7 @@ struct RowTile {
   typedef Block<DP> B;
   u32x4 q[KSTEPS];
   f32x4 o[DTILES];
-  float m, l;
+  float base, l;  // weights are exp2(score * scale - base)
   int32_t limit;
   int32_t odd_from;  // the first block whose infinities and NaN of V were left out
 
@@ -714,27 +719,28 @@ struct RowTile {
         for (int r = 0; r < 4; ++r)
           if (!(sees >> (i * 16 + r) & 1)) s[i][r] = -INFINITY;
     }
-    float top = m;
+    float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
     top = max_across32(max_across16(top));
-    const float base = top == -INFINITY ? 0.f : top * a.scale;
-    const float shrink = exp2_of(m * a.scale - base);  // 0 from -inf
+    const float grown = fmaxf(base, top * a.scale - T::kScaledUp);
+    const float from = grown == -INFINITY ? 0.f : grown;
+    const float shrink = exp2_of(base - from);  // 0 from -inf
     u32x4 p;
     float sum = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
-        const float x = exp2_of(__builtin_fmaf(s[i][r], a.scale, -base));
-        const float y = exp2_of(__builtin_fmaf(s[i][r + 1], a.scale, -base));
+        const float x = exp2_of(__builtin_fmaf(s[i][r], a.scale, -from));
+        const float y = exp2_of(__builtin_fmaf(s[i][r + 1], a.scale, -from));
         p[i * 2 + r / 2] = T::pack(x, y);
         sum += x + y;
       }
     l = l * shrink + sum;
-    m = top;
+    base = grown;
 #pragma unroll
     for (int d = 0; d < DTILES; ++d) {
       const char* from = my_v + (quad * 4 + n / 4) * VSTRIDE + (d * 16 + n % 4 * 4) * 2;
@@ -757,6 +763,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
   typedef Block<DP> B;
   constexpr int KSTEPS = Tile::KSTEPS, DTILES = Tile::DTILES, VSTRIDE = Tile::VSTRIDE;
   constexpr int OSTRIDE = DP + 4;
+  constexpr float kUnscaled = 1.f / (1 << (int)T::kScaledUp);
   static_assert(kTile * OSTRIDE * 4 <= kBlock * VSTRIDE, "a wavefront's O takes the place of its V");
   typedef float Stats[2][kTile];
   Stats* const stats = reinterpret_cast<Stats*>(lds + kWaves * kBlock * VSTRIDE);
@@ -765,7 +772,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
   const int32_t D = a.head_dim;
   {
     Tile tile = {};
-    tile.m = -INFINITY;
+    tile.base = -INFINITY;
     tile.odd_from = INT32_MAX;
     if (n < item.rows) {
       const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
@@ -829,23 +836,23 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (quad == 0) {
-      stats[wave][0][n] = tile.m;
+      stats[wave][0][n] = tile.base;
       stats[wave][1][n] = l;
     }
     __syncthreads();
-    float all_m = -INFINITY, all_l = 0;
+    float top = -INFINITY, all_l = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) all_m = fmaxf(all_m, stats[w][0][n]);
-    const float base = all_m == -INFINITY ? 0.f : all_m * a.scale;
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][0][n]);
+    const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) all_l += stats[w][1][n] * exp2_of(stats[w][0][n] * a.scale - base);
-    const float part = exp2_of(tile.m * a.scale - base) * (all_l == 0 ? 0.f : 1.f / all_l);
+    for (int w = 0; w < kWaves; ++w) all_l += stats[w][1][n] * exp2_of(stats[w][0][n] - base);
+    const float part = exp2_of(tile.base - base) * (all_l == 0 ? 0.f : 1.f / all_l);
     float* my_o = reinterpret_cast<float*>(my_v);
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
       *reinterpret_cast<f32x4*>(my_o + n * OSTRIDE + d * 16 + quad * 4) = tile.o[d] * part;
     if (wave == 0 && quad == 0 && n < item.rows) {
-      const float lse2 = all_l == 0 ? -INFINITY : base + __log2f(all_l);
+      const float lse2 = all_l == 0 ? -INFINITY : base + T::kScaledUp + __log2f(all_l * kUnscaled);
       if (item.slot >= 0) {
         a.partial_lse[0][((int64_t)item.slot * a.kv_heads + h) * kTile + n] = lse2;
       } else if (a.lse) {
@@ -892,7 +899,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
   constexpr int KSTRIDE = DP * 2 + 16, VSTRIDE = DP * 2 + kVPad;
   constexpr int LPR = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // lanes to a row
   constexpr int RPW = 64 / LPR, ROUNDS = kStep / (RPW * kWaves);
-  constexpr float kOutgrown = 8;
+  constexpr float kScaledUp = T::kScaledUp / 2, kOutgrown = 8 + kScaledUp, kUnscaled = 1.f / (1 << (int)kScaledUp);
   typedef char KStep[kStep * KSTRIDE];
   typedef char VStep[kStep * VSTRIDE];
   KStep* const k_lds = reinterpret_cast<KStep*>(lds);
@@ -927,7 +934,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
     __syncthreads();
     const int32_t tile_least = min(min(leasts[0], leasts[1]), min(leasts[2], leasts[3]));
     f32x16 o[DTILES] = {};
-    float base = -INFINITY, l = 0;  // weights are exp2(score * scale - base)
+    float base = -INFINITY, l = 0;  // as in a narrow tile
     u32x4 kr[ROUNDS], vr[ROUNDS];
     uint32_t group_lo = 0, group_hi = 0;  // where the groups of 16 keys of 16 windows lie, one to a lane
     uint64_t groups = 0;                  // and which of them are there
@@ -1061,10 +1068,10 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
       return max_across32(top);
     };
     // A base that has been outgrown. It is a whole number, so that what was made with the old one, the weights that wait
-    // for their product among it, is scaled exactly.
+    // for their product among it, is scaled exactly (in f16 those that stay above 2^-21 of a weight of 1, others to 2^-32 of it).
     const auto grow = [&](float top, uint32_t* waiting) {
       if (__ballot(top * a.scale > base + kOutgrown)) {
-        const float grown = fmaxf(base, __builtin_ceilf(top * a.scale));
+        const float grown = fmaxf(base, __builtin_ceilf(top * a.scale) - kScaledUp);
         const float shrink = exp2_of(base - (grown == -INFINITY ? 0.f : grown));  // 0 from -inf
 #pragma unroll
         for (int d = 0; d < DTILES; ++d) o[d] *= shrink;
@@ -1194,7 +1201,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
       }
     }
     l += __shfl_xor(l, 32);
-    const float inv = l == 0 ? 0.f : 1.f / l, lse2 = l == 0 ? -INFINITY : base + __log2f(l);
+    const float inv = l == 0 ? 0.f : 1.f / l, lse2 = l == 0 ? -INFINITY : base + kScaledUp + __log2f(l * kUnscaled);
     if (my_row < item.rows) {
       if (item.slot >= 0) {
         const int64_t row = ((int64_t)item.slot * a.kv_heads + h) * kWide + my_row;

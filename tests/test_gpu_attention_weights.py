@@ -1,0 +1,60 @@
+"""Softmax weights far below the largest: many of them together count, however small each is."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import attention_oracle as ao
+from tests.test_gpu_attention import Step
+
+pytestmark = pytest.mark.gpu
+
+
+def sink_step(lengths, heads, kv_heads, D, page, dtype, above, at, seed=30):
+    """One key of every request stands `above` the others, whose scores are about 0, and its value is 0."""
+    s = Step(lengths, heads, kv_heads, D, page, dtype, seed=seed)
+    rng = np.random.default_rng(seed)
+    q = rng.standard_normal(D).astype(np.float32)
+    s.query = torch.from_numpy(np.broadcast_to(q, (s.T, heads, D)).copy()).to(s.dtype)
+    s.cache[:, 0] *= 0.1
+    s.cache[:, 1] = 1 + 0.3 * s.cache[:, 1]
+    q = s.query[0, 0].float().numpy()
+    for b in range(len(lengths)):
+        p = s.indices[s.indptr[b] + at // page]
+        s.cache[p, 0, at % page] = torch.from_numpy(q * (above / s.scale / (q * q).sum())).to(s.dtype)
+        s.cache[p, 1, at % page] = 0
+    return s
+
+
+def check(s, out, lse):
+    """As Step.check, but with a bound on a weight's rounding that has no floor at the type's smallest number. What is left of one:
+    weights are at most 2^-7 of the type's range below it, half a step of the smallest numbers is 2^-25, and a base stands
+    up to 1 above the largest score: 2^-31 of the largest weight."""
+    want, want_lse, weighted, values, products = s.oracle()
+    tol, tol_lse = ao.attention_tolerances(want, want_lse, weighted, values, products, s.D, s.scale, s.eps, 0.0)
+    # (the output's own smallest numbers)
+    tol = tol + values * 2.0 ** -31 * (s.denormal > 0) + s.denormal
+    got = out.cpu().double().numpy().reshape(want.shape)
+    err = np.abs(got - want)
+    assert (err <= tol).all(), f"off by {np.nanmax(err / tol):.3g} of the bound, {np.nanmax(err / np.abs(want)):.3g} of the value"
+    assert (np.abs(lse.cpu().double().numpy() - want_lse) <= tol_lse).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("above", [9.0, 16.5, 18.0])
+@pytest.mark.parametrize("lengths,heads,kv_heads,D,page", [
+    ([(1, 7001)], 4, 2, 64, 16), ([(1, 900), (2, 700)], 4, 1, 128, 16), ([(1, 3000)], 4, 1, 80, 20),   # narrow tiles
+    ([(40, 3000)], 4, 1, 64, 16), ([(40, 900), (35, 2001)], 4, 2, 128, 20), ([(40, 6000)], 128, 128, 8, 16)])   # wide
+def test_one_key_far_above_many(gpu, lengths, heads, kv_heads, D, page, above, dtype):
+    s = sink_step(lengths, heads, kv_heads, D, page, dtype, above, 100)
+    out, lse = s.plan(gpu).run(s.query.to(gpu), s.cache.to(gpu), return_lse=True)
+    check(s, out, lse)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_the_far_key_comes_late(gpu, new, dtype):
+    """What was summed before it, and the weights that wait for their product, are scaled down by as much."""
+    for at in (160, 1499, 2950):
+        s = sink_step([(new, 3000)], 4, 1, 64, 16, dtype, 16.5, at)
+        out, lse = s.plan(gpu).run(s.query.to(gpu), s.cache.to(gpu), return_lse=True)
+        check(s, out, lse)
