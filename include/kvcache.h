@@ -591,8 +591,12 @@ int kvc_rotary_plan_run_norm(const kvc_rotary_plan* plan, const void* query, con
  * last key, or is masked, does not reach the result, infinities and NaN included.
  * qo_indptr and kv_indptr do not decrease; where one does, the step is not computed and no row written.
  * Rows behind qo_indptr[batch_size] are left as they were. Sums and softmax
- * statistics are fp32, the weights are rounded to the storage type for the
- * matrix instruction, the output once.
+ * statistics are fp32, the output is rounded once. Requests of more than 32
+ * rows (tokens times num_heads / num_kv_heads; more than 16 where there is much work), and a
+ * prefix that many rows share, have their weights rounded to the storage type for the matrix
+ * instruction, each by at most half a step of itself; those of the others keep twice as many bits.
+ * Scores, times log2(e), are below 2^24 in magnitude: beyond that a step of fp32 is
+ * more than 1, and weights may leave the type's range.
  *
  * max_q_len: the most tokens that a request has, 0 if not known. It helps to choose
  * kernels and is no limit. shared_pages: the leading pages that the requests of the batch share (a

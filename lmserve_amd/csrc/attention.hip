@@ -663,9 +663,10 @@ struct Block {
 //   S^T = K Q^T: the keys' rows are the matrix instruction's A operand as they lie in memory, 16 bytes a lane.
 //   O^T = V^T P^T: a lane's 8 probabilities, of keys 4q..4q+3 and 16+4q..16+4q+3 (q = lane / 16), are the B operand as S^T
 //   left them; the A operand wants the same keys of one column of V, which the transposing LDS read gives.
-// P is rounded to the storage type for the matrix instruction, each weight by at most half a step of itself, as the inputs
-// were (in f16 from 2^-28 of the largest on; smaller ones by at most 2^-39 of it); the sum l is of the weights before that, since
-// lse is an output in 32 bits.
+// The matrix instruction takes 16 bits: a weight goes in as two numbers of the storage type, itself rounded and the rest rounded, off
+// by a half step's square. The second product is on a unit that waits for keys: decode of 256 requests 405.4 us with one
+// product and 405.7 with both, one request 17.5 and 17.9, the error against 64 bits 2.02e-3 and 1.65e-3 of the outputs' size, which is
+// their own rounding. (f16: from 2^-28 of the largest weight on; smaller ones are off by at most 2^-39 of it.)
 template <typename T, int DP>
 struct RowTile {
   static constexpr int KSTEPS = DP / 32, DTILES = DP / 16;
@@ -728,7 +729,7 @@ struct RowTile {
     const float grown = fmaxf(base, top * a.scale - T::kScaledUp);
     const float from = grown == -INFINITY ? 0.f : grown;
     const float shrink = exp2_of(base - from);  // 0 from -inf
-    u32x4 p;
+    u32x4 p, rest;
     float sum = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -736,11 +737,14 @@ struct RowTile {
       for (int r = 0; r < 4; r += 2) {
         const float x = exp2_of(__builtin_fmaf(s[i][r], a.scale, -from));
         const float y = exp2_of(__builtin_fmaf(s[i][r + 1], a.scale, -from));
-        p[i * 2 + r / 2] = T::pack(x, y);
+        const uint32_t two = T::pack(x, y);
+        p[i * 2 + r / 2] = two;
+        rest[i * 2 + r / 2] = T::pack(x - T::wide(two & 0xffffu), y - T::wide(two >> 16));
         sum += x + y;
       }
     l = l * shrink + sum;
     base = grown;
+    u32x4 last = {};
 #pragma unroll
     for (int d = 0; d < DTILES; ++d) {
       const char* from = my_v + (quad * 4 + n / 4) * VSTRIDE + (d * 16 + n % 4 * 4) * 2;
@@ -750,7 +754,10 @@ struct RowTile {
       const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
       const u32x4 v = {x[0], x[1], y[0], y[1]};
       o[d] = T::mfma(v, p, o[d] * shrink);
+      if (d) o[d - 1] = T::mfma(last, rest, o[d - 1]);
+      last = v;
     }
+    o[DTILES - 1] = T::mfma(last, rest, o[DTILES - 1]);
   }
 };
 
@@ -1084,6 +1091,9 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
     // 32 keys: their weights from the scores s, while the scores of the keys behind them and the product of the weights
     // before them, that waited, with V are on the matrix unit. The order is written out, a product with what goes on beside
     // it to a line: pieces from LDS for the products kAhead further on, half a pair of weights, the next scores' maximum.
+    // A weight is rounded to the storage type for its product, off by at most half a step of itself; their sum l is of the weights
+    // before that. The rest as a second product, as in a narrow tile, would cost what the matrix unit is bound by: 2048 new
+    // tokens 800 us so and 1043 with both, the error against 64 bits 2.33e-3 and 1.66e-3 of the outputs' size.
     const auto take = [&](const f32x16& s, uint32_t* p, f32x16& next, float& top, const uint32_t* waiting, int buf, auto which,
                           u32x4* piece) {
       constexpr int PIECES = KSTEPS + 2 * DTILES, HALF = decltype(which)::value;

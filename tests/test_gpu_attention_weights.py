@@ -58,3 +58,20 @@ def test_the_far_key_comes_late(gpu, new, dtype):
         s = sink_step([(new, 3000)], 4, 1, 64, 16, dtype, 16.5, at)
         out, lse = s.plan(gpu).run(s.query.to(gpu), s.cache.to(gpu), return_lse=True)
         check(s, out, lse)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lengths,heads,kv_heads,D,page,shared", [
+    ([(1, 40), (1, 700), (2, 65), (1, 2001)], 8, 2, 128, 16, 0), ([(4, 300), (1, 33)], 8, 2, 64, 16, 0), ([(1, 900)], 16, 1, 80, 20, 0),
+    ([(3, 500), (1, 77)], 5, 1, 256, 32, 0), ([(1, 400 + 9 * i) for i in range(4)], 8, 2, 96, 8, 40)])
+def test_few_rows_round_their_outputs_only(gpu, lengths, heads, kv_heads, D, page, shared, dtype):
+    """Narrow tiles: the weights' two parts are off by 2^-16 (bf16) and 2^-22 of themselves, 32-bit sums by less, and the output's
+    rounding is all that shows: the error's root mean square is that of the exact outputs rounded, to 1 %. (A weight in one
+    part adds as much again as its own rounding, a quarter.)"""
+    s = Step(lengths, heads, kv_heads, D, page, dtype, shared=shared, seed=31)
+    out, lse = s.plan(gpu, max_q_len=max(n for n, _ in lengths)).run(s.query.to(gpu), s.cache.to(gpu), return_lse=True)
+    s.check(out, lse)
+    want = torch.from_numpy(s.oracle()[0])
+    rms = lambda x: x.square().mean().sqrt().item()
+    rounded = rms(want.to(s.dtype).double() - want)
+    assert rms(out.cpu().double().reshape(want.shape) - want) <= 1.01 * rounded
