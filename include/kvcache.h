@@ -612,6 +612,9 @@ int kvc_rotary_plan_run_norm(const kvc_rotary_plan* plan, const void* query, con
  * (kvc_attention_plan_bytes, device memory, aligned to 256, kept by the caller while the plan
  * is used); _run must be ordered after it. _run works in `workspace`
  * (kvc_attention_workspace_bytes, aligned to 256): runs that may overlap need a workspace each.
+ * It holds partial results: up to 9 MB (32 / 8 heads of 128) where every request has few rows and
+ * none share, up to 340 MB where the capacities admit long contexts under many rows, more with more
+ * key heads and wider ones (64 of 256 with a shared prefix 1.4 GB).
  * query [num_tokens, num_heads*head_dim] with a token stride in elements,
  * rows and pages aligned to 16 bytes; out [num_tokens, num_heads*head_dim]
  * contiguous; lse fp32 [num_tokens, num_heads] or NULL. `out` may be the query

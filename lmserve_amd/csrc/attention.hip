@@ -1413,32 +1413,41 @@ Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
   return l;
 }
 
-// Row tiles are at most rows / tile and one more for every request that has tokens, and those of the shared prefix. A narrow
-// tile's part in a workgroup has place tile + workgroup in the list; two parts of a workgroup need slots, and, where a prefix is
-// shared, every tile's first part. Wide tiles cut into ranges of at least the rounds' share of all keys make at most
-// the rounds' items and one more a tile; those of two ranges or more, which need slots, at most twice the rounds' items.
+// What a step of these capacities can need. Requests with tokens are at most `requests`; those of more than `narrow_rows` rows are
+// wide, the others narrow, and only narrow ones share a prefix. Tiles of a kind are at most their rows / tile and one more a
+// request. A narrow tile's part in a workgroup has place tile + workgroup in the list; two parts of a workgroup that the line reaches need slots, and,
+// where a prefix is shared, every tile's first part. Wide tiles cut into ranges of at least the rounds' share of all keys make at most
+// the rounds' items and one more a tile. Slots are for those of two ranges or more: they have no more tiles than rounds'
+// items, and no more ranges than the tables' keys hold of the least length (heads of 128: 20 tokens of 4 x 8 heads over 900 keys 1.5 MB
+// of workspace, 256 tokens of 256 requests 8, or 188 where any request may have them all, 2048 tokens of 7 x 4 heads behind long
+// contexts 175).
 Sizes sizes_of(const kvc_attention_plan& p) {
   Sizes n;
-  const int64_t rows = p.num_tokens * (p.num_heads / p.num_kv_heads);
+  const int64_t rows = p.num_tokens * (p.num_heads / p.num_kv_heads), keys = p.num_kv_indices * p.page_size;
   const bool shared = p.shared_pages > 0;
   n.wide = rows > p.narrow_rows || (shared && wide_prefix(rows, p.shared_pages * p.page_size));
   const int64_t groups = n.wide ? kStepGroups : 256 * narrow_residents((int)p.head_dim);
   n.groups = std::min<int64_t>(kMaxGroups, std::max<int64_t>(1, groups / p.num_kv_heads));
   n.residents = std::max<int64_t>(1, kResidents / p.num_kv_heads);
-  const auto shared_tiles = [&](int64_t tile) { return shared ? rows / tile + 1 : 0; };
-  const auto tiles = [&](int64_t tile) { return rows / tile + std::min(p.batch_size, p.num_tokens) + shared_tiles(tile); };
-  n.max_items[0] = tiles(kTile) + n.groups;
-  n.max_slots[0] = 2 * n.groups + (shared ? tiles(kTile) : 0);
-  n.max_items[1] = n.wide ? tiles(kWide) + kMaxRounds * n.residents : 0;
-  n.max_slots[1] = n.wide ? 2 * kMaxRounds * n.residents + shared_tiles(kWide) : 0;
+  const int64_t requests = std::min(p.batch_size, p.num_tokens), of_narrow = std::min(rows, p.narrow_rows);
+  const int64_t narrow_tiles = std::min(rows / kTile + requests, requests * ((of_narrow + kTile - 1) / kTile));
+  const int64_t wide_tiles = rows / kWide + std::min(requests, rows / (p.narrow_rows + 1));
+  const auto shared_tiles = [&](int64_t tile) { return shared ? std::min(rows, requests * of_narrow) / tile + 1 : 0; };
+  const auto ranges = [](int64_t of) { return of > kMinChunk ? (of + kMinChunk - 1) / kMinChunk : 0; };
+  const int64_t rounds = kMaxRounds * n.residents;
+  n.max_items[0] = narrow_tiles + shared_tiles(kTile) + n.groups;
+  // The line of work of the narrow tiles. It counts a request's keys once a tile (Tiles::before), or its tokens where they are
+  // more than its keys; a request has as many tiles as `narrow_rows` allow, all of them where a hint made every request narrow.
+  const int64_t each = kTileWork + kTile + 2, request_tokens = of_narrow / (p.num_heads / p.num_kv_heads);
+  const int64_t line = (of_narrow + kTile - 1) / kTile * (keys + p.num_tokens) + narrow_tiles * each;
+  n.max_slots[0] = shared ? 2 * n.groups + narrow_tiles + shared_tiles(kTile) : 2 * std::min(n.groups, line / kMinShare + 2);
+  n.max_items[1] = n.wide ? wide_tiles + shared_tiles(kWide) + rounds : 0;
+  n.max_slots[1] = n.wide ? std::min(rounds + std::min(wide_tiles, rounds) + shared_tiles(kWide),
+                                     wide_tiles * ranges(keys) + shared_tiles(kWide) * std::max<int64_t>(ranges(p.shared_pages * p.page_size), 1))
+                          : 0;
   n.max_shared_tiles = shared_tiles(kTile);
-  // Where no tile can be cut none is joined. Narrow ones are cut where the line of work is longer than all shares of the least length,
-  // or a tile as long as one. The line counts a request's keys once a tile (Tiles::before), or its tokens where they are more than
-  // its keys; a request has as many tiles as `narrow_rows` allow, all of them where a hint made every request narrow. Wide
-  // ones are cut where a request has more keys than the least range.
-  const int64_t group = p.num_heads / p.num_kv_heads, keys = p.num_kv_indices * p.page_size, each = kTileWork + kTile + 2;
-  const int64_t request_rows = std::min(rows, p.narrow_rows), request_tokens = request_rows / group;
-  const int64_t line = (request_rows + kTile - 1) / kTile * (keys + p.num_tokens) + tiles(kTile) * each;
+  // Where no tile can be cut none is joined. Narrow ones are cut where the line is longer than all shares of the least length,
+  // or a tile as long as one, wide ones where a request has more keys than the least range.
   n.join = shared || line > kMinShare * n.groups || std::max(keys, request_tokens) + each >= kMinShare || (n.wide && keys > kMinChunk);
   n.max_entries = n.join ? rows : 0;
   return n;
