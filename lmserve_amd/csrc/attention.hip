@@ -1360,6 +1360,14 @@ __global__ __launch_bounds__(kThreads, 6) void attend_join_kernel(AttendArgs a) 
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
+struct Memory {  // of an argument (which may be null)
+  const void* p;
+  int64_t bytes;
+  bool meets(const Memory& o) const {
+    return p && o.p && (uintptr_t)p < (uintptr_t)o.p + (uint64_t)o.bytes && (uintptr_t)o.p < (uintptr_t)p + (uint64_t)bytes;
+  }
+};
+
 // The sizes that follow from the capacities: of narrow and of wide items
 struct Sizes {
   int64_t groups, residents, max_items[2], max_slots[2], max_shared_tiles, max_entries;
@@ -1543,6 +1551,10 @@ int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buf
   if (!plan) return fail(KVC_ERR_INVALID_ARG, "%s: null plan", fn);
   if (!buffer || (uintptr_t)buffer % 256 || buffer_bytes < plan->plan_bytes)
     return fail(KVC_ERR_STAGING, "%s: the plan needs %lld bytes, aligned to 256", fn, (long long)plan->plan_bytes);
+  const Memory to{buffer, plan->plan_bytes};
+  if (to.meets({plan->qo_indptr, (plan->batch_size + 1) * 4}) || to.meets({plan->kv_indices, plan->num_kv_indices * 4}) ||
+      to.meets({plan->kv_indptr, (plan->batch_size + 1) * 4}) || to.meets({plan->kv_last_page_len, plan->batch_size * 4}))
+    return fail(KVC_ERR_INVALID_ARG, "%s: the buffer overlaps the index arrays", fn);
   plan->buffer = (char*)buffer;
   if (plan->batch_size == 0 || plan->num_tokens == 0) return KVC_OK;
   PlanArgs a{plan->qo_indptr, plan->kv_indices, plan->kv_indptr, plan->kv_last_page_len, (int32_t)plan->batch_size,
@@ -1578,20 +1590,20 @@ int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query, in
     return fail(KVC_ERR_STAGING, "%s: the workspace needs %lld bytes", fn, (long long)plan->workspace_bytes);
   if (!plan->buffer) return fail(KVC_ERR_INVALID_ARG, "%s: the plan is not built", fn);
   // A row of the query is read before the same row of the output is written, and by no one else afterwards; nothing else that
-  // is read or written may share memory with the output
-  const auto meet = [](const void* x, int64_t n, const void* y, int64_t m) {
-    return x && y && (uintptr_t)x < (uintptr_t)y + (uint64_t)m && (uintptr_t)y < (uintptr_t)x + (uint64_t)n;
-  };
-  const int64_t q_row = plan->num_heads * plan->head_dim * 2, out_bytes = plan->num_tokens * q_row;
-  const int64_t q_bytes = (plan->num_tokens - 1) * q_token_stride * 2 + q_row, lse_bytes = plan->num_tokens * plan->num_heads * 4;
-  const int64_t cache_bytes = num_pages > 0 ? (num_pages - 1) * page_stride * 2 + page * 2 : 0;
+  // is read or written may share memory with what is written
+  const int64_t q_row = plan->num_heads * plan->head_dim * 2;
   const bool in_place = out == query && (plan->num_tokens == 1 || q_token_stride * 2 == q_row);
-  if ((!in_place && meet(out, out_bytes, query, q_bytes)) || meet(out, out_bytes, paged_kv_cache, cache_bytes) ||
-      meet(lse, lse_bytes, query, q_bytes) || meet(lse, lse_bytes, paged_kv_cache, cache_bytes) ||
-      meet(lse, lse_bytes, out, out_bytes) || meet(workspace, plan->workspace_bytes, query, q_bytes) ||
-      meet(workspace, plan->workspace_bytes, paged_kv_cache, cache_bytes) || meet(workspace, plan->workspace_bytes, out, out_bytes) ||
-      meet(workspace, plan->workspace_bytes, lse, lse_bytes) || meet(workspace, plan->workspace_bytes, plan->buffer, plan->plan_bytes))
-    return fail(KVC_ERR_INVALID_ARG, "%s: what is written overlaps what is read (the output may be the query itself)", fn);
+  const Memory written[] = {{out, plan->num_tokens * q_row}, {lse, plan->num_tokens * plan->num_heads * 4}, {workspace, plan->workspace_bytes}};
+  const Memory read[] = {{query, (plan->num_tokens - 1) * q_token_stride * 2 + q_row},
+                         {paged_kv_cache, num_pages > 0 ? (num_pages - 1) * page_stride * 2 + page * 2 : 0},
+                         {plan->buffer, plan->plan_bytes},
+                         {plan->kv_indices, plan->num_kv_indices * 4}};
+  bool apart = true;
+  for (const Memory& w : written) {
+    for (const Memory& r : read) apart = apart && (!w.meets(r) || (&w == written && &r == read && in_place));
+    for (const Memory* x = written; x < &w; ++x) apart = apart && !w.meets(*x);
+  }
+  if (!apart) return fail(KVC_ERR_INVALID_ARG, "%s: what is written overlaps what is read (the output may be the query itself)", fn);
   AttendArgs a{};
   a.query = (const char*)query;
   a.cache = (const char*)paged_kv_cache;

@@ -436,6 +436,23 @@ int run_norm(const char* fn, const void* query, const void* key, const void* val
       }
     if (c->batch_indices && (c->batch_size == 0 || c->num_kv_indices == 0)) a.key_cache = nullptr;  // every token is skipped
   }
+  // nor may what is written, rows and cache planes, share memory with the arrays beside the rows
+  const auto span = [&](const Rows& r) { return r.p ? (__int128)(tokens - 1) * r.stride + r.row : (__int128)0; };
+  const __int128 plane = c && c->num_cache_blocks > 0
+                             ? (__int128)(c->num_cache_blocks - 1) * a.cache_block_stride + (__int128)(c->block_size - 1) * a.cache_slot_stride + k_row * E
+                             : (__int128)0;
+  struct Memory {
+    const void* p;
+    __int128 bytes;
+  };
+  const Memory written[] = {{a.query_out, span(out_q)}, {a.key_out, span(out_k)}, {c ? c->key_cache : nullptr, plane}, {c ? c->value_cache : nullptr, plane}};
+  const Memory arrays[] = {{q_weight, head_dim * E}, {k_weight, head_dim * E}, {positions, tokens * pos_bytes},
+                           {cos_sin_cache, (__int128)max_position * 2 * rotary_dim * E},
+                           {c ? c->slot_mapping : nullptr, c ? tokens * c->slot_bytes : 0}, {c ? c->batch_indices : nullptr, tokens * 4},
+                           {c ? c->kv_indices : nullptr, c ? (__int128)c->num_kv_indices * 4 : 0}, {c ? c->kv_indptr : nullptr, c ? (__int128)(c->batch_size + 1) * 4 : 0}};
+  for (const Memory& w : written)
+    for (const Memory& r : arrays)
+      if (w.p && r.p && (uintptr_t)w.p < (uintptr_t)r.p + r.bytes && (uintptr_t)r.p < (uintptr_t)w.p + w.bytes) apart = false;
   if (!apart)
     return fail(KVC_ERR_INVALID_ARG, "%s: an output overlaps an input or another output (only a whole output on its own input's rows may)", fn);
   const int n = 16 / E;

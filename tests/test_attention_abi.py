@@ -129,3 +129,43 @@ def test_common_prefix_pages():
     assert f([[5, 2], [4, 2]]) == 0
     assert f(t for t in ([7] * 4, [7] * 6)) == 4
     assert f([np.arange(1000, dtype=np.int32), list(range(999)) + [5, 6]]) == 999
+
+
+def test_what_is_written_may_not_be_what_is_read():
+    """The arrays beside the rows, against everything that is written: index arrays and the attention plan's buffer; the norm's
+    weights, tables and indices and its outputs and cache planes. (A run of the attention needs a plan that was built.)"""
+    L = _lib.lib()
+    h = ctypes.c_void_p()
+    assert create(h) == OK
+    need = L.kvc_attention_plan_bytes(h)
+    for at in (4096, 8192, 12288, 16384):        # the index arrays that `create` gives
+        at = at // 256 * 256
+        assert L.kvc_attention_plan_build(h, at, need, None) == INVALID and "overlaps" in _lib.last_error()
+    L.kvc_attention_plan_destroy(h)
+    page = 2 * 16 * 2 * 64 * 2
+    good = dict(q=1 << 20, k=2 << 20, v=3 << 20, qw=4 << 20, kw=5 << 20, eps=1e-6, pos=6 << 20, pb=4, cs=7 << 20, maxp=100, tokens=4,
+                hq=8, hk=2, d=64, rd=64, qs=512, ks=128, vs=128, qo=8 << 20, ko=9 << 20, qos=512, kos=128, kc=16 << 20,
+                vc=(16 << 20) + page // 2, slots=10 << 20, sb=8, bs=16, bstride=page // 2, sstride=128, nb=8, dtype=BF16)
+
+    def run(**kw):
+        a = dict(good)
+        a.update(kw)
+        return L.kvc_qk_norm_rotary_pos_emb_and_cache(*a.values(), None)
+
+    ends = dict(qw=128, kw=128, pos=16, cs=100 * 2 * 64 * 2, slots=32)      # bytes of the arrays
+    outs = dict(qo=4 * 512 * 2, ko=4 * 128 * 2, kc=8 * page, vc=8 * page - page // 2)
+    for array, n in ends.items():
+        for out in outs:
+            at = good[out] if out != "vc" else good["kc"] + page // 2
+            for where in (at, at + 16, at - n + 16):
+                if out == "vc" and where < good["vc"]:
+                    continue
+                assert run(**{array: where}) == INVALID and "overlaps" in _lib.last_error(), (array, out, where - at)
+    paged = dict(q=1 << 20, k=2 << 20, v=3 << 20, qw=4 << 20, kw=5 << 20, eps=1e-6, batch=6 << 20, pos=7 << 20, cs=8 << 20, maxp=100,
+                 nnz=4, hq=8, hk=2, d=64, rd=64, qs=512, ks=128, vs=128, qo=9 << 20, ko=10 << 20, qos=512, kos=128, cache=16 << 20,
+                 idx=11 << 20, ptr=12 << 20, b=3, n=9, page=16, stride=page // 2, pages=8, dtype=BF16)
+    for array in ("qw", "kw", "batch", "pos", "cs", "idx", "ptr"):
+        for out in ("qo", "ko", "cache"):
+            a = dict(paged)
+            a[array] = paged[out] + 16
+            assert L.kvc_qk_norm_rotary_pos_emb_and_append_paged(*a.values(), None) == INVALID and "overlaps" in _lib.last_error(), (array, out)
