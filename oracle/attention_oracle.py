@@ -50,12 +50,13 @@ def attention_tolerances(out, lse, weighted, values, products, D, scale, dtype_e
 
     A score is D products summed in 32 bits: off by at most (D + 2) 2^-24 sum|q||k|, times the scale, and by 2^-22 of the
     exponent's own size for scale, maximum and difference; a weight by that (relative) and by half a step of the storage type
-    (dtype_eps / 2, or half the smallest denormal); sums of weights and of weighted values by 2^-24 a term in the
-    chains of up to 600 terms the sizes here make; the output is rounded once more."""
+    (dtype_eps / 2; or half the smallest denormal of f16, of weights that are scaled up by 2^7 and more against a base that stands up to
+    1 above the largest score: 2^-6 of that, as a part of the largest weight); sums of weights and of weighted values by 2^-24 a
+    term in the chains of up to 600 terms the sizes here make; the output is rounded once more."""
     ds = scale * products * (D + 2) * 2.0 ** -24 + (1 + scale * products) * 2.0 ** -22
     chain = 600 * 2.0 ** -24
     rel = 2 * ds + 2 * chain
-    tol = weighted * (dtype_eps / 2 + rel[..., None]) * 1.05 + np.abs(out) * dtype_eps / 2 * 1.05 + values * denormal + denormal
+    tol = weighted * (dtype_eps / 2 + rel[..., None]) * 1.05 + np.abs(out) * dtype_eps / 2 * 1.05 + values * denormal * 2.0 ** -6 + denormal
     return tol, ds + chain + np.abs(np.where(np.isfinite(lse), lse, 0)) * 2.0 ** -22 + 2.0 ** -22
 
 
