@@ -35,7 +35,7 @@ class PagedAttentionPlan:
     sm_scale: of the scores, `head_dim ** -0.5` when None.
     max_q_len: the most tokens a request has, if known: of help to the choice of kernels, not a limit.
 
-    The step's work is laid out on the device at construction, by two small launches on the current
+    The step's work is laid out on the device at construction, by a small launch (two with shared pages) on the current
     stream; `build()` does it again after the index buffers were written for another step, and can
     be recorded with the runs into a hipGraph (keep the plan while that is replayed). Runs must be ordered after it. The
     plan keeps references to the index tensors; a step whose `qo_indptr` or `kv_indptr` decreases is not computed. Every run takes a workspace of its own from torch's allocator, so runs on
@@ -86,7 +86,7 @@ class PagedAttentionPlan:
             self._destroy(plan)
 
     def build(self) -> None:
-        """Lay out the step that the index buffers hold (two small launches on the current stream)."""
+        """Lay out the step that the index buffers hold (a small launch on the current stream, two with shared pages)."""
         with _on_device_of(self._buffer):
             if _stream_of(self._buffer) != self._stream:
                 self._buffer.record_stream(torch.cuda.current_stream())

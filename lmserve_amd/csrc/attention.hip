@@ -7,7 +7,7 @@
 // Ranges of keys that different workgroups took are joined by their lse = m + log l: o = sum_c exp(lse_c - lse) o_c.
 // Exponentials are taken to base 2, with scale * log2(e) in the exponent's multiply-add.
 //
-// A step's work is laid out on the device, from the index tensors (two small launches, once per step): items of
+// A step's work is laid out on the device, from the index tensors (a small launch, two with a shared prefix, once per step): items of
 // (row tile, key range) of about equal length, as many as fill the card, however the lengths are spread. The leading
 // pages that the requests of a batch share are items of their own, whose rows are those of ALL these requests.
 
@@ -51,8 +51,9 @@ __device__ constexpr int kTileWork = 64, kMinShare = 1024, kMinSharedShare = 256
 __device__ constexpr int kMinChunk = 512, kWideTileWork = 128, kWidePartWork = 384;
 constexpr int32_t kMaxKeys = INT32_MAX - 8192;  // of a request: a key that is looked up ahead stays below 2^31
 // The rows of all sharing requests are wide tiles where they are more than kNarrowSharedRows, or more than a narrow tile and
-// rows times keys above kNarrowWork: 96 rows over 4096 keys 26.8 us wide and 33.6 narrow, 128 rows 28.6 and 40.7, 64 rows
-// 26 either way; 91 rows over 2000 keys 24.7 and 20.8, 104 over 1024 18.1 and 15.7.
+// rows times keys above kNarrowWork. 8 key heads of 128, wide and narrow: 96 rows over 4096 keys 27.3 and 33.9 us, 128 rows 28.5 and
+// 40.8, 64 rows 25.7 and 26.6; 96 over 1024 23.2 and 21.2, 24 over 2000 23.1 and 16.7. (With fewer key heads the narrow tiles have
+// more of the card to themselves, which the rule does not look at: one key head, 128 rows over 4096 keys 25.2 and 18.1.)
 __host__ __device__ constexpr bool wide_prefix(int64_t rows, int64_t keys) {
   constexpr int64_t kNarrowSharedRows = 128, kNarrowWork = 1 << 18;
   return rows > kNarrowSharedRows || (rows > kTile && rows * keys > kNarrowWork);
@@ -895,8 +896,8 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
 // The maximum that the weights are taken against grows only when a row's has outgrown it by 2^8: until then the larger weights
 // (below 2^8) and sums say the same, and the rescaling of O, 64 registers at 128 columns, is left out of nearly every step.
 // Bound by the instructions that two wavefronts a SIMD can have under way: the matrix unit is busy for 41 % of the cycles
-// (2048 new tokens behind 13 to 30 thousand keys, 7 query heads to a key head of 128: 740 to 830 us as the clock is, up to 965
-// TFLOP/s).
+// (2048 new tokens behind 13 to 30 thousand keys, 7 query heads to a key head of 128: 781 us at least and 822 in the median of 30
+// launches, 865 to 910 TFLOP/s).
 template <int DP>
 constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16 + DP * 2 + kVPad) + (kWaves + 1) * 4; }
 
@@ -1398,8 +1399,8 @@ constexpr int64_t kResidents = 512;           // wide items on the card at a tim
 constexpr int64_t kMaxRounds = 4;             // of them in a step, where a range of keys is longer than the least
 // The most rows of a request for narrow tiles, with more it is cut into wide ones: one narrow tile where there is work to
 // fill the card, that is, where all rows together, over the requests' average of keys, make more than kMuchWork, else two. 32 rows
-// each: 64 requests of 2000 keys 125 us wide and 132 in two narrow tiles, 256 of 600 172 and 221, one of 16000 32 and 40, of
-// 131000 131 and 190; one of 2000 24.8 and 23.0, four of 20 rows and 900 keys 23.1 and 17.5. (48 rows, 64 requests: 127 and 258.)
+// each over 8 key heads: 64 requests of 2000 keys 125 us wide and 133 in two narrow tiles, 256 of 600 169 and 220, one of 16000 31 and 40,
+// of 131000 130 and 189; one of 2000 24.8 and 23.0, four of 20 rows and 900 keys 23.1 and 17.3. (One key head, one of 131000: 44 and 29.)
 constexpr int64_t kNarrowRows = 32, kMuchWork = 1 << 18;
 
 Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {

@@ -179,7 +179,7 @@ class KVWriteStep:
     # ------------------------------------------------------------------ launches
     def build_index(self) -> None:
         """One launch on the current stream: every index tensor of the step that
-        the buffers hold, written in place. With attention two more lay out its work."""
+        the buffers hold, written in place. With attention one more lays out its work (two with shared pages)."""
         build_write_index(self.input_lens, self.context_lens, self.num_blocks, self.kv_indices,
                           self.page_size, self.max_tokens, out=self._out)
         if self.attention_plan is not None:
