@@ -589,8 +589,8 @@ int kvc_rotary_plan_run_norm(const kvc_rotary_plan* plan, const void* query, con
  * -inf. A page outside [0, num_pages) has no keys; nor has a request more than
  * 2^31 - 8193. What lies behind a request's
  * last key, or is masked, does not reach the result, infinities and NaN included. An
- * infinite value that a row does see makes that column infinite, or NaN where its weight is too
- * small for fp32 (which of the two may depend on the other rows of the step).
+ * infinite value that a row does see makes that column infinite, however small its weight is (NaN
+ * with both signs, or a NaN among the values).
  * qo_indptr and kv_indptr do not decrease; where one does, the step is not computed and no row written.
  * Rows behind qo_indptr[batch_size] are left as they were. Sums and softmax
  * statistics are fp32, the output is rounded once. Requests of more than 32

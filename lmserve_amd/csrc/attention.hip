@@ -562,6 +562,10 @@ __device__ __forceinline__ float max_across16(float x) {
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+__device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) <= 3.402823466e38f; }
+// The least weight of a part: however far below the others it is, what is infinite in it stays
+constexpr float kLeastWeight = 1.401298464e-45f;
+
 // How an item's keys are reached
 enum Reach : int {
   kAnyPage,   // pages of any size: a lane looks up every key it loads
@@ -823,12 +827,34 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
         present = coming;
       }
     }
-    // infinities and NaN of V that were left out, where rows stop, go to the rows that see their keys. (A weight is taken for
-    // 1: what it scales is infinite. The opaque zero keeps the compiler from working on this ahead.)
-    if (tile.odd_from < item.key_end) {
+    // the sum over the four quads' keys
+    float l = tile.l;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    // Infinities and NaN of V: those that were left out, where rows stop, and where a product with one of them is in O (that may
+    // be NaN, from a weight's second part or a weight of 0), go to the rows that see their keys with a weight of 1: what it scales
+    // is infinite. (The opaque zero keeps the compiler from working on this ahead.)
+    f32x4 probe = {};
+#pragma unroll
+    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) probe[e] = __builtin_fmaf(tile.o[d][e], 0.f, probe[e]);
+    const bool mine = !finite((probe[0] + probe[1]) + (probe[2] + probe[3])) && finite(l);
+    const bool some = __ballot(mine) != 0;
+    if (__builtin_expect(some || tile.odd_from < item.key_end, 0)) {
       int32_t zero = 0;
       asm volatile("" : "+v"(zero));
-      for (int32_t b0 = tile.odd_from; b0 < item.key_end; b0 += STEP)
+      uint32_t odd[(DTILES + 7) / 8] = {};
+      if (mine)
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!finite(tile.o[d][e])) {
+              odd[d / 8] |= 1u << (d % 8 * 4 + e);
+              tile.o[d][e] = 0;
+            }
+      for (int32_t b0 = some ? item.key_begin + wave * kBlock : tile.odd_from; b0 < item.key_end; b0 += STEP)
 #pragma unroll 1
         for (int32_t key = b0; key < min(b0 + kBlock, item.key_end); ++key) {
           const int64_t off = key_offset(a, item.table, key, item.key_end);
@@ -838,11 +864,15 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
           for (int d = 0; d < DTILES; ++d)
             if (d * 16 + quad * 4 < D) tile.o[d] += infinite_part<T>(*reinterpret_cast<const u32x2*>(row + d * 32));
         }
+#pragma unroll
+      for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((odd[d / 8] >> (d % 8 * 4 + e) & 1) && tile.o[d][e] == 0) tile.o[d][e] = NAN;  // (no value was: a sum left fp32)
+          if (l == 0) tile.o[d][e] = 0;
+        }
     }
-    // the sum over the four quads' keys, then over the wavefronts
-    float l = tile.l;
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    // over the wavefronts
     if (quad == 0) {
       stats[wave][0][n] = tile.base;
       stats[wave][1][n] = l;
@@ -854,7 +884,8 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
     const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) all_l += stats[w][1][n] * exp2_of(stats[w][0][n] - base);
-    const float part = exp2_of(tile.base - base) * (all_l == 0 ? 0.f : 1.f / all_l);
+    const float weight = exp2_of(tile.base - base) * (all_l == 0 ? 0.f : 1.f / all_l);
+    const float part = weight < kLeastWeight ? kLeastWeight : weight;  // (NaN stays)
     float* my_o = reinterpret_cast<float*>(my_v);
 #pragma unroll
     for (int d = 0; d < DTILES; ++d)
@@ -1191,10 +1222,29 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
       }
     }
     __syncthreads();  // (left_out is complete, and the buffers are free)
-    if (left_out) {  // as above
+    l += __shfl_xor(l, 32);
+    f32x4 probe = {};
+#pragma unroll
+    for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) probe[r % 4] = __builtin_fmaf(o[d][r], 0.f, probe[r % 4]);
+    const bool mine = !finite((probe[0] + probe[1]) + (probe[2] + probe[3])) && finite(l);
+    const bool some = __ballot(mine) != 0;
+    if (__builtin_expect(some || left_out, 0)) {  // as above
       int32_t zero = 0;
       asm volatile("" : "+v"(zero));
-      const int32_t from = item.key_begin + max((max(tile_least - item.key_begin, 0) + kStep / 2) / kStep * kStep - kStep / 2, 0);
+      uint32_t odd[(DTILES + 1) / 2] = {};
+      if (mine)
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!finite(o[d][r])) {
+              odd[d / 2] |= 1u << (d % 2 * 16 + r);
+              o[d][r] = 0;
+            }
+      const int32_t from = some ? item.key_begin
+                                : item.key_begin + max((max(tile_least - item.key_begin, 0) + kStep / 2) / kStep * kStep - kStep / 2, 0);
 #pragma unroll 1
       for (int32_t key = from; key < item.key_end; ++key) {
         const int64_t off = key_offset(a, item.table, key, item.key_end);
@@ -1210,8 +1260,14 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
               for (int e = 0; e < 4; ++e) o[d][i * 4 + e] += x[e];
             }
       }
+#pragma unroll
+      for (int d = 0; d < DTILES; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if ((odd[d / 2] >> (d % 2 * 16 + r) & 1) && o[d][r] == 0) o[d][r] = NAN;
+          if (l == 0) o[d][r] = 0;
+        }
     }
-    l += __shfl_xor(l, 32);
     const float inv = l == 0 ? 0.f : 1.f / l, lse2 = l == 0 ? -INFINITY : base + kScaledUp + __log2f(l * kUnscaled);
     if (my_row < item.rows) {
       if (item.slot >= 0) {
@@ -1339,7 +1395,7 @@ __global__ __launch_bounds__(kThreads, 6) void attend_join_kernel(AttendArgs a) 
         f32x4 x = {};
 #pragma unroll 4
         for (int32_t c = from; c < parts; c += step)
-          x += *reinterpret_cast<const f32x4*>((c < own ? own_o : shared_o) + row_of(c) * D + d) * exp2_of(lse_of(c) - base);
+          x += *reinterpret_cast<const f32x4*>((c < own ? own_o : shared_o) + row_of(c) * D + d) * fmaxf(exp2_of(lse_of(c) - base), kLeastWeight);
         return x;
       };
       if (!many) {
