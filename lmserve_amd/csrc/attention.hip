@@ -282,13 +282,13 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
   // ends before all its work is done, the narrow tiles' (a key of which takes about 4/5 of the time) among it; where that is the
   // larger part, ranges may last as long, at two thirds of the time that they take beside their like: behind a shared
   // prompt of 4096 keys and 256 requests' own of 1 to 512, ranges of 512 keys 119 us, of 1024 113, of 2048 107.
-  int32_t chunk = 1 << 30;
+  int32_t chunk = kMaxKeys;
   const int64_t all_wide = (int64_t)wide_work + (shared_wide ? (int64_t)shared_tiles * shared_len : 0);
   if (all_wide) {
     const int32_t most = max(longest, shared_wide ? shared_len : 0), listed = min(a.batch_size, 1024);
     const auto chunk_of = [&](int32_t x) {
       const double keys = __builtin_ceil((double)all_wide * 16 / ((double)a.residents * (x + 1)));
-      return round_up((int32_t)(keys < kMinChunk ? kMinChunk : keys < (1 << 30) ? keys : 1 << 30), kStep);
+      return round_up((int32_t)(keys < kMinChunk ? kMinChunk : keys < kMaxKeys ? keys : kMaxKeys), kStep);
     };
     for (int32_t x = wave; x < 64; x += 16) {
       const int32_t keys = chunk_of(x);
@@ -1421,7 +1421,7 @@ struct Memory {  // of an argument (which may be null)
   const void* p;
   int64_t bytes;
   bool meets(const Memory& o) const {
-    return p && o.p && (uintptr_t)p < (uintptr_t)o.p + (uint64_t)o.bytes && (uintptr_t)o.p < (uintptr_t)p + (uint64_t)bytes;
+    return p && o.p && bytes > 0 && o.bytes > 0 && (uintptr_t)p < (uintptr_t)o.p + (uint64_t)o.bytes && (uintptr_t)o.p < (uintptr_t)p + (uint64_t)bytes;
   }
 };
 

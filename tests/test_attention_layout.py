@@ -200,3 +200,17 @@ def test_slots_of_narrow_tiles_are_there():
         last = max((group for group, count in parts if count > 1), default=-1)
         have = workspace(lens, hk * group, hk, d, page, max_q) // (16 * hk * (d + 1) * 4)
         assert 2 * (last + 1) <= have, (lens, hk, group)
+
+
+def test_slots_of_the_longest_requests_are_there():
+    """Requests of nearly 2^31 keys under so many rows that an even share of the work is a longer range than any request has: none is cut."""
+    longest = (1 << 31) - 1 - 8192
+    for hk, group, n, requests in ((1, 1, 1 << 20, 1), (8, 1, 1 << 20, 2), (1, 8, 1 << 22, 3)):
+        lens = [(n, longest)] * requests
+        residents = max(1, 512 // hk)
+        work = sum(ceil(n * group, 128) * k for n, k in lens)
+        assert ceil(work * 16, residents * 64) > longest
+        have = workspace(lens, hk * group, hk, 64, 1024)
+        for x in range(64):
+            chunk = ceil(min(max(512, ceil(work * 16, residents * (x + 1))), longest), 64) * 64
+            assert slots_of_wide_tiles(lens, group, residents, 32, chunk) * 128 * hk * 65 * 4 <= have, (lens, x)
