@@ -51,6 +51,10 @@ class PagedAttentionPlan:
         self._plan = None
         self.qo_indptr, self.kv_indices = _i32(qo_indptr, "qo_indptr"), _i32(kv_indices, "kv_indices")
         self.kv_indptr, self.kv_last_page_len = _i32(kv_indptr, "kv_indptr"), _i32(kv_last_page_len, "kv_last_page_len")
+        # index tensors that are no dense arrays: the launches read copies, which `build` makes anew
+        self._copies = [(copy, given) for copy, given in ((self.qo_indptr, qo_indptr), (self.kv_indices, kv_indices),
+                                                          (self.kv_indptr, kv_indptr), (self.kv_last_page_len, kv_last_page_len))
+                        if copy is not given]
         batch = self.kv_last_page_len.numel()
         if self.kv_indptr.numel() != batch + 1 or self.qo_indptr.numel() != batch + 1:
             raise ValueError("qo_indptr and kv_indptr must have batch_size + 1 entries")
@@ -88,10 +92,18 @@ class PagedAttentionPlan:
     def build(self) -> None:
         """Lay out the step that the index buffers hold (a small launch on the current stream, two with shared pages)."""
         with _on_device_of(self._buffer):
-            if _stream_of(self._buffer) != self._stream:
-                self._buffer.record_stream(torch.cuda.current_stream())
+            self._used_here()
+            for copy, given in self._copies:
+                copy.copy_(given)
             _lib.check(_lib.lib().kvc_attention_plan_build(self._plan, self._buffer.data_ptr(), self._buffer.numel(),
                                                            _stream_of(self._buffer)))
+
+    def _used_here(self) -> None:
+        """What the plan owns stays allocated until the current stream's launches are done with it."""
+        if _stream_of(self._buffer) != self._stream:
+            stream = torch.cuda.current_stream()
+            for owned in (self._buffer, *(copy for copy, _ in self._copies)):
+                owned.record_stream(stream)
 
     def run(self, query: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, lse: Optional[torch.Tensor] = None):
@@ -147,8 +159,7 @@ class PagedAttentionPlan:
         if T:
             with _on_device_of(q2):
                 stream = _stream_of(q2)
-                if stream != self._stream:
-                    self._buffer.record_stream(torch.cuda.current_stream())
+                self._used_here()
                 workspace = torch.empty(self._workspace_bytes, dtype=torch.uint8, device=self.device)
                 _lib.check(_lib.lib().kvc_attention_plan_run(
                     self._plan, q2.data_ptr(), q2.stride(0) if T > 1 else row, paged_kv_cache.data_ptr(),
