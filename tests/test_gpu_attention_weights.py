@@ -75,3 +75,32 @@ def test_few_rows_round_their_outputs_only(gpu, lengths, heads, kv_heads, D, pag
     rms = lambda x: x.square().mean().sqrt().item()
     rounded = rms(want.to(s.dtype).double() - want)
     assert rms(out.cpu().double().reshape(want.shape) - want) <= 1.01 * rounded
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lengths", [[(1, 900), (2, 40)], [(40, 700), (1, 33)]])
+def test_scores_of_millions(gpu, lengths, dtype):
+    """Scores up to 2^23 times log2(e), hundreds of thousands apart: a row is the value v of its highest key. In narrow tiles the
+    weight w goes in as w1 + w2 with |w1 + w2 - w| <= (eps / 2)^2 w, so that o = v (w1 + w2) / w is nearer to v than the quarter step
+    from which a value of the type would round to another: the same bits. In wide ones only w1 with |w1 - w| <= eps / 2 w does: o is
+    off by eps / 2 |v|, and its rounding by eps / 2 |o|: eps (1 + eps / 4) |v| together."""
+    s = Step(lengths, 8, 2, 128, 16, dtype, seed=32, scale_q=4096.0)
+    s.cache[:, 0] *= 512
+    out, lse = s.plan(gpu).run(s.query.to(gpu), s.cache.to(gpu), return_lse=True)
+    out, lse = out.cpu(), lse.cpu().double()
+    for b, (n, k) in enumerate(lengths):
+        pages = torch.from_numpy(s.indices[s.indptr[b]:s.indptr[b + 1]].astype(np.int64))
+        keys, values = (s.cache[pages, i].reshape(-1, 2, 128)[:k] for i in (0, 1))
+        for j in range(n):
+            t = int(s.qo[b]) + j
+            for x in range(8):
+                score = keys[:k - n + j + 1, x // 4].double() @ s.query[t, x].double() * s.scale
+                top = score.topk(min(2, len(score)))
+                if len(score) > 1 and top.values[0] - top.values[1] < 200 + 2.0 ** -16 * top.values.abs().max():
+                    continue      # (too close to tell in 32 bits)
+                v = values[top.indices[0], x // 4]
+                if n * 4 > 32:
+                    assert ((out[t, x].double() - v.double()).abs() <= s.eps * 1.01 * v.double().abs() + s.denormal).all()
+                else:
+                    assert torch.equal(out[t, x], v)
+                assert abs(lse[t, x] - top.values[0]) <= 2.0 ** -16 * top.values[0].abs() + 1
