@@ -668,10 +668,10 @@ struct Block {
 //   S^T = K Q^T: the keys' rows are the matrix instruction's A operand as they lie in memory, 16 bytes a lane.
 //   O^T = V^T P^T: a lane's 8 probabilities, of keys 4q..4q+3 and 16+4q..16+4q+3 (q = lane / 16), are the B operand as S^T
 //   left them; the A operand wants the same keys of one column of V, which the transposing LDS read gives.
-// The matrix instruction takes 16 bits: a weight goes in as two numbers of the storage type, itself rounded and the rest rounded, off
-// by a half step's square. The second product is on a unit that waits for keys: decode of 256 requests 405.4 us with one
-// product and 405.7 with both, one request 17.5 and 17.9, the error against 64 bits 2.02e-3 and 1.65e-3 of the outputs' size, which is
-// their own rounding. (f16: from 2^-28 of the largest weight on; smaller ones are off by at most 2^-39 of it.)
+// The matrix instruction takes 16 bits: a weight goes in as two numbers of the storage type, itself rounded and the rest
+// rounded, off by a half step's square. The second product is on a unit that waits for keys: decode of 256 requests 405.4 us with
+// one product and 405.7 with both, one request 17.5 and 17.9, the error against 64 bits 2.02e-3 and 1.65e-3 of the outputs' size,
+// which is their own rounding. (f16: from 2^-28 of the largest weight on; smaller ones are off by at most 2^-39 of it.)
 template <typename T, int DP>
 struct RowTile {
   static constexpr int KSTEPS = DP / 32, DTILES = DP / 16;
@@ -927,8 +927,8 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
 // The maximum that the weights are taken against grows only when a row's has outgrown it by 2^8: until then the larger weights
 // (below 2^8) and sums say the same, and the rescaling of O, 64 registers at 128 columns, is left out of nearly every step.
 // Bound by the instructions that two wavefronts a SIMD can have under way: the matrix unit is busy for 41 % of the cycles
-// (2048 new tokens behind 13 to 30 thousand keys, 7 query heads to a key head of 128: 781 us at least and 822 in the median of 30
-// launches, 865 to 910 TFLOP/s).
+// (2048 new tokens behind 13 to 30 thousand keys, 7 query heads to a key head of 128: 780 us at least and 825 in the median of 30
+// launches, 860 to 910 TFLOP/s).
 template <int DP>
 constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16 + DP * 2 + kVPad) + (kWaves + 1) * 4; }
 
@@ -1478,14 +1478,14 @@ Layout layout_of(const kvc_attention_plan& p, char* buffer, int64_t* bytes) {
   return l;
 }
 
-// What a step of these capacities can need. Requests with tokens are at most `requests`; those of more than `narrow_rows` rows are
-// wide, the others narrow, and only narrow ones share a prefix. Tiles of a kind are at most their rows / tile and one more a
-// request. A narrow tile's part in a workgroup has place tile + workgroup in the list; two parts of a workgroup that the line reaches need slots, and,
-// where a prefix is shared, every tile's first part. Wide tiles cut into ranges of at least the rounds' share of all keys make at most
-// the rounds' items and one more a tile. Slots are for those of two ranges or more: they have no more tiles than rounds'
-// items, and no more ranges than the tables' keys hold of the least length (heads of 128: 20 tokens of 4 x 8 heads over 900 keys 1.5 MB
-// of workspace, 256 tokens of 256 requests 8, or 188 where any request may have them all, 2048 tokens of 7 x 4 heads behind long
-// contexts 175).
+// What a step of these capacities can need. Requests with tokens are at most `requests`; those of more than `narrow_rows` rows
+// are wide, the others narrow, and only narrow ones share a prefix. Tiles of a kind are at most their rows / tile and one more
+// a request. A narrow tile's part in a workgroup has place tile + workgroup in the list; two parts of a workgroup that the line
+// reaches need slots, and, where a prefix is shared, every tile's first part. Wide tiles cut into ranges of at least the rounds'
+// share of all keys make at most the rounds' items and one more a tile. Slots are for those of two ranges or more: they have no
+// more tiles than rounds' items, and no more ranges than the tables' keys hold of the least length. (Heads of 128: 20 tokens of
+// 4 x 8 heads over 900 keys 1.5 MB of workspace, 256 tokens of 256 requests 8, or 188 where any request may have them all, 2048
+// tokens of 7 x 4 heads behind long contexts 175.)
 Sizes sizes_of(const kvc_attention_plan& p) {
   Sizes n;
   const int64_t rows = p.num_tokens * (p.num_heads / p.num_kv_heads), keys = p.num_kv_indices * p.page_size;
