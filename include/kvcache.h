@@ -640,6 +640,69 @@ int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query,
                            void* workspace, int64_t workspace_bytes, void* stream);
 int kvc_attention_plan_destroy(kvc_attention_plan* plan);
 
+/* ---------------------------------------------------------------------------
+ * The cache in 8 bits: half the bytes of K and V, quantised as they are written.
+ * Stands beside the 16-bit write of the same call site
+ *   (runtime/worker/llm_worker/models/layers/attention.py:76-85).
+ * A page of one layer is kvc_q8_page_bytes(H, D, page_size) bytes, page_size / 16
+ * groups of 16 tokens one after another. A group holds codes (OCP e4m3) and
+ * exponents, padded to whole 128 bytes:
+ *   K [H][token / 4][D / 16][token % 4][D % 16], V [H][D][token],
+ *   exponents [H][K, V], one byte each, plus 127.
+ * value = code * 2^exponent, the exponent shared by a group's 16 tokens, for every
+ * head and for K and V by itself. It is the least one from -100 to 120 with which
+ * the largest finite magnitude that was written into the group is at most 448 (-100 where all are 0); a code
+ * is the value times 2^-exponent, rounded once, ties to even. An infinity or NaN becomes
+ * NaN and has no part in the exponent.
+ *
+ * Writes are those of kvc_reshape_and_cache and kvc_append_paged_kv_cache: the same
+ * slots, index arrays and tokens that are skipped. The tokens of a request come in the order of their
+ * positions, as the index build gives them: those of a group lie one behind another in a call's arrays, and
+ * calls go from its first place up. A call that begins at a group's first place
+ * begins it anew. One that goes on with it leaves the exponent where it is enough;
+ * where it is not, the codes before the new ones are rounded to the greater one. Places
+ * behind the last token written are left as they were. (Tokens of one group in another
+ * order, or twice, leave that group's contents undefined, and no other's.)
+ *
+ * Reads are the way back: the rows of the tokens, in any order, rounded once to
+ * bf16 or f16. Rows of tokens that are skipped are left as they were.
+ *
+ * key, value: bf16 or f16 rows of H * D, strides in elements, rows and pages
+ * aligned to 16 bytes; page_stride in BYTES. head_dim a multiple of 16 up to 256, page_size a
+ * multiple of 16. What is written may not overlap what is read. Whole blocks are moved
+ * as bytes by kvc_copy_blocks, the swaps and the disk tier: their exponents go with them.
+ * ------------------------------------------------------------------------- */
+int64_t kvc_q8_page_bytes(int64_t num_kv_heads, int64_t head_dim, int64_t page_size);
+
+int kvc_reshape_and_cache_q8(const void* key, const void* value, void* kv_cache,
+                             const void* slot_mapping, int slot_bytes, int64_t num_tokens,
+                             int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                             int64_t key_token_stride, int64_t value_token_stride,
+                             int64_t page_stride, int64_t num_pages, int dtype, void* stream);
+
+int kvc_append_paged_kv_cache_q8(const void* append_key, const void* append_value,
+                                 const int32_t* batch_indices, const int32_t* positions,
+                                 void* paged_kv_cache, const int32_t* kv_indices,
+                                 const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                                 int64_t nnz, int64_t batch_size, int64_t num_kv_indices,
+                                 int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                 int64_t key_token_stride, int64_t value_token_stride,
+                                 int64_t page_stride, int64_t num_pages, int dtype, void* stream);
+
+int kvc_read_cache_q8(const void* kv_cache, const void* slot_mapping, int slot_bytes, void* key,
+                      void* value, int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
+                      int64_t page_size, int64_t key_token_stride, int64_t value_token_stride,
+                      int64_t page_stride, int64_t num_pages, int dtype, void* stream);
+
+int kvc_read_paged_kv_cache_q8(const int32_t* batch_indices, const int32_t* positions,
+                               const void* paged_kv_cache, const int32_t* kv_indices,
+                               const int32_t* kv_indptr, const int32_t* kv_last_page_len, void* key,
+                               void* value, int64_t nnz, int64_t batch_size,
+                               int64_t num_kv_indices, int64_t num_kv_heads, int64_t head_dim,
+                               int64_t page_size, int64_t key_token_stride,
+                               int64_t value_token_stride, int64_t page_stride, int64_t num_pages,
+                               int dtype, void* stream);
+
 /* The on-device half of a swap on its own: gather scattered pool blocks into a
  * dense device buffer laid out like the host pool, [n, layer_end-layer_begin,
  * block_bytes], or scatter such a buffer back:

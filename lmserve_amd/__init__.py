@@ -3,6 +3,7 @@
     cache_ops   copy_blocks, fill_key_cache, reshape_and_cache(_layers), gather/scatter_blocks,
                 swap_out / swap_in (functional form of the GPU <-> host swap)
     paged       append_paged_kv_cache(_layers), get_seq_lens, get_batch_indices_positions
+    quantized   the cache in 8 bits: quantised as it is written, read back, its layout
     kv_worker   KVWorker (GPU <-> pinned host swap), Device, BlockMapping
     index_prep  host-side block-table / slot-mapping construction
     attention   causal attention over the paged cache, a shared prefix read once for the batch
@@ -32,6 +33,8 @@ from .kv_pool import (CachePlan, KVWorkerHandle, KVWorkerParams, LayerSyncHooks,
 from .kv_service import serve_kv_worker
 from .kv_worker import (BlockMapping, BlockMappingEntry, Device, KVWorker, PinnedHostPool,
                         flatten_block_mappings)
+from .quantized import (allocate_q8_kv_caches, append_paged_kv_cache_q8, plan_q8_cache, q8_page_bytes, read_cache_q8,
+                        read_paged_kv_cache_q8, reshape_and_cache_q8)
 from .rotary import (PagedRotaryWritePlan, RotaryEmbedding, make_cos_sin_cache, qk_norm_rotary_pos_emb,
                      qk_norm_rotary_pos_emb_and_append_paged, qk_norm_rotary_pos_emb_and_cache, rotary_pos_emb,
                      rotary_pos_emb_and_append_paged, rotary_pos_emb_and_cache)
@@ -56,6 +59,8 @@ __all__ = [
     "InferInput", "KVIndexInputs", "make_kv_index_inputs", "to_device", "to_device_one_launch",
     "build_write_index", "BlockRuns", "max_block_runs", "slot_block_runs", "write_block_runs_layers",
     "KVWriteStep",
+    "q8_page_bytes", "plan_q8_cache", "allocate_q8_kv_caches", "reshape_and_cache_q8", "append_paged_kv_cache_q8",
+    "read_cache_q8", "read_paged_kv_cache_q8",
     "PagedAttentionPlan", "paged_attention", "common_prefix_pages",
     "qk_norm_rotary_pos_emb", "qk_norm_rotary_pos_emb_and_cache", "qk_norm_rotary_pos_emb_and_append_paged",
 ]

@@ -154,6 +154,13 @@ SIGNATURES = {
     "kvc_attention_plan_build": (c_int, [_P, _P, _I64, _P]),
     "kvc_attention_plan_run": (c_int, [_P, _P, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P]),
     "kvc_attention_plan_destroy": (c_int, [_P]),
+    "kvc_q8_page_bytes": (_I64, [_I64, _I64, _I64]),
+    "kvc_reshape_and_cache_q8": (c_int, [_P, _P, _P, _P, c_int, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, c_int, _P]),
+    "kvc_append_paged_kv_cache_q8": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                             _I64, _I64, _I64, c_int, _P]),
+    "kvc_read_cache_q8": (c_int, [_P, _P, c_int, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, c_int, _P]),
+    "kvc_read_paged_kv_cache_q8": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
+                                           _I64, _I64, _I64, c_int, _P]),
     "kvc_copy_blocks": (c_int, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P]),
     "kvc_gather_blocks": (c_int, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
     "kvc_scatter_blocks": (c_int, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P]),

@@ -16,6 +16,7 @@ SOURCES = [os.path.join(PKG_DIR, "csrc", "kvcache.hip"),
            os.path.join(PKG_DIR, "csrc", "rope_cache.hip"),
            os.path.join(PKG_DIR, "csrc", "qk_norm.hip"),
            os.path.join(PKG_DIR, "csrc", "attention.hip"),
+           os.path.join(PKG_DIR, "csrc", "quantized.hip"),
            os.path.join(PKG_DIR, "csrc", "disk_tier.cpp"),
            os.path.join(PKG_DIR, "csrc", "host_rows.cpp")]
 INCLUDE = os.path.join(REPO_ROOT, "include")
@@ -92,7 +93,8 @@ def build_fastcall(verbose: bool = False) -> str:
     return FAST_PATH
 
 
-HEADERS = [os.path.join(PKG_DIR, "csrc", "common.h"), os.path.join(PKG_DIR, "csrc", "device.h"),
+HEADERS = [os.path.join(PKG_DIR, "csrc", "common.h"), os.path.join(PKG_DIR, "csrc", "attention.h"),
+           os.path.join(PKG_DIR, "csrc", "types.h"), os.path.join(PKG_DIR, "csrc", "q8.h"), os.path.join(PKG_DIR, "csrc", "device.h"),
            os.path.join(PKG_DIR, "csrc", "staging.h"),
            os.path.join(INCLUDE, "kvcache.h"), os.path.join(INCLUDE, "kvcache_experimental.h")]
 

@@ -1,0 +1,93 @@
+// What the kernels of the attention over a 16-bit cache and over an 8-bit one share: the step's layout, as the plan's launch
+// writes it, and the launch's arguments.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "types.h"
+
+namespace kvc {
+namespace attn {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kTile = 16;          // rows of a narrow item
+constexpr int kWide = 32 * kWaves; // rows of a wide item: 32 to a wavefront
+constexpr int kStep = 64;          // keys that a workgroup takes at once of a wide item
+constexpr int kAhead = 3;          // pieces of a wide item's K and V that are read from LDS ahead of their product
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct Item {  // 32 bytes: a tile or a part of one
+  int32_t q_begin;  // first token of the request; -1: the rows of all sharing requests, through shared_tokens
+  int32_t row0, rows, table, key_begin, key_end;
+  int32_t slot;     // of its partial; -1: the whole tile
+  int32_t limit;    // keys that the request's first token sees, each further one a key more (less than 1: none)
+};
+struct Parts {  // 16 bytes: of a tile: the slot of the first, and of the c-th further one next + c * step
+  int32_t slot, next, step, count;
+};
+struct Entry {  // 32 bytes: rows of one tile that are joined from partials
+  int32_t q_begin, row0;
+  int16_t rows, many;   // (a single one, of many parts)
+  int32_t shared_row0;  // the first row among those of the sharing requests, or -1
+  Parts parts;
+};
+struct Range {
+  int32_t begin, end;
+};
+struct Header {
+  int32_t wide_items, narrow_entries, wide_entries, shared_wide;  // (narrow entries from the front, wide ones from the back)
+};
+
+struct Layout {  // the plan's device buffer
+  Header* header;
+  int32_t* shares;         // [B] 1: its leading pages are the shared ones
+  int2* shared_tokens;     // [T] token, and the keys it sees
+  Range* ranges;           // [groups] narrow items of a workgroup
+  Item* items[2];          // narrow: tile t's part in workgroup w at t + w: those of a workgroup lie side by side
+  Parts* shared_parts;     // of the tiles of the sharing requests' rows
+  Entry* entries;
+};
+
+__device__ __forceinline__ int32_t clamp(int32_t x, int32_t lo, int32_t hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+struct AttendArgs {
+  const char* query;
+  const char* cache;
+  const int32_t* kv_indices;
+  char* out;
+  float* lse;              // may be null
+  float* partial[2];       // narrow, wide: [slots][kv heads][rows of a tile][head_dim]
+  float* partial_lse[2];   // [slots][kv heads][rows of a tile], to base 2
+  int64_t q_stride;        // bytes
+  uint32_t page_stride, row_stride, plane;  // bytes: page to page, key to key in a page (none in an 8-bit cache), K to V
+  int32_t num_pages, page_size, page_shift;
+  int32_t kv_heads, group, head_dim;
+  int32_t narrow_groups, wide_groups;  // workgroups, of all key heads
+  int32_t max_entries;
+  uint32_t group_stride, exponents;    // of an 8-bit cache, bytes: group to group of 16 keys, a group's exponents
+  float scale;             // times log2(e)
+  Layout l;
+};
+
+// The larger of a lane's value and that of the lane 32 (16) further on or before, without LDS
+__device__ __forceinline__ float max_across32(float x) {
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float max_across16(float x) {
+  const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) <= 3.402823466e38f; }
+// The least weight of a part: however far below the others it is, what is infinite in it stays
+constexpr float kLeastWeight = 1.401298464e-45f;
+
+}  // namespace attn
+}  // namespace kvc

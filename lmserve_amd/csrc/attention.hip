@@ -19,29 +19,18 @@
 #include <new>
 #include <type_traits>
 
+#include "attention.h"
 #include "common.h"
 #include "device.h"
 #include "kvcache.h"
 
 namespace {
 
-using kvc::fail;
-using kvc::log2_exact;
-using kvc::u32x4;
+using namespace kvc;
+using namespace kvc::attn;
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kTile = 16;          // rows of a narrow item
-constexpr int kWide = 32 * kWaves; // rows of a wide item: 32 to a wavefront
 constexpr int kBlock = 32;         // keys that a wavefront takes at once of a narrow item
-constexpr int kStep = 64;          // keys that a workgroup takes at once of a wide item
 constexpr int kVPad = 64;          // bytes between a wide item's rows of V in LDS
-constexpr int kAhead = 3;          // pieces of a wide item's K and V that are read from LDS ahead of their product
 constexpr int kMaxGroups = 1024;    // workgroups of a key head
 // In keys: what a narrow tile costs beside its own, a workgroup's least share, the least part of a tile. With the least
 // share there are workgroups to spare, and a part is half of it: a short tile in one piece is done sooner than cut
@@ -59,8 +48,6 @@ __host__ __device__ constexpr bool wide_prefix(int64_t rows, int64_t keys) {
   return rows > kNarrowSharedRows || (rows > kTile && rows * keys > kNarrowWork);
 }
 constexpr int kManyParts = 16;     // a row of more partials is joined by a workgroup
-constexpr float kLn2 = 0.69314718055994530942f;
-constexpr float kLog2e = 1.44269504088896340736f;
 
 // ---- the step's layout ---------------------------------------------------------------------------------------------
 // Row tiles are of 16 rows (narrow, of requests of few rows) or of 128 (wide), each over the keys that its last row sees.
@@ -72,38 +59,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 //   neighbours in the list and run on one XCD, whose L2 the range then comes to once (2048 new
 //   tokens behind 13 to 30 thousand keys 834 us; the tiles dealt to all XCDs in turn 854).
 // A part of a tile leaves its rows' unfinished result in a slot of the workspace, and the parts are joined at the end.
-struct Item {  // 32 bytes: a tile or a part of one
-  int32_t q_begin;  // first token of the request; -1: the rows of all sharing requests, through shared_tokens
-  int32_t row0, rows, table, key_begin, key_end;
-  int32_t slot;     // of its partial; -1: the whole tile
-  int32_t limit;    // keys that the request's first token sees, each further one a key more (less than 1: none)
-};
-struct Parts {  // 16 bytes: of a tile: the slot of the first, and of the c-th further one next + c * step
-  int32_t slot, next, step, count;
-};
-struct Entry {  // 32 bytes: rows of one tile that are joined from partials
-  int32_t q_begin, row0;
-  int16_t rows, many;   // (a single one, of many parts)
-  int32_t shared_row0;  // the first row among those of the sharing requests, or -1
-  Parts parts;
-};
-struct Range {
-  int32_t begin, end;
-};
-struct Header {
-  int32_t wide_items, narrow_entries, wide_entries, shared_wide;  // (narrow entries from the front, wide ones from the back)
-};
-
-struct Layout {  // the plan's device buffer
-  Header* header;
-  int32_t* shares;         // [B] 1: its leading pages are the shared ones
-  int2* shared_tokens;     // [T] token, and the keys it sees
-  Range* ranges;           // [groups] narrow items of a workgroup
-  Item* items[2];          // narrow: tile t's part in workgroup w at t + w: those of a workgroup lie side by side
-  Parts* shared_parts;     // of the tiles of the sharing requests' rows
-  Entry* entries;
-};
-
+// (The lists are those of attention.h.)
 struct PlanArgs {
   const int32_t *qo_indptr, *kv_indices, *kv_indptr, *kv_last_page_len;
   int32_t batch_size, num_tokens, num_kv_indices, page_size, shared_pages, group;
@@ -112,8 +68,6 @@ struct PlanArgs {
   int32_t max_items[2], max_entries;
   Layout l;
 };
-
-__device__ __forceinline__ int32_t clamp(int32_t x, int32_t lo, int32_t hi) { return x < lo ? lo : x > hi ? hi : x; }
 
 struct Table {
   int32_t begin, pages;
@@ -452,58 +406,6 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     a.l.ranges[w] = last_item[w] < 0 ? Range{0, 0} : Range{first_item[w], last_item[w] + 1};
 }
 
-// ---- storage types -------------------------------------------------------------------------------------------------
-struct BF16 {
-  typedef __bf16 V8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    const f32x2 v = {lo, hi};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2));
-  }
-  static __device__ __forceinline__ float wide(uint32_t half) { return __uint_as_float(half << 16); }
-  static constexpr uint32_t kExponent = 0x7f80u;
-  static constexpr float kScaledUp = 0;
-};
-struct F16 {
-  typedef _Float16 V8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const h2 v = {(_Float16)lo, (_Float16)hi};
-    return __builtin_bit_cast(uint32_t, v);
-  }
-  static __device__ __forceinline__ float wide(uint32_t half) {
-    return (float)__builtin_bit_cast(_Float16, (uint16_t)half);
-  }
-  static constexpr uint32_t kExponent = 0x7c00u;
-  // log2 of what weights are scaled up by, so that small ones, of which there may be many, are numbers of the type: a weight of 1 is
-  // then 2^14 in a narrow tile, and one of kOutgrown, 2^8, is 2^15 in a wide tile. Both keep a step of the type below its largest.
-  static constexpr float kScaledUp = 14;
-};
-// Is an infinity or NaN among the 16-bit values that were taken in? (The largest exponent of either half.)
-template <typename T>
-struct Oddities {
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-  u16x2 top = {};
-  __device__ __forceinline__ void take(u32x4 v) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[w] & (T::kExponent << 16 | T::kExponent)));
-  }
-  __device__ __forceinline__ bool any() const { return max((uint32_t)top[0], (uint32_t)top[1]) == T::kExponent; }
-};
 // The infinities and NaN among 4 values, 0 for the others
 template <typename T>
 __device__ __forceinline__ f32x4 infinite_part(u32x2 four) {
@@ -515,32 +417,6 @@ __device__ __forceinline__ f32x4 infinite_part(u32x2 four) {
   }
   return x;
 }
-template <typename T>
-__device__ __forceinline__ u32x4 finite_part(u32x4 v) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v[i] = ((v[i] & T::kExponent) == T::kExponent ? 0 : v[i] & 0xffffu) | ((v[i] >> 16 & T::kExponent) == T::kExponent ? 0 : v[i] & 0xffff0000u);
-  return v;
-}
-
-struct AttendArgs {
-  const char* query;
-  const char* cache;
-  const int32_t* kv_indices;
-  char* out;
-  float* lse;              // may be null
-  float* partial[2];       // narrow, wide: [slots][kv heads][rows of a tile][head_dim]
-  float* partial_lse[2];   // [slots][kv heads][rows of a tile], to base 2
-  int64_t q_stride;        // bytes
-  uint32_t page_stride, row_stride, plane;  // bytes: page to page, key to key in a page, K to V
-  int32_t num_pages, page_size, page_shift;
-  int32_t kv_heads, group, head_dim;
-  int32_t narrow_groups, wide_groups;  // workgroups, of all key heads
-  int32_t max_entries;
-  float scale;             // times log2(e)
-  Layout l;
-};
-
 // Byte offset of a key's row, or -1 where there is none to read: beyond `end`, or on a page that the cache does not have
 __device__ __forceinline__ int64_t key_offset(const AttendArgs& a, int32_t table, int32_t key, int32_t end) {
   if (key >= end) return -1;
@@ -549,22 +425,6 @@ __device__ __forceinline__ int64_t key_offset(const AttendArgs& a, int32_t table
   if (page < 0 || page >= a.num_pages) return -1;
   return (int64_t)page * a.page_stride + (int64_t)(key - p * a.page_size) * a.row_stride;
 }
-
-// The larger of a lane's value and that of the lane 32 (16) further on or before, without LDS
-__device__ __forceinline__ float max_across32(float x) {
-  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-}
-__device__ __forceinline__ float max_across16(float x) {
-  const auto both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-}
-
-__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
-
-__device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) <= 3.402823466e38f; }
-// The least weight of a part: however far below the others it is, what is infinite in it stays
-constexpr float kLeastWeight = 1.401298464e-45f;
 
 // How an item's keys are reached
 enum Reach : int {
@@ -1416,14 +1276,6 @@ __global__ __launch_bounds__(kThreads, 6) void attend_join_kernel(AttendArgs a) 
 }
 
 int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
-
-struct Memory {  // of an argument (which may be null)
-  const void* p;
-  int64_t bytes;
-  bool meets(const Memory& o) const {
-    return p && o.p && bytes > 0 && o.bytes > 0 && (uintptr_t)p < (uintptr_t)o.p + (uint64_t)o.bytes && (uintptr_t)o.p < (uintptr_t)p + (uint64_t)bytes;
-  }
-};
 
 // The sizes that follow from the capacities: of narrow and of wide items
 struct Sizes {

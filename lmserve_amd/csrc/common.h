@@ -20,6 +20,14 @@ inline int log2_exact(int64_t x) {
   return s;
 }
 
+struct Memory {  // of an argument (which may be null)
+  const void* p;
+  int64_t bytes;
+  bool meets(const Memory& o) const {
+    return p && o.p && bytes > 0 && o.bytes > 0 && (uintptr_t)p < (uintptr_t)o.p + (uint64_t)o.bytes && (uintptr_t)o.p < (uintptr_t)p + (uint64_t)bytes;
+  }
+};
+
 // Launch shape of the rotation kernel, set through kvc_set_tuning
 // ("rope_threads": 64/128/192/256 lanes per workgroup, 0 = by size; "rope_nt":
 // non-temporal loads, bit 0 the K and V rows, bit 1 the Q rows, 4 = plain loads,

@@ -81,6 +81,7 @@ dtype_map = {
     torch.float16: np.float16,
     torch.bfloat16: np.uint16,
     torch.int32: np.int32,
+    torch.uint8: np.uint8,      # blocks of an 8-bit cache
 }
 
 SWAP_MODES = {"staged": _lib.KVC_SWAP_STAGED, "direct": _lib.KVC_SWAP_DIRECT, "auto": _lib.KVC_SWAP_AUTO}
