@@ -640,6 +640,24 @@ int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query,
                            void* workspace, int64_t workspace_bytes, void* stream);
 int kvc_attention_plan_destroy(kvc_attention_plan* plan);
 
+/* The same over a cache in 8 bits (kvc_q8_page_bytes has its layout): a plan made by
+ * _create_q8 is built, sized and destroyed as the others and run by _run_q8, page_stride in
+ * BYTES. head_dim and page_size are multiples of 16. What the codes stand for is
+ * what is attended to: a code that is NaN has that value in the rows that see it, and those alone.
+ * Weights go into the product with V in f16, scaled up by 2^7 or 2^14, whatever dtype is,
+ * with f16 queries of few rows in two parts. Values are kept to 2^-41 of the largest
+ * that the keys of the same request may have (448 times their groups' largest scale). */
+int kvc_attention_plan_create_q8(const int32_t* qo_indptr, const int32_t* kv_indices,
+                                 const int32_t* kv_indptr, const int32_t* kv_last_page_len,
+                                 int64_t batch_size, int64_t num_tokens, int64_t num_kv_indices,
+                                 int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                 int64_t page_size, int64_t max_q_len, int64_t shared_pages,
+                                 float sm_scale, int dtype, kvc_attention_plan** out);
+int kvc_attention_plan_run_q8(const kvc_attention_plan* plan, const void* query,
+                              int64_t q_token_stride, const void* paged_kv_cache,
+                              int64_t page_stride, int64_t num_pages, void* out, float* lse,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------
  * The cache in 8 bits: half the bytes of K and V, quantised as they are written.
  * Stands beside the 16-bit write of the same call site

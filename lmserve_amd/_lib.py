@@ -154,6 +154,9 @@ SIGNATURES = {
     "kvc_attention_plan_build": (c_int, [_P, _P, _I64, _P]),
     "kvc_attention_plan_run": (c_int, [_P, _P, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P]),
     "kvc_attention_plan_destroy": (c_int, [_P]),
+    "kvc_attention_plan_create_q8": (c_int, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, c_float,
+                                          c_int, ctypes.POINTER(_P)]),
+    "kvc_attention_plan_run_q8": (c_int, [_P, _P, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _P]),
     "kvc_q8_page_bytes": (_I64, [_I64, _I64, _I64]),
     "kvc_reshape_and_cache_q8": (c_int, [_P, _P, _P, _P, c_int, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, c_int, _P]),
     "kvc_append_paged_kv_cache_q8": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64,

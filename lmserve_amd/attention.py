@@ -16,6 +16,7 @@ import torch
 from . import _lib
 from .cache_ops import _on_device_of, _require_gpu, _stream_of
 from .paged import _i32
+from .quantized import _pages
 from .rotary import _DTYPES
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -34,6 +35,9 @@ class PagedAttentionPlan:
       computed by themselves: the number changes the time and not the result.
     sm_scale: of the scores, `head_dim ** -0.5` when None.
     max_q_len: the most tokens a request has, if known: of help to the choice of kernels, not a limit.
+    kv_dtype: `torch.float8_e4m3fn` for a cache in 8 bits (`lmserve_amd.quantized`), whose layers are
+      `[num_pages, page_bytes]` of uint8; `dtype` is then the queries' and outputs'. `head_dim` and `page_size` are
+      multiples of 16 with it.
 
     The step's work is laid out on the device at construction, by a small launch (two with shared pages) on the current
     stream; `build()` does it again after the index buffers were written for another step, and can
@@ -45,7 +49,7 @@ class PagedAttentionPlan:
     def __init__(self, qo_indptr: torch.Tensor, kv_indices: torch.Tensor, kv_indptr: torch.Tensor,
                  kv_last_page_len: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                  dtype: torch.dtype, num_tokens: int, max_q_len: Optional[int] = None, shared_pages: int = 0,
-                 sm_scale: Optional[float] = None, kv_layout: str = "NHD"):
+                 sm_scale: Optional[float] = None, kv_layout: str = "NHD", kv_dtype: Optional[torch.dtype] = None):
         if kv_layout != "NHD":
             raise ValueError(f"kv_layout {kv_layout!r} is not supported (the reference uses 'NHD')")
         self._plan = None
@@ -64,11 +68,15 @@ class PagedAttentionPlan:
         kd = _DTYPES.get(dtype)
         if kd is None:
             raise TypeError(f"Unsupported dtype: {dtype}")
+        if kv_dtype not in (None, dtype, torch.float8_e4m3fn):
+            raise TypeError(f"Unsupported kv_dtype: {kv_dtype} (the cache holds {dtype} or float8_e4m3fn)")
+        self.q8 = kv_dtype == torch.float8_e4m3fn
         self.dtype, self.num_tokens = dtype, int(num_tokens)
         self.Hq, self.H, self.D, self.page_size = int(num_heads), int(num_kv_heads), int(head_dim), int(page_size)
         lib = _lib.lib()
         handle = ctypes.c_void_p()
-        _lib.check(lib.kvc_attention_plan_create(
+        create = lib.kvc_attention_plan_create_q8 if self.q8 else lib.kvc_attention_plan_create
+        _lib.check(create(
             self.qo_indptr.data_ptr(), self.kv_indices.data_ptr(), self.kv_indptr.data_ptr(),
             self.kv_last_page_len.data_ptr(), batch, self.num_tokens, self.kv_indices.numel(), self.Hq, self.H,
             self.D, self.page_size, int(max_q_len or 0), int(shared_pages), self.D ** -0.5 if sm_scale is None else float(sm_scale), kd,
@@ -79,7 +87,7 @@ class PagedAttentionPlan:
         self._workspace_bytes = lib.kvc_attention_workspace_bytes(self._plan)
         self._stream = _stream_of(self._buffer)      # whose allocator the buffer is from
         self._dev_index = self.device.index
-        fast = _lib.fast()
+        fast = None if self.q8 else _lib.fast()
         self._fast_run = fast.attention_plan_run if fast else None
         self._dtype_code = fast.scalar_type_code(torch.empty(0, dtype=dtype)) if fast else -1
         self.build()
@@ -108,7 +116,7 @@ class PagedAttentionPlan:
     def run(self, query: torch.Tensor, paged_kv_cache: torch.Tensor, out: Optional[torch.Tensor] = None,
             return_lse: bool = False, lse: Optional[torch.Tensor] = None):
         """One layer: `query [num_tokens, Hq, D]` (or `[num_tokens, Hq*D]`; rows may be slices
-        of a fused projection) over `paged_kv_cache [num_pages, 2, page_size, H, D]`.
+        of a fused projection) over `paged_kv_cache [num_pages, 2, page_size, H, D]`, or `[num_pages, page_bytes]` in 8 bits.
         Returns `out` in the query's shape, with `return_lse` also the fp32 `[num_tokens, Hq]` logarithms of the
         softmax sums. `out` / `lse` may be contiguous buffers of the caller's (`out` the query itself, but no other
         memory that is read); without one, rows
@@ -126,7 +134,7 @@ class PagedAttentionPlan:
                     _lib.check(got)
         for t, n in ((query, "query"), (paged_kv_cache, "paged_kv_cache")):
             _require_gpu(t, n)
-            if t.dtype != self.dtype or t.device != self.device:
+            if t.dtype != (torch.uint8 if self.q8 and t is paged_kv_cache else self.dtype) or t.device != self.device:
                 raise TypeError(f"{n} must have the plan's dtype and device")
         T, row = self.num_tokens, self.Hq * self.D
         if query.dim() not in (2, 3) or query.shape[0] != T or query.numel() != T * row \
@@ -140,11 +148,17 @@ class PagedAttentionPlan:
                 q2 = q2.clone()
         shape, st = paged_kv_cache.shape, paged_kv_cache.stride()
         kv_row = self.H * self.D
-        if len(shape) != 5 or shape[1:] != (2, self.page_size, self.H, self.D):
+        if self.q8:
+            pages, page_size, page_stride = _pages(paged_kv_cache, self.H, self.D, "paged_kv_cache")
+            if page_size != self.page_size:
+                raise ValueError(f"paged_kv_cache has pages of {page_size} tokens, the plan of {self.page_size}")
+        elif len(shape) != 5 or shape[1:] != (2, self.page_size, self.H, self.D):
             raise ValueError("paged_kv_cache must be [num_pages, 2, page_size, H, D]")
-        pages = shape[0]
-        page = 2 * self.page_size * kv_row
-        if pages and (st[4] != 1 or (st[3] != self.D and self.H > 1) or (st[2] != kv_row and self.page_size > 1)
+        else:
+            pages = shape[0]
+            page = 2 * self.page_size * kv_row
+            page_stride = st[0] if pages > 1 else page
+        if pages and not self.q8 and (st[4] != 1 or (st[3] != self.D and self.H > 1) or (st[2] != kv_row and self.page_size > 1)
                       or st[1] != page // 2):
             raise ValueError("every page of paged_kv_cache must be contiguous [2, page_size, H, D]")
         if out is None:
@@ -161,9 +175,10 @@ class PagedAttentionPlan:
                 stream = _stream_of(q2)
                 self._used_here()
                 workspace = torch.empty(self._workspace_bytes, dtype=torch.uint8, device=self.device)
-                _lib.check(_lib.lib().kvc_attention_plan_run(
+                run = _lib.lib().kvc_attention_plan_run_q8 if self.q8 else _lib.lib().kvc_attention_plan_run
+                _lib.check(run(
                     self._plan, q2.data_ptr(), q2.stride(0) if T > 1 else row, paged_kv_cache.data_ptr(),
-                    st[0] if pages > 1 else page, pages, out.data_ptr(), None if lse is None else lse.data_ptr(),
+                    page_stride, pages, out.data_ptr(), None if lse is None else lse.data_ptr(),
                     workspace.data_ptr(), workspace.numel(), stream))
         return (out, lse) if return_lse else out
 
@@ -171,11 +186,17 @@ class PagedAttentionPlan:
 def paged_attention(query: torch.Tensor, paged_kv_cache: torch.Tensor, qo_indptr: torch.Tensor,
                     kv_indices: torch.Tensor, kv_indptr: torch.Tensor, kv_last_page_len: torch.Tensor,
                     max_q_len: Optional[int] = None, shared_pages: int = 0, sm_scale: Optional[float] = None,
-                    out: Optional[torch.Tensor] = None, return_lse: bool = False, kv_layout: str = "NHD"):
+                    out: Optional[torch.Tensor] = None, return_lse: bool = False, kv_layout: str = "NHD",
+                    num_kv_heads: Optional[int] = None):
     """`PagedAttentionPlan` made and run once: attention of one layer with index tensors that
-    serve no other (a model's layers share a plan). Arguments and results are the plan's."""
+    serve no other (a model's layers share a plan). Arguments and results are the plan's. A cache
+    `[num_pages, page_bytes]` of uint8 is one in 8 bits: `query` is then `[T, Hq, D]`, and `num_kv_heads` has to be given."""
+    if isinstance(paged_kv_cache, torch.Tensor) and paged_kv_cache.dtype == torch.uint8:
+        return _paged_attention_q8(query, paged_kv_cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len,
+                                   shared_pages, sm_scale, out, return_lse, kv_layout, num_kv_heads)
     fast = _lib.fast_entry("paged_attention")
-    if fast is not None and kv_layout == "NHD" and isinstance(paged_kv_cache, torch.Tensor) and paged_kv_cache.is_cuda:
+    if fast is not None and kv_layout == "NHD" and isinstance(paged_kv_cache, torch.Tensor) and paged_kv_cache.is_cuda \
+            and num_kv_heads is None:
         # common layouts: checked and launched from C++ (1 = not one of them: fall through)
         dev = paged_kv_cache.device.index
         got = fast(query, paged_kv_cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len or 0, shared_pages,
@@ -190,10 +211,26 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: torch.Tensor, qo_indptr
     if paged_kv_cache.dim() != 5 or paged_kv_cache.shape[1] != 2:
         raise ValueError("paged_kv_cache must be [num_pages, 2, page_size, H, D]")
     _, _, page_size, H, D = paged_kv_cache.shape
+    if num_kv_heads not in (None, H):
+        raise ValueError(f"num_kv_heads is {num_kv_heads}, the cache has {H}")
     if query.dim() not in (2, 3) or D == 0 or query.shape[-1] % D:
         raise ValueError("query must be [T, Hq, D] or [T, Hq*D]")
     heads = query.shape[1] if query.dim() == 3 else query.shape[1] // D
     plan = PagedAttentionPlan(qo_indptr, kv_indices, kv_indptr, kv_last_page_len, heads, H, D, page_size, query.dtype,
                               query.shape[0], max_q_len=max_q_len, shared_pages=shared_pages, sm_scale=sm_scale,
                               kv_layout=kv_layout)
+    return plan.run(query, paged_kv_cache, out=out, return_lse=return_lse)
+
+
+def _paged_attention_q8(query, paged_kv_cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len, shared_pages,
+                        sm_scale, out, return_lse, kv_layout, num_kv_heads):
+    for t, n in ((query, "query"), (paged_kv_cache, "paged_kv_cache")):
+        _require_gpu(t, n)
+    if query.dim() != 3 or num_kv_heads is None:
+        raise ValueError("over a cache in 8 bits query must be [T, Hq, D] and num_kv_heads given")
+    _, heads, D = query.shape
+    _, page_size, _ = _pages(paged_kv_cache, int(num_kv_heads), D, "paged_kv_cache")
+    plan = PagedAttentionPlan(qo_indptr, kv_indices, kv_indptr, kv_last_page_len, heads, num_kv_heads, D, page_size, query.dtype,
+                              query.shape[0], max_q_len=max_q_len, shared_pages=shared_pages, sm_scale=sm_scale,
+                              kv_layout=kv_layout, kv_dtype=torch.float8_e4m3fn)
     return plan.run(query, paged_kv_cache, out=out, return_lse=return_lse)

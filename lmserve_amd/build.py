@@ -16,6 +16,7 @@ SOURCES = [os.path.join(PKG_DIR, "csrc", "kvcache.hip"),
            os.path.join(PKG_DIR, "csrc", "rope_cache.hip"),
            os.path.join(PKG_DIR, "csrc", "qk_norm.hip"),
            os.path.join(PKG_DIR, "csrc", "attention.hip"),
+           os.path.join(PKG_DIR, "csrc", "attention_q8.hip"),
            os.path.join(PKG_DIR, "csrc", "quantized.hip"),
            os.path.join(PKG_DIR, "csrc", "disk_tier.cpp"),
            os.path.join(PKG_DIR, "csrc", "host_rows.cpp")]

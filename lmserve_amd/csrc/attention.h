@@ -89,5 +89,49 @@ __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) <= 3
 // The least weight of a part: however far below the others it is, what is infinite in it stays
 constexpr float kLeastWeight = 1.401298464e-45f;
 
+// A workgroup of a key head takes its share's items one after the other
+template <typename Narrow>
+__device__ __forceinline__ void take_share(const AttendArgs& a, int32_t at, const Narrow& narrow) {
+  const int32_t group = at / a.kv_heads, h = at - group * a.kv_heads;
+  const Range range = a.l.ranges[group];
+  for (int32_t i = range.begin; i < range.end; ++i) narrow(a.l.items[0][i], h);
+}
+
+// Steps that may have wide tiles: both kinds in one launch, side by side on the card, as the narrow ones wait for memory and
+// the wide ones for the matrix units. 32 workgroups of a kind in turn: they are dealt to the 8 XCDs and there to 4 shader
+// engines in rotation (8 in turn put all wide ones on half of the engines: 2048 new tokens 1218 us, 917 so). The wide items, of one key head
+// after the other, are dealt to the XCDs in eight runs, so that items that read the same keys share an L2.
+template <typename Narrow, typename Wide>
+__device__ __forceinline__ void take_step(const AttendArgs& a, const Narrow& narrow_item, const Wide& wide_item) {
+  const int32_t narrow = a.narrow_groups;
+  const int32_t both = (narrow < a.wide_groups ? narrow : a.wide_groups) & ~31;
+  int32_t at = blockIdx.x;
+  bool is_wide;
+  if (at < 2 * both) {
+    is_wide = (at & 32) == 0;
+    at = (at >> 6) * 32 + (at & 31);
+  } else {
+    at -= both;  // what is left of either, the wide first
+    is_wide = at < a.wide_groups;
+    if (!is_wide) at = at - a.wide_groups + both;
+  }
+  if (!is_wide) {
+    take_share(a, at, narrow_item);
+    return;
+  }
+  const int32_t items = a.l.header->wide_items, all = items * a.kv_heads, run = (all + 7) / 8;
+  for (int32_t i = at >> 3; i < run; i += a.wide_groups >> 3) {
+    const int32_t x = (at & 7) * run + i;
+    if (x >= all) break;
+    const int32_t h = x / items;
+    const Item item = a.l.items[1][x - h * items];
+    if (item.rows) wide_item(item, h);
+  }
+}
+
+// The 8-bit cache's kernels (attention_q8.hip): the step's tiles, `wide` where there may be wide ones
+void launch_q8(const AttendArgs& a, bool f16, bool wide, bool past_the_caches, hipStream_t s);
+constexpr int q8_narrow_residents(int dim) { return dim <= 64 ? 3 : dim <= 128 ? 2 : 1; }  // narrow workgroups of a CU
+
 }  // namespace attn
 }  // namespace kvc

@@ -23,6 +23,7 @@
 #include "common.h"
 #include "device.h"
 #include "kvcache.h"
+#include "q8.h"
 
 namespace {
 
@@ -1160,52 +1161,20 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
   }
 }
 
-// A workgroup of a key head takes its share's items one after the other
-template <typename T, int DP, Reach REACH, bool NT>
-__device__ __forceinline__ void narrow_share(const AttendArgs& a, int32_t at, char* lds) {
-  const int32_t group = at / a.kv_heads, h = at - group * a.kv_heads;
-  const Range range = a.l.ranges[group];
-  for (int32_t i = range.begin; i < range.end; ++i) narrow_item<T, DP, REACH, NT>(a, a.l.items[0][i], h, lds);
-}
 // As many workgroups as are on the card at once, by their registers. NT: keys by non-temporal loads, see launch_attend.
 constexpr int narrow_residents(int dp) { return dp <= 64 ? 4 : dp <= 128 ? 2 : 1; }  // of a CU
 template <typename T, int DP, Reach REACH, bool NT = false>
 __global__ __launch_bounds__(kThreads, narrow_residents(DP)) void attend_rows_kernel(AttendArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[narrow_lds<T, DP>()];
-  narrow_share<T, DP, REACH, NT>(a, blockIdx.x, lds);
+  take_share(a, blockIdx.x, [&](const Item& item, int32_t h) { narrow_item<T, DP, REACH, NT>(a, item, h, lds); });
 }
 
-// Steps that may have wide tiles: both kinds in one launch, side by side on the card, as the narrow ones wait for memory and
-// the wide ones for the matrix units. 32 workgroups of a kind in turn: they are dealt to the 8 XCDs and there to 4 shader
-// engines in rotation (8 in turn put all wide ones on half of the engines: 2048 new tokens 1218 us, 917 so). The wide items, of one key head
-// after the other, are dealt to the XCDs in eight runs, so that items that read the same keys share an L2.
 template <typename T, int DP, Reach REACH>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_step_kernel(AttendArgs a) {
   constexpr int LDS = wide_lds<DP>() > narrow_lds<T, DP>() ? wide_lds<DP>() : narrow_lds<T, DP>();
   __shared__ __attribute__((aligned(16))) char lds[LDS];
-  const int32_t narrow = a.narrow_groups, both = min(narrow, a.wide_groups) & ~31;
-  int32_t at = blockIdx.x;
-  bool is_wide;
-  if (at < 2 * both) {
-    is_wide = (at & 32) == 0;
-    at = (at >> 6) * 32 + (at & 31);
-  } else {
-    at -= both;  // what is left of either, the wide first
-    is_wide = at < a.wide_groups;
-    if (!is_wide) at = at - a.wide_groups + both;
-  }
-  if (!is_wide) {
-    narrow_share<T, DP, REACH, false>(a, at, lds);
-    return;
-  }
-  const int32_t items = a.l.header->wide_items, all = items * a.kv_heads, run = (all + 7) / 8;
-  for (int32_t i = at >> 3; i < run; i += a.wide_groups >> 3) {
-    const int32_t x = (at & 7) * run + i;
-    if (x >= all) break;
-    const int32_t h = x / items;
-    const Item item = a.l.items[1][x - h * items];
-    if (item.rows) wide_item<T, DP, REACH>(a, item, h, lds);
-  }
+  take_step(a, [&](const Item& item, int32_t h) { narrow_item<T, DP, REACH, false>(a, item, h, lds); },
+            [&](const Item& item, int32_t h) { wide_item<T, DP, REACH>(a, item, h, lds); });
 }
 
 // Joins a row's partials: weights exp2(lse_c - lse). An entry of several rows, of few parts each, takes half a wavefront a row,
@@ -1292,6 +1261,7 @@ struct kvc_attention_plan {
   int64_t batch_size, num_tokens, num_kv_indices, num_heads, num_kv_heads, head_dim, page_size, shared_pages;
   int64_t narrow_rows;
   int dtype;
+  bool q8;  // the cache is in 8 bits
   float scale;
   Sizes n;
   int64_t plan_bytes, workspace_bytes;
@@ -1343,7 +1313,7 @@ Sizes sizes_of(const kvc_attention_plan& p) {
   const int64_t rows = p.num_tokens * (p.num_heads / p.num_kv_heads), keys = p.num_kv_indices * p.page_size;
   const bool shared = p.shared_pages > 0;
   n.wide = rows > p.narrow_rows || (shared && wide_prefix(rows, p.shared_pages * p.page_size));
-  const int64_t groups = n.wide ? kStepGroups : 256 * narrow_residents((int)p.head_dim);
+  const int64_t groups = n.wide ? kStepGroups : 256 * (p.q8 ? q8_narrow_residents((int)p.head_dim) : narrow_residents((int)p.head_dim));
   n.groups = std::min<int64_t>(kMaxGroups, std::max<int64_t>(1, groups / p.num_kv_heads));
   n.residents = std::max<int64_t>(1, kResidents / p.num_kv_heads);
   const int64_t requests = std::min(p.batch_size, p.num_tokens), of_narrow = std::min(rows, p.narrow_rows);
@@ -1370,14 +1340,18 @@ Sizes sizes_of(const kvc_attention_plan& p) {
   return n;
 }
 
+// Keys that no cache holds, and that are read once, by non-temporal loads (decode of 256 requests, 2.2 GB: 421 and 406 us;
+// one of 131001 keys, 0.5 GB: 108 and 103; behind a shared prompt, 0.27 GB of which 16 MB are read again and again, 126
+// and 130)
+bool past_the_caches(const kvc_attention_plan& p, int64_t element) {
+  return p.shared_pages == 0 && p.num_kv_indices * 2 * p.page_size * p.num_kv_heads * p.head_dim * element >= (int64_t(256) << 20);
+}
+
 template <typename T, int DP>
 void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
   const dim3 block(kThreads), grid((unsigned)(a.narrow_groups + a.wide_groups));
   const bool any = a.page_size % 16 != 0, full = a.head_dim == DP;
-  // Keys that no cache holds, and that are read once, by non-temporal loads (decode of 256 requests, 2.2 GB: 421 and 406 us;
-  // one of 131001 keys, 0.5 GB: 108 and 103; behind a shared prompt, 0.27 GB of which 16 MB are read again and again, 126
-  // and 130)
-  const bool nt = p.shared_pages == 0 && p.num_kv_indices * 2 * p.page_size * p.num_kv_heads * p.head_dim * 2 >= (int64_t(256) << 20);
+  const bool nt = past_the_caches(p, 2);
   if (p.n.wide) {
     if (any) kvc::launch((attend_step_kernel<T, DP, kAnyPage>), grid, block, 0, s, a);
     else if (!full) kvc::launch((attend_step_kernel<T, DP, kGroups>), grid, block, 0, s, a);
@@ -1391,7 +1365,8 @@ void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t
 }
 template <typename T>
 void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t s) {
-  if (p.head_dim <= 64) launch_attend<T, 64>(a, p, s);
+  if (p.q8) launch_q8(a, std::is_same<T, F16>::value, p.n.wide, past_the_caches(p, 1), s);
+  else if (p.head_dim <= 64) launch_attend<T, 64>(a, p, s);
   else if (p.head_dim <= 96) launch_attend<T, 96>(a, p, s);
   else if (p.head_dim <= 128) launch_attend<T, 128>(a, p, s);
   else launch_attend<T, 256>(a, p, s);
@@ -1402,14 +1377,12 @@ void launch_attend(const AttendArgs& a, const kvc_attention_plan& p, hipStream_t
 
 }  // namespace
 
-extern "C" {
+namespace {
 
-int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* kv_indptr,
-                              const int32_t* kv_last_page_len, int64_t batch_size, int64_t num_tokens,
-                              int64_t num_kv_indices, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
-                              int64_t page_size, int64_t max_q_len, int64_t shared_pages, float sm_scale, int dtype,
-                              kvc_attention_plan** out) {
-  constexpr const char* fn = "kvc_attention_plan_create";
+int create_plan(const char* fn, bool q8, const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* kv_indptr,
+                const int32_t* kv_last_page_len, int64_t batch_size, int64_t num_tokens, int64_t num_kv_indices, int64_t num_heads,
+                int64_t num_kv_heads, int64_t head_dim, int64_t page_size, int64_t max_q_len, int64_t shared_pages, float sm_scale,
+                int dtype, kvc_attention_plan** out) {
   if (!out) return fail(KVC_ERR_INVALID_ARG, "%s: null out", fn);
   *out = nullptr;
   if (dtype != KVC_DTYPE_BF16 && dtype != KVC_DTYPE_F16)
@@ -1423,6 +1396,9 @@ int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indice
     return fail(KVC_ERR_UNSUPPORTED, "%s: head_dim %lld (need a multiple of 8 up to 256)", fn, (long long)head_dim);
   if (page_size <= 0 || page_size > (1 << 20))
     return fail(KVC_ERR_INVALID_ARG, "%s: page_size %lld", fn, (long long)page_size);
+  if (q8 && (head_dim % 16 || page_size % q8::kGroup))
+    return fail(KVC_ERR_UNSUPPORTED, "%s: head_dim %lld, page_size %lld (an 8-bit cache needs multiples of 16)", fn, (long long)head_dim,
+                (long long)page_size);
   if (!(sm_scale > 0) || !std::isfinite(sm_scale))
     return fail(KVC_ERR_INVALID_ARG, "%s: the scale must be positive and finite", fn);
   if (batch_size >= (1 << 24) || num_kv_indices >= (int64_t(1) << 31) || num_heads > 0xffff ||
@@ -1430,11 +1406,13 @@ int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indice
     return fail(KVC_ERR_UNSUPPORTED, "%s: too many requests, pages, tokens or heads", fn);
   if (batch_size > 0 && (!qo_indptr || !kv_indptr || !kv_last_page_len || (num_kv_indices > 0 && !kv_indices)))
     return fail(KVC_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (q8 && page_size / q8::kGroup * q8::group_bytes(num_kv_heads, head_dim) >= int64_t(1) << 32)
+    return fail(KVC_ERR_UNSUPPORTED, "%s: pages of 4 GiB and more", fn);
   // more pages than the tables hold are shared by no one
   if (shared_pages > num_kv_indices || shared_pages * page_size > (1 << 30)) shared_pages = 0;
   kvc_attention_plan* p = new (std::nothrow) kvc_attention_plan{
       qo_indptr, kv_indices, kv_indptr, kv_last_page_len, batch_size, num_tokens, num_kv_indices, num_heads, num_kv_heads,
-      head_dim, page_size, shared_pages, kNarrowRows, dtype, sm_scale, {}, 0, 0, nullptr};
+      head_dim, page_size, shared_pages, kNarrowRows, dtype, q8, sm_scale, {}, 0, 0, nullptr};
   if (!p) return fail(KVC_ERR_HIP, "%s: out of host memory", fn);
   const int64_t rows = num_tokens * (num_heads / num_kv_heads), keys = num_kv_indices * page_size / std::max<int64_t>(batch_size, 1);
   if ((double)rows * (double)keys > (double)kMuchWork) p->narrow_rows = kTile;
@@ -1446,6 +1424,107 @@ int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indice
   p->workspace_bytes = round_up(std::max<int64_t>(p->workspace_bytes, 1), 256);
   *out = p;
   return KVC_OK;
+}
+
+// `page_stride` in bytes
+int run_plan(const char* fn, bool q8, const kvc_attention_plan* plan, const void* query, int64_t q_token_stride, const void* paged_kv_cache,
+             int64_t page_stride, int64_t num_pages, void* out, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!plan) return fail(KVC_ERR_INVALID_ARG, "%s: null plan", fn);
+  if (plan->q8 != q8) return fail(KVC_ERR_INVALID_ARG, "%s: the plan is for a cache in %d bits", fn, plan->q8 ? 8 : 16);
+  if (plan->batch_size == 0 || plan->num_tokens == 0) return KVC_OK;
+  const int64_t row = plan->num_kv_heads * plan->head_dim, group = q8::group_bytes(plan->num_kv_heads, plan->head_dim);
+  const int64_t page = q8 ? plan->page_size / q8::kGroup * group : 2 * plan->page_size * row * 2;
+  if (!query || !out || !workspace || (num_pages > 0 && !paged_kv_cache))
+    return fail(KVC_ERR_INVALID_ARG, "%s: null pointer", fn);
+  if (num_pages < 0 || num_pages >= (int64_t(1) << 31) || page_stride < page || page_stride >= (int64_t(1) << 32))
+    return fail(KVC_ERR_INVALID_ARG, "%s: bad cache geometry", fn);
+  if (q_token_stride < plan->num_heads * plan->head_dim)
+    return fail(KVC_ERR_INVALID_ARG, "%s: token stride smaller than a row", fn);
+  if (((uintptr_t)query | (uintptr_t)paged_kv_cache | (uint64_t)q_token_stride * 2 | (uint64_t)page_stride) % 16 ||
+      (uintptr_t)out % 8 || (uintptr_t)lse % 4 || (uintptr_t)workspace % 256)
+    return fail(KVC_ERR_INVALID_ARG, "%s: rows must be aligned to 16 bytes, the output to 8", fn);
+  if (workspace_bytes < plan->workspace_bytes)
+    return fail(KVC_ERR_STAGING, "%s: the workspace needs %lld bytes", fn, (long long)plan->workspace_bytes);
+  if (!plan->buffer) return fail(KVC_ERR_INVALID_ARG, "%s: the plan is not built", fn);
+  // A row of the query is read before the same row of the output is written, and by no one else afterwards; nothing else that
+  // is read or written may share memory with what is written
+  const int64_t q_row = plan->num_heads * plan->head_dim * 2;
+  const bool in_place = out == query && (plan->num_tokens == 1 || q_token_stride * 2 == q_row);
+  const Memory written[] = {{out, plan->num_tokens * q_row}, {lse, plan->num_tokens * plan->num_heads * 4}, {workspace, plan->workspace_bytes}};
+  const Memory read[] = {{query, (plan->num_tokens - 1) * q_token_stride * 2 + q_row},
+                         {paged_kv_cache, num_pages > 0 ? (num_pages - 1) * page_stride + page : 0},
+                         {plan->buffer, plan->plan_bytes},
+                         {plan->kv_indices, plan->num_kv_indices * 4}};
+  bool apart = true;
+  for (const Memory& w : written) {
+    for (const Memory& r : read) apart = apart && (!w.meets(r) || (&w == written && &r == read && in_place));
+    for (const Memory* x = written; x < &w; ++x) apart = apart && !w.meets(*x);
+  }
+  if (!apart) return fail(KVC_ERR_INVALID_ARG, "%s: what is written overlaps what is read (the output may be the query itself)", fn);
+  AttendArgs a{};
+  a.query = (const char*)query;
+  a.cache = (const char*)paged_kv_cache;
+  a.kv_indices = plan->kv_indices;
+  a.out = (char*)out;
+  a.lse = lse;
+  float* at = (float*)workspace;
+  for (int k = 0; k < 2; ++k) {
+    const int64_t rows = plan->n.max_slots[k] * plan->num_kv_heads * (k ? kWide : kTile);
+    a.partial[k] = at;
+    at += rows * plan->head_dim;
+  }
+  for (int k = 0; k < 2; ++k) {
+    a.partial_lse[k] = at;
+    at += plan->n.max_slots[k] * plan->num_kv_heads * (k ? kWide : kTile);
+  }
+  a.q_stride = q_token_stride * 2;
+  a.page_stride = (uint32_t)page_stride;
+  if (q8) {
+    a.plane = (uint32_t)q8::plane_bytes(plan->num_kv_heads, plan->head_dim);
+    a.group_stride = (uint32_t)group;
+    a.exponents = 2 * a.plane;
+  } else {
+    a.row_stride = (uint32_t)(row * 2);
+    a.plane = (uint32_t)(plan->page_size * row * 2);
+  }
+  a.num_pages = (int32_t)num_pages;
+  a.page_size = (int32_t)plan->page_size;
+  a.page_shift = log2_exact(plan->page_size);
+  a.kv_heads = (int32_t)plan->num_kv_heads;
+  a.group = (int32_t)(plan->num_heads / plan->num_kv_heads);
+  a.head_dim = (int32_t)plan->head_dim;
+  a.narrow_groups = (int32_t)(plan->n.groups * plan->num_kv_heads);
+  // (a workgroup takes further items where there are more than these)
+  a.wide_groups = (int32_t)round_up(std::min<int64_t>(plan->n.max_items[1] * plan->num_kv_heads, 4096), 8);
+  a.max_entries = (int32_t)plan->n.max_entries;
+  a.scale = plan->scale * kLog2e;
+  a.l = layout_of(*plan, plan->buffer, nullptr);
+  if (plan->dtype == KVC_DTYPE_BF16) launch_attend<BF16>(a, *plan, (hipStream_t)stream);
+  else launch_attend<F16>(a, *plan, (hipStream_t)stream);
+  KVC_HIP(hipGetLastError());
+  return KVC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kvc_attention_plan_create(const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* kv_indptr,
+                              const int32_t* kv_last_page_len, int64_t batch_size, int64_t num_tokens,
+                              int64_t num_kv_indices, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                              int64_t page_size, int64_t max_q_len, int64_t shared_pages, float sm_scale, int dtype,
+                              kvc_attention_plan** out) {
+  return create_plan("kvc_attention_plan_create", false, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, batch_size, num_tokens,
+                     num_kv_indices, num_heads, num_kv_heads, head_dim, page_size, max_q_len, shared_pages, sm_scale, dtype, out);
+}
+
+int kvc_attention_plan_create_q8(const int32_t* qo_indptr, const int32_t* kv_indices, const int32_t* kv_indptr,
+                                 const int32_t* kv_last_page_len, int64_t batch_size, int64_t num_tokens,
+                                 int64_t num_kv_indices, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                 int64_t page_size, int64_t max_q_len, int64_t shared_pages, float sm_scale, int dtype,
+                                 kvc_attention_plan** out) {
+  return create_plan("kvc_attention_plan_create_q8", true, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, batch_size, num_tokens,
+                     num_kv_indices, num_heads, num_kv_heads, head_dim, page_size, max_q_len, shared_pages, sm_scale, dtype, out);
 }
 
 int64_t kvc_attention_plan_bytes(const kvc_attention_plan* plan) {
@@ -1482,73 +1561,17 @@ int kvc_attention_plan_build(kvc_attention_plan* plan, void* buffer, int64_t buf
 int kvc_attention_plan_run(const kvc_attention_plan* plan, const void* query, int64_t q_token_stride,
                            const void* paged_kv_cache, int64_t page_stride, int64_t num_pages, void* out, float* lse,
                            void* workspace, int64_t workspace_bytes, void* stream) {
-  constexpr const char* fn = "kvc_attention_plan_run";
-  if (!plan) return fail(KVC_ERR_INVALID_ARG, "%s: null plan", fn);
-  if (plan->batch_size == 0 || plan->num_tokens == 0) return KVC_OK;
-  const int64_t row = plan->num_kv_heads * plan->head_dim, page = 2 * plan->page_size * row;
-  if (!query || !out || !workspace || (num_pages > 0 && !paged_kv_cache))
-    return fail(KVC_ERR_INVALID_ARG, "%s: null pointer", fn);
-  if (num_pages < 0 || num_pages >= (int64_t(1) << 31) || page_stride < page || page_stride * 2 >= (int64_t(1) << 32))
-    return fail(KVC_ERR_INVALID_ARG, "%s: bad cache geometry", fn);
-  if (q_token_stride < plan->num_heads * plan->head_dim)
-    return fail(KVC_ERR_INVALID_ARG, "%s: token stride smaller than a row", fn);
-  if (((uintptr_t)query | (uintptr_t)paged_kv_cache | (uint64_t)q_token_stride * 2 | (uint64_t)page_stride * 2) % 16 ||
-      (uintptr_t)out % 8 || (uintptr_t)lse % 4 || (uintptr_t)workspace % 256)
-    return fail(KVC_ERR_INVALID_ARG, "%s: rows must be aligned to 16 bytes, the output to 8", fn);
-  if (workspace_bytes < plan->workspace_bytes)
-    return fail(KVC_ERR_STAGING, "%s: the workspace needs %lld bytes", fn, (long long)plan->workspace_bytes);
-  if (!plan->buffer) return fail(KVC_ERR_INVALID_ARG, "%s: the plan is not built", fn);
-  // A row of the query is read before the same row of the output is written, and by no one else afterwards; nothing else that
-  // is read or written may share memory with what is written
-  const int64_t q_row = plan->num_heads * plan->head_dim * 2;
-  const bool in_place = out == query && (plan->num_tokens == 1 || q_token_stride * 2 == q_row);
-  const Memory written[] = {{out, plan->num_tokens * q_row}, {lse, plan->num_tokens * plan->num_heads * 4}, {workspace, plan->workspace_bytes}};
-  const Memory read[] = {{query, (plan->num_tokens - 1) * q_token_stride * 2 + q_row},
-                         {paged_kv_cache, num_pages > 0 ? (num_pages - 1) * page_stride * 2 + page * 2 : 0},
-                         {plan->buffer, plan->plan_bytes},
-                         {plan->kv_indices, plan->num_kv_indices * 4}};
-  bool apart = true;
-  for (const Memory& w : written) {
-    for (const Memory& r : read) apart = apart && (!w.meets(r) || (&w == written && &r == read && in_place));
-    for (const Memory* x = written; x < &w; ++x) apart = apart && !w.meets(*x);
-  }
-  if (!apart) return fail(KVC_ERR_INVALID_ARG, "%s: what is written overlaps what is read (the output may be the query itself)", fn);
-  AttendArgs a{};
-  a.query = (const char*)query;
-  a.cache = (const char*)paged_kv_cache;
-  a.kv_indices = plan->kv_indices;
-  a.out = (char*)out;
-  a.lse = lse;
-  float* at = (float*)workspace;
-  for (int k = 0; k < 2; ++k) {
-    const int64_t rows = plan->n.max_slots[k] * plan->num_kv_heads * (k ? kWide : kTile);
-    a.partial[k] = at;
-    at += rows * plan->head_dim;
-  }
-  for (int k = 0; k < 2; ++k) {
-    a.partial_lse[k] = at;
-    at += plan->n.max_slots[k] * plan->num_kv_heads * (k ? kWide : kTile);
-  }
-  a.q_stride = q_token_stride * 2;
-  a.page_stride = (uint32_t)(page_stride * 2);
-  a.row_stride = (uint32_t)(row * 2);
-  a.plane = (uint32_t)(plan->page_size * row * 2);
-  a.num_pages = (int32_t)num_pages;
-  a.page_size = (int32_t)plan->page_size;
-  a.page_shift = log2_exact(plan->page_size);
-  a.kv_heads = (int32_t)plan->num_kv_heads;
-  a.group = (int32_t)(plan->num_heads / plan->num_kv_heads);
-  a.head_dim = (int32_t)plan->head_dim;
-  a.narrow_groups = (int32_t)(plan->n.groups * plan->num_kv_heads);
-  // (a workgroup takes further items where there are more than these)
-  a.wide_groups = (int32_t)round_up(std::min<int64_t>(plan->n.max_items[1] * plan->num_kv_heads, 4096), 8);
-  a.max_entries = (int32_t)plan->n.max_entries;
-  a.scale = plan->scale * kLog2e;
-  a.l = layout_of(*plan, plan->buffer, nullptr);
-  if (plan->dtype == KVC_DTYPE_BF16) launch_attend<BF16>(a, *plan, (hipStream_t)stream);
-  else launch_attend<F16>(a, *plan, (hipStream_t)stream);
-  KVC_HIP(hipGetLastError());
-  return KVC_OK;
+  // (a stride whose bytes would not be a number is too large as it is)
+  const int64_t bytes = page_stride > -(int64_t(1) << 40) && page_stride < int64_t(1) << 40 ? page_stride * 2 : page_stride;
+  return run_plan("kvc_attention_plan_run", false, plan, query, q_token_stride, paged_kv_cache, bytes, num_pages, out, lse, workspace,
+                  workspace_bytes, stream);
+}
+
+int kvc_attention_plan_run_q8(const kvc_attention_plan* plan, const void* query, int64_t q_token_stride,
+                              const void* paged_kv_cache, int64_t page_stride, int64_t num_pages, void* out, float* lse,
+                              void* workspace, int64_t workspace_bytes, void* stream) {
+  return run_plan("kvc_attention_plan_run_q8", true, plan, query, q_token_stride, paged_kv_cache, page_stride, num_pages, out, lse,
+                  workspace, workspace_bytes, stream);
 }
 
 int kvc_attention_plan_destroy(kvc_attention_plan* plan) {
