@@ -57,7 +57,7 @@ KVC_LAUNCH_RUN = 9
 KVC_LAUNCH_THROUGH = 10
 
 KVC_ABI_VERSION = 6
-FAST_INTERFACE = 3      # names and arguments of the `_kvc_fast` extension's functions
+FAST_INTERFACE = 4      # names and arguments of the `_kvc_fast` extension's functions
 KVC_NOALLOC_MAX_BLOCKS = 8192
 
 KVC_DTYPE_BF16 = 0

@@ -87,8 +87,8 @@ class PagedAttentionPlan:
         self._workspace_bytes = lib.kvc_attention_workspace_bytes(self._plan)
         self._stream = _stream_of(self._buffer)      # whose allocator the buffer is from
         self._dev_index = self.device.index
-        fast = None if self.q8 else _lib.fast()
-        self._fast_run = fast.attention_plan_run if fast else None
+        fast = _lib.fast()
+        self._fast_run = (fast.attention_plan_run_q8 if self.q8 else fast.attention_plan_run) if fast else None
         self._dtype_code = fast.scalar_type_code(torch.empty(0, dtype=dtype)) if fast else -1
         self.build()
 
@@ -224,6 +224,17 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: torch.Tensor, qo_indptr
 
 def _paged_attention_q8(query, paged_kv_cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len, shared_pages,
                         sm_scale, out, return_lse, kv_layout, num_kv_heads):
+    fast = _lib.fast_entry("paged_attention")
+    if fast is not None and num_kv_heads is not None and kv_layout == "NHD" and paged_kv_cache.is_cuda and query.dim() == 3:
+        # as for 16 bits
+        dev = paged_kv_cache.device.index
+        got = fast(query, paged_kv_cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len or 0, shared_pages,
+                   (query.shape[2] or 1) ** -0.5 if sm_scale is None else sm_scale, out, return_lse, dev, _raw_stream(dev),
+                   num_kv_heads)
+        if type(got) is not int:
+            return got
+        if got < 0:
+            _lib.check(got)
     for t, n in ((query, "query"), (paged_kv_cache, "paged_kv_cache")):
         _require_gpu(t, n)
     if query.dim() != 3 or num_kv_heads is None:

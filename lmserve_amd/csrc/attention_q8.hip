@@ -44,17 +44,8 @@ __device__ __forceinline__ Item uniform(const Item& x) {
 // 8 codes as 8 numbers, times a power of two
 template <typename T>
 __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi, float by) {
-  if constexpr (std::is_same<T, BF16>::value) {
-    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, by, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, by, true)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, by, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, by, true))};
-  } else {
-    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, by, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, by, true)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, by, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, by, true))};
-  }
+  return u32x4{T::template from_codes<false>(lo, by), T::template from_codes<true>(lo, by), T::template from_codes<false>(hi, by),
+               T::template from_codes<true>(hi, by)};
 }
 // 2^n for n from -126 up, less for a lesser one
 __device__ __forceinline__ float power(int32_t n) { return __uint_as_float((uint32_t)(max(n, -127) + 127) << 23); }

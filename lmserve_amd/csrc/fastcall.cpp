@@ -44,7 +44,7 @@
 namespace {
 
 constexpr long NOT_FAST = 1;
-constexpr long kInterface = 3;  // changes with the names or arguments of the functions below; _lib.py checks it
+constexpr long kInterface = 4;  // changes with the names or arguments of the functions below; _lib.py checks it
 
 bool as_ptr(PyObject* o, void** out) {
   if (o == Py_None) {
@@ -534,8 +534,119 @@ PyObject* fast_rotary_plan_run_norm(PyObject*, PyObject* const* args, Py_ssize_t
   END_HANDLE_TH_ERRORS
 }
 
+// One layer of an 8-bit pool, [num_pages, page_bytes] of bytes: the page stride in bytes, or -1. Rows that it reads are aligned to 16 bytes.
+int64_t q8_stride(const at::Tensor& c, int64_t heads, int64_t dim, int device, int64_t* num_pages, int64_t* page_size) {
+  if (c.scalar_type() != at::kByte || !c.is_cuda() || c.device().index() != device || c.dim() != 2 || heads < 1 || dim < 1) return -1;
+  const int64_t pages = c.sizes()[0], bytes = c.sizes()[1], group = kvc_q8_page_bytes(heads, dim, 16);
+  if (pages < 1 || group < 1 || bytes < group || bytes % group || c.strides()[1] != 1) return -1;
+  const int64_t stride = pages > 1 ? c.strides()[0] : bytes;
+  if (stride < bytes || stride % 16 || (uintptr_t)c.data_ptr() % 16) return -1;
+  *num_pages = pages;
+  *page_size = bytes / group * 16;
+  return stride;
+}
+int64_t aligned_rows(const at::Tensor& t, int64_t n, int64_t width, int dtype, int device) {
+  const int64_t stride = row_stride_at_least(t, n, width, dtype, device);
+  return stride < 0 || (n > 1 && stride % 8) || (uintptr_t)t.data_ptr() % 16 ? -1 : stride;
+}
+
+// The tokens' places: by slots, or by batch_indices, positions, kv_indices, kv_indptr. The number of tokens, or -1.
+struct Places {
+  const at::Tensor* t[4] = {};
+  int slot_bytes = 0;
+  int64_t count(int device) {
+    if (!t[1]) {
+      if (!t[0]) return -1;
+      slot_bytes = t[0]->scalar_type() == at::kLong ? 8 : 4;
+      return index_array(*t[0], device, slot_bytes == 8 ? at::kLong : at::kInt) ? t[0]->sizes()[0] : -1;
+    }
+    for (const at::Tensor* x : t)
+      if (!x || !index_array(*x, device, at::kInt)) return -1;
+    return t[0]->sizes()[0] == t[1]->sizes()[0] && t[3]->sizes()[0] > 0 ? t[0]->sizes()[0] : -1;
+  }
+  int run(bool read, void* k, void* v, void* c, int64_t n, int64_t heads, int64_t dim, int64_t page_size, int64_t ks, int64_t vs, int64_t stride,
+          int64_t pages, int dtype, void* stream) const {
+    const auto i32 = [&](int i) { return (const int32_t*)t[i]->data_ptr(); };
+    if (!t[1])
+      return read ? kvc_read_cache_q8(c, t[0]->data_ptr(), slot_bytes, k, v, n, heads, dim, page_size, ks, vs, stride, pages, dtype, stream)
+                  : kvc_reshape_and_cache_q8(k, v, c, t[0]->data_ptr(), slot_bytes, n, heads, dim, page_size, ks, vs, stride, pages, dtype, stream);
+    const int64_t batch = t[3]->sizes()[0] - 1, ids = t[2]->sizes()[0];
+    return read ? kvc_read_paged_kv_cache_q8(i32(0), i32(1), c, i32(2), i32(3), nullptr, k, v, n, batch, ids, heads, dim, page_size, ks, vs, stride,
+                                             pages, dtype, stream)
+                : kvc_append_paged_kv_cache_q8(k, v, i32(0), i32(1), c, i32(2), i32(3), nullptr, n, batch, ids, heads, dim, page_size, ks, vs,
+                                               stride, pages, dtype, stream);
+  }
+};
+
+/* write_q8(key, value, cache, device, stream, slot_mapping) or (..., batch_indices, positions, kv_indices, kv_indptr):
+ * kvc_reshape_and_cache_q8 or kvc_append_paged_kv_cache_q8 on tensors */
+PyObject* fast_write_q8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 6 && nargs != 9) {
+    PyErr_SetString(PyExc_TypeError, "write_q8 takes 6 or 9 arguments");
+    return nullptr;
+  }
+  int64_t device;
+  void* stream;
+  if (!as_i64(args[3], &device) || !as_ptr(args[4], &stream)) return nullptr;
+  const at::Tensor *k = tensor_of(args[0]), *v = tensor_of(args[1]), *c = tensor_of(args[2]);
+  const int dev = (int)device;
+  Places at;
+  for (int i = 0; i < nargs - 5; ++i)
+    if (!(at.t[i] = tensor_of(args[5 + i]))) return PyLong_FromLong(NOT_FAST);
+  if (!k || !v || !c || k->dim() != 3 || v->dim() < 2 || !on_current_device(dev)) return PyLong_FromLong(NOT_FAST);
+  const int64_t n = at.count(dev), heads = k->sizes()[1], dim = k->sizes()[2], row = heads * dim;
+  const at::ScalarType type = k->scalar_type();
+  if (n < 1 || (type != at::kBFloat16 && type != at::kHalf)) return PyLong_FromLong(NOT_FAST);
+  // (slots are of all rows, index entries may be of fewer)
+  if (nargs == 6 && (k->sizes()[0] != n || v->sizes()[0] != n)) return PyLong_FromLong(NOT_FAST);
+  if (v->dim() == 3 ? v->sizes()[1] != heads || v->sizes()[2] != dim : v->sizes()[1] != row) return PyLong_FromLong(NOT_FAST);
+  int64_t pages, page_size;
+  const int64_t stride = q8_stride(*c, heads, dim, dev, &pages, &page_size), ks = aligned_rows(*k, n, row, (int)type, dev),
+                vs = aligned_rows(*v, n, row, (int)type, dev);
+  if (stride < 0 || ks < 0 || vs < 0) return PyLong_FromLong(NOT_FAST);
+  return PyLong_FromLong(at.run(false, k->data_ptr(), v->data_ptr(), c->data_ptr(), n, heads, dim, page_size, ks, vs, stride, pages,
+                                kvc_dtype_of(type), stream));
+}
+
+/* read_q8(cache, heads, dim, dtype, device, stream, slot_mapping) or (..., batch_indices, positions, kv_indices, kv_indptr)
+ * -> 1, a negative kvc_status or (key, value): kvc_read_cache_q8 or kvc_read_paged_kv_cache_q8 into new tensors */
+PyObject* fast_read_q8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7 && nargs != 10) {
+    PyErr_SetString(PyExc_TypeError, "read_q8 takes 7 or 10 arguments");
+    return nullptr;
+  }
+  int64_t heads, dim, dtype, device;
+  void* stream;
+  if (!as_i64(args[1], &heads) || !as_i64(args[2], &dim) || !as_i64(args[3], &dtype) || !as_i64(args[4], &device) || !as_ptr(args[5], &stream))
+    return nullptr;
+  const at::Tensor* c = tensor_of(args[0]);
+  const int dev = (int)device;
+  Places at;
+  for (int i = 0; i < nargs - 6; ++i)
+    if (!(at.t[i] = tensor_of(args[6 + i]))) return PyLong_FromLong(NOT_FAST);
+  if (!c || !on_current_device(dev)) return PyLong_FromLong(NOT_FAST);
+  const int64_t n = at.count(dev);
+  int64_t pages, page_size;
+  const int64_t stride = q8_stride(*c, heads, dim, dev, &pages, &page_size);
+  if (n < 1 || stride < 0) return PyLong_FromLong(NOT_FAST);
+  const at::ScalarType type = dtype == KVC_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
+  at::Tensor k, v;
+  {
+    pybind11::gil_scoped_release no_lock;  // the allocator may wait
+    const auto options = at::TensorOptions().dtype(type).device(c->device());
+    k = at::empty({n, heads, dim}, options);
+    v = at::empty({n, heads, dim}, options);
+  }
+  const int rc = at.run(true, k.data_ptr(), v.data_ptr(), c->data_ptr(), n, heads, dim, page_size, heads * dim, heads * dim, stride, pages,
+                        (int)dtype, stream);
+  if (rc < 0) return PyLong_FromLong(rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
+  END_HANDLE_TH_ERRORS
+}
+
 // A plan's run into new tensors (or `given`): out, or (out, lse)
-PyObject* attend(const kvc_attention_plan* plan, const at::Tensor& q, int64_t q_stride, int64_t tokens, int64_t q_heads, int64_t dim,
+PyObject* attend(bool q8, const kvc_attention_plan* plan, const at::Tensor& q, int64_t q_stride, int64_t tokens, int64_t q_heads, int64_t dim,
                  const at::Tensor& c, int64_t pages, int64_t stride, const at::Tensor* given, bool with_lse, void* stream) {
   at::Tensor out, lse, work;
   {
@@ -545,15 +656,17 @@ PyObject* attend(const kvc_attention_plan* plan, const at::Tensor& q, int64_t q_
     if (with_lse) lse = at::empty({tokens, q_heads}, on_device.dtype(at::kFloat));
     work = at::empty({kvc_attention_workspace_bytes(plan)}, on_device.dtype(at::kByte));
   }
-  const int rc = kvc_attention_plan_run(plan, q.data_ptr(), q_stride, c.data_ptr(), stride, pages, out.data_ptr(),
-                                        with_lse ? lse.data_ptr<float>() : nullptr, work.data_ptr(), work.numel(), stream);
+  const auto run = q8 ? kvc_attention_plan_run_q8 : kvc_attention_plan_run;
+  const int rc = run(plan, q.data_ptr(), q_stride, c.data_ptr(), stride, pages, out.data_ptr(),
+                     with_lse ? lse.data_ptr<float>() : nullptr, work.data_ptr(), work.numel(), stream);
   if (rc < 0) return PyLong_FromLong(rc);
   if (!with_lse) return THPVariable_Wrap(std::move(out));
   return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
 }
 
 /* attention_plan_run(plan, tokens, q_heads, heads, dim, page_size, dtype, device, query, cache, out | None, return_lse, stream)
- * -> 1, a negative kvc_status, out or (out, lse): kvc_attention_plan_run on tensors */
+ * -> 1, a negative kvc_status, out or (out, lse): kvc_attention_plan_run on tensors (or _run_q8) */
+template <bool Q8>
 PyObject* fast_attention_plan_run(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   void *plan, *stream;
@@ -571,30 +684,32 @@ PyObject* fast_attention_plan_run(PyObject*, PyObject* const* args, Py_ssize_t n
   const at::Tensor* given = args[10] == Py_None ? nullptr : tensor_of(args[10]);
   if (!q || !c || (args[10] != Py_None && !given) || tokens == 0 || !on_current_device((int)device)) return PyLong_FromLong(NOT_FAST);
   const int64_t row = q_heads * dim, qs = row_stride(*q, tokens, row, (int)dtype, (int)device);
-  int64_t pages = 0;
-  const int64_t ps = page_stride(*c, page_size, heads, dim, (int)dtype, (int)device, &pages);
-  if (qs < 0 || ps < 0 || (q->dim() == 3 && q->sizes()[2] != dim) || qs % 8 || (uintptr_t)q->data_ptr() % 16 ||
+  int64_t pages = 0, found = page_size;
+  const int64_t ps = Q8 ? q8_stride(*c, heads, dim, (int)device, &pages, &found) : page_stride(*c, page_size, heads, dim, (int)dtype, (int)device, &pages);
+  if (qs < 0 || ps < 0 || found != page_size || (q->dim() == 3 && q->sizes()[2] != dim) || qs % 8 || (uintptr_t)q->data_ptr() % 16 ||
       (given && (row_stride(*given, tokens, row, (int)dtype, (int)device) != row)))
     return PyLong_FromLong(NOT_FAST);
-  return attend((const kvc_attention_plan*)plan, *q, qs, tokens, q_heads, dim, *c, pages, ps, given, with_lse, stream);
+  return attend(Q8, (const kvc_attention_plan*)plan, *q, qs, tokens, q_heads, dim, *c, pages, ps, given, with_lse, stream);
   END_HANDLE_TH_ERRORS
 }
 
 /* paged_attention(query, cache, qo_indptr, kv_indices, kv_indptr, kv_last_page_len, max_q_len, shared_pages, sm_scale,
- *                 out | None, return_lse, device, stream) -> 1, a negative kvc_status, out or (out, lse): a plan made, built,
+ *                 out | None, return_lse, device, stream[, kv_heads of an 8-bit cache]) -> 1, a negative kvc_status, out or (out, lse): a plan made, built,
  * run once and given back (one request's call through the interpreter 27 us, so the 17 that its two kernels take) */
 PyObject* fast_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   int64_t max_q_len, shared_pages, device;
   float scale;
   void* stream;
-  if (nargs != 13) {
-    PyErr_SetString(PyExc_TypeError, "paged_attention takes 13 arguments");
+  int64_t heads = 0;
+  if (nargs != 13 && nargs != 14) {
+    PyErr_SetString(PyExc_TypeError, "paged_attention takes 13 or 14 arguments");
     return nullptr;
   }
+  const bool q8 = nargs == 14;
   const int with_lse = PyObject_IsTrue(args[10]);
   if (!as_i64(args[6], &max_q_len) || !as_i64(args[7], &shared_pages) || !as_f32(args[8], &scale) || with_lse < 0 ||
-      !as_i64(args[11], &device) || !as_ptr(args[12], &stream))
+      !as_i64(args[11], &device) || !as_ptr(args[12], &stream) || (q8 && !as_i64(args[13], &heads)))
     return nullptr;
   const at::Tensor* t[6];
   for (int i = 0; i < 6; ++i)
@@ -602,23 +717,26 @@ PyObject* fast_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t narg
   const at::Tensor &q = *t[0], &c = *t[1], &qo = *t[2], &ind = *t[3], &ptr = *t[4], &last = *t[5];
   const at::Tensor* given = args[9] == Py_None ? nullptr : tensor_of(args[9]);
   const int dev = (int)device;
-  if ((args[9] != Py_None && !given) || !on_current_device(dev) || c.dim() != 5 || (q.dim() != 2 && q.dim() != 3))
+  if ((args[9] != Py_None && !given) || !on_current_device(dev) || (q8 ? q.dim() != 3 : c.dim() != 5 || (q.dim() != 2 && q.dim() != 3)))
     return PyLong_FromLong(NOT_FAST);
   for (int i = 2; i < 6; ++i)
     if (!index_array(*t[i], dev, at::kInt)) return PyLong_FromLong(NOT_FAST);
   const at::ScalarType type = q.scalar_type();
-  const int64_t batch = last.sizes()[0], tokens = q.sizes()[0], page_size = c.sizes()[2], heads = c.sizes()[3], dim = c.sizes()[4];
+  const int64_t batch = last.sizes()[0], tokens = q.sizes()[0], dim = q8 ? q.sizes()[2] : c.sizes()[4];
+  int64_t page_size = q8 ? 0 : c.sizes()[2];
+  if (!q8) heads = c.sizes()[3];
   const int64_t row = q.dim() == 3 ? q.sizes()[1] * q.sizes()[2] : q.sizes()[1];
   int64_t pages = 0;
-  const int64_t qs = row_stride(q, tokens, row, (int)type, dev), ps = page_stride(c, page_size, heads, dim, (int)type, dev, &pages);
+  const int64_t qs = row_stride(q, tokens, row, (int)type, dev);
+  const int64_t ps = q8 ? q8_stride(c, heads, dim, dev, &pages, &page_size) : page_stride(c, page_size, heads, dim, (int)type, dev, &pages);
   if (kvc_dtype_of(type) < 0 || tokens == 0 || qs < 0 || ps < 0 || dim == 0 || row % dim || (q.dim() == 3 && q.sizes()[2] != dim) ||
       qo.sizes()[0] != batch + 1 || ptr.sizes()[0] != batch + 1 || qs % 8 || (uintptr_t)q.data_ptr() % 16 ||
       (given && row_stride(*given, tokens, row, (int)type, dev) != row))
     return PyLong_FromLong(NOT_FAST);
   kvc_attention_plan* plan = nullptr;
-  int rc = kvc_attention_plan_create((const int32_t*)qo.data_ptr(), (const int32_t*)ind.data_ptr(), (const int32_t*)ptr.data_ptr(),
-                                     (const int32_t*)last.data_ptr(), batch, tokens, ind.sizes()[0], row / dim, heads, dim, page_size,
-                                     max_q_len, shared_pages, scale, kvc_dtype_of(type), &plan);
+  const auto create = q8 ? kvc_attention_plan_create_q8 : kvc_attention_plan_create;
+  int rc = create((const int32_t*)qo.data_ptr(), (const int32_t*)ind.data_ptr(), (const int32_t*)ptr.data_ptr(), (const int32_t*)last.data_ptr(),
+                  batch, tokens, ind.sizes()[0], row / dim, heads, dim, page_size, max_q_len, shared_pages, scale, kvc_dtype_of(type), &plan);
   if (rc < 0) return PyLong_FromLong(rc);
   struct Owner {
     kvc_attention_plan* p;
@@ -631,7 +749,7 @@ PyObject* fast_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t narg
   }
   rc = kvc_attention_plan_build(plan, buffer.data_ptr(), buffer.numel(), stream);
   if (rc < 0) return PyLong_FromLong(rc);
-  return attend(plan, q, qs, tokens, row / dim, dim, c, pages, ps, given, with_lse, stream);
+  return attend(q8, plan, q, qs, tokens, row / dim, dim, c, pages, ps, given, with_lse, stream);
   END_HANDLE_TH_ERRORS
 }
 
@@ -1088,8 +1206,14 @@ PyMethodDef methods[] = {
      "kvc_qk_norm_rotary_pos_emb and its forms on tensors; the outputs, 1 = not the fast layout, or a negative kvc_status."},
     {"rotary_plan_run_norm", (PyCFunction)(void (*)(void))fast_rotary_plan_run_norm, METH_FASTCALL,
      "kvc_rotary_plan_run_norm on tensors; the outputs, 1 = not the fast layout, or a negative kvc_status."},
-    {"attention_plan_run", (PyCFunction)(void (*)(void))fast_attention_plan_run, METH_FASTCALL,
+    {"attention_plan_run", (PyCFunction)(void (*)(void))fast_attention_plan_run<false>, METH_FASTCALL,
      "kvc_attention_plan_run on tensors; the outputs, 1 = not the fast layout, or a negative kvc_status."},
+    {"attention_plan_run_q8", (PyCFunction)(void (*)(void))fast_attention_plan_run<true>, METH_FASTCALL,
+     "kvc_attention_plan_run_q8 on tensors; the outputs, 1 = not the fast layout, or a negative kvc_status."},
+    {"write_q8", (PyCFunction)(void (*)(void))fast_write_q8, METH_FASTCALL,
+     "The write into an 8-bit cache on tensors; 0, 1 = not the fast layout, or a negative kvc_status."},
+    {"read_q8", (PyCFunction)(void (*)(void))fast_read_q8, METH_FASTCALL,
+     "Rows of an 8-bit cache in new tensors; (key, value), 1 = not the fast layout, or a negative kvc_status."},
     {"paged_attention", (PyCFunction)(void (*)(void))fast_paged_attention, METH_FASTCALL,
      "An attention plan made and run once; the outputs, 1 = not the fast layout, or a negative kvc_status."},
     {"build_index", (PyCFunction)(void (*)(void))fast_build_index, METH_FASTCALL,

@@ -34,20 +34,6 @@ __device__ __forceinline__ int32_t exponent_of(float top) {
   return e < kLeast + kBias ? kLeast + kBias : e > kMost + kBias ? kMost + kBias : e;
 }
 
-// Two values to two codes in the lower or the upper half of `old`, rounded to nearest, ties to even
-template <bool UPPER>
-__device__ __forceinline__ uint32_t encode(float x, float y, uint32_t old) {
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, y, (int)old, UPPER);
-}
-__device__ __forceinline__ uint32_t encode(float x0, float x1, float x2, float x3) { return encode<true>(x2, x3, encode<false>(x0, x1, 0)); }
-
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-template <bool UPPER>
-__device__ __forceinline__ f32x2 decode(uint32_t codes) {
-  const auto v = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, UPPER);
-  return f32x2{v[0], v[1]};
-}
-
 // Where a code is NaN: bit 7 of its byte
 __device__ __forceinline__ uint32_t nan_codes(uint32_t codes) { return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 // The bytes of those of 4 codes, from token `first` on, that are among tokens [0, n)

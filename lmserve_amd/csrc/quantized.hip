@@ -30,6 +30,7 @@ using namespace kvc::q8;
 
 constexpr int kThreads = 256, kWavesPerGroup = kThreads / 64;
 constexpr int kChunk = 16;  // tokens of a workgroup
+constexpr int64_t kPastBytes = int64_t(64) << 20;  // rows that are read into more than this
 
 struct Args {
   char *key, *value;  // rows, read or written
@@ -98,35 +99,27 @@ __device__ __forceinline__ float largest(const uint32_t (&words)[N], bool& odd) 
   return T::wide(one);
 }
 
-// The group's exponent, stored, when tokens up to `top` join those before `first`; how far it has grown
-__device__ __forceinline__ int32_t grow(const Run& r, uint32_t at, float top, int32_t& grown) {
+// The group's exponent, stored, when tokens up to `top` join those before `first`, which had `had`; how far it has grown
+__device__ __forceinline__ int32_t grow(const Run& r, int32_t had, float top, int32_t& grown) {
   const int32_t need = exponent_of(top);
-  grown = 0;
-  if (r.first == 0) return need;
-  const int32_t had = min(max((int32_t)*reinterpret_cast<const uint8_t*>(r.group + at), kLeast + kBias), kMost + kBias);
-  if (need > had) grown = need - had;
+  had = r.first == 0 ? 0 : min(max(had, kLeast + kBias), kMost + kBias);
+  grown = r.first && need > had ? need - had : 0;
   return max(need, had);
 }
-// 2^-n for what the codes of a group are scaled by that has grown by n
-__device__ __forceinline__ float shrink_of(int32_t n) { return n < 64 ? __uint_as_float((uint32_t)(kBias - n) << 23) : 0.f; }
 
-__device__ __forceinline__ uint32_t rescaled(uint32_t codes, float by) {
-  const f32x2 lo = decode<false>(codes), hi = decode<true>(codes);
-  const uint32_t odd = (nan_codes(codes) >> 7) * 0xffu;
-  return (encode(lo[0] * by, lo[1] * by, hi[0] * by, hi[1] * by) & ~odd) | (0x7f7f7f7fu & odd);
+// Codes of a group that has grown by 2^n, rounded again (exact up to there: codes are numbers of f16); NaN stays
+__device__ __forceinline__ uint32_t rescaled(uint32_t codes, int32_t n) {
+  const float scale = power_of((uint32_t)(kBias + min(n, 64)));
+  const uint32_t lo = F16::from_codes<false>(codes, 1.f), hi = F16::from_codes<true>(codes, 1.f);
+  const uint32_t c = F16::to_codes<true>(hi, scale, F16::to_codes<false>(lo, scale, 0));
+  return c & ~nan_codes(c);
 }
 
-// Codes of 4 values, two to a word; an infinity or NaN is NaN
+// Codes of 4 values, two to a word; an infinity or NaN is the positive NaN
 template <typename T>
-__device__ __forceinline__ uint32_t codes_of(uint32_t x, uint32_t y, float by, bool odd) {
-  uint32_t c = encode(T::wide(x & 0xffffu) * by, T::wide(x >> 16) * by, T::wide(y & 0xffffu) * by, T::wide(y >> 16) * by);
-  if (odd) {
-    const uint32_t v[4] = {x & 0x7fffu, x >> 16 & 0x7fffu, y & 0x7fffu, y >> 16 & 0x7fffu};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (v[e] >= T::kExponent) c = (c & ~(0xffu << e * 8)) | 0x7fu << e * 8;
-  }
-  return c;
+__device__ __forceinline__ uint32_t codes_of(uint32_t x, uint32_t y, float scale, bool odd) {
+  const uint32_t c = T::template to_codes<true>(y, scale, T::template to_codes<false>(x, scale, 0));
+  return odd ? c & ~nan_codes(c) : c;
 }
 
 // LPR: lanes to a row of 16-byte vectors
@@ -142,6 +135,8 @@ struct Head {
     const bool there = col * 8 < D;
     const char* from = a.key + r.token * a.k_stride + ((int64_t)h * D + col * 8) * 2;
     char* const to = r.group + h * kGroup * D + col / 2 * 64 + col % 2 * 8;
+    uint8_t* const exponent = reinterpret_cast<uint8_t*>(r.group + 2 * kGroup * a.heads * D + 2 * h);
+    const int32_t had = *exponent;
     uint32_t x[PASSES * 4] = {};
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
@@ -155,67 +150,72 @@ struct Head {
     bool odd;
     int32_t grown;
     const float top = largest<T>(x, odd);
-    const uint32_t at = 2 * kGroup * a.heads * D + 2 * h;
-    const int32_t e = grow(r, at, top, grown);
-    const float by = power_of(2 * kBias - e), old_by = shrink_of(grown);
+    const int32_t e = grow(r, had, top, grown);
+    const float scale = power_of(e);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int32_t t = p * RPP + row;
       u32x2* const tile = reinterpret_cast<u32x2*>(to + t / 4 * (4 * D) + t % 4 * 16);
       if (!there || t >= r.end) continue;
       if (t >= r.first) {
-        *tile = u32x2{codes_of<T>(x[p * 4], x[p * 4 + 1], by, odd), codes_of<T>(x[p * 4 + 2], x[p * 4 + 3], by, odd)};
+        *tile = u32x2{codes_of<T>(x[p * 4], x[p * 4 + 1], scale, odd), codes_of<T>(x[p * 4 + 2], x[p * 4 + 3], scale, odd)};
       } else if (grown) {
         const u32x2 c = *tile;
-        *tile = u32x2{rescaled(c[0], old_by), rescaled(c[1], old_by)};
+        *tile = u32x2{rescaled(c[0], grown), rescaled(c[1], grown)};
       }
     }
-    if (lane == 0) *reinterpret_cast<uint8_t*>(r.group + at) = (uint8_t)e;
+    if (lane == 0) *exponent = (uint8_t)e;
   }
 
   static __device__ __forceinline__ void write_v(const Args& a, const Run& r, int32_t h, int32_t lane) {
     const int32_t D = a.dim, t0 = TPL == 8 ? lane / 32 * 8 : 0, pair = TPL == 8 ? lane % 32 : lane;
     const char* from = a.value + r.token * a.v_stride + ((int64_t)h * D + pair * 2) * 2;
     char* const to = r.group + kGroup * a.heads * D + (int64_t)h * kGroup * D + pair * 2 * kGroup + t0;
-    uint32_t x[COLUMNS * TPL] = {};
+    uint8_t* const exponent = reinterpret_cast<uint8_t*>(r.group + 2 * kGroup * a.heads * D + 2 * h + 1);
+    const int32_t had = *exponent;
+    const bool whole = r.first == 0 && r.end == kGroup;
+    uint32_t x[COLUMNS * TPL] = {}, old[COLUMNS][2][WORDS] = {};
 #pragma unroll
-    for (int i = 0; i < TPL; ++i) {
-      const int32_t t = t0 + i;
+    for (int c = 0; c < COLUMNS; ++c)
+      if ((c * 64 + pair) * 2 < D) {
+        if (whole) {
 #pragma unroll
-      for (int c = 0; c < COLUMNS; ++c)
-        if (t >= r.first && t < r.end && (c * 64 + pair) * 2 < D)
-          x[c * TPL + i] = *reinterpret_cast<const uint32_t*>(from + (t - r.first) * a.v_stride + c * 256);
-    }
+          for (int i = 0; i < TPL; ++i) x[c * TPL + i] = *reinterpret_cast<const uint32_t*>(from + (t0 + i) * a.v_stride + c * 256);
+        } else {
+#pragma unroll
+          for (int i = 0; i < TPL; ++i)
+            if (t0 + i >= r.first && t0 + i < r.end)
+              x[c * TPL + i] = *reinterpret_cast<const uint32_t*>(from + (t0 + i - r.first) * a.v_stride + c * 256);
+#pragma unroll
+          for (int d = 0; d < 2; ++d) load(reinterpret_cast<const uint32_t*>(to + c * 128 * kGroup + d * kGroup), old[c][d]);
+        }
+      }
     bool odd;
     int32_t grown;
     const float top = largest<T>(x, odd);
-    const uint32_t at = 2 * kGroup * a.heads * D + 2 * h + 1;
-    const int32_t e = grow(r, at, top, grown);
-    const float by = power_of(2 * kBias - e), old_by = shrink_of(grown);
-    const bool whole = r.first == 0 && r.end == kGroup;
+    const int32_t e = grow(r, had, top, grown);
+    const float scale = power_of(e);
 #pragma unroll
     for (int c = 0; c < COLUMNS; ++c) {
       if ((c * 64 + pair) * 2 >= D) continue;
 #pragma unroll
       for (int d = 0; d < 2; ++d) {
-        uint32_t* const tile = reinterpret_cast<uint32_t*>(to + c * 128 * kGroup + d * kGroup);
-        uint32_t old[WORDS] = {}, now[WORDS];
-        if (!whole) load(tile, old);
+        uint32_t now[WORDS];
 #pragma unroll
         for (int w = 0; w < WORDS; ++w) {
           const uint32_t* y = x + c * TPL + w * 4;
-          const auto two = [&](int i) { return d ? (y[i] >> 16) | (y[i + 1] & 0xffff0000u) : (y[i] & 0xffffu) | y[i + 1] << 16; };
-          now[w] = codes_of<T>(two(0), two(2), by, odd);
+          const auto two = [&](int i) { return __builtin_amdgcn_perm(y[i + 1], y[i], d ? 0x07060302u : 0x05040100u); };
+          now[w] = codes_of<T>(two(0), two(2), scale, odd);
           if (!whole) {
             const uint32_t before = bytes_below(r.first, t0 + w * 4), until = bytes_below(r.end, t0 + w * 4);
-            const uint32_t kept = grown ? rescaled(old[w], old_by) : old[w];
-            now[w] = (kept & before) | (now[w] & until & ~before) | (old[w] & ~until);
+            const uint32_t kept = grown ? rescaled(old[c][d][w], grown) : old[c][d][w];
+            now[w] = (kept & before) | (now[w] & until & ~before) | (old[c][d][w] & ~until);
           }
         }
-        store(tile, now);
+        store(reinterpret_cast<uint32_t*>(to + c * 128 * kGroup + d * kGroup), now);
       }
     }
-    if (lane == 0) *reinterpret_cast<uint8_t*>(r.group + at) = (uint8_t)e;
+    if (lane == 0) *exponent = (uint8_t)e;
   }
 
   static __device__ __forceinline__ void load(const uint32_t* p, uint32_t (&v)[WORDS]) {
@@ -231,34 +231,41 @@ struct Head {
     if constexpr (WORDS == 4) *reinterpret_cast<u32x4*>(p) = u32x4{v[0], v[1], v[2], v[3]};
     else *reinterpret_cast<u32x2*>(p) = u32x2{v[0], v[1]};
   }
+  template <typename V>
+  static __device__ __forceinline__ void put(char* p, V v, bool past) {
+    if (past) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+    else *reinterpret_cast<V*>(p) = v;
+  }
 
+  static __device__ __forceinline__ float scale_at(const char* exponent) {
+    return power_of(max((uint32_t)*reinterpret_cast<const uint8_t*>(exponent), 1u));
+  }
+
+  template <bool PAST>
   static __device__ __forceinline__ void read_k(const Args& a, const Run& r, int32_t h, int32_t lane) {
     const int32_t row = lane / LPR, col = lane % LPR, D = a.dim;
     if (col * 8 >= D) return;
     const char* const from = r.group + h * kGroup * D + col / 2 * 64 + col % 2 * 8;
     char* to = a.key + r.token * a.k_stride + ((int64_t)h * D + col * 8) * 2;
-    const float by = power_of(max((uint32_t)*reinterpret_cast<const uint8_t*>(r.group + 2 * kGroup * a.heads * D + 2 * h), 1u));
+    const float by = scale_at(r.group + 2 * kGroup * a.heads * D + 2 * h);
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       const int32_t t = p * RPP + row;
       if (t < r.first || t >= r.end) continue;
       const u32x2 c = *reinterpret_cast<const u32x2*>(from + t / 4 * (4 * D) + t % 4 * 16);
-      u32x4 v;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const f32x2 lo = decode<false>(c[w]), hi = decode<true>(c[w]);
-        v[w * 2] = T::pack(lo[0] * by, lo[1] * by);
-        v[w * 2 + 1] = T::pack(hi[0] * by, hi[1] * by);
-      }
-      *reinterpret_cast<u32x4*>(to + (t - r.first) * a.k_stride) = v;
+      put(to + (t - r.first) * a.k_stride,
+          u32x4{T::template from_codes<false>(c[0], by), T::template from_codes<true>(c[0], by), T::template from_codes<false>(c[1], by),
+                T::template from_codes<true>(c[1], by)},
+          PAST);
     }
   }
 
+  template <bool PAST>
   static __device__ __forceinline__ void read_v(const Args& a, const Run& r, int32_t h, int32_t lane) {
     const int32_t D = a.dim, t0 = TPL == 8 ? lane / 32 * 8 : 0, pair = TPL == 8 ? lane % 32 : lane;
     char* to = a.value + r.token * a.v_stride + ((int64_t)h * D + pair * 2) * 2;
     const char* const from = r.group + kGroup * a.heads * D + (int64_t)h * kGroup * D + pair * 2 * kGroup + t0;
-    const float by = power_of(max((uint32_t)*reinterpret_cast<const uint8_t*>(r.group + 2 * kGroup * a.heads * D + 2 * h + 1), 1u));
+    const float by = scale_at(r.group + 2 * kGroup * a.heads * D + 2 * h + 1);
 #pragma unroll
     for (int c = 0; c < COLUMNS; ++c) {
       if ((c * 64 + pair) * 2 >= D) continue;
@@ -267,19 +274,23 @@ struct Head {
       for (int d = 0; d < 2; ++d) load(reinterpret_cast<const uint32_t*>(from + c * 128 * kGroup + d * kGroup), x[d]);
 #pragma unroll
       for (int w = 0; w < WORDS; ++w) {
-        const f32x2 even[2] = {decode<false>(x[0][w]), decode<true>(x[0][w])}, odd[2] = {decode<false>(x[1][w]), decode<true>(x[1][w])};
+        // tokens 2 i and 2 i + 1 of both columns
+        const uint32_t column[2][2] = {{T::template from_codes<false>(x[0][w], by), T::template from_codes<true>(x[0][w], by)},
+                                       {T::template from_codes<false>(x[1][w], by), T::template from_codes<true>(x[1][w], by)}};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int32_t t = t0 + w * 4 + i;
           if (t >= r.first && t < r.end)
-            *reinterpret_cast<uint32_t*>(to + (t - r.first) * a.v_stride + c * 256) = T::pack(even[i / 2][i % 2] * by, odd[i / 2][i % 2] * by);
+            put(to + (t - r.first) * a.v_stride + c * 256,
+                (uint32_t)__builtin_amdgcn_perm(column[1][i / 2], column[0][i / 2], i % 2 ? 0x07060302u : 0x05040100u), PAST);
         }
       }
     }
   }
 };
 
-template <typename T, int LPR, bool READ>
+enum Way : int { kWrite, kRead, kReadPast };
+template <typename T, int LPR, Way WAY>
 __global__ __launch_bounds__(kThreads) void rows_kernel(Args a) {
   const int32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int64_t chunk = blockIdx.x / a.splits;
@@ -305,9 +316,9 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Args a) {
     r.token = chunk * kChunk - 1 + first;
     r.first = entry % kGroup;
     r.end = r.first + 1 + __builtin_ctz(~(continues >> (first + 1)));
-    if constexpr (READ) {
-      if (rest & 1) Head<T, LPR>::read_v(a, r, rest >> 1, lane);
-      else Head<T, LPR>::read_k(a, r, rest >> 1, lane);
+    if constexpr (WAY != kWrite) {
+      if (rest & 1) Head<T, LPR>::template read_v<WAY == kReadPast>(a, r, rest >> 1, lane);
+      else Head<T, LPR>::template read_k<WAY == kReadPast>(a, r, rest >> 1, lane);
     } else {
       if (rest & 1) Head<T, LPR>::write_v(a, r, rest >> 1, lane);
       else Head<T, LPR>::write_k(a, r, rest >> 1, lane);
@@ -315,11 +326,11 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Args a) {
   }
 }
 
-template <typename T, bool READ>
+template <typename T, Way WAY>
 void launch_rows(const Args& a, unsigned grid, hipStream_t s) {
-  if (a.dim <= 64) kvc::launch((rows_kernel<T, 8, READ>), dim3(grid), dim3(kThreads), 0, s, a);
-  else if (a.dim <= 128) kvc::launch((rows_kernel<T, 16, READ>), dim3(grid), dim3(kThreads), 0, s, a);
-  else kvc::launch((rows_kernel<T, 32, READ>), dim3(grid), dim3(kThreads), 0, s, a);
+  if (a.dim <= 64) kvc::launch((rows_kernel<T, 8, WAY>), dim3(grid), dim3(kThreads), 0, s, a);
+  else if (a.dim <= 128) kvc::launch((rows_kernel<T, 16, WAY>), dim3(grid), dim3(kThreads), 0, s, a);
+  else kvc::launch((rows_kernel<T, 32, WAY>), dim3(grid), dim3(kThreads), 0, s, a);
 }
 
 int check_geometry(const char* fn, int64_t heads, int64_t dim, int64_t page_size) {
@@ -381,8 +392,10 @@ int run_rows(const char* fn, bool read, const void* key, const void* value, void
          (uint32_t)group_bytes(heads, dim)};
   const unsigned grid = (unsigned)(chunks * splits);
   hipStream_t s = (hipStream_t)stream;
-  if (read) dtype == KVC_DTYPE_BF16 ? launch_rows<BF16, true>(a, grid, s) : launch_rows<F16, true>(a, grid, s);
-  else dtype == KVC_DTYPE_BF16 ? launch_rows<BF16, false>(a, grid, s) : launch_rows<F16, false>(a, grid, s);
+  const bool bf16 = dtype == KVC_DTYPE_BF16, past = read && num_tokens * row * 4 >= kPastBytes;
+  if (past) bf16 ? launch_rows<BF16, kReadPast>(a, grid, s) : launch_rows<F16, kReadPast>(a, grid, s);
+  else if (read) bf16 ? launch_rows<BF16, kRead>(a, grid, s) : launch_rows<F16, kRead>(a, grid, s);
+  else bf16 ? launch_rows<BF16, kWrite>(a, grid, s) : launch_rows<F16, kWrite>(a, grid, s);
   KVC_HIP(hipGetLastError());
   return KVC_OK;
 }

@@ -29,6 +29,17 @@ struct BF16 {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2));
   }
   static __device__ __forceinline__ float wide(uint32_t half) { return __uint_as_float(half << 16); }
+  // e4m3 codes, two at a time, from and to the lower or upper half of a word: times, and divided by, a power of two, rounded once. (An infinity becomes NaN.)
+  template <bool UPPER>
+  static __device__ __forceinline__ uint32_t from_codes(uint32_t codes, float by) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, by, UPPER));
+  }
+  template <bool UPPER>
+  static __device__ __forceinline__ uint32_t to_codes(uint32_t two, float scale, uint32_t old) {
+    typedef short s2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(__builtin_bit_cast(s2, old), __builtin_bit_cast(b2, two), scale, UPPER));
+  }
   static constexpr uint32_t kExponent = 0x7f80u;
   static constexpr float kScaledUp = 0;
 };
@@ -47,6 +58,16 @@ struct F16 {
   }
   static __device__ __forceinline__ float wide(uint32_t half) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)half);
+  }
+  template <bool UPPER>
+  static __device__ __forceinline__ uint32_t from_codes(uint32_t codes, float by) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, by, UPPER));
+  }
+  template <bool UPPER>
+  static __device__ __forceinline__ uint32_t to_codes(uint32_t two, float scale, uint32_t old) {
+    typedef short s2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(s2, old), __builtin_bit_cast(h2, two), scale, UPPER));
   }
   static constexpr uint32_t kExponent = 0x7c00u;
   // log2 of what weights are scaled up by, so that small ones, of which there may be many, are numbers of the type: a weight of 1 is

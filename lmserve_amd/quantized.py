@@ -26,6 +26,9 @@ from .paged import _paged_common
 from .rotary import _DTYPES
 
 GROUP = 16      # tokens that share an exponent
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_fast_entry = _lib.fast_entry
+_READ_DTYPES = {torch.bfloat16: _lib.KVC_DTYPE_BF16, torch.float16: _lib.KVC_DTYPE_F16}
 
 
 def q8_page_bytes(num_kv_heads: int, head_dim: int, page_size: int) -> int:
@@ -112,6 +115,15 @@ def reshape_and_cache_q8(key: torch.Tensor, value: torch.Tensor, kv_cache: torch
     key, value: `[T, H, D]`, bf16 or f16 (rows may be slices of a fused projection); kv_cache: uint8
     `[num_blocks, block_bytes]`, `kv_caches[l]` of the pool; slot_mapping: `[T]` int32/int64 on the device.
     """
+    fast = _fast_entry("write_q8")
+    if fast is not None and isinstance(kv_cache, torch.Tensor) and kv_cache.is_cuda:
+        # common layouts: checked and launched from C++ (1 = not one of them: fall through)
+        dev = kv_cache.device.index
+        rc = fast(key, value, kv_cache, dev, _raw_stream(dev), slot_mapping)
+        if rc == 0:
+            return
+        if rc < 0:
+            _lib.check(rc)
     H, D = _heads_of(key, "key")
     pages, page_size, stride = _pages(kv_cache, H, D, "kv_cache")
     _require_gpu(slot_mapping, "slot_mapping")
@@ -136,6 +148,16 @@ def append_paged_kv_cache_q8(append_key: torch.Tensor, append_value: torch.Tenso
                              kv_indptr: torch.Tensor, kv_last_page_len: torch.Tensor, kv_layout: str = "NHD") -> None:
     """`append_paged_kv_cache` into one layer of an 8-bit pool, `[num_pages, page_bytes]` of uint8: token `i` to
     place `p % page_size` of page `kv_indices[kv_indptr[b] + p // page_size]`, `b = batch_indices[i]`, `p = positions[i]`."""
+    fast = _fast_entry("write_q8")
+    if fast is not None and kv_layout == "NHD" and isinstance(paged_kv_cache, torch.Tensor) and paged_kv_cache.is_cuda \
+            and kv_last_page_len.is_cuda and kv_last_page_len.dtype == torch.int32:
+        # common layouts: checked and launched from C++ (1 = not one of them: fall through)
+        dev = paged_kv_cache.device.index
+        rc = fast(append_key, append_value, paged_kv_cache, dev, _raw_stream(dev), batch_indices, positions, kv_indices, kv_indptr)
+        if rc == 0:
+            return
+        if rc < 0:
+            _lib.check(rc)
     H, D = _heads_of(append_key, "append_key")
     pages, page_size, stride = _pages(paged_kv_cache, H, D, "paged_kv_cache")
     batch_indices, positions, kv_indices, kv_indptr, kv_last_page_len = _paged_common(
@@ -177,6 +199,15 @@ def read_cache_q8(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, num_kv_hea
     the way back of `reshape_and_cache_q8`, slots in any order. `key` / `value` may be buffers of the
     caller's; rows of slots outside the cache are left as they were."""
     H, D = int(num_kv_heads), int(head_dim)
+    fast = _fast_entry("read_q8")
+    if fast is not None and key is None and value is None and dtype in _READ_DTYPES and kv_cache.is_cuda:
+        # common layouts: checked and launched from C++ (1 = not one of them: fall through)
+        dev = kv_cache.device.index
+        got = fast(kv_cache, H, D, _READ_DTYPES[dtype], dev, _raw_stream(dev), slot_mapping)
+        if type(got) is not int:
+            return got
+        if got < 0:
+            _lib.check(got)
     pages, page_size, stride = _pages(kv_cache, H, D, "kv_cache")
     _require_gpu(slot_mapping, "slot_mapping")
     slot_mapping, slot_bytes = _slot_args(slot_mapping)
@@ -199,6 +230,16 @@ def read_paged_kv_cache_q8(batch_indices: torch.Tensor, positions: torch.Tensor,
                            kv_layout: str = "NHD") -> Tuple[torch.Tensor, torch.Tensor]:
     """`read_cache_q8` by the page table: the way back of `append_paged_kv_cache_q8`, tokens in any order."""
     H, D = int(num_kv_heads), int(head_dim)
+    fast = _fast_entry("read_q8")
+    if fast is not None and kv_layout == "NHD" and key is None and value is None and dtype in _READ_DTYPES and paged_kv_cache.is_cuda \
+            and kv_last_page_len.is_cuda and kv_last_page_len.dtype == torch.int32:
+        # common layouts: checked and launched from C++ (1 = not one of them: fall through)
+        dev = paged_kv_cache.device.index
+        got = fast(paged_kv_cache, H, D, _READ_DTYPES[dtype], dev, _raw_stream(dev), batch_indices, positions, kv_indices, kv_indptr)
+        if type(got) is not int:
+            return got
+        if got < 0:
+            _lib.check(got)
     pages, page_size, stride = _pages(paged_kv_cache, H, D, "paged_kv_cache")
     batch_indices, positions, kv_indices, kv_indptr, kv_last_page_len = _paged_common(
         None, None, batch_indices, positions, kv_indices, kv_indptr, kv_last_page_len, kv_layout)
