@@ -37,6 +37,10 @@ __device__ __forceinline__ void st_through_nt(char* p, u32x4 v) {
   asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" ::"v"(p), "v"(v) : "memory");
 }
 
+__device__ __forceinline__ void st_through_nt(char* p, uint32_t v) {
+  asm volatile("global_store_dword %0, %1, off sc1 nt" ::"v"(p), "v"(v) : "memory");
+}
+
 // A kernel launch whose arguments go straight to the runtime. The launch by <<<>>> and its macro first store the
 // configuration for a host stub that fetches it again, 0.1 to 0.15 us of the 2.3 a launch costs, and a launch per layer at
 // decode sizes is bound by that. Errors are in hipGetLastError, as with the macro.

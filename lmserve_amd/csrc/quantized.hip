@@ -30,7 +30,11 @@ using namespace kvc::q8;
 
 constexpr int kThreads = 256, kWavesPerGroup = kThreads / 64;
 constexpr int kChunk = 16;  // tokens of a workgroup
-constexpr int64_t kPastBytes = int64_t(64) << 20;  // rows that are read into more than this
+// Rows beyond so many bytes go past the caches. What is read back: stores past them (8 heads of 128, 8192 tokens, 32 MiB of rows, 10.7 us without and
+// 9.4 so, 32768 43.4 and 31.2, 131001 158 and 144); what is written: loads (32768 tokens, 128 MiB of rows, 42.6 us without and 36.7 so, 65536 82
+// and 69; 16384 18.6 and 20.9, whose rows a projection before them leaves in the caches). The codes are stored plainly, through the
+// caches they cost 23 us at 16384.
+constexpr int64_t kReadPastBytes = int64_t(32) << 20, kWritePastBytes = int64_t(128) << 20;
 
 struct Args {
   char *key, *value;  // rows, read or written
@@ -40,8 +44,8 @@ struct Args {
   const int32_t *batch_indices, *positions, *kv_indices, *kv_indptr;
   int64_t num_tokens, num_slots;
   int32_t slot_bytes, batch_size, num_kv_indices, num_pages, page_size, page_shift;
-  int32_t heads, dim, splits;
-  uint32_t page_stride, group_stride;
+  int32_t heads, dim;
+  uint32_t splits, page_stride, group_stride;
 };
 
 // A token's place in the cache, page * page_size + entry, or -1: none
@@ -130,6 +134,7 @@ struct Head {
   static constexpr int COLUMNS = LPR == 32 ? 2 : 1;     // pairs of columns of a lane
   static constexpr int WORDS = TPL / 4;
 
+  template <bool PAST>
   static __device__ __forceinline__ void write_k(const Args& a, const Run& r, int32_t h, int32_t lane) {
     const int32_t row = lane / LPR, col = lane % LPR, D = a.dim;
     const bool there = col * 8 < D;
@@ -142,7 +147,7 @@ struct Head {
     for (int p = 0; p < PASSES; ++p) {
       const int32_t t = p * RPP + row;
       if (there && t >= r.first && t < r.end) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(from + (t - r.first) * a.k_stride);
+        const u32x4 v = get<PAST, u32x4>(from + (t - r.first) * a.k_stride);
 #pragma unroll
         for (int w = 0; w < 4; ++w) x[p * 4 + w] = v[w];
       }
@@ -167,6 +172,7 @@ struct Head {
     if (lane == 0) *exponent = (uint8_t)e;
   }
 
+  template <bool PAST>
   static __device__ __forceinline__ void write_v(const Args& a, const Run& r, int32_t h, int32_t lane) {
     const int32_t D = a.dim, t0 = TPL == 8 ? lane / 32 * 8 : 0, pair = TPL == 8 ? lane % 32 : lane;
     const char* from = a.value + r.token * a.v_stride + ((int64_t)h * D + pair * 2) * 2;
@@ -180,12 +186,12 @@ struct Head {
       if ((c * 64 + pair) * 2 < D) {
         if (whole) {
 #pragma unroll
-          for (int i = 0; i < TPL; ++i) x[c * TPL + i] = *reinterpret_cast<const uint32_t*>(from + (t0 + i) * a.v_stride + c * 256);
+          for (int i = 0; i < TPL; ++i) x[c * TPL + i] = get<PAST, uint32_t>(from + (t0 + i) * a.v_stride + c * 256);
         } else {
 #pragma unroll
           for (int i = 0; i < TPL; ++i)
             if (t0 + i >= r.first && t0 + i < r.end)
-              x[c * TPL + i] = *reinterpret_cast<const uint32_t*>(from + (t0 + i - r.first) * a.v_stride + c * 256);
+              x[c * TPL + i] = get<PAST, uint32_t>(from + (t0 + i - r.first) * a.v_stride + c * 256);
 #pragma unroll
           for (int d = 0; d < 2; ++d) load(reinterpret_cast<const uint32_t*>(to + c * 128 * kGroup + d * kGroup), old[c][d]);
         }
@@ -231,10 +237,15 @@ struct Head {
     if constexpr (WORDS == 4) *reinterpret_cast<u32x4*>(p) = u32x4{v[0], v[1], v[2], v[3]};
     else *reinterpret_cast<u32x2*>(p) = u32x2{v[0], v[1]};
   }
-  template <typename V>
-  static __device__ __forceinline__ void put(char* p, V v, bool past) {
-    if (past) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+  template <bool PAST, typename V>
+  static __device__ __forceinline__ void put(char* p, V v) {
+    if constexpr (PAST) st_through_nt(p, v);
     else *reinterpret_cast<V*>(p) = v;
+  }
+  template <bool PAST, typename V>
+  static __device__ __forceinline__ V get(const char* p) {
+    if constexpr (PAST) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    else return *reinterpret_cast<const V*>(p);
   }
 
   static __device__ __forceinline__ float scale_at(const char* exponent) {
@@ -253,10 +264,9 @@ struct Head {
       const int32_t t = p * RPP + row;
       if (t < r.first || t >= r.end) continue;
       const u32x2 c = *reinterpret_cast<const u32x2*>(from + t / 4 * (4 * D) + t % 4 * 16);
-      put(to + (t - r.first) * a.k_stride,
-          u32x4{T::template from_codes<false>(c[0], by), T::template from_codes<true>(c[0], by), T::template from_codes<false>(c[1], by),
-                T::template from_codes<true>(c[1], by)},
-          PAST);
+      put<PAST>(to + (t - r.first) * a.k_stride,
+                u32x4{T::template from_codes<false>(c[0], by), T::template from_codes<true>(c[0], by), T::template from_codes<false>(c[1], by),
+                      T::template from_codes<true>(c[1], by)});
     }
   }
 
@@ -281,19 +291,23 @@ struct Head {
         for (int i = 0; i < 4; ++i) {
           const int32_t t = t0 + w * 4 + i;
           if (t >= r.first && t < r.end)
-            put(to + (t - r.first) * a.v_stride + c * 256,
-                (uint32_t)__builtin_amdgcn_perm(column[1][i / 2], column[0][i / 2], i % 2 ? 0x07060302u : 0x05040100u), PAST);
+            put<PAST>(to + (t - r.first) * a.v_stride + c * 256,
+                      (uint32_t)__builtin_amdgcn_perm(column[1][i / 2], column[0][i / 2], i % 2 ? 0x07060302u : 0x05040100u));
         }
       }
     }
   }
 };
 
-enum Way : int { kWrite, kRead, kReadPast };
+enum Way : int { kWrite, kWritePast, kRead, kReadPast };
 template <typename T, int LPR, Way WAY>
 __global__ __launch_bounds__(kThreads) void rows_kernel(Args a) {
   const int32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t chunk = blockIdx.x / a.splits;
+  // The workgroups of 16 tokens on one XCD, of 8 that take such runs of workgroups in turn (16384 tokens written 19.7 us in the plain order, 18.1 so)
+  const uint32_t turn = 8 * a.splits, whole = gridDim.x / turn * turn, in = blockIdx.x / 8;
+  const bool dealt = blockIdx.x < whole;
+  const int64_t chunk = dealt ? in / a.splits * 8 + blockIdx.x % 8 : blockIdx.x / a.splits;
+  const int32_t split = dealt ? in % a.splits : blockIdx.x % a.splits;
   const int32_t waves = a.splits * kWavesPerGroup;
   // the 16 tokens are lanes 1 to 16; the one before them, and those behind them that their groups may reach
   const int64_t slot = lane < 2 * kChunk ? slot_of(a, chunk * kChunk - 1 + lane) : -1;
@@ -303,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Args a) {
   uint32_t opens = (uint32_t)__ballot(lane >= 1 && lane <= kChunk && slot >= 0 && !follows);
   const int32_t tasks = __popc(opens) * a.heads * 2;
   int32_t at = 0;
-  for (int32_t i = (int32_t)(blockIdx.x % a.splits) * kWavesPerGroup + wave; i < tasks; i += waves) {
+  for (int32_t i = split * kWavesPerGroup + wave; i < tasks; i += waves) {
     const int32_t run = i / (2 * a.heads), rest = i - run * 2 * a.heads;
     for (; at < run; ++at) opens &= opens - 1;
     const int32_t first = __builtin_ctz(opens);
@@ -316,12 +330,13 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(Args a) {
     r.token = chunk * kChunk - 1 + first;
     r.first = entry % kGroup;
     r.end = r.first + 1 + __builtin_ctz(~(continues >> (first + 1)));
-    if constexpr (WAY != kWrite) {
-      if (rest & 1) Head<T, LPR>::template read_v<WAY == kReadPast>(a, r, rest >> 1, lane);
-      else Head<T, LPR>::template read_k<WAY == kReadPast>(a, r, rest >> 1, lane);
+    constexpr bool PAST = WAY == kWritePast || WAY == kReadPast;
+    if constexpr (WAY >= kRead) {
+      if (rest & 1) Head<T, LPR>::template read_v<PAST>(a, r, rest >> 1, lane);
+      else Head<T, LPR>::template read_k<PAST>(a, r, rest >> 1, lane);
     } else {
-      if (rest & 1) Head<T, LPR>::write_v(a, r, rest >> 1, lane);
-      else Head<T, LPR>::write_k(a, r, rest >> 1, lane);
+      if (rest & 1) Head<T, LPR>::template write_v<PAST>(a, r, rest >> 1, lane);
+      else Head<T, LPR>::template write_k<PAST>(a, r, rest >> 1, lane);
     }
   }
 }
@@ -381,21 +396,24 @@ int run_rows(const char* fn, bool read, const void* key, const void* value, void
   for (const Memory& m : index) apart = apart && (read ? !m.meets(rows[0]) && !m.meets(rows[1]) : !m.meets(pages));
   if (!apart) return fail(KVC_ERR_INVALID_ARG, "%s: what is written overlaps what is read", fn);
   const int64_t chunks = (num_tokens + kChunk - 1) / kChunk;
-  // As many wavefronts for 16 tokens as their runs can use, from 2 for a head (one run, K and V) up to 32 (16 runs), as long as all
-  // are on the card at once.
-  const int64_t waves = std::min(std::max<int64_t>(8192 / chunks, 2 * heads), 2 * heads * kChunk);
+  // As many wavefronts for 16 tokens as their runs can use, from 2 for a head (one run, K and V) up to 32 (16 runs), 4096 in all as far as that
+  // allows (8 heads of 128: 256 requests' tokens 6.7 us, 7.5 with 2048; 4 heads, 2048 tokens of four requests 5.2, 4.3 with 2048 and 6.5 with 8192).
+  const int64_t waves = std::min(std::max<int64_t>(4096 / chunks, 2 * heads), 2 * heads * kChunk);
   const int64_t splits = (waves + kWavesPerGroup - 1) / kWavesPerGroup;
   if (chunks * splits >= (int64_t(1) << 31)) return fail(KVC_ERR_UNSUPPORTED, "%s: too many tokens", fn);
   Args a{(char*)key, (char*)value, k_stride * 2, v_stride * 2, (char*)cache, x.slots, x.batch_indices, x.positions, x.kv_indices, x.kv_indptr,
          num_tokens, num_pages * page_size, x.slot_bytes, (int32_t)x.batch_size, (int32_t)x.num_kv_indices, (int32_t)num_pages,
-         (int32_t)page_size, log2_exact(page_size), (int32_t)heads, (int32_t)dim, (int32_t)splits, (uint32_t)page_stride,
+         (int32_t)page_size, log2_exact(page_size), (int32_t)heads, (int32_t)dim, (uint32_t)splits, (uint32_t)page_stride,
          (uint32_t)group_bytes(heads, dim)};
   const unsigned grid = (unsigned)(chunks * splits);
   hipStream_t s = (hipStream_t)stream;
-  const bool bf16 = dtype == KVC_DTYPE_BF16, past = read && num_tokens * row * 4 >= kPastBytes;
-  if (past) bf16 ? launch_rows<BF16, kReadPast>(a, grid, s) : launch_rows<F16, kReadPast>(a, grid, s);
-  else if (read) bf16 ? launch_rows<BF16, kRead>(a, grid, s) : launch_rows<F16, kRead>(a, grid, s);
-  else bf16 ? launch_rows<BF16, kWrite>(a, grid, s) : launch_rows<F16, kWrite>(a, grid, s);
+  const bool bf16 = dtype == KVC_DTYPE_BF16, past = num_tokens * row * 4 >= (read ? kReadPastBytes : kWritePastBytes);
+  switch (read ? past ? kReadPast : kRead : past ? kWritePast : kWrite) {
+    case kWrite: bf16 ? launch_rows<BF16, kWrite>(a, grid, s) : launch_rows<F16, kWrite>(a, grid, s); break;
+    case kWritePast: bf16 ? launch_rows<BF16, kWritePast>(a, grid, s) : launch_rows<F16, kWritePast>(a, grid, s); break;
+    case kRead: bf16 ? launch_rows<BF16, kRead>(a, grid, s) : launch_rows<F16, kRead>(a, grid, s); break;
+    case kReadPast: bf16 ? launch_rows<BF16, kReadPast>(a, grid, s) : launch_rows<F16, kReadPast>(a, grid, s); break;
+  }
   KVC_HIP(hipGetLastError());
   return KVC_OK;
 }

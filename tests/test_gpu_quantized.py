@@ -318,3 +318,24 @@ def test_refusals(gpu):
     write(none, none, cache, at[:0])
     write(k, k, cache[:0], at)
     assert kvc.read_cache_q8(cache, at[:0], H, D)[0].shape == (0, H, D)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_large_calls_are_what_smaller_ones_are(gpu, dtype):
+    """Sizes from which rows go past the caches, against the same tokens in calls below them."""
+    H, D, page, T = 8, 128, 16, 33000
+    g = torch.Generator(device=gpu).manual_seed(1)
+    k, v = (torch.randn(T, H, D, generator=g, device=gpu).to(TYPES[dtype]) for _ in range(2))
+    slots = torch.randperm(T // 16 + 9, generator=g, device=gpu)[torch.arange(T, device=gpu) // 16] * 16 + torch.arange(T, device=gpu) % 16
+    one = kvc.allocate_q8_kv_caches(1, T // 16 + 9, page, H, D, gpu)[0]
+    one.fill_(40)
+    many = one.clone()
+    kvc.reshape_and_cache_q8(k, v, one, slots)
+    for t in range(0, T, 4000):
+        kvc.reshape_and_cache_q8(k[t:t + 4000], v[t:t + 4000], many, slots[t:t + 4000])
+    assert torch.equal(one, many)
+    got = kvc.read_cache_q8(one, slots, H, D, TYPES[dtype])
+    for t in range(0, T, 4000):
+        for a, b in zip(got, kvc.read_cache_q8(one, slots[t:t + 4000], H, D, TYPES[dtype])):
+            assert torch.equal(a[t:t + 4000], b)
+    assert (got[0] - k).abs().max() < 0.3 and (got[1] - v).abs().max() < 0.3
