@@ -40,6 +40,7 @@ struct Range {
 };
 struct Header {
   int32_t wide_items, narrow_entries, wide_entries, shared_wide;  // (narrow entries from the front, wide ones from the back)
+  int32_t shared_tiles, shared_count;  // of wide tiles of the sharing rows: tile t's parts are t + c * shared_tiles
 };
 
 struct Layout {  // the plan's device buffer

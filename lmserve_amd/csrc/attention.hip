@@ -284,13 +284,15 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     return begin + clamp(((int32_t)before + kStep / 2) / kStep * kStep, 0, end - begin);
   };
 
+  int32_t shared_count = 0;
   if (shared_rows) {
     const int32_t table = table_of(a, some_request).begin;
     const int32_t each = shared_wide ? round_up(ceil_div(shared_len, shared_chunks), kStep) : 0;
+    if (shared_wide) shared_count = ceil_div(shared_len, each);
     for (int32_t i = tid; i < shared_tiles; i += 1024) {
       const int32_t row0 = i * shared_tile, rows = min(shared_tile, shared_rows - row0);
       if (shared_wide) {
-        a.l.shared_parts[i] = {i, i, shared_tiles, ceil_div(shared_len, each)};
+        a.l.shared_parts[i] = {i, i, shared_tiles, shared_count};
       } else {
         const Cuts p = cuts_of(a, i * shared_work, shared_work, share, sliver);
         a.l.shared_parts[i] = {2 * a.groups + i, 2 * p.group, 2, p.count};
@@ -402,7 +404,8 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     __syncthreads();
   }
   if (tid == 0)
-    *a.l.header = {min(carry[2], a.max_items[1]), min(entries[0], a.max_entries), min(entries[1], a.max_entries), shared_wide};
+    *a.l.header = {min(carry[2], a.max_items[1]), min(entries[0], a.max_entries), min(entries[1], a.max_entries), shared_wide,
+                   shared_tiles, shared_count};
   for (int32_t w = tid; w < a.groups; w += 1024)
     a.l.ranges[w] = last_item[w] < 0 ? Range{0, 0} : Range{first_item[w], last_item[w] + 1};
 }
@@ -1179,64 +1182,110 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_step_kerne
 
 // Joins a row's partials: weights exp2(lse_c - lse). An entry of several rows, of few parts each, takes half a wavefront a row,
 // its lanes over the columns; one of a single row of many parts a workgroup, the parts over the eight halves.
-// Bound by the chain of loads (entry, lse, partials) at few rows, by the partials' bytes at many.
+// Bound by the chain of loads at few rows, by the partials' bytes at many: the header and the entry that is likely, then the parts' lse and their first
+// kJoined values, are asked for together (over 8 bits, the attention of
+// 256 requests behind a shared prompt 70.3 us with one after the other, 65.3 so, of 13 behind one 17.0 and 14.2; with registers spilled it is slower than either).
+constexpr int kJoined = 8;
 template <typename T>
-__global__ __launch_bounds__(kThreads, 6) void attend_join_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void attend_join_kernel(AttendArgs a) {
   __shared__ f32x4 sums[8][64];
   const int32_t half = threadIdx.x >> 5, column = threadIdx.x & 31;
-  const Header head = *a.l.header;
-  const bool shared_wide = head.shared_wide;
-  const int32_t D = a.head_dim, entries = head.narrow_entries + head.wide_entries;
+  const int32_t D = a.head_dim;
+  Entry likely = a.l.entries[min((int32_t)blockIdx.x / a.kv_heads, a.max_entries - 1)];
+  const Header given = *a.l.header;
+  const int32_t narrow_entries = __builtin_amdgcn_readfirstlane(given.narrow_entries), shared_tiles = __builtin_amdgcn_readfirstlane(given.shared_tiles),
+                shared_count = __builtin_amdgcn_readfirstlane(given.shared_count);
+  const bool shared_wide = __builtin_amdgcn_readfirstlane(given.shared_wide);
+  const int32_t entries = narrow_entries + __builtin_amdgcn_readfirstlane(given.wide_entries);
   for (int32_t at = blockIdx.x; at < entries * a.kv_heads; at += gridDim.x) {
     const int32_t it = at / a.kv_heads, h = at - it * a.kv_heads;
-    const bool wide = it >= head.narrow_entries;
-    const Entry e = a.l.entries[wide ? a.max_entries - 1 - (it - head.narrow_entries) : it];
+    const bool wide = it >= narrow_entries;
+    if (wide || at != (int32_t)blockIdx.x) likely = a.l.entries[wide ? a.max_entries - 1 - (it - narrow_entries) : it];
+    // (the same in all lanes)
+    const auto one = [](int32_t v) { return __builtin_amdgcn_readfirstlane(v); };
+    const Entry e = {one(likely.q_begin), one(likely.row0), (int16_t)one(likely.rows), (int16_t)one(likely.many), one(likely.shared_row0),
+                     {one(likely.parts.slot), one(likely.parts.next), one(likely.parts.step), one(likely.parts.count)}};
     const int32_t own_tile = wide ? kWide : kTile, shared_tile = shared_wide ? kWide : kTile;
     const float* const own_lse = a.partial_lse[wide], * const shared_lse = a.partial_lse[shared_wide];
     const float* const own_o = a.partial[wide], * const shared_o = a.partial[shared_wide];
     const bool many = e.many;
     for (int32_t r = many ? 0 : half; r < e.rows; r += 8) {
-      const int32_t row = e.row0 + r, shared_row = e.shared_row0 + r;
-      const Parts sh = e.shared_row0 >= 0 ? a.l.shared_parts[shared_row / shared_tile] : Parts{};
+      const int32_t row = e.row0 + r, shared_row = e.shared_row0 + r, shared_at = shared_row / shared_tile;
+      Parts sh = {};
+      if (e.shared_row0 >= 0) {
+        if (shared_wide) sh = {shared_at, shared_at, shared_tiles, shared_count};
+        else sh = a.l.shared_parts[shared_at];
+      }
       const int32_t own = e.parts.count, parts = own + sh.count;
-      const auto row_of = [&](int32_t c) -> int64_t {  // of part c
-        if (c < own) return ((int64_t)(c ? e.parts.next + c * e.parts.step : e.parts.slot) * a.kv_heads + h) * own_tile + row % own_tile;
+      const auto row_of = [&](int32_t c) -> uint32_t {  // of part c (a workspace of 16 GB has 2^28 rows at most)
+        if (c < own) return (uint32_t)((c ? e.parts.next + c * e.parts.step : e.parts.slot) * a.kv_heads + h) * own_tile + row % own_tile;
         c -= own;
-        return ((int64_t)(c ? sh.next + c * sh.step : sh.slot) * a.kv_heads + h) * shared_tile + shared_row % shared_tile;
+        return (uint32_t)((c ? sh.next + c * sh.step : sh.slot) * a.kv_heads + h) * shared_tile + shared_row % shared_tile;
       };
       const auto lse_of = [&](int32_t c) { return (c < own ? own_lse : shared_lse)[row_of(c)]; };
-      float top = -INFINITY;
-      for (int32_t c = column; c < parts; c += 32) top = fmaxf(top, lse_of(c));
-      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-      const float base = top == -INFINITY ? 0.f : top;
-      float total = 0;
-      for (int32_t c = column; c < parts; c += 32) total += exp2_of(lse_of(c) - base);
-      for (int d = 16; d; d >>= 1) total += __shfl_xor(total, d);
-      const float inv = total == 0 ? 0.f : 1.f / total;
+      const auto values_at = [&](int32_t c, uint32_t row, int32_t d) {
+        return *reinterpret_cast<const f32x4*>((c < own ? own_o : shared_o) + (uint64_t)row * D + d);
+      };
       const int32_t i = row / a.group, g = row - i * a.group;
       const int64_t out_row = ((int64_t)(e.q_begin + i) * a.kv_heads + h) * a.group + g;
-      if (a.lse && column == 0 && (!many || half == 0)) a.lse[out_row] = (total == 0 ? -INFINITY : base + __log2f(total)) * kLn2;
       const auto put = [&](int32_t d, f32x4 x) {
-        x *= inv;
         *reinterpret_cast<u32x2*>(a.out + (out_row * D + d) * 2) = u32x2{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
       };
-      const auto sum_of = [&](int32_t d, int32_t from, int32_t step) {
-        f32x4 x = {};
-#pragma unroll 4
-        for (int32_t c = from; c < parts; c += step)
-          x += *reinterpret_cast<const f32x4*>((c < own ? own_o : shared_o) + row_of(c) * D + d) * fmaxf(exp2_of(lse_of(c) - base), kLeastWeight);
-        return x;
-      };
       if (!many) {
-        for (int32_t d = column * 4; d < D; d += 128) put(d, sum_of(d, 0, 1));
+        // up to kManyParts parts, each a lane's: where its values are, its lse, its weight; the values are asked for ahead of what they are weighed by
+        const int32_t mine = min(column, parts - 1);
+        const float lse = column < parts ? lse_of(mine) : -INFINITY;
+        const uint64_t at_mine = (uint64_t)(uintptr_t)((mine < own ? own_o : shared_o) + (uint64_t)row_of(mine) * D);
+        f32x4 value[kJoined];
+        const auto ask = [&](int32_t c0, int32_t d) {
+#pragma unroll
+          for (int j = 0; j < kJoined; ++j) {
+            const uint64_t from = (uint64_t)(uint32_t)__shfl((int)(at_mine >> 32), c0 + j, 32) << 32 | (uint32_t)__shfl((int)at_mine, c0 + j, 32);
+            if (c0 + j < parts && d < D) value[j] = *reinterpret_cast<const f32x4*>((uintptr_t)from + d * 4);
+          }
+        };
+        ask(0, column * 4);
+        float top = lse;
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float base = top == -INFINITY ? 0.f : top, weight = exp2_of(lse - base);
+        float total = column < parts ? weight : 0.f;
+        for (int d = 16; d; d >>= 1) total += __shfl_xor(total, d);
+        const float inv = total == 0 ? 0.f : 1.f / total, least = fmaxf(weight, kLeastWeight);
+        if (a.lse && column == 0) a.lse[out_row] = (total == 0 ? -INFINITY : base + __log2f(total)) * kLn2;
+        for (int32_t d = column * 4; d < D + column * 4; d += 128) {
+          f32x4 x = {};
+          for (int32_t c0 = 0; c0 < parts; c0 += kJoined) {
+            if (c0 || d >= 128) ask(c0, d);
+#pragma unroll
+            for (int j = 0; j < kJoined; ++j) {
+              const float w = __shfl(least, c0 + j, 32);
+              if (c0 + j < parts) x += value[j] * w;
+            }
+          }
+          if (d < D) put(d, x * inv);
+        }
       } else {
-        for (int32_t d = column; d < D / 4; d += 32) sums[half][d] = sum_of(d * 4, half, 8);
+        float top = -INFINITY;
+        for (int32_t c = column; c < parts; c += 32) top = fmaxf(top, lse_of(c));
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float base = top == -INFINITY ? 0.f : top;
+        float total = 0;
+        for (int32_t c = column; c < parts; c += 32) total += exp2_of(lse_of(c) - base);
+        for (int d = 16; d; d >>= 1) total += __shfl_xor(total, d);
+        const float inv = total == 0 ? 0.f : 1.f / total;
+        if (a.lse && column == 0 && half == 0) a.lse[out_row] = (total == 0 ? -INFINITY : base + __log2f(total)) * kLn2;
+        for (int32_t d = column; d < D / 4; d += 32) {
+          f32x4 x = {};
+#pragma unroll 4
+          for (int32_t c = half; c < parts; c += 8) x += values_at(c, row_of(c), d * 4) * fmaxf(exp2_of(lse_of(c) - base), kLeastWeight);
+          sums[half][d] = x;
+        }
         __syncthreads();
         for (int32_t d = threadIdx.x; d < D / 4; d += kThreads) {
           f32x4 x = {};
 #pragma unroll
           for (int w = 0; w < 8; ++w) x += sums[w][d];
-          put(d * 4, x);
+          put(d * 4, x * inv);
         }
         __syncthreads();
       }
@@ -1343,8 +1392,10 @@ Sizes sizes_of(const kvc_attention_plan& p) {
 // Keys that no cache holds, and that are read once, by non-temporal loads (decode of 256 requests, 2.2 GB: 421 and 406 us;
 // one of 131001 keys, 0.5 GB: 108 and 103; behind a shared prompt, 0.27 GB of which 16 MB are read again and again, 126
 // and 130)
+// Over 8 bits from less on: one of 131001 keys, 0.25 GB, 67 and 63; 64 of 1000, 0.13 GB, 37.6 and 38.1.
 bool past_the_caches(const kvc_attention_plan& p, int64_t element) {
-  return p.shared_pages == 0 && p.num_kv_indices * 2 * p.page_size * p.num_kv_heads * p.head_dim * element >= (int64_t(256) << 20);
+  return p.shared_pages == 0 &&
+         p.num_kv_indices * 2 * p.page_size * p.num_kv_heads * p.head_dim * element >= (int64_t(p.q8 ? 192 : 256) << 20);
 }
 
 template <typename T, int DP>
