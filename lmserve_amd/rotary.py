@@ -282,6 +282,36 @@ def qk_norm_rotary_pos_emb(query: torch.Tensor, key: torch.Tensor, query_weight:
     return q_out.view(query.shape), k_out.view(key.shape)
 
 
+def rotate_into(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, cos_sin_cache: torch.Tensor, head_dim: int,
+                query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None,
+                query_weight: Optional[torch.Tensor] = None, key_weight: Optional[torch.Tensor] = None,
+                eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`rotary_pos_emb`, or with weights `qk_norm_rotary_pos_emb`, into contiguous buffers of the caller's where they are
+    given. Tokens at positions without a cos/sin row (padding) are left alone: their rows of the outputs stay as they were."""
+    if (query_weight is None) != (key_weight is None):
+        raise ValueError("query_weight and key_weight come together")
+    q2, k2, positions, pos_bytes, kd, T = _prep(query, key, positions, cos_sin_cache, head_dim)
+    outs = []
+    for given, rows, name in ((query_out, q2, "query_out"), (key_out, k2, "key_out")):
+        if given is None:
+            given = torch.empty_like(rows, memory_format=torch.contiguous_format)
+        elif given.dtype != rows.dtype or given.device != rows.device or given.numel() != rows.numel() or not given.is_contiguous():
+            raise ValueError(f"{name} must be contiguous, of the rows' size, dtype and device")
+        outs.append(given)
+    q_out, k_out = outs
+    if T > 0:
+        weights = () if query_weight is None else _norm_weights(query_weight, key_weight, query, head_dim)
+        with _on_device_of(q2):
+            lib = _lib.lib()
+            call = lib.kvc_qk_norm_rotary_pos_emb if weights else lib.kvc_rotary_pos_emb
+            _lib.check(call(
+                q2.data_ptr(), k2.data_ptr(), *((w.data_ptr() for w in weights)), *((eps,) if weights else ()), positions.data_ptr(),
+                pos_bytes, cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], T, q2.shape[1] // head_dim, k2.shape[1] // head_dim,
+                head_dim, cos_sin_cache.shape[1] // 2, _tok_stride(q2), _tok_stride(k2), q_out.data_ptr(), k_out.data_ptr(),
+                q2.shape[1], k2.shape[1], kd, _stream_of(q2)))
+    return q_out, k_out
+
+
 def qk_norm_rotary_pos_emb_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                                      query_weight: torch.Tensor, key_weight: torch.Tensor, positions: torch.Tensor,
                                      cos_sin_cache: torch.Tensor, head_dim: int, kv_cache: torch.Tensor,

@@ -37,7 +37,8 @@ from . import _lib, streams
 from .attention import PagedAttentionPlan
 from .index_prep import InferInput
 from .paged import BlockRuns, PagedKVWritePlan, build_write_index, max_block_runs
-from .rotary import PagedRotaryWritePlan
+from .quantized import q8_page_bytes, reshape_and_cache_q8
+from .rotary import PagedRotaryWritePlan, rotate_into
 
 
 class KVWriteStep:
@@ -52,6 +53,8 @@ class KVWriteStep:
     with_runs: also have the index build emit the step's block runs (`self.runs`).
     with_attention: `attend` is available (needs `num_heads`), and the index build lays out its work;
       shared_pages, sm_scale and max_q_len are `PagedAttentionPlan`'s, for all steps to come.
+    kv_dtype: `torch.float8_e4m3fn` for a pool in 8 bits (`allocate_q8_kv_caches`): `append`, `rotate_and_append` and
+      `attend` take its layers, `[num_pages, page_bytes]` of uint8; `dtype` is the projections'. The rotation is then a launch before the write's.
 
     The buffers hold one step: the sequences recorded from one object run one after another.
     """
@@ -60,7 +63,16 @@ class KVWriteStep:
                  max_requests: int, max_tokens: int, max_block_ids: int,
                  cos_sin_cache: Optional[torch.Tensor] = None, num_heads: int = 0,
                  with_runs: bool = False, with_attention: bool = False, shared_pages: int = 0,
-                 sm_scale: Optional[float] = None, max_q_len: Optional[int] = None):
+                 sm_scale: Optional[float] = None, max_q_len: Optional[int] = None,
+                 kv_dtype: Optional[torch.dtype] = None):
+        if kv_dtype not in (None, dtype, torch.float8_e4m3fn):
+            raise TypeError(f"Unsupported kv_dtype: {kv_dtype} (the cache holds {dtype} or float8_e4m3fn)")
+        self.q8 = kv_dtype == torch.float8_e4m3fn
+        if self.q8:
+            q8_page_bytes(num_kv_heads, head_dim, page_size)       # says what it does not take
+            if dtype not in (torch.bfloat16, torch.float16):
+                raise TypeError(f"Unsupported dtype: {dtype} (keys and values of an 8-bit cache are bf16 or f16)")
+        self.num_kv_heads, self.head_dim = int(num_kv_heads), int(head_dim)
         if with_attention and num_heads < 1:
             raise ValueError("with_attention needs num_heads")
         self.device = torch.device(device)
@@ -94,11 +106,12 @@ class KVWriteStep:
             self.runs = BlockRuns(torch.zeros(cap, 4, **i32), torch.zeros(1, **i32), torch.zeros(B + 1, **i32))
         self._out = (self.cu_seqlens_q, self.kv_indptr, self.kv_last_page_len, self.batch_indices,
                      self.positions, self.slot_mapping) + ((self.runs,) if with_runs else ())
-        self.plan = PagedKVWritePlan(self.batch_indices, self.positions, self.kv_indices, self.kv_indptr,
+        self.plan = None if self.q8 else PagedKVWritePlan(self.batch_indices, self.positions, self.kv_indices, self.kv_indptr,
                                      self.kv_last_page_len, num_kv_heads, head_dim, page_size, dtype,
                                      slots=self.slot_mapping)
         self.rotary_plan = None
-        if cos_sin_cache is not None:
+        self.cos_sin_cache = cos_sin_cache
+        if cos_sin_cache is not None and not self.q8:
             self.rotary_plan = PagedRotaryWritePlan(self.batch_indices, self.positions, self.kv_indices,
                                                     self.kv_indptr, self.kv_last_page_len, cos_sin_cache,
                                                     num_heads, num_kv_heads, head_dim, page_size,
@@ -108,7 +121,7 @@ class KVWriteStep:
             self.attention_plan = PagedAttentionPlan(self.cu_seqlens_q, self.kv_indices, self.kv_indptr,
                                                      self.kv_last_page_len, num_heads, num_kv_heads, head_dim, page_size,
                                                      dtype, T, max_q_len=max_q_len, shared_pages=shared_pages,
-                                                     sm_scale=sm_scale)
+                                                     sm_scale=sm_scale, kv_dtype=kv_dtype)
         self.num_tokens = 0       # of the step last packed (host-side knowledge)
         self.num_requests = 0
 
@@ -188,13 +201,23 @@ class KVWriteStep:
     def append(self, key: torch.Tensor, value: torch.Tensor, paged_kv_cache: torch.Tensor) -> None:
         """One layer's write; `key` / `value` hold `max_tokens` rows, of which the
         step's first `num_tokens` are written."""
+        if self.q8:
+            heads = (self.num_kv_heads, self.head_dim)
+            key, value = (t.unflatten(1, heads) if t.dim() == 2 else t for t in (key, value))
+            reshape_and_cache_q8(key, value, paged_kv_cache, self.slot_mapping)
+            return
         self.plan.append(key, value, paged_kv_cache)
 
     def rotate_and_append(self, query, key, value, paged_kv_cache, query_out=None, key_out=None,
                           query_weight=None, key_weight=None, eps: float = 1e-6):
         """One layer's rotation and write; with the layer's `query_weight` and `key_weight` its heads are normed first."""
-        if self.rotary_plan is None:
+        if self.cos_sin_cache is None:
             raise ValueError("this step was made without a cos/sin table")
+        if self.q8:
+            query_out, rotated = rotate_into(query, key, self.positions, self.cos_sin_cache, self.head_dim, query_out, key_out,
+                                             query_weight, key_weight, eps)
+            self.append(rotated, value, paged_kv_cache)
+            return query_out, key_out
         return self.rotary_plan.run(query, key, value, paged_kv_cache, query_out=query_out, key_out=key_out,
                                     query_weight=query_weight, key_weight=key_weight, eps=eps)
 
@@ -224,7 +247,7 @@ class KVWriteStep:
         if attention_outs is not None:
             if self.attention_plan is None:
                 raise ValueError("this step was made without attention")
-            if queries is None or (self.rotary_plan is not None and query_outs is None):
+            if queries is None or (self.cos_sin_cache is not None and query_outs is None):
                 raise ValueError("attention_outs need queries, and query_outs where they are rotated")
 
         def body():
@@ -232,7 +255,7 @@ class KVWriteStep:
             if attention_outs is not None or norm_weights is not None:
                 for l, (k, v, c) in enumerate(zip(keys, values, caches)):
                     q = queries[l]
-                    if self.rotary_plan is None and norm_weights is None:
+                    if self.cos_sin_cache is None and norm_weights is None:
                         self.append(k, v, c)
                     else:
                         qw, kw = norm_weights[l] if norm_weights is not None else (None, None)
