@@ -298,3 +298,49 @@ def test_refusals(gpu):
     wide = kvc.PagedAttentionPlan(*index, 4, 2, 64, 16, s.dtype, 1, kv_dtype=s.dtype)
     with pytest.raises(TypeError):
         wide.run(q, pages)
+
+
+def test_one_plan_on_two_streams_at_once(gpu):
+    """Every run has a workspace of its own."""
+    s = Step([(1, 3000), (40, 900), (1, 700)], 8, 2, 128, 16, seed=21)
+    plan, pages = s.plan(gpu), s.pages(gpu)
+    q = [s.query.to(gpu), (s.query * 2).to(gpu)]
+    want = [plan.run(x, pages) for x in q]
+    s.check(want[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(plan.run(q[i], pages))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_write_then_attend(gpu):
+    """A prompt in chunks and single tokens, written and attended to through the eager calls, on what the write left."""
+    H, HQ, D, page = 2, 8, 128, 32
+    rng = np.random.default_rng(22)
+    pool = kvc.allocate_q8_kv_caches(1, 20, page, H, D, gpu)[0].fill_(127)
+    table = rng.permutation(20)[:10].astype(np.int32)
+    i32 = dict(dtype=torch.int32, device=gpu)
+    have = 0
+    for new in (150, 1, 1, 33, 1, 14):
+        k, v = (torch.from_numpy(rng.standard_normal((new, H, D)).astype(np.float32)).to(torch.bfloat16).to(gpu) for _ in range(2))
+        q = torch.from_numpy(rng.standard_normal((new, HQ, D)).astype(np.float32)).to(torch.bfloat16).to(gpu)
+        positions = torch.arange(have, have + new, **i32)
+        have += new
+        pages = -(-have // page)
+        index = [torch.from_numpy(table[:pages]).to(gpu), torch.tensor([0, pages], **i32), torch.tensor([(have - 1) % page + 1], **i32)]
+        kvc.append_paged_kv_cache_q8(k, v, torch.zeros(new, **i32), positions, pool, *index)
+        out, lse = kvc.paged_attention(q, pool, torch.tensor([0, new], **i32), *index, return_lse=True, num_kv_heads=H)
+        s = Step.__new__(Step)
+        s.page, s.H, s.Hq, s.D, s.eps = page, H, HQ, D, 2.0 ** -7
+        s.cache, s.query, s.scale = qo.Cache(pool.cpu().numpy(), H, D), q.cpu(), D ** -0.5
+        s.qo, s.indices, s.indptr, s.last = np.array([0, new]), table[:pages], np.array([0, pages]), np.array([(have - 1) % page + 1])
+        s.check(out, lse)
+        # the rows that come back are those that were attended to
+        bk, bv = kvc.read_paged_kv_cache_q8(torch.zeros(new, **i32), positions, pool, *index, H, D)
+        assert (bk - k).abs().max() < 0.3 and (bv - v).abs().max() < 0.3

@@ -339,3 +339,50 @@ def test_large_calls_are_what_smaller_ones_are(gpu, dtype):
         for a, b in zip(got, kvc.read_cache_q8(one, slots[t:t + 4000], H, D, TYPES[dtype])):
             assert torch.equal(a[t:t + 4000], b)
     assert (got[0] - k).abs().max() < 0.3 and (got[1] - v).abs().max() < 0.3
+
+
+def test_a_group_in_another_order_or_twice_harms_no_other(gpu):
+    """Places of one group in falling order, twice, and in two parts of a call: its own contents are undefined, every other group's are right."""
+    H, D, page = 4, 128, 32
+    s = Step([64, 64], H, D, page, "bf16", seed=31)
+    cache = torch.from_numpy(s.raw).to(gpu)
+    base = s.indices.astype(np.int64) * page
+    bad = [base[0] + 7, base[0] + 6, base[0] + 5, base[0] + 6, base[0] + 1, base[0] + 2, base[0] + 15, base[0] + 15]
+    good = [base[1] + i for i in range(20)] + [base[2] + 16 + i for i in range(3)]
+    slots = np.array(bad[:3] + good[:9] + bad[3:6] + good[9:] + bad[6:], np.int64)
+    k, v = (rows(s.rng, len(slots), H, D, "bf16") for _ in range(2))
+    keep = [i for i, t in enumerate(slots) if t not in bad]
+    # (the good tokens are one run of the call with a break inside a group: what follows it goes on with the group)
+    first, second = [i for i in keep if i < 12], [i for i in keep if i > 12]
+    for part in (first, second):
+        s.oracle.write(k[part].double().numpy(), v[part].double().numpy(), slots[part])
+    for part in (slice(0, 12), slice(12, None)):
+        kvc.reshape_and_cache_q8(k[part].to(gpu), v[part].to(gpu), cache, torch.from_numpy(slots[part]).to(gpu))
+    group = group_bytes(H, D)
+    got, want = cache.cpu().numpy().reshape(-1, group), s.oracle.pages().reshape(-1, group)
+    others = np.delete(np.arange(len(got)), base[0] // 16)
+    assert np.array_equal(got[others], want[others])
+    back = kvc.read_cache_q8(cache, torch.from_numpy(slots[::-1].copy()).to(gpu), H, D)      # any order, twice the same
+    where = torch.from_numpy(Cache(cache.cpu().numpy(), H, D).values()[slots[::-1]]).to(torch.bfloat16)
+    for g, w in zip(back, (where[:, 0], where[:, 1])):
+        assert torch.equal(torch.isnan(g.cpu()), torch.isnan(w)) and torch.equal(g.cpu().nan_to_num(1), w.nan_to_num(1))
+
+
+def test_writes_on_two_streams_at_once(gpu):
+    """Calls that write different groups of the same pages side by side."""
+    H, D, page = 8, 64, 64
+    s = Step([64 * 8], H, D, page, "f16", seed=32)
+    cache = torch.from_numpy(s.raw).to(gpu)
+    k, v = (rows(s.rng, 512, H, D, "f16") for _ in range(2))
+    slots = (s.indices.astype(np.int64)[:, None] * page + np.arange(page)).ravel()
+    s.oracle.write(k.double().numpy(), v.double().numpy(), slots)
+    halves = [np.flatnonzero(np.arange(512) // 16 % 2 == h) for h in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    given = [(k[h].to(gpu), v[h].to(gpu), torch.from_numpy(slots[h]).to(gpu)) for h in halves]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for stream, (a, b, at) in zip(streams, given):
+            with torch.cuda.stream(stream):
+                kvc.reshape_and_cache_q8(a, b, cache, at)
+    torch.cuda.synchronize()
+    same(cache, s.oracle)

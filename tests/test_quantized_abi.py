@@ -90,3 +90,61 @@ def test_no_cpu_path():
     k = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="GPU"):
         kvc.reshape_and_cache_q8(k, k, torch.zeros(2, kvc.q8_page_bytes(2, 64, 16), dtype=torch.uint8), torch.arange(3))
+
+
+def test_attention_plans_over_8_bits_that_are_refused():
+    import ctypes
+    L = _lib.lib()
+    good = dict(qo=4096, idx=8192, ptr=12288, last=16384, batch=3, tokens=7, nidx=9, hq=8, hk=2, d=64, page=32, max_q=0, shared=0,
+                scale=0.125, dtype=0)
+
+    def create(fn, **kw):
+        a = dict(good)
+        a.update(kw)
+        h = ctypes.c_void_p()
+        return fn(*a.values(), ctypes.byref(h)), h
+
+    for change, code in ((dict(d=72), UNSUPPORTED), (dict(d=8), UNSUPPORTED), (dict(d=272), UNSUPPORTED), (dict(page=20), UNSUPPORTED),
+                         (dict(page=8), UNSUPPORTED), (dict(page=0), INVALID), (dict(dtype=2), UNSUPPORTED), (dict(hq=7), INVALID),
+                         (dict(scale=0.0), INVALID), (dict(batch=-1), INVALID), (dict(qo=None), INVALID),
+                         (dict(page=1 << 20, hk=64, hq=64, d=256), UNSUPPORTED)):
+        rc, h = create(L.kvc_attention_plan_create_q8, **change)
+        assert rc == code and h.value is None, change
+        assert "kvc_attention_plan_create_q8" in _lib.last_error()
+    rc, h = create(L.kvc_attention_plan_create_q8)
+    rc16, h16 = create(L.kvc_attention_plan_create)
+    assert rc == rc16 == OK
+    work, page = L.kvc_attention_workspace_bytes(h), kvc.q8_page_bytes(2, 64, 32)
+    run = dict(q=1 << 20, qs=512, cache=1 << 24, ps=page, pages=4, out=2 << 20, lse=None, ws=1 << 30, wb=work)
+
+    def go(fn, plan, **kw):
+        a = dict(run)
+        a.update(kw)
+        return fn(plan, *a.values(), None)
+
+    assert go(L.kvc_attention_plan_run_q8, None) == INVALID
+    for fn, plan, bits in ((L.kvc_attention_plan_run_q8, h16, 16), (L.kvc_attention_plan_run, h, 8)):
+        assert go(fn, plan) == INVALID and f"{bits} bits" in _lib.last_error()
+    assert go(L.kvc_attention_plan_run_q8, h) == INVALID and "not built" in _lib.last_error()     # every other argument is in order
+    for change, word in ((dict(q=None), "null"), (dict(out=None), "null"), (dict(cache=None), "null"), (dict(ps=page - 16), "geometry"),
+                         (dict(ps=1 << 32), "geometry"), (dict(pages=-1), "geometry"), (dict(qs=504), "stride"), (dict(ps=page + 8), "aligned"),
+                         (dict(cache=(1 << 24) + 8), "aligned"), (dict(q=(1 << 20) + 8), "aligned"), (dict(ws=(1 << 30) + 64), "aligned")):
+        assert go(L.kvc_attention_plan_run_q8, h, **change) == INVALID and word in _lib.last_error(), change
+    assert go(L.kvc_attention_plan_run_q8, h, wb=work - 1) == _lib.KVC_ERR_STAGING
+    for x in (h, h16):
+        L.kvc_attention_plan_destroy(x)
+
+
+def test_blocks_of_bytes_on_disk(tmp_path):
+    """The disk tier holds 8-bit blocks as bytes."""
+    rng = np.random.default_rng(0)
+    shape = (6, 2, kvc.q8_page_bytes(2, 64, 16))
+    host = rng.integers(0, 256, shape, dtype=np.uint8)
+    tier = kvc.DiskTier(str(tmp_path / "blocks.npy"), shape, np.uint8)
+    try:
+        tier.save_blocks(host, np.array([0, 3, 5]), np.array([4, 1, 0]))
+        back = np.zeros_like(host)
+        tier.load_blocks(back, np.array([4, 1, 0]), np.array([2, 1, 4]))
+    finally:
+        tier.close()
+    assert np.array_equal(back[[2, 1, 4]], host[[0, 3, 5]]) and not back[[0, 3, 5]].any()
