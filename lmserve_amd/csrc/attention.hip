@@ -1176,7 +1176,7 @@ template <typename T, int DP, Reach REACH>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_step_kernel(AttendArgs a) {
   constexpr int LDS = wide_lds<DP>() > narrow_lds<T, DP>() ? wide_lds<DP>() : narrow_lds<T, DP>();
   __shared__ __attribute__((aligned(16))) char lds[LDS];
-  take_step(a, [&](const Item& item, int32_t h) { narrow_item<T, DP, REACH, false>(a, item, h, lds); },
+  take_step<false>(a, [&](const Item& item, int32_t h) { narrow_item<T, DP, REACH, false>(a, item, h, lds); },
             [&](const Item& item, int32_t h) { wide_item<T, DP, REACH>(a, item, h, lds); });
 }
 
@@ -1546,7 +1546,7 @@ int run_plan(const char* fn, bool q8, const kvc_attention_plan* plan, const void
   a.head_dim = (int32_t)plan->head_dim;
   a.narrow_groups = (int32_t)(plan->n.groups * plan->num_kv_heads);
   // (a workgroup takes further items where there are more than these)
-  a.wide_groups = (int32_t)round_up(std::min<int64_t>(plan->n.max_items[1] * plan->num_kv_heads, 4096), 8);
+  a.wide_groups = (int32_t)round_up(std::min<int64_t>(plan->n.max_items[1] * plan->num_kv_heads, q8 ? 2048 : 4096), 8);
   a.max_entries = (int32_t)plan->n.max_entries;
   a.scale = plan->scale * kLog2e;
   a.l = layout_of(*plan, plan->buffer, nullptr);

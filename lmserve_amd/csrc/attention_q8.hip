@@ -86,6 +86,11 @@ __device__ __forceinline__ bool is_nan(const char* column, int32_t token) { retu
 //   of K the columns 64 s + 16 quad.. of token 4 i + n % 4 of group n / 4: two operands of the product i,
 //   of V the column 16 d + n of group quad: 16 tokens, two operands,
 // and holds the scores and weights of row n and group quad.
+// Bound by HBM where there are many keys: decode of 256 requests, 1.13 GB of codes, 182 us (6.2 TB/s; the 16-bit cache 400), one
+// request of 131001 keys 45 to 63; by the chain of item, pages, keys and the joining of wavefronts where there are few: 900 keys of one
+// request 6.7 us. Two workgroups a CU by their registers (three, with 45 of them spilled, are slower); asking for the next item's
+// record, pages, queries and keys ahead cost more in code and registers than it hid (one request of 900 keys 6.7 to 7.3 us, one of 32000 keys 26.6 to 29.2).
+// f16 queries have their weights in two parts, as over 16 bits; with bf16 outputs the rest of an f16 weight, 2^-12 of it, is below their rounding.
 template <int DP>
 constexpr int narrow_lds() { return kWaves * kTile * (DP + 4) * 4 + kWaves * kTile * 12; }
 
@@ -321,7 +326,9 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
 // As the wide tiles over 16 bits (attention.hip): 32 rows to a wavefront, K half a step ahead of V, one barrier a step. What is
 // staged in LDS is 16 bits: K as the query's type, its rows permuted, V as f16 columns in units of 2^(E - kUp), so a group is converted once for
 // all four wavefronts; a wavefront converts the group of the window that is its own number. E goes with a window, and
-// O is scaled to it before the window's product.
+// O is scaled to it before the window's product. V's columns lie in LDS as the product takes them, so it reads them whole, without the transposing read.
+// Bound as over 16 bits, by what two wavefronts a SIMD have under way: 2048 new tokens behind 13 to 30 thousand keys 740 to 810 us from card to
+// card (16 bits: 770 on one where this takes 752), 880 to 960 TFLOP/s.
 template <int DP>
 constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16) + 2 * DP * (kStep * 2 + kVPad) + (kWaves + 1) * 4; }
 
@@ -689,7 +696,7 @@ template <typename T, int DP, bool FULL>
 __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void step_kernel(AttendArgs a) {
   constexpr int LDS = wide_lds<DP>() > narrow_lds<DP>() ? wide_lds<DP>() : narrow_lds<DP>();
   __shared__ __attribute__((aligned(16))) char lds[LDS];
-  take_step(a, [&](const Item& item, int32_t h) { narrow_item<T, DP, FULL, false>(a, item, h, lds); },
+  take_step<true>(a, [&](const Item& item, int32_t h) { narrow_item<T, DP, FULL, false>(a, item, h, lds); },
             [&](const Item& item, int32_t h) { wide_item<T, DP, FULL>(a, item, h, lds); });
 }
 
