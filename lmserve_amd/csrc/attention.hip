@@ -1177,7 +1177,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_step_kerne
   constexpr int LDS = wide_lds<DP>() > narrow_lds<T, DP>() ? wide_lds<DP>() : narrow_lds<T, DP>();
   __shared__ __attribute__((aligned(16))) char lds[LDS];
   take_step<false>(a, [&](const Item& item, int32_t h) { narrow_item<T, DP, REACH, false>(a, item, h, lds); },
-            [&](const Item& item, int32_t h) { wide_item<T, DP, REACH>(a, item, h, lds); });
+                   [&](const Item& item, int32_t h) { wide_item<T, DP, REACH>(a, item, h, lds); });
 }
 
 // Joins a row's partials: weights exp2(lse_c - lse). An entry of several rows, of few parts each, takes half a wavefront a row,

@@ -697,7 +697,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void step_kernel(Atten
   constexpr int LDS = wide_lds<DP>() > narrow_lds<DP>() ? wide_lds<DP>() : narrow_lds<DP>();
   __shared__ __attribute__((aligned(16))) char lds[LDS];
   take_step<true>(a, [&](const Item& item, int32_t h) { narrow_item<T, DP, FULL, false>(a, item, h, lds); },
-            [&](const Item& item, int32_t h) { wide_item<T, DP, FULL>(a, item, h, lds); });
+                  [&](const Item& item, int32_t h) { wide_item<T, DP, FULL>(a, item, h, lds); });
 }
 
 template <typename T, int DP>
