@@ -111,6 +111,13 @@ class KVWriteStep:
                                      slots=self.slot_mapping)
         self.rotary_plan = None
         self.cos_sin_cache = cos_sin_cache
+        # An 8-bit cache's write behind a rotation skips the tokens that have no cos/sin row, as the rotation does. Without one that
+        # any slot of the tables could lack, the slots are the step's own.
+        self._rotated_slots = self.slot_mapping
+        if self.q8 and cos_sin_cache is not None and cos_sin_cache.shape[0] < N * self.page_size:
+            self._rotated_slots = torch.full_like(self.slot_mapping, -1)
+            self._has_row = torch.zeros(T, dtype=torch.bool, device=self.device)
+            self._no_slot = torch.full((), -1, dtype=torch.int64, device=self.device)
         if cos_sin_cache is not None and not self.q8:
             self.rotary_plan = PagedRotaryWritePlan(self.batch_indices, self.positions, self.kv_indices,
                                                     self.kv_indptr, self.kv_last_page_len, cos_sin_cache,
@@ -192,9 +199,13 @@ class KVWriteStep:
     # ------------------------------------------------------------------ launches
     def build_index(self) -> None:
         """One launch on the current stream: every index tensor of the step that
-        the buffers hold, written in place. With attention one more lays out its work (two with shared pages)."""
+        the buffers hold, written in place. With attention one more lays out its work (two with shared pages), and
+        with a pool in 8 bits and a cos/sin table of fewer positions than the block tables reach two more find the tokens beyond it."""
         build_write_index(self.input_lens, self.context_lens, self.num_blocks, self.kv_indices,
                           self.page_size, self.max_tokens, out=self._out)
+        if self._rotated_slots is not self.slot_mapping:
+            torch.lt(self.positions, self.cos_sin_cache.shape[0], out=self._has_row)
+            torch.where(self._has_row, self.slot_mapping, self._no_slot, out=self._rotated_slots)
         if self.attention_plan is not None:
             self.attention_plan.build()
 
@@ -202,21 +213,25 @@ class KVWriteStep:
         """One layer's write; `key` / `value` hold `max_tokens` rows, of which the
         step's first `num_tokens` are written."""
         if self.q8:
-            heads = (self.num_kv_heads, self.head_dim)
-            key, value = (t.unflatten(1, heads) if t.dim() == 2 else t for t in (key, value))
-            reshape_and_cache_q8(key, value, paged_kv_cache, self.slot_mapping)
+            self._append_q8(key, value, paged_kv_cache, self.slot_mapping)
             return
         self.plan.append(key, value, paged_kv_cache)
 
+    def _append_q8(self, key, value, paged_kv_cache, slots) -> None:
+        heads = (self.num_kv_heads, self.head_dim)
+        key, value = (t.unflatten(1, heads) if t.dim() == 2 else t for t in (key, value))
+        reshape_and_cache_q8(key, value, paged_kv_cache, slots)
+
     def rotate_and_append(self, query, key, value, paged_kv_cache, query_out=None, key_out=None,
                           query_weight=None, key_weight=None, eps: float = 1e-6):
-        """One layer's rotation and write; with the layer's `query_weight` and `key_weight` its heads are normed first."""
+        """One layer's rotation and write; with the layer's `query_weight` and `key_weight` its heads are normed first.
+        Tokens at positions without a cos/sin row are left alone: neither rotated nor written."""
         if self.cos_sin_cache is None:
             raise ValueError("this step was made without a cos/sin table")
         if self.q8:
             query_out, rotated = rotate_into(query, key, self.positions, self.cos_sin_cache, self.head_dim, query_out, key_out,
                                              query_weight, key_weight, eps)
-            self.append(rotated, value, paged_kv_cache)
+            self._append_q8(rotated, value, paged_kv_cache, self._rotated_slots)
             return query_out, key_out
         return self.rotary_plan.run(query, key, value, paged_kv_cache, query_out=query_out, key_out=key_out,
                                     query_weight=query_weight, key_weight=key_weight, eps=eps)

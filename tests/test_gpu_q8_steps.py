@@ -144,3 +144,66 @@ def test_operators_of_the_dispatcher(gpu):
     torch.ops.kvcache.append_paged_kv_cache_q8(k, v, torch.zeros(20, **i32), slots.int(), b, torch.arange(2, **i32),
                                                torch.tensor([0, 2], **i32), torch.tensor([4], **i32))
     assert torch.equal(a, b) and a.any()
+
+
+@pytest.mark.parametrize("norms", [False, True])
+@pytest.mark.parametrize("key_out", [False, True])
+@pytest.mark.parametrize("recorded", [False, True])
+def test_tokens_beyond_the_cos_sin_table_are_left_alone(gpu, recorded, key_out, norms):
+    """A table that ends inside a request's context, inside a group: the tokens that have no row are not written either, and the
+    codes and exponents that their groups hold stay, whatever the rotated keys' memory held before."""
+    rows = 37
+    cs = kvc.make_cos_sin_cache(D, rows, 10000.0, dtype=torch.bfloat16).to(gpu)
+    step = step_of(gpu, cos_sin_cache=cs)
+    g = torch.Generator().manual_seed(0)
+    weights = [(1 + 0.2 * torch.randn(D, generator=g)).to(torch.bfloat16).to(gpu) for _ in range(2)] if norms else [None, None]
+    pool = kvc.allocate_q8_kv_caches(1, BLOCKS, PAGE, H, D, gpu)
+    pool.random_(0, 256, generator=torch.Generator(device=gpu).manual_seed(1))
+    oracle = qo.Cache(pool[0].cpu().numpy(), H, D)
+    reqs = Requests(5)
+    (q, k, v), = projections(reqs.rng, gpu, 1)
+    q_out = torch.zeros(TOKENS, HQ * D, dtype=torch.bfloat16, device=gpu)
+    k_out = torch.zeros(TOKENS, H * D, dtype=torch.bfloat16, device=gpu) if key_out else None
+    graph = None
+    for new in ((26, 33, 5), (5, 1, 20), (1, 1, 1), (0, 4, 30)):
+        inputs = reqs.next(new)
+        tokens = sum(new)
+        for t, x in zip((q, k, v), projections(reqs.rng, gpu, 1)[0]):
+            t.copy_(x)
+        step.set_requests(inputs)
+        # what earlier steps may have left where the rotation writes nothing
+        junk = torch.full((TOKENS, H * D), 3e38, dtype=torch.bfloat16, device=gpu)
+        if key_out:
+            k_out.copy_(junk)
+        del junk
+        q_out.fill_(7)
+        if recorded and graph is None:
+            def body():
+                step.build_index()
+                step.rotate_and_append(q, k, v, pool[0], query_out=q_out, key_out=k_out, query_weight=weights[0], key_weight=weights[1])
+            body()      # (writing a step twice is writing it once)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                body()
+        if recorded:
+            graph.replay()
+        else:
+            step.build_index()
+            step.rotate_and_append(q, k, v, pool[0], query_out=q_out, key_out=k_out, query_weight=weights[0], key_weight=weights[1])
+        torch.cuda.synchronize()
+        positions = step.positions[:tokens].cpu().numpy()
+        slots = step.slot_mapping[:tokens].cpu().numpy()
+        there = positions < rows
+        assert (q_out[:tokens].cpu()[torch.from_numpy(~there)] == 7).all()
+        call = (lambda *a: kvc.qk_norm_rotary_pos_emb(a[0], a[1], *weights, *a[2:])) if norms else kvc.rotary_pos_emb
+        _, rk = call(q[:tokens].contiguous(), k[:tokens].contiguous(), step.positions[:tokens].clamp(max=rows - 1), cs, D)
+        oracle.write(rk.double().cpu().numpy().reshape(tokens, H, D), v[:tokens].double().cpu().numpy().reshape(tokens, H, D),
+                     np.where(there, slots, -1))
+        assert np.array_equal(pool[0].cpu().numpy(), oracle.pages()), new
+    assert max(reqs.have) > rows + PAGE
+    # without the rotation every token of the step is written
+    before = pool.clone()
+    step.append(k, v, pool[0])
+    oracle.write(k[:tokens].double().cpu().numpy().reshape(tokens, H, D), v[:tokens].double().cpu().numpy().reshape(tokens, H, D), slots)
+    assert np.array_equal(pool[0].cpu().numpy(), oracle.pages()) and not torch.equal(before, pool)
