@@ -118,11 +118,17 @@ class KVWriteStep:
             self._rotated_slots = torch.full_like(self.slot_mapping, -1)
             self._has_row = torch.zeros(T, dtype=torch.bool, device=self.device)
             self._no_slot = torch.full((), -1, dtype=torch.int64, device=self.device)
-        if cos_sin_cache is not None and not self.q8:
-            self.rotary_plan = PagedRotaryWritePlan(self.batch_indices, self.positions, self.kv_indices,
-                                                    self.kv_indptr, self.kv_last_page_len, cos_sin_cache,
-                                                    num_heads, num_kv_heads, head_dim, page_size,
-                                                    slots=self.slot_mapping)
+        if cos_sin_cache is not None:
+            plan = PagedRotaryWritePlan(self.batch_indices, self.positions, self.kv_indices,
+                                        self.kv_indptr, self.kv_last_page_len, cos_sin_cache,
+                                        num_heads, num_kv_heads, head_dim, page_size,
+                                        slots=self.slot_mapping)
+            if self.q8:
+                if cos_sin_cache.dtype != dtype or cos_sin_cache.device != self.slot_mapping.device:
+                    raise TypeError("cos_sin_cache must have the step's dtype and device")
+                self._q_row = plan.q_row      # (the plan checked the table)
+            else:
+                self.rotary_plan = plan
         self.attention_plan = None
         if with_attention:
             self.attention_plan = PagedAttentionPlan(self.cu_seqlens_q, self.kv_indices, self.kv_indptr,
@@ -229,6 +235,12 @@ class KVWriteStep:
         if self.cos_sin_cache is None:
             raise ValueError("this step was made without a cos/sin table")
         if self.q8:
+            kv_row = self.num_kv_heads * self.head_dim
+            for t, width, name in ((query, self._q_row, "query"), (key, kv_row, "key"), (value, kv_row, "value")):
+                if t.dtype != self.cos_sin_cache.dtype or t.device != self.cos_sin_cache.device:
+                    raise TypeError(f"{name} must have the step's dtype and device")
+                if t.dim() < 2 or t.shape[0] != self.max_tokens or t.numel() != self.max_tokens * width:
+                    raise ValueError(f"{name} must hold [{self.max_tokens}, {width}] elements")
             query_out, rotated = rotate_into(query, key, self.positions, self.cos_sin_cache, self.head_dim, query_out, key_out,
                                              query_weight, key_weight, eps)
             self._append_q8(rotated, value, paged_kv_cache, self._rotated_slots)

@@ -207,3 +207,44 @@ def test_tokens_beyond_the_cos_sin_table_are_left_alone(gpu, recorded, key_out, 
     step.append(k, v, pool[0])
     oracle.write(k[:tokens].double().cpu().numpy().reshape(tokens, H, D), v[:tokens].double().cpu().numpy().reshape(tokens, H, D), slots)
     assert np.array_equal(pool[0].cpu().numpy(), oracle.pages()) and not torch.equal(before, pool)
+
+
+def test_what_a_rotating_step_refuses(gpu):
+    """As over 16 bits: a table that is not one at construction, rows of another number or width at every call."""
+    cs = kvc.make_cos_sin_cache(D, 64, 10000.0, dtype=torch.bfloat16).to(gpu)
+    args = (H, D, PAGE, torch.bfloat16, gpu, 4, TOKENS, 20)
+    for error, kw in ((TypeError, dict(cos_sin_cache=cs.half(), num_heads=HQ)), (ValueError, dict(cos_sin_cache=cs.t(), num_heads=HQ)),
+                      (ValueError, dict(cos_sin_cache=cs[0], num_heads=HQ))):
+        with pytest.raises(error):
+            kvc.KVWriteStep(*args, kv_dtype=F8, **kw)
+    with pytest.raises((TypeError, ValueError, RuntimeError)):
+        kvc.KVWriteStep(*args, kv_dtype=F8, cos_sin_cache=cs.cpu(), num_heads=HQ)
+    pool = kvc.allocate_q8_kv_caches(1, BLOCKS, PAGE, H, D, gpu).zero_()
+    step = kvc.KVWriteStep(*args, kv_dtype=F8, cos_sin_cache=cs, num_heads=HQ)
+    reqs = Requests(6)
+    step.set_requests(reqs.next((20, 5)))
+    step.build_index()
+    (q, k, v), = projections(reqs.rng, gpu, 1)
+    half = TOKENS // 2
+    with pytest.raises(ValueError):      # (of a step without query heads)
+        kvc.KVWriteStep(*args, kv_dtype=F8, cos_sin_cache=cs).rotate_and_append(q, k, v, pool[0])
+    for bad in ((q[:half], k, v), (q, k[:half], v), (q, k, v[:half]), (q[:, D:], k, v), (q.reshape(2 * TOKENS, -1), k, v),
+                (q.reshape(-1), k, v), (q, torch.cat((k, k), 1), v), (q, k, torch.cat((v, v), 1)), (q, k, v[:, D:])):
+        with pytest.raises(ValueError):
+            step.rotate_and_append(*bad, pool[0])
+    for bad in ((q.half(), k, v), (q, k.half(), v), (q, k, v.half())):
+        with pytest.raises(TypeError):
+            step.rotate_and_append(*bad, pool[0])
+    with pytest.raises(ValueError):
+        step.rotate_and_append(q, k, v, pool[0], query_out=torch.empty(half, HQ * D, dtype=torch.bfloat16, device=gpu))
+    with pytest.raises(ValueError):
+        step.rotate_and_append(q, k, v, pool[0], query_weight=torch.ones(D, dtype=torch.bfloat16, device=gpu))
+    torch.cuda.synchronize()
+    assert not pool.any()
+    rotated, _ = step.rotate_and_append(q, k, v, pool[0])
+    assert rotated.shape == (TOKENS, HQ * D) and pool.any()
+    # rows of any layout are rows
+    apart = q.reshape(TOKENS, HQ, D).transpose(1, 2).contiguous().transpose(1, 2)
+    again, _ = step.rotate_and_append(apart, k, v, pool[0])
+    n = step.num_tokens
+    assert torch.equal(again.reshape(TOKENS, -1)[:n], rotated[:n])
