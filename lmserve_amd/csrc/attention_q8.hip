@@ -49,6 +49,11 @@ __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi, float by) {
 }
 // 2^n for n from -126 up, less for a lesser one
 __device__ __forceinline__ float power(int32_t n) { return __uint_as_float((uint32_t)(max(n, -127) + 127) << 23); }
+// What the scores of a group of K are scaled by. A product beyond fp32's normal numbers would make 0 * inf or -inf * 0 of scores that are
+// 0 or masked; at their ends it has the same weights, as scores of that size are equal, or infinitely apart, in fp32.
+__device__ __forceinline__ float score_scale(float scale, uint32_t ek) {
+  return __builtin_amdgcn_fmed3f(scale * power_of(ek), 1.17549435e-38f, 3.402823466e38f);
+}
 // what V's codes of a group are scaled by
 __device__ __forceinline__ float v_scale(int32_t ev, int32_t E) { return power(max(ev - E + kUp, -126)); }
 
@@ -218,7 +223,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
             for (int w = 0; w < 4; ++w) b.v[d][w] = without_nan(b.v[d][w]);
         }
       }
-      const float scale = a.scale * power_of(ek);
+      const float scale = score_scale(a.scale, ek);
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -486,7 +491,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
   // the scale of the lane's scores of a half of a window
   const auto scale_of = [&](const Window& x, int half) {
     const uint32_t two = (uint32_t)(x.exps >> half * 32);
-    return a.scale * power_of(max((hi ? two >> 16 : two) & 255, 1u));
+    return score_scale(a.scale, max((hi ? two >> 16 : two) & 255, 1u));
   };
   const auto highest = [&](f32x16& s) {
     float top = s[0];

@@ -19,7 +19,8 @@ namespace q8 {
 
 constexpr int kGroup = 16;               // tokens of a group
 constexpr int kBias = 127;               // of a stored exponent
-constexpr int kLeast = -100, kMost = 120;  // exponents: a product of 2^e with a score's scale stays a normal fp32
+// Exponents. With a score's scale from 2^-26 to 2^8 / log2(e) the product with 2^e is a normal fp32; the attention holds others to those.
+constexpr int kLeast = -100, kMost = 120;
 
 inline int64_t plane_bytes(int64_t heads, int64_t dim) { return kGroup * heads * dim; }
 inline int64_t group_bytes(int64_t heads, int64_t dim) { return (2 * plane_bytes(heads, dim) + 2 * heads + 127) / 128 * 128; }

@@ -344,3 +344,25 @@ def test_write_then_attend(gpu):
         # the rows that come back are those that were attended to
         bk, bv = kvc.read_paged_kv_cache_q8(torch.zeros(new, **i32), positions, pool, *index, H, D)
         assert (bk - k).abs().max() < 0.3 and (bv - v).abs().max() < 0.3
+
+
+@pytest.mark.parametrize("lengths", [[(1, 100), (3, 40), (1, 16)], [(60, 200), (40, 40)]])
+@pytest.mark.parametrize("scale,exponent", [(2.0 ** -60, -100), (1e-30, -100), (2.0 ** -120, 0), (2.0 ** -26, -100), (400.0, 120), (3e5, 118), (1e30, 100)])
+def test_scales_of_any_size(gpu, lengths, scale, exponent):
+    """A softmax scale whose product with a group's 2^e is no normal fp32. The small ones: groups of zeros among keys whose scores are then equal;
+    the large ones: keys that lie in a column that the queries do not have, scores of 0."""
+    s = Step(lengths, 4, 2, 64, 16, seed=23, spread=0)
+    c = s.cache
+    groups = np.unique(s.indices)[::2]
+    by_group = c.codes.reshape(-1, 16, 2, 2, 64)
+    if scale < 1:
+        by_group[groups, :, 0] = 0
+    else:
+        s.query[..., 5] = 0
+        there = (by_group[:, :, 0] & 127) != 127
+        by_group[:, :, 0] = np.where(there, 0, by_group[:, :, 0])
+        by_group[:, :, 0, :, 5] = np.where(there[..., 5], 120, by_group[:, :, 0, :, 5])
+    c.exponents[groups, :, 0] = exponent
+    s.scale = scale
+    out, lse = s.plan(gpu, sm_scale=scale).run(s.query.to(gpu), s.pages(gpu), return_lse=True)
+    s.check(out, lse)
