@@ -644,9 +644,12 @@ int kvc_attention_plan_destroy(kvc_attention_plan* plan);
  * _create_q8 is built, sized and destroyed as the others and run by _run_q8, page_stride in
  * BYTES. head_dim and page_size are multiples of 16. What the codes stand for is
  * what is attended to: a code that is NaN has that value in the rows that see it, and those alone.
- * Weights go into the product with V in f16, scaled up by 2^7 or 2^14, whatever dtype is,
- * with f16 queries of few rows in two parts. Values are kept to 2^-41 of the largest
- * that the keys of the same request may have (448 times their groups' largest scale). */
+ * A weight times its group's scale of V goes into the product in f16, whatever dtype is, so that
+ * the row's largest such stands at 2^6 or more: others are kept to half a step of f16, or to
+ * 2^-30 of that largest. With f16 queries of few rows in two parts. What a row does not see has
+ * no part in that; nor do a group's sizes where the weights make up for them (to 2^-115 of
+ * the largest scale that the row sees). sm_scale times a scale of K is held to the normal
+ * numbers of fp32. */
 int kvc_attention_plan_create_q8(const int32_t* qo_indptr, const int32_t* kv_indices,
                                  const int32_t* kv_indptr, const int32_t* kv_last_page_len,
                                  int64_t batch_size, int64_t num_tokens, int64_t num_kv_indices,

@@ -4,10 +4,10 @@
 // number of bf16 and of f16, so nothing is rounded on the way to them:
 //   the scores are those of the codes, and 2^ek goes with the softmax's scale into the exponent's multiply-add: a lane's scores
 //   are of one group, so that is one register;
-//   V's codes are scaled by 2^(ev - E) in their conversion, E the greatest ev of the keys so far, and O is in units of 2^E: what has been
-//   summed is scaled where E grows. (f16 holds codes scaled up by 2^7 down to ev - E = -22; below that they lose bits to 2^-41 of
-//   the largest value that the same keys may have.)
-// The weights are f16, scaled up as in the 16-bit kernels, whatever the query's type.
+//   V's codes are the product's as they are, and 2^ev goes with the weights: a weight is exp2(score - base) 2^(ev - E) there, and O in units of
+//   2^(base + E). base and E are a row's own: base follows its highest score, base + E the greatest score + ev of the keys that it sees. So
+//   what a row does not see has no part in its units, and a weight is rounded as a part of the row's largest term, weight times group's size.
+// The weights are f16, scaled up as in the 16-bit kernels, whatever the query's type. base and E are whole numbers, so what has been summed is scaled exactly.
 //
 // The keys are permuted: which row of the matrix instruction's A a key is does not matter, and with
 //   row 4 g + r of the i-th product = token 4 i + r of group g        (16 rows, 4 groups, products i = 0..3)
@@ -30,7 +30,12 @@ using namespace kvc;
 using namespace kvc::attn;
 using namespace kvc::q8;
 
-constexpr int kUp = 7;  // log2 of what V's codes are scaled up by
+constexpr float kLowest = -1000;  // E before the row's first key
+// What 2^(ev - E) goes to. Above: E is at least 100 below the greatest ev of the keys that the row sees, however small their weights. Below:
+// weights of f16 come to nothing long before, and in the sum of weights one of 2^-126 is lost, 2^-62 without the factor.
+constexpr int32_t kNear = -64, kFar = 100, kLag = -40;
+// From here on a base is too large to have ev - E added to it in fp32
+constexpr float kHuge = 1 << 22;
 constexpr int kVPad = 16;  // bytes between a wide item's columns of V in LDS
 
 // The code below keeps the lanes of a wavefront together: what differs between lanes is selected, loads go to an address that is there for
@@ -47,16 +52,11 @@ __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi, float by) {
   return u32x4{T::template from_codes<false>(lo, by), T::template from_codes<true>(lo, by), T::template from_codes<false>(hi, by),
                T::template from_codes<true>(hi, by)};
 }
-// 2^n for n from -126 up, less for a lesser one
-__device__ __forceinline__ float power(int32_t n) { return __uint_as_float((uint32_t)(max(n, -127) + 127) << 23); }
 // What the scores of a group of K are scaled by. A product beyond fp32's normal numbers would make 0 * inf or -inf * 0 of scores that are
 // 0 or masked; at their ends it has the same weights, as scores of that size are equal, or infinitely apart, in fp32.
 __device__ __forceinline__ float score_scale(float scale, uint32_t ek) {
   return __builtin_amdgcn_fmed3f(scale * power_of(ek), 1.17549435e-38f, 3.402823466e38f);
 }
-// what V's codes of a group are scaled by
-__device__ __forceinline__ float v_scale(int32_t ev, int32_t E) { return power(max(ev - E + kUp, -126)); }
-
 // Is a key before `end` (of an item that has keys), and on a page of the cache? Where its group lies (that of what is not there: at the cache's beginning)
 __device__ __forceinline__ bool find_group(const AttendArgs& a, int32_t table, int32_t key, int32_t end, uint64_t& at) {
   const int32_t k = min(max(key, 0), end - 1);
@@ -72,13 +72,6 @@ template <bool NT, typename V>
 __device__ __forceinline__ V load(const char* p) {
   if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
   else return *reinterpret_cast<const V*>(p);
-}
-
-__device__ __forceinline__ int32_t max_of_quads(int32_t x) {
-  const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
-  x = max((int32_t)a[0], (int32_t)a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
-  return max((int32_t)b[0], (int32_t)b[1]);
 }
 
 // NaN among V's codes of 4 tokens, which a weight of 0 does not cancel, taken out
@@ -154,7 +147,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
   typedef Narrow<T, DP, FULL, NT> Block;
   constexpr int KS = Block::KS, DTILES = Block::DTILES, OSTRIDE = DP + 4, STEP = kWaves * kStep;
   constexpr bool kRest = std::is_same<T, F16>::value;
-  constexpr float kScaledUp = F16::kScaledUp, kUnscaled = 1.f / (1 << (int)kScaledUp);
+  constexpr float kScaledUp = F16::kScaledUp, kOutgrown = kScaledUp + 1, kUnscaled = 1.f / (1 << (int)kScaledUp);
   float(*const stats)[3][kTile] = reinterpret_cast<float(*)[3][kTile]>(lds + kWaves * kTile * OSTRIDE * 4);
   const int32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int32_t n = lane & 15, quad = lane >> 4, D = a.head_dim;
@@ -163,7 +156,8 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
   u32x4 q[KS][2] = {};
   f32x4 o[DTILES] = {};
   float base = -INFINITY, l = 0;  // weights are exp2(score * scale - base)
-  int32_t limit = 0, E = 0, odd_from = INT32_MAX;
+  float E = kLowest;              // O is in units of 2^(base + E)
+  int32_t limit = 0, odd_from = INT32_MAX;
   {
     const int32_t row = item.row0 + min(n, item.rows - 1), i = row / a.group, g = row - i * a.group;  // (rows that are not there: the last)
     const int2 x = item.q_begin >= 0 ? make_int2(item.q_begin + i, item.limit + i) : a.l.shared_tokens[i];
@@ -195,7 +189,8 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
           s[i] = T::mfma(widen<T>(b.k[i][c][2], b.k[i][c][3], 1.f), q[c][1], s[i]);
         }
       const int32_t avail = b.avail, first = k0 + quad * kGroup;
-      const int32_t ek = avail ? max((int32_t)(b.exps & 255), 1) : kBias, ev = avail ? (int32_t)(b.exps >> 8) : 0;
+      const int32_t ek = avail ? (int32_t)(b.exps & 255) : kBias;
+      const float ev = (float)(b.exps >> 8);
       if (more) {
         if ((it & 15) == 0) b.look_up(a, item, k0 + STEP, lane);
         b.load_k(a, item, h, k0 + STEP, it, lane);
@@ -229,31 +224,43 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][r]);
-      top = max_across32(max_across16(top * scale));
-      const float grown = fmaxf(base, top - kScaledUp);
+      const float mine = top * scale;  // of the lane's group
+      top = max_across32(max_across16(mine));
+      const float grown = fmaxf(base, __builtin_ceilf(top) - kScaledUp);
       const float from = grown == -INFINITY ? 0.f : grown;
-      const int32_t greatest = max(E, max_of_quads(ev));
       const float by_weight = exp2_of(base - from);  // 0 from -inf
-      const float shrink = by_weight * power(E - greatest);
-      const float by = v_scale(ev, greatest);
-      E = greatest;
+      E = fmaxf(E + (base - from), kLowest);  // O's units stay (or it comes to nothing below)
       base = grown;
+      const float need = (mine == -INFINITY ? 3 * kLowest : ev) - E + fmaxf(mine - from, kOutgrown - kFar);
+      if (__ballot(need > kOutgrown)) {
+        const float up = fmaxf(__builtin_ceilf(max_across32(max_across16(need))) - kScaledUp, 0.f), shrink = exp2_of(-up);
+#pragma unroll
+        for (int d = 0; d < DTILES; ++d) o[d] *= shrink;
+        E += up;
+      }
+      const float t = fminf(fmaxf(ev - E, kNear), kFar);
+      float by = scale, minus = t - from;
+      if (__ballot(__builtin_fabsf(from) > kHuge)) {
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) s[j / 4][j % 4] = __builtin_fmaf(s[j / 4][j % 4], scale, -from);
+        by = 1, minus = t;
+      }
       u32x4 p[2], rest[2];
       float sum = 0;
 #pragma unroll
       for (int j = 0; j < kGroup; j += 2) {
-        const float x = exp2_of(__builtin_fmaf(s[j / 4][j % 4], scale, -from));
-        const float y = exp2_of(__builtin_fmaf(s[j / 4][j % 4 + 1], scale, -from));
+        const float x = exp2_of(__builtin_fmaf(s[j / 4][j % 4], by, minus));
+        const float y = exp2_of(__builtin_fmaf(s[j / 4][j % 4 + 1], by, minus));
         const uint32_t two = F16::pack(x, y);
         p[j / 8][j % 8 / 2] = two;
         if (kRest) rest[j / 8][j % 8 / 2] = F16::pack(x - F16::wide(two & 0xffffu), y - F16::wide(two >> 16));
         sum += x + y;
       }
-      l = l * by_weight + sum;
+      l = l * by_weight + sum * exp2_of(-t);
 #pragma unroll
       for (int d = 0; d < DTILES; ++d) {
-        const u32x4 lo = widen<F16>(b.v[d][0], b.v[d][1], by), hi = widen<F16>(b.v[d][2], b.v[d][3], by);
-        o[d] = F16::mfma(lo, p[0], o[d] * shrink);
+        const u32x4 lo = widen<F16>(b.v[d][0], b.v[d][1], 1.f), hi = widen<F16>(b.v[d][2], b.v[d][3], 1.f);
+        o[d] = F16::mfma(lo, p[0], o[d]);
         o[d] = F16::mfma(hi, p[1], o[d]);
         if (kRest) {
           o[d] = F16::mfma(lo, rest[0], o[d]);
@@ -297,7 +304,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
   for (int d = 0; d < DTILES; ++d) {
     f32x4 x;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = l == 0 ? 0.f : __builtin_ldexpf(o[d][e] * weight, E - kBias - kUp);
+    for (int e = 0; e < 4; ++e) x[e] = l == 0 ? 0.f : __builtin_ldexpf(o[d][e] * weight, (int32_t)E - kBias);
     *reinterpret_cast<f32x4*>(my_o + n * OSTRIDE + d * 16 + quad * 4) = x;
   }
   if (wave == 0 && quad == 0 && n < item.rows) {
@@ -329,9 +336,10 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
 
 // ---- wide items: up to 128 rows, a workgroup takes 64 keys at once ------------------------------------------------------
 // As the wide tiles over 16 bits (attention.hip): 32 rows to a wavefront, K half a step ahead of V, one barrier a step. What is
-// staged in LDS is 16 bits: K as the query's type, its rows permuted, V as f16 columns in units of 2^(E - kUp), so a group is converted once for
-// all four wavefronts; a wavefront converts the group of the window that is its own number. E goes with a window, and
-// O is scaled to it before the window's product. V's columns lie in LDS as the product takes them, so it reads them whole, without the transposing read.
+// staged in LDS is 16 bits: K as the query's type, its rows permuted, V as f16 columns, so a group is converted once for
+// all four wavefronts; a wavefront converts the group of the window that is its own number.
+// V's columns lie in LDS as the product takes them, so it reads them whole, without the transposing read.
+// Heads of 64 have three workgroups a CU (a step of 3 chunks and 60 single tokens 62 us with two, 182 registers, 57 with three, 168 and 24 bytes spilled).
 // Bound as over 16 bits, by what two wavefronts a SIMD have under way: 2048 new tokens behind 13 to 30 thousand keys 740 to 810 us from card to
 // card (16 bits: 770 on one where this takes 752), 880 to 960 TFLOP/s.
 template <int DP>
@@ -340,7 +348,6 @@ constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16) + 2 * DP * (kStep * 
 struct Window {  // of 64 keys
   uint64_t present;  // which are there
   uint64_t exps;     // its groups' exponents, 16 bits each
-  int32_t E;         // the greatest of V up to here
 };
 
 template <typename T, int DP, bool FULL>
@@ -387,13 +394,13 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
   const int32_t tile_least = min(min(leasts[0], leasts[1]), min(leasts[2], leasts[3]));
   f32x16 o[DTILES] = {};
   float base = -INFINITY, l = 0;  // as in a narrow tile
-  int32_t E = 0;                  // O's
+  int32_t E = (int32_t)kLowest, least_E = E, most_E = E;  // (of the wavefront's rows that see keys)
+  bool huge = false;
   u32x4 kr[ROUNDS], vr[ROUNDS];
   // where the groups of 16 windows lie, one to a lane, which of them are there, their exponents
   uint32_t group_lo = 0, group_hi = 0, group_exps = 0;
   uint64_t groups = 0;
   const char* place = nullptr;  // of the wavefront's group of the window that K was last asked of
-  int32_t greatest = 0;         // E of that window
   // Keys come in windows of 64: window w begins 32 before the item's 64 w-th key, so that what a step reads, K of the 64
   // keys from its own 32nd on and V of the 64 keys up to its own 32nd, are the windows w + 1 and w.
   const auto window = [&](int32_t w) { return item.key_begin + w * kStep - kStep / 2; };
@@ -410,7 +417,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
       group_lo = (uint32_t)at;
       group_hi = (uint32_t)(at >> 32);
       const uint32_t exps = *reinterpret_cast<const uint16_t*>(a.cache + at + a.exponents + 2 * h);
-      group_exps = there ? exps : kBias;
+      group_exps = there ? exps : kBias << 8 | kBias;
     }
     const uint32_t four = (uint32_t)(groups >> (w & 15) * 4) & 15, left = (uint32_t)(item.key_end - first);
     Window x;
@@ -425,9 +432,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
     for (int i = 0; i < 4; ++i) {
       const uint32_t e = (uint32_t)__builtin_amdgcn_readlane((int)group_exps, (w & 15) * 4 + i);
       x.exps |= (uint64_t)e << (i * 16);
-      greatest = max(greatest, (int32_t)(e >> 8));
     }
-    x.E = greatest;
     place = heads + (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)group_hi, (w & 15) * 4 + wave) << 32 |
                               (uint32_t)__builtin_amdgcn_readlane((int)group_lo, (w & 15) * 4 + wave));
 #pragma unroll
@@ -472,12 +477,11 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
           for (int j = 0; j < 4; ++j) vr[i][j] = without_nan(vr[i][j]);
       }
     }
-    const float by = v_scale((int32_t)(x.exps >> (wave * 16 + 8)) & 255, x.E);
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
       char* const to = v_lds[buf] + piece_of(i) * VSTRIDE + wave * 32;
-      *reinterpret_cast<u32x4*>(to) = widen<F16>(vr[i][0], vr[i][1], by);
-      *reinterpret_cast<u32x4*>(to + 16) = widen<F16>(vr[i][2], vr[i][3], by);
+      *reinterpret_cast<u32x4*>(to) = widen<F16>(vr[i][0], vr[i][1], 1.f);
+      *reinterpret_cast<u32x4*>(to + 16) = widen<F16>(vr[i][2], vr[i][3], 1.f);
     }
   };
 
@@ -488,10 +492,15 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
   const auto v_piece = [&](int buf, int half, int j) {
     return *reinterpret_cast<const u32x4*>(v_lds[buf] + (j % DTILES * 32 + n) * VSTRIDE + half * 64 + hi * 32 + j / DTILES * 16);
   };
-  // the scale of the lane's scores of a half of a window
-  const auto scale_of = [&](const Window& x, int half) {
+  // the exponents of the lane's group of a half of a window; the scale of its scores
+  const auto exps_of = [&](const Window& x, int half) {
     const uint32_t two = (uint32_t)(x.exps >> half * 32);
-    return score_scale(a.scale, max((hi ? two >> 16 : two) & 255, 1u));
+    return hi ? two >> 16 : two & 0xffffu;
+  };
+  const auto scale_of = [&](uint32_t exps) { return score_scale(a.scale, exps & 255); };
+  const auto evs_of = [&](const Window& x, int half) {
+    const uint32_t two = (uint32_t)(x.exps >> half * 32);
+    return make_int2(two >> 8 & 255, two >> 24);
   };
   const auto highest = [&](f32x16& s) {
     float top = s[0];
@@ -499,7 +508,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
     return top;
   };
-  // the row's highest score of 32 keys, scaled, those of keys that it does not see taken out
+  // the highest score of the lane's group of 32 keys, scaled, those of keys that the row does not see taken out
   const auto mask = [&](f32x16& s, float top, float scale, int32_t k0, uint32_t present) {
     if (least < k0 + 32 || ~present) {
       const int32_t left = clamp(limit - k0 - hi * 16, 0, 16);
@@ -509,37 +518,49 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
         if (!(sees >> r & 1)) s[r] = -INFINITY;
       top = highest(s);
     }
-    return max_across32(top * scale);
+    return top * scale;
   };
-  // A base that has been outgrown, as over 16 bits
-  const auto grow = [&](float top, uint32_t* waiting) {
-    if (__ballot(top > base + kOutgrown)) {
-      const float grown = fmaxf(base, __builtin_ceilf(top) - kScaledUp);
-      const float shrink = exp2_of(base - (grown == -INFINITY ? 0.f : grown));  // 0 from -inf
+  // Units of O that have been outgrown, and with them the base, as over 16 bits. (The base may be outgrown by more, as its weights stay in
+  // fp32: by kOutgrown - kLag, while no ev is further below E than that.) The exponents of the weights to come, s * scale + minus, in
+  // which they are scaled by 2^(ev - E); what their sum is scaled back by. `evs` are those of both groups.
+  const auto grow = [&](f32x16& s, float& scale, float mine, int32_t ev, int2 evs, uint32_t* waiting, float& minus) {
+    const float need = mine - base + (float)(ev - E);
+    if (__ballot(need > kOutgrown) || max(evs.x, evs.y) - least_E > kFar || min(evs.x, evs.y) - most_E < kLag) {
+      const float top = max_across32(mine), grown = top > base + kOutgrown ? __builtin_ceilf(top) - kScaledUp : base;
+      const float by = base - (grown == -INFINITY ? 0.f : grown);  // -inf from -inf
+      l *= exp2_of(by);
+      E = max(E + (int32_t)fmaxf(by, kLowest), (int32_t)kLowest);  // O's units stay (or it comes to nothing here)
+      base = grown;
+      const float above = max_across32(mine == -INFINITY ? mine : fmaxf(mine - base, kOutgrown - kFar) + (float)(ev - E));
+      const float up = above > kOutgrown ? __builtin_ceilf(above) - kScaledUp : 0.f, shrink = exp2_of(-up);
 #pragma unroll
       for (int d = 0; d < DTILES; ++d) o[d] *= shrink;
 #pragma unroll
       for (int i = 0; i < 8; ++i) waiting[i] = F16::pack(F16::wide(waiting[i] & 0xffffu) * shrink, F16::wide(waiting[i] >> 16) * shrink);
-      l *= shrink;
-      base = grown;
+      E += (int32_t)up;
+      int32_t x = limit > item.key_begin ? E : INT32_MAX, y = limit > item.key_begin ? E : INT32_MIN / 2;
+      for (int d = 16; d; d >>= 1) x = min(x, __shfl_xor(x, d)), y = max(y, __shfl_xor(y, d));
+      least_E = __builtin_amdgcn_readfirstlane(x);
+      most_E = __builtin_amdgcn_readfirstlane(y);
+      huge = __ballot(__builtin_fabsf(base) > kHuge && base != -INFINITY);
     }
-  };
-  // O in the units of the window whose V comes next
-  const auto in_units = [&](int32_t to) {
-    if (to != E) {
-      const float by = power(E - to);
+    const int32_t t = clamp(ev - E, kNear, kFar);
+    const float from = base == -INFINITY ? 0.f : base;
+    minus = (float)t - from;
+    if (__builtin_expect(huge, 0)) {
 #pragma unroll
-      for (int d = 0; d < DTILES; ++d) o[d] *= by;
-      E = to;
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale, -from);
+      scale = 1;
+      minus = (float)t;
     }
+    return __uint_as_float((uint32_t)(kBias - t) << 23);
   };
   // 32 keys: their weights from the scores s, while the scores of the keys behind them and the product of the weights
   // before them, that waited, with V are on the matrix unit, in the order of attention.hip.
-  const auto take = [&](const f32x16& s, float scale, uint32_t* p, f32x16& next, float& top, const uint32_t* waiting, int buf, auto which,
+  const auto take = [&](const f32x16& s, float scale, float minus, float back, uint32_t* p, f32x16& next, float& top, const uint32_t* waiting, int buf, auto which,
                         u32x4* piece) {
     constexpr int PIECES = KSTEPS + 2 * DTILES, HALF = decltype(which)::value;
     static_assert(PIECES % (kAhead + 1) == 0, "the second half's first pieces are asked for at the end of the first's");
-    const float minus = base == -INFINITY ? 0.f : -base;
     float sum[2] = {}, weight[3] = {};
     next = f32x16{};
     // a weight is used behind the next one's exponential, whose result the adder would wait for
@@ -579,7 +600,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
       __builtin_amdgcn_sched_barrier(0);
     }
     add(15);
-    l += sum[0] + sum[1];
+    l = __builtin_fmaf(sum[0] + sum[1], back, l);
   };
   const int32_t steps = a.num_pages > 0 ? (item.key_end - item.key_begin + kStep - 1) / kStep : 0;
   if (steps > 0) {
@@ -590,7 +611,6 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
     fetch_v();
     stage_k(1);
     stage_v(0, 0, before);
-    int32_t units = before.E;  // of the window whose V is staged
     Window now = fetch_k(1), coming = {}, then = {};  // the windows i + 1, i + 2, i + 3
     fetch_v();
     stage_k(0);
@@ -599,7 +619,9 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
     f32x16 s0 = {}, s1;
 #pragma unroll
     for (int j = 0; j < KSTEPS; ++j) s0 = T::mfma(k_piece(1, 1, j), q[j], s0);
-    float scale0 = scale_of(before, 1);
+    uint32_t exps0 = exps_of(before, 1);
+    int2 evs0 = evs_of(before, 1);
+    float scale0 = scale_of(exps0);
     float top = mask(s0, highest(s0), scale0, k0, (uint32_t)(before.present >> 32));
     for (int32_t i = 0; i < steps; ++i, k0 += kStep) {
       const int buf = i & 1;
@@ -611,24 +633,25 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
         fetch_v();
         if (i + 2 < steps) then = fetch_k(i + 3);
       }
-      in_units(units);
       // before the other workgroup's wavefronts that stage
       __builtin_amdgcn_s_setprio(1);
-      grow(top, p1);
-      take(s0, scale0, p0, s1, top, p1, buf, std::integral_constant<int, 0>{}, piece);
-      const float scale1 = scale_of(now, 0);
+      float minus;
+      const float back0 = grow(s0, scale0, top, (int32_t)(exps0 >> 8), evs0, p1, minus);
+      take(s0, scale0, minus, back0, p0, s1, top, p1, buf, std::integral_constant<int, 0>{}, piece);
+      const uint32_t exps1 = exps_of(now, 0);
+      float scale1 = scale_of(exps1);
       top = mask(s1, top, scale1, k0 + 32, (uint32_t)now.present);
-      grow(top, p0);
-      take(s1, scale1, p1, s0, top, p0, buf, std::integral_constant<int, 1>{}, piece);  // (after the last step: scores of keys that are not there)
-      scale0 = scale_of(now, 1);
+      const float back1 = grow(s1, scale1, top, (int32_t)(exps1 >> 8), evs_of(now, 0), p0, minus);
+      take(s1, scale1, minus, back1, p1, s0, top, p0, buf, std::integral_constant<int, 1>{}, piece);  // (after the last step: scores of keys that are not there)
+      exps0 = exps_of(now, 1);
+      evs0 = evs_of(now, 1);
+      scale0 = scale_of(exps0);
       top = mask(s0, top, scale0, k0 + kStep, (uint32_t)(now.present >> 32));
       __builtin_amdgcn_s_setprio(0);
-      units = now.E;
       now = coming;
       coming = then;
     }
     __syncthreads();
-    in_units(units);
     // the last weights' product
 #pragma unroll
     for (int j = 0; j < 2 * DTILES; ++j) {
@@ -661,7 +684,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
     const auto four = [&](int d, int i) {
       f32x4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = l == 0 ? 0.f : __builtin_ldexpf(o[d][i * 4 + e] * inv, E - kBias - kUp);
+      for (int e = 0; e < 4; ++e) x[e] = l == 0 ? 0.f : __builtin_ldexpf(o[d][i * 4 + e] * inv, E - kBias);
       return x;
     };
     if (item.slot >= 0) {
@@ -698,7 +721,7 @@ __global__ __launch_bounds__(kThreads, q8_narrow_residents(DP)) void rows_kernel
   take_share(a, blockIdx.x, [&](const Item& item, int32_t h) { narrow_item<T, DP, FULL, NT>(a, item, h, lds); });
 }
 template <typename T, int DP, bool FULL>
-__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void step_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kThreads, DP <= 64 && FULL ? 3 : DP <= 128 ? 2 : 1) void step_kernel(AttendArgs a) {
   constexpr int LDS = wide_lds<DP>() > narrow_lds<DP>() ? wide_lds<DP>() : narrow_lds<DP>();
   __shared__ __attribute__((aligned(16))) char lds[LDS];
   take_step<true>(a, [&](const Item& item, int32_t h) { narrow_item<T, DP, FULL, false>(a, item, h, lds); },
