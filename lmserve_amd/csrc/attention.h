@@ -74,6 +74,11 @@ struct AttendArgs {
   Layout l;
 };
 
+// Row r of the tile of a key head whose partial is in a slot. In 64 bits: with 8 columns a workspace of 155 GB has 2^32 rows.
+__host__ __device__ constexpr int64_t partial_row(int32_t slot, int32_t kv_heads, int32_t h, int32_t tile, int32_t r) {
+  return ((int64_t)slot * kv_heads + h) * tile + r;
+}
+
 // The larger of a lane's value and that of the lane 32 (16) further on or before, without LDS
 __device__ __forceinline__ float max_across32(float x) {
   const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

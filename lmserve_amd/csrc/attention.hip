@@ -757,7 +757,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
     if (wave == 0 && quad == 0 && n < item.rows) {
       const float lse2 = all_l == 0 ? -INFINITY : base + T::kScaledUp + __log2f(all_l * kUnscaled);
       if (item.slot >= 0) {
-        a.partial_lse[0][((int64_t)item.slot * a.kv_heads + h) * kTile + n] = lse2;
+        a.partial_lse[0][partial_row(item.slot, a.kv_heads, h, kTile, n)] = lse2;
       } else if (a.lse) {
         const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
         a.lse[(int64_t)(item.q_begin + i) * a.kv_heads * a.group + h * a.group + g] = lse2 * kLn2;
@@ -772,7 +772,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& ite
       for (int w = 0; w < kWaves; ++w)
         x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(lds + w * (kBlock * VSTRIDE)) + r * OSTRIDE + d);
       if (item.slot >= 0) {
-        *reinterpret_cast<f32x4*>(a.partial[0] + (((int64_t)item.slot * a.kv_heads + h) * kTile + r) * D + d) = x;
+        *reinterpret_cast<f32x4*>(a.partial[0] + partial_row(item.slot, a.kv_heads, h, kTile, r) * D + d) = x;
       } else {
         const int32_t row = item.row0 + r, i = row / a.group, g = row - i * a.group;
         const u32x2 two = {T::pack(x[0], x[1]), T::pack(x[2], x[3])};
@@ -1135,7 +1135,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& item,
     const float inv = l == 0 ? 0.f : 1.f / l, lse2 = l == 0 ? -INFINITY : base + kScaledUp + __log2f(l * kUnscaled);
     if (my_row < item.rows) {
       if (item.slot >= 0) {
-        const int64_t row = ((int64_t)item.slot * a.kv_heads + h) * kWide + my_row;
+        const int64_t row = partial_row(item.slot, a.kv_heads, h, kWide, my_row);
         if (hi == 0) a.partial_lse[1][row] = lse2;
 #pragma unroll
         for (int d = 0; d < DTILES; ++d)
@@ -1217,14 +1217,14 @@ __global__ __launch_bounds__(kThreads, 4) void attend_join_kernel(AttendArgs a) 
         else sh = a.l.shared_parts[shared_at];
       }
       const int32_t own = e.parts.count, parts = own + sh.count;
-      const auto row_of = [&](int32_t c) -> uint32_t {  // of part c (a workspace of 16 GB has 2^28 rows at most)
-        if (c < own) return (uint32_t)((c ? e.parts.next + c * e.parts.step : e.parts.slot) * a.kv_heads + h) * own_tile + row % own_tile;
+      const auto row_of = [&](int32_t c) {  // of part c
+        if (c < own) return partial_row(c ? e.parts.next + c * e.parts.step : e.parts.slot, a.kv_heads, h, own_tile, row % own_tile);
         c -= own;
-        return (uint32_t)((c ? sh.next + c * sh.step : sh.slot) * a.kv_heads + h) * shared_tile + shared_row % shared_tile;
+        return partial_row(c ? sh.next + c * sh.step : sh.slot, a.kv_heads, h, shared_tile, shared_row % shared_tile);
       };
       const auto lse_of = [&](int32_t c) { return (c < own ? own_lse : shared_lse)[row_of(c)]; };
-      const auto values_at = [&](int32_t c, uint32_t row, int32_t d) {
-        return *reinterpret_cast<const f32x4*>((c < own ? own_o : shared_o) + (uint64_t)row * D + d);
+      const auto values_at = [&](int32_t c, int64_t row, int32_t d) {
+        return *reinterpret_cast<const f32x4*>((c < own ? own_o : shared_o) + row * D + d);
       };
       const int32_t i = row / a.group, g = row - i * a.group;
       const int64_t out_row = ((int64_t)(e.q_begin + i) * a.kv_heads + h) * a.group + g;
@@ -1235,7 +1235,7 @@ __global__ __launch_bounds__(kThreads, 4) void attend_join_kernel(AttendArgs a) 
         // up to kManyParts parts, each a lane's: where its values are, its lse, its weight; the values are asked for ahead of what they are weighed by
         const int32_t mine = min(column, parts - 1);
         const float lse = column < parts ? lse_of(mine) : -INFINITY;
-        const uint64_t at_mine = (uint64_t)(uintptr_t)((mine < own ? own_o : shared_o) + (uint64_t)row_of(mine) * D);
+        const uint64_t at_mine = (uint64_t)(uintptr_t)((mine < own ? own_o : shared_o) + row_of(mine) * D);
         f32x4 value[kJoined];
         const auto ask = [&](int32_t c0, int32_t d) {
 #pragma unroll

@@ -310,7 +310,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
   if (wave == 0 && quad == 0 && n < item.rows) {
     const float lse2 = all_l == 0 ? -INFINITY : from + kScaledUp + __log2f(all_l * kUnscaled);
     if (item.slot >= 0) {
-      a.partial_lse[0][((int64_t)item.slot * a.kv_heads + h) * kTile + n] = lse2;
+      a.partial_lse[0][partial_row(item.slot, a.kv_heads, h, kTile, n)] = lse2;
     } else if (a.lse) {
       const int32_t row = item.row0 + n, i = row / a.group, g = row - i * a.group;
       a.lse[(int64_t)(item.q_begin + i) * a.kv_heads * a.group + h * a.group + g] = lse2 * kLn2;
@@ -324,7 +324,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) x += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(lds) + (w * kTile + r) * OSTRIDE + d);
     if (item.slot >= 0) {
-      *reinterpret_cast<f32x4*>(a.partial[0] + (((int64_t)item.slot * a.kv_heads + h) * kTile + r) * D + d) = x;
+      *reinterpret_cast<f32x4*>(a.partial[0] + partial_row(item.slot, a.kv_heads, h, kTile, r) * D + d) = x;
     } else {
       const int32_t row = item.row0 + r, i = row / a.group, g = row - i * a.group;
       *reinterpret_cast<u32x2*>(a.out + (((int64_t)(item.q_begin + i) * a.kv_heads + h) * a.group + g) * D * 2 + d * 2) =
@@ -688,7 +688,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
       return x;
     };
     if (item.slot >= 0) {
-      const int64_t row = ((int64_t)item.slot * a.kv_heads + h) * kWide + my_row;
+      const int64_t row = partial_row(item.slot, a.kv_heads, h, kWide, my_row);
       if (hi == 0) a.partial_lse[1][row] = lse2;
 #pragma unroll
       for (int d = 0; d < DTILES; ++d)
