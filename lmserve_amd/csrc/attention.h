@@ -49,7 +49,7 @@ struct Layout {  // the plan's device buffer
   int2* shared_tokens;     // [T] token, and the keys it sees
   Range* ranges;           // [groups] narrow items of a workgroup
   Item* items[2];          // narrow: tile t's part in workgroup w at t + w: those of a workgroup lie side by side
-  Parts* shared_parts;     // of the tiles of the sharing requests' rows
+  Parts* shared_parts;     // of the narrow tiles of the sharing requests' rows (of wide ones the header has them)
   Entry* entries;
 };
 

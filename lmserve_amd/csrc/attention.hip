@@ -289,18 +289,14 @@ __global__ __launch_bounds__(1024) void attend_schedule_kernel(PlanArgs a) {
     const int32_t table = table_of(a, some_request).begin;
     const int32_t each = shared_wide ? round_up(ceil_div(shared_len, shared_chunks), kStep) : 0;
     if (shared_wide) shared_count = ceil_div(shared_len, each);
-    for (int32_t i = tid; i < shared_tiles; i += 1024) {
-      const int32_t row0 = i * shared_tile, rows = min(shared_tile, shared_rows - row0);
-      if (shared_wide) {
-        a.l.shared_parts[i] = {i, i, shared_tiles, shared_count};
-      } else {
-        const Cuts p = cuts_of(a, i * shared_work, shared_work, share, sliver);
-        a.l.shared_parts[i] = {2 * a.groups + i, 2 * p.group, 2, p.count};
-        for (int32_t c = 0; c < p.count; ++c)
-          put(i, p.group + c,
-              {-1, row0, rows, table, cut_key(i * shared_work, shared_work, p, c, 0, shared_len),
-               cut_key(i * shared_work, shared_work, p, c + 1, 0, shared_len), c ? 2 * (p.group + c) : 2 * a.groups + i, 0});
-      }
+    for (int32_t i = tid; i < shared_tiles && !shared_wide; i += 1024) {
+      const int32_t row0 = i * kTile, rows = min(kTile, shared_rows - row0);
+      const Cuts p = cuts_of(a, i * shared_work, shared_work, share, sliver);
+      a.l.shared_parts[i] = {2 * a.groups + i, 2 * p.group, 2, p.count};
+      for (int32_t c = 0; c < p.count; ++c)
+        put(i, p.group + c,
+            {-1, row0, rows, table, cut_key(i * shared_work, shared_work, p, c, 0, shared_len),
+             cut_key(i * shared_work, shared_work, p, c + 1, 0, shared_len), c ? 2 * (p.group + c) : 2 * a.groups + i, 0});
     }
     for (int32_t i = tid; i < shared_items && i < a.max_items[1]; i += 1024) {
       const int32_t c = i / shared_tiles, row0 = (i - c * shared_tiles) * kWide, from = min(c * each, shared_len);
@@ -1232,7 +1228,9 @@ __global__ __launch_bounds__(kThreads, 4) void attend_join_kernel(AttendArgs a) 
         *reinterpret_cast<u32x2*>(a.out + (out_row * D + d) * 2) = u32x2{T::pack(x[0], x[1]), T::pack(x[2], x[3])};
       };
       if (!many) {
-        // up to kManyParts parts, each a lane's: where its values are, its lse, its weight; the values are asked for ahead of what they are weighed by
+        // Each part a lane's: where its values are, its lse, its weight; the values are asked for ahead of what they are weighed by. Parts are up to kManyParts
+        // in the tile that the entry was made for, and up to two more where its rows go on in the prefix's next tile: tiles as long, cut at the same
+        // distances, differ by one cut, and by one more where the line ends. So they are below the half wavefront's 32.
         const int32_t mine = min(column, parts - 1);
         const float lse = column < parts ? lse_of(mine) : -INFINITY;
         const uint64_t at_mine = (uint64_t)(uintptr_t)((mine < own ? own_o : shared_o) + row_of(mine) * D);
