@@ -123,6 +123,7 @@ bool on_current_device(int device) {
 /* append_paged(key, value, batch_indices, positions, cache, kv_indices, kv_indptr,
  *              kv_last_page_len, device, stream): kvc_append_paged_kv_cache on tensors */
 PyObject* fast_append_paged(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS  // (a tensor without strides throws where they are read)
   if (nargs != 10) {
     PyErr_SetString(PyExc_TypeError, "append_paged takes 10 arguments");
     return nullptr;
@@ -155,11 +156,13 @@ PyObject* fast_append_paged(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
       c.data_ptr(), (const int32_t*)ind.data_ptr(), (const int32_t*)ptr.data_ptr(),
       (const int32_t*)last.data_ptr(), nnz, ptr.sizes()[0] - 1, ind.sizes()[0], heads, dim, page_size,
       ks, vs, ps, num_pages, (int)c.element_size(), stream));
+  END_HANDLE_TH_ERRORS
 }
 
 /* reshape_and_cache(key, value, cache, slot_mapping, device, stream): kvc_reshape_and_cache
  * on one layer of the interleaved pool, [num_blocks, 2, block_size, H, D] */
 PyObject* fast_reshape_and_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   if (nargs != 6) {
     PyErr_SetString(PyExc_TypeError, "reshape_and_cache takes 6 arguments");
     return nullptr;
@@ -190,10 +193,12 @@ PyObject* fast_reshape_and_cache(PyObject*, PyObject* const* args, Py_ssize_t na
                                                kc + bs * row * (int64_t)c->element_size(), sl->data_ptr(),
                                                slot_bytes, n, row, ks, vs, bs, stride, row, num_blocks,
                                                (int)c->element_size(), stream));
+  END_HANDLE_TH_ERRORS
 }
 
 /* write_plan_append(plan, nnz, heads, dim, page_size, dtype, device, key, value, cache, stream) */
 PyObject* fast_write_plan_append(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   void *plan, *stream;
   int64_t nnz, heads, dim, page_size, dtype, device;
   if (nargs != 11) {
@@ -216,11 +221,13 @@ PyObject* fast_write_plan_append(PyObject*, PyObject* const* args, Py_ssize_t na
   if (ks < 0 || vs < 0 || ps < 0) return PyLong_FromLong(NOT_FAST);
   return PyLong_FromLong(kvc_write_plan_append((const kvc_write_plan*)plan, k->data_ptr(), v->data_ptr(),
                                                ks, vs, c->data_ptr(), ps, num_pages, stream));
+  END_HANDLE_TH_ERRORS
 }
 
 /* rotary_plan_run(plan, nnz, q_heads, heads, dim, page_size, dtype, device,
  *                 query, key, value, query_out, key_out | None, cache, stream) */
 PyObject* fast_rotary_plan_run(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   void *plan, *stream;
   int64_t nnz, q_heads, heads, dim, page_size, dtype, device;
   if (nargs != 15) {
@@ -254,6 +261,7 @@ PyObject* fast_rotary_plan_run(PyObject*, PyObject* const* args, Py_ssize_t narg
                                              v->data_ptr(), qs, ks, vs, qo->data_ptr(),
                                              ko ? ko->data_ptr() : nullptr, c->data_ptr(), ps, num_pages,
                                              stream));
+  END_HANDLE_TH_ERRORS
 }
 
 // [n, width] or [n, heads, dim] rows, dense inside a token: width and token stride, or false
@@ -326,6 +334,7 @@ PyObject* fast_rotary_pos_emb(PyObject*, PyObject* const* args, Py_ssize_t nargs
  *                     kv_indices, kv_indptr, kv_last_page_len, query_out, key_out | None, device, stream):
  * kvc_rotary_pos_emb_and_append_paged on tensors */
 PyObject* fast_rotary_append_paged(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   if (nargs != 15) {
     PyErr_SetString(PyExc_TypeError, "rotary_append_paged takes 15 arguments");
     return nullptr;
@@ -372,6 +381,7 @@ PyObject* fast_rotary_append_paged(PyObject*, PyObject* const* args, Py_ssize_t 
       cs->sizes()[1] / 2, qs, ks, vs, qo->data_ptr(), ko ? ko->data_ptr() : nullptr, qw, row, c->data_ptr(),
       (const int32_t*)ind->data_ptr(), (const int32_t*)ptr->data_ptr(), ptr->sizes()[0] - 1,
       ind->sizes()[0], page_size, ps, num_pages, kd, stream));
+  END_HANDLE_TH_ERRORS
 }
 
 bool as_f32(PyObject* o, float* out) {
@@ -581,6 +591,7 @@ struct Places {
 /* write_q8(key, value, cache, device, stream, slot_mapping) or (..., batch_indices, positions, kv_indices, kv_indptr):
  * kvc_reshape_and_cache_q8 or kvc_append_paged_kv_cache_q8 on tensors */
 PyObject* fast_write_q8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
   if (nargs != 6 && nargs != 9) {
     PyErr_SetString(PyExc_TypeError, "write_q8 takes 6 or 9 arguments");
     return nullptr;
@@ -606,6 +617,7 @@ PyObject* fast_write_q8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (stride < 0 || ks < 0 || vs < 0) return PyLong_FromLong(NOT_FAST);
   return PyLong_FromLong(at.run(false, k->data_ptr(), v->data_ptr(), c->data_ptr(), n, heads, dim, page_size, ks, vs, stride, pages,
                                 kvc_dtype_of(type), stream));
+  END_HANDLE_TH_ERRORS
 }
 
 /* read_q8(cache, heads, dim, dtype, device, stream, slot_mapping) or (..., batch_indices, positions, kv_indices, kv_indptr)
