@@ -1390,7 +1390,9 @@ Sizes sizes_of(const kvc_attention_plan& p) {
 // Keys that no cache holds, and that are read once, by non-temporal loads (decode of 256 requests, 2.2 GB: 421 and 406 us;
 // one of 131001 keys, 0.5 GB: 108 and 103; behind a shared prompt, 0.27 GB of which 16 MB are read again and again, 126
 // and 130)
-// Over 8 bits from less on: one of 131001 keys, 0.25 GB, 67 and 63; 64 of 1000, 0.13 GB, 37.6 and 38.1.
+// Over 8 bits from 192 MiB on: such a layer and another one leave nothing of each other in the last-level cache (256 MiB), and keys that come from memory are
+// read faster so at every size (16 MiB 15.6 and 15.1, 126 MiB 33.0 and 30.6, 250 MiB 55.9 and 52.1, 1000 MiB 186 and 175); those of a layer that
+// the cache still holds slower (64 MiB 18.9 and 20.0, 188 MiB 29.7 and 34.6, 250 MiB 38.0 and 44.5; 376 MiB 75.2 and 71.1).
 bool past_the_caches(const kvc_attention_plan& p, int64_t element) {
   return p.shared_pages == 0 &&
          p.num_kv_indices * 2 * p.page_size * p.num_kv_heads * p.head_dim * element >= (int64_t(p.q8 ? 192 : 256) << 20);
@@ -1543,8 +1545,9 @@ int run_plan(const char* fn, bool q8, const kvc_attention_plan* plan, const void
   a.group = (int32_t)(plan->num_heads / plan->num_kv_heads);
   a.head_dim = (int32_t)plan->head_dim;
   a.narrow_groups = (int32_t)(plan->n.groups * plan->num_kv_heads);
-  // (a workgroup takes further items where there are more than these)
-  a.wide_groups = (int32_t)round_up(std::min<int64_t>(plan->n.max_items[1] * plan->num_kv_heads, q8 ? 2048 : 4096), 8);
+  // A workgroup takes further items where there are more than these. (Over 8 bits, 1024, 2048 and 4096: 16 chunks of 512 tokens 153, 145 and 144 us,
+  // 64 requests behind a shared prompt 29.5, 26.0 and 26.2, 256 67.6, 67.5 and 66.2, 4 of 4096 tokens 3945, 3904 and 3826.)
+  a.wide_groups = (int32_t)round_up(std::min<int64_t>(plan->n.max_items[1] * plan->num_kv_heads, 4096), 8);
   a.max_entries = (int32_t)plan->n.max_entries;
   a.scale = plan->scale * kLog2e;
   a.l = layout_of(*plan, plan->buffer, nullptr);
