@@ -682,7 +682,9 @@ int kvc_attention_plan_run_q8(const kvc_attention_plan* plan, const void* query,
  * calls go from its first place up. A call that begins at a group's first place
  * begins it anew. One that goes on with it leaves the exponent where it is enough;
  * where it is not, the codes before the new ones are rounded to the greater one. Places
- * behind the last token written are left as they were. (Tokens of one group in another
+ * behind the last token written are left as they were. Going on with a group stores its other
+ * tokens again: what reads or moves them has to be ordered with the write, which over 16 bits
+ * it need not be. (Tokens of one group in another
  * order, or twice, leave that group's contents undefined, and no other's.)
  *
  * Reads are the way back: the rows of the tokens, in any order, rounded once to

@@ -12,8 +12,9 @@
 //   K: a lane has 8 columns of a row, 16 bytes as they come, and stores their 8 codes.
 //   V: a lane has 2 columns of all tokens, 4 bytes a token, 256 bytes a wavefront, and stores 16 codes of each: the group's
 //   transposition needs no LDS. A group that is continued is read, and written whole.
-// Bound by HBM and the caches from some thousand tokens on (16384 tokens of 8 heads of 128, 101 MB: 18.6 us, 5.4 TB/s; 131001 read back, 0.8 GB: 144 us,
-// 5.6 TB/s), by launch and the chain of slots, rows and exponents below (256 single tokens 6.7 us in a graph, one token 4.3).
+// Bound by HBM and the caches from some thousand tokens on (16384 tokens of 8 heads of 128, 101 MB: 20.2 to 21.9 us, 4.6 to 5.0 TB/s, and 17.8 where a
+// graph writes the same rows again, which the last-level cache then holds; 131001 read back, 0.8 GB: 144 us, 5.6 TB/s), by launch and the chain of slots,
+// rows and exponents below (256 single tokens, each of which has a group of V read and written whole, 7.7 us in a graph, 6.5 over the same rows; one token 4.0).
 
 #include <hip/hip_runtime.h>
 

@@ -9,7 +9,8 @@ every head and for K and V (include/kvcache.h has the layout). Blocks move as by
 
 A group's exponent is that of the largest value written into it. A request's tokens come in the order
 of their positions: a call that begins at a group's first place begins the group anew, and one that goes on with it
-rounds what is there to a greater exponent where it has to.
+rounds what is there to a greater exponent where it has to. It stores the group's other tokens again, so whatever reads
+or moves a block that is still being filled is ordered with the writes into it.
 
 `PagedAttentionPlan(kv_dtype=torch.float8_e4m3fn)` and `paged_attention` attend to such a cache.
 """
