@@ -646,7 +646,8 @@ int kvc_attention_plan_destroy(kvc_attention_plan* plan);
  * what is attended to: a code that is NaN has that value in the rows that see it, and those alone.
  * A weight times its group's scale of V goes into the product in f16, whatever dtype is, so that
  * the row's largest such stands at 2^6 or more: others are kept to half a step of f16, or to
- * 2^-30 of that largest. With f16 queries of few rows in two parts. What a row does not see has
+ * 2^-30 of that largest. With f16 queries of few rows in two parts, of many rows divided by
+ * the sum of the weights as they were rounded (lse is of the unrounded ones). What a row does not see has
  * no part in that; nor do a group's sizes where the weights make up for them (to 2^-115 of
  * the largest scale that the row sees). sm_scale times a scale of K is held to the normal
  * numbers of fp32. */

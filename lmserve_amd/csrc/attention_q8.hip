@@ -339,7 +339,7 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
 // staged in LDS is 16 bits: K as the query's type, its rows permuted, V as f16 columns, so a group is converted once for
 // all four wavefronts; a wavefront converts the group of the window that is its own number.
 // V's columns lie in LDS as the product takes them, so it reads them whole, without the transposing read.
-// Heads of 64 have three workgroups a CU (a step of 3 chunks and 60 single tokens 62 us with two, 182 registers, 57 with three, 168 and 24 bytes spilled).
+// Heads of 64 have three workgroups a CU (a step of 3 chunks and 60 single tokens 62 us with two, 182 registers, 57 with three, 168 and 24 to 28 bytes spilled).
 // Bound as over 16 bits, by what two wavefronts a SIMD have under way: 2048 new tokens behind 13 to 30 thousand keys 740 to 810 us from card to
 // card (16 bits: 770 on one where this takes 752), 880 to 960 TFLOP/s.
 template <int DP>
@@ -394,6 +394,11 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
   const int32_t tile_least = min(min(leasts[0], leasts[1]), min(leasts[2], leasts[3]));
   f32x16 o[DTILES] = {};
   float base = -INFINITY, l = 0;  // as in a narrow tile
+  // The sum of the weights as they went into the product, rounded: what O is divided by with f16 outputs, as a row of few keys then keeps what their weights'
+  // roundings have in common (chunks of 5 to 50 tokens from their first key on: up to 1.63 times the plain form's error without, 1.46 so; a step of 3 chunks
+  // and 60 single tokens 57.0 and 59.5 us). Beside bf16's rounding there is no difference.
+  constexpr bool kRounded = std::is_same<T, F16>::value;
+  float rounded = 0;
   int32_t E = (int32_t)kLowest, least_E = E, most_E = E;  // (of the wavefront's rows that see keys)
   bool huge = false;
   u32x4 kr[ROUNDS], vr[ROUNDS];
@@ -529,6 +534,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
       const float top = max_across32(mine), grown = top > base + kOutgrown ? __builtin_ceilf(top) - kScaledUp : base;
       const float by = base - (grown == -INFINITY ? 0.f : grown);  // -inf from -inf
       l *= exp2_of(by);
+      if (kRounded) rounded *= exp2_of(by);
       E = max(E + (int32_t)fmaxf(by, kLowest), (int32_t)kLowest);  // O's units stay (or it comes to nothing here)
       base = grown;
       const float above = max_across32(mine == -INFINITY ? mine : fmaxf(mine - base, kOutgrown - kFar) + (float)(ev - E));
@@ -561,7 +567,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
                         u32x4* piece) {
     constexpr int PIECES = KSTEPS + 2 * DTILES, HALF = decltype(which)::value;
     static_assert(PIECES % (kAhead + 1) == 0, "the second half's first pieces are asked for at the end of the first's");
-    float sum[2] = {}, weight[3] = {};
+    float sum[2] = {}, weight[3] = {}, used = 0;
     next = f32x16{};
     // a weight is used behind the next one's exponential, whose result the adder would wait for
     const auto add = [&](int r) {
@@ -570,6 +576,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
       if (r % 2) {
         p[r / 2] = F16::pack(weight[(r + 2) % 3], weight[r % 3]);
         asm volatile("" : "+v"(p[r / 2]));
+        if (kRounded) used = F16::sum(p[r / 2], used);
       }
     };
     const auto ask = [&](int j) {
@@ -600,7 +607,10 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
       __builtin_amdgcn_sched_barrier(0);
     }
     add(15);
-    l = __builtin_fmaf(sum[0] + sum[1], back, l);
+    const float all = sum[0] + sum[1];
+    l = __builtin_fmaf(all, back, l);
+    // (where they are further off than numbers of f16 are rounded, 2^(ev - E) has scaled them to below f16's: values that count for nothing, weights that do)
+    if (kRounded) rounded = __builtin_fmaf(__builtin_fabsf(used - all) <= all * (1.f / 2048) ? used : all, back, rounded);
   };
   const int32_t steps = a.num_pages > 0 ? (item.key_end - item.key_begin + kStep - 1) / kStep : 0;
   if (steps > 0) {
@@ -661,6 +671,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
   }
   __syncthreads();  // (left_out is complete, and the buffers are free)
   l += __shfl_xor(l, 32);
+  if (kRounded) rounded += __shfl_xor(rounded, 32);
   if (__builtin_expect(left_out, 0)) {  // as above
     const int32_t from = item.key_begin + max((max(tile_least - item.key_begin, 0) + kStep / 2) / kStep * kStep - kStep / 2, 0);
 #pragma unroll 1
@@ -679,7 +690,7 @@ __device__ __forceinline__ void wide_item(const AttendArgs& a, const Item& given
         }
     }
   }
-  const float inv = l == 0 ? 0.f : 1.f / l, lse2 = l == 0 ? -INFINITY : base + kScaledUp + __log2f(l * kUnscaled);
+  const float inv = l == 0 ? 0.f : 1.f / (kRounded ? rounded : l), lse2 = l == 0 ? -INFINITY : base + kScaledUp + __log2f(l * kUnscaled);
   if (my_row < item.rows) {
     const auto four = [&](int d, int i) {
       f32x4 x;

@@ -69,6 +69,11 @@ struct F16 {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(s2, old), __builtin_bit_cast(h2, two), scale, UPPER));
   }
+  // the two numbers of a word, and x
+  static __device__ __forceinline__ float sum(uint32_t two, float x) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, two), h2{1, 1}, x, false);
+  }
   static constexpr uint32_t kExponent = 0x7c00u;
   // log2 of what weights are scaled up by, so that small ones, of which there may be many, are numbers of the type: a weight of 1 is
   // then 2^14 in a narrow tile, and one of kOutgrown, 2^8, is 2^15 in a wide tile. Both keep a step of the type below its largest.

@@ -86,3 +86,22 @@ def test_f16_weights_in_two_parts(gpu, D, shared):
     out = s.plan(gpu, max_q_len=1).run(s.query.to(gpu), s.pages(gpu)).cpu().double().numpy()
     err = np.abs(out - want)
     assert (err <= tol).all(), f"off by {(err / tol).max():.3g} of the bound"
+
+
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_a_row_of_one_key_is_its_value(gpu, D):
+    """f16, wide tiles, whose weights are rounded once: what O is divided by is rounded with them. Codes times 2^-6 are numbers of f16, so the first row of a prompt
+    comes out as its key's value, and one whose keys have one value as that value."""
+    s = Step([(40, 40)] * 24 + [(70, 70)] * 8, 4, 2, D, 16, "f16", seed=33, spread=0)
+    c = s.cache
+    for b in range(24, 32):
+        table = s.indices[s.indptr[b]:s.indptr[b + 1]].astype(np.int64)
+        slots = (table[:, None] * 16 + np.arange(16)).ravel()[:70]
+        c.codes[slots, 1] = c.codes[slots[0], 1]
+    out = s.plan(gpu).run(s.query.to(gpu), s.pages(gpu)).cpu().double().numpy()
+    values = c.values()[:, 1]
+    for b in range(32):
+        v = np.repeat(values[int(s.indices[s.indptr[b]]) * 16], 2, axis=0)
+        rows = out[s.qo[b]] if b < 24 else out[s.qo[b]:s.qo[b + 1]]
+        # (sums in 32 bits: far less than half a step of f16, so the rounding takes it off)
+        assert (np.abs(rows - v) <= 2.0 ** -20 * np.abs(v)).all(), b
