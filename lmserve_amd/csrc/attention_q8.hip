@@ -31,8 +31,8 @@ using namespace kvc::attn;
 using namespace kvc::q8;
 
 constexpr float kLowest = -1000;  // E before the row's first key
-// What 2^(ev - E) goes to. Above: E is at least 100 below the greatest ev of the keys that the row sees, however small their weights. Below:
-// weights of f16 come to nothing long before, and in the sum of weights one of 2^-126 is lost, 2^-62 without the factor.
+// What ev - E is held to. At most kFar: E is raised to the greatest ev of the keys that the row sees less that, however small their weights. At least
+// kNear: what f16 holds of a weight ends long before, and the sum, in fp32, keeps weights from 2^-62 on. From kLag down a base is looked after by itself.
 constexpr int32_t kNear = -64, kFar = 100, kLag = -40;
 // From here on a base is too large to have ev - E added to it in fp32
 constexpr float kHuge = 1 << 22;
@@ -340,8 +340,8 @@ __device__ __forceinline__ void narrow_item(const AttendArgs& a, const Item& giv
 // all four wavefronts; a wavefront converts the group of the window that is its own number.
 // V's columns lie in LDS as the product takes them, so it reads them whole, without the transposing read.
 // Heads of 64 have three workgroups a CU (a step of 3 chunks and 60 single tokens 62 us with two, 182 registers, 57 with three, 168 and 24 to 28 bytes spilled).
-// Bound as over 16 bits, by what two wavefronts a SIMD have under way: 2048 new tokens behind 13 to 30 thousand keys 740 to 810 us from card to
-// card (16 bits: 770 on one where this takes 752), 880 to 960 TFLOP/s.
+// Bound as over 16 bits, by what two wavefronts a SIMD have under way: 2048 new tokens behind 13 to 30 thousand keys 773 to 860 us from card to
+// card (16 bits: 770 to 820), 830 to 925 TFLOP/s.
 template <int DP>
 constexpr int wide_lds() { return 2 * kStep * (DP * 2 + 16) + 2 * DP * (kStep * 2 + kVPad) + (kWaves + 1) * 4; }
 
